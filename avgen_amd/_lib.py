@@ -280,6 +280,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_ptr, c_i64p, c_i32, c_i32, c_ptr, c_ptr, c_i64, c_ptr, c_i64p,
          c_ptr],
     ),
+    "avattn_position_tables": (
+        ctypes.c_int,
+        [c_ptr, c_i32, c_i64, c_i32, c_i32, c_i32, c_ptr, ctypes.c_double, c_ptr, c_ptr, c_ptr],
+    ),
+    "avattn_rotate": (
+        ctypes.c_int,
+        [c_ptr, c_i64p, c_i32, c_ptr, c_i64p,
+         c_ptr, c_i64p, c_i32, c_ptr, c_i64p,
+         c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+         c_ptr, c_ptr, c_i64, c_i32,
+         c_ptr],
+    ),
+    "avattn_add_rms_norm": (
+        ctypes.c_int,
+        [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i32, c_i64, c_i64, c_i32, c_f32, c_ptr, c_ptr, c_ptr, c_ptr],
+    ),
+    "avattn_add_rms_norm_bwd_workspace_size": (c_size, [c_i64, c_i64]),
+    "avattn_add_rms_norm_bwd": (
+        ctypes.c_int,
+        [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i32, c_i64, c_i64, c_i32, c_f32, c_ptr, c_ptr,
+         c_ptr, c_size, c_ptr],
+    ),
 }
 
 # Status codes (include/avattn.h).
@@ -386,6 +408,9 @@ KERNEL_IDS = {
     "ring_dq_finish": 13,
     "dkv_reduce": 14,
     "diag_dq_partials": 15,
+    "add_rms_norm": 16,
+    "add_rms_norm_bwd": 17,
+    "attn_fwd_few": 18,
 }
 
 

@@ -1,0 +1,429 @@
+"""Ops of the steps around attention in a block: the rotation of part of each
+head by sequence positions, and the residual addition with its RMS norm.
+
+Registered as ``torch.library`` ops like those of :mod:`avgen_amd.ops`
+(same checks, streams, workspaces and errors; plain eager calls skip the
+dispatcher's Python layers).  Ops (namespace ``avgen_amd``):
+
+* ``rotate(x, cos, sin, start, half, inverse)`` and ``rotate_pair(q, k, ...)``
+  (one launch for both), differentiable in the tensors;
+* ``add_rms_norm(x, residual, weight, eps) -> (norm, sum)``, differentiable,
+  with ``add_rms_norm_bwd``;
+* ``add_rms_norm_fp8(x, residual, weight, eps) -> (codes, scale, sum)``.
+
+Tensors are bf16 or float32, on one device; unlike the attention ops these
+take any width, stride and alignment.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from contextlib import nullcontext
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .ops import _direct, _grad_direct, _ptr, _require_gpu, _stream, _strides3, _workspace
+
+__all__ = [
+    "MAX_TABLE_PAIRS",
+    "add_rms_norm",
+    "add_rms_norm_bwd",
+    "add_rms_norm_fp8",
+    "position_tables",
+    "rotate",
+    "rotate_pair",
+]
+
+#: Most pairs of one position table (``avattn_position_tables``).
+MAX_TABLE_PAIRS = 256
+
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+def _one_device(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All tensors on one GPU."""
+    _require_gpu(name, *tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise RuntimeError(f"{name}: tensors on different devices: {sorted(map(str, devices))}")
+
+
+def _on(device: torch.device):
+    """Launches on ``device``, whichever is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
+
+
+def _packed_last(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with a contiguous last dimension."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+# ---------------------------------------------------------------------------
+# Rotation
+# ---------------------------------------------------------------------------
+
+
+def position_tables(positions: torch.Tensor, frequencies: list[float], amplitude: float):
+    """cos/sin tables ``(B, 1, L, pairs)`` float32 of integer ``positions``
+    ``(B, L)``: ``amplitude * cos(position * frequency)``, the angle in
+    double."""
+    name = "avgen_amd.position_tables"
+    if positions.ndim != 2:
+        raise ValueError(f"{name}: positions must be (batch, length); got {tuple(positions.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: positions must be int32 or int64; got {positions.dtype}")
+    P = len(frequencies)
+    if not 1 <= P <= MAX_TABLE_PAIRS:
+        raise ValueError(f"{name}: 1 to {MAX_TABLE_PAIRS} pairs; got {P}")
+    _require_gpu(name, positions)
+    positions = _packed_last(positions)
+    B, L = positions.shape
+    stride = positions.stride(0) if B > 1 else 0
+    if 0 < stride < L or stride < 0:
+        positions = positions.contiguous()
+        stride = L
+    cos = torch.empty((B, 1, L, P), device=positions.device, dtype=torch.float32)
+    sin = torch.empty_like(cos)
+    freq = (ctypes.c_double * P)(*frequencies)
+    with _on(positions.device):
+        st = _lib.load().avattn_position_tables(
+            _ptr(positions), int(positions.dtype is torch.int64), stride, B, L, P,
+            ctypes.cast(freq, ctypes.c_void_p), float(amplitude), _ptr(cos), _ptr(sin), _stream(positions.device))
+    _lib.check(st, name)
+    return cos, sin
+
+
+def _check_rotation(name, tensors, cos, sin, start):
+    """Shapes and dtypes; the tables contiguous, with their batch stride."""
+    x = tensors[0]
+    for t in tensors:
+        if t.ndim != 4:
+            raise ValueError(f"{name}: rotary input must be (batch, heads, length, head_dim); got {tuple(t.shape)}")
+        if t.dtype not in _FLOATS or t.dtype is not x.dtype:
+            raise TypeError(f"{name}: inputs must all be bfloat16 or all float32; got {t.dtype}")
+        if t.shape[0] != x.shape[0] or t.shape[2:] != x.shape[2:]:
+            raise ValueError(f"{name}: {tuple(x.shape)} and {tuple(t.shape)} differ in more than their heads")
+    if cos.ndim != 4 or cos.shape != sin.shape:
+        raise ValueError(f"{name}: rotary tables must be (batch, 1, length, pairs) and agree")
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
+        raise TypeError(f"{name}: rotary tables must be float32")
+    B, _, L, D = x.shape
+    P = cos.shape[-1]
+    if P < 1 or start < 0 or start + 2 * P > D:
+        raise ValueError(f"{name}: channels [{start}, {start + 2 * P}) do not lie in a head of {D}")
+    if cos.shape[-2] != L:
+        raise ValueError(f"{name}: sequence length {L} does not match rotary tables built for length {cos.shape[-2]}")
+    if cos.shape[0] not in (1, B) or cos.shape[1] != 1:
+        raise ValueError(f"{name}: rotary tables batch {cos.shape[0]} does not broadcast to {B}")
+    _one_device(name, *tensors, cos, sin)
+    cos, sin = cos.contiguous(), sin.contiguous()
+    return cos, sin, (0 if cos.shape[0] == 1 else L * P)
+
+
+def _rotate_launch(name, q, k, cos, sin, start, half, inverse):
+    cos, sin, tsb = _check_rotation(name, (q,) if k is None else (q, k), cos, sin, start)
+    B, H, L, D = q.shape
+    ins = [_packed_last(t) for t in (q, k) if t is not None]
+    outs = []
+    for t in ins:
+        o = torch.empty_like(t, memory_format=torch.preserve_format)
+        outs.append(o if o.stride(-1) == 1 or D <= 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device))
+    args = []
+    for t, o in zip(ins, outs):
+        args += [_ptr(t), _strides3(t), t.shape[1], _ptr(o), _strides3(o)]
+    if k is None:
+        args += [None, None, 0, None, None]
+    with _on(q.device):
+        st = _lib.load().avattn_rotate(
+            *args, B, L, D, cos.shape[-1], int(start), int(bool(half)), int(q.dtype is torch.float32),
+            _ptr(cos), _ptr(sin), tsb, int(bool(inverse)), _stream(q.device))
+    _lib.check(st, name)
+    return outs
+
+
+def _rotate_impl(x, cos, sin, start, half, inverse):
+    return _rotate_launch("avgen_amd.rotate", x, None, cos, sin, start, half, inverse)[0]
+
+
+def _rotate_pair_impl(q, k, cos, sin, start, half, inverse):
+    return tuple(_rotate_launch("avgen_amd.rotate_pair", q, k, cos, sin, start, half, inverse))
+
+
+@torch.library.custom_op("avgen_amd::rotate", mutates_args=())
+def _rotate_op(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, start: int, half: bool,
+               inverse: bool) -> torch.Tensor:
+    """Rotation (or its transpose) of channels [start, start + 2 pairs)."""
+    return _rotate_impl(x, cos, sin, start, half, inverse)
+
+
+@_rotate_op.register_fake
+def _(x, cos, sin, start, half, inverse):
+    return torch.empty_like(x)
+
+
+@torch.library.custom_op("avgen_amd::rotate_pair", mutates_args=())
+def _rotate_pair_op(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, start: int, half: bool,
+                    inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rotate`` of a query and a key by the same tables, in one launch."""
+    return _rotate_pair_impl(q, k, cos, sin, start, half, inverse)
+
+
+@_rotate_pair_op.register_fake
+def _(q, k, cos, sin, start, half, inverse):
+    return torch.empty_like(q), torch.empty_like(k)
+
+
+def rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, start: int, half: bool,
+           inverse: bool) -> torch.Tensor:
+    """Rotation (or its transpose) of channels [start, start + 2 pairs)."""
+    return _direct(_Rotate, _rotate_op, _rotate_impl, (x, cos, sin, start, half, inverse), (x, cos, sin))
+
+
+def rotate_pair(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, start: int, half: bool,
+                inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rotate`` of a query and a key by the same tables, in one launch."""
+    return _direct(_RotatePair, _rotate_pair_op, _rotate_pair_impl, (q, k, cos, sin, start, half, inverse),
+                   (q, k, cos, sin))
+
+
+def _rotate_setup(ctx, inputs, output):
+    _x, cos, sin, ctx.start, ctx.half, ctx.inverse = inputs
+    ctx.save_for_backward(cos, sin)
+
+
+def _rotate_backward(ctx, grad):
+    cos, sin = ctx.saved_tensors
+    return rotate(grad, cos, sin, ctx.start, ctx.half, not ctx.inverse), None, None, None, None, None
+
+
+def _rotate_pair_setup(ctx, inputs, output):
+    _q, _k, cos, sin, ctx.start, ctx.half, ctx.inverse = inputs
+    ctx.save_for_backward(cos, sin)
+
+
+def _rotate_pair_backward(ctx, gq, gk):
+    cos, sin = ctx.saved_tensors
+    how = (cos, sin, ctx.start, ctx.half, not ctx.inverse)
+    if gq is not None and gk is not None:
+        gq, gk = rotate_pair(gq, gk, *how)
+    else:
+        gq, gk = (None if g is None else rotate(g, *how) for g in (gq, gk))
+    return gq, gk, None, None, None, None, None
+
+
+torch.library.register_autograd("avgen_amd::rotate", _rotate_backward, setup_context=_rotate_setup)
+torch.library.register_autograd("avgen_amd::rotate_pair", _rotate_pair_backward, setup_context=_rotate_pair_setup)
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        result = _rotate_impl(*args)
+        _rotate_setup(ctx, args, result)
+        return result
+
+    backward = staticmethod(_rotate_backward)
+
+
+class _RotatePair(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        result = _rotate_pair_impl(*args)
+        ctx.set_materialize_grads(False)
+        _rotate_pair_setup(ctx, args, result)
+        return result
+
+    backward = staticmethod(_rotate_pair_backward)
+
+
+# ---------------------------------------------------------------------------
+# Residual + RMS norm
+# ---------------------------------------------------------------------------
+
+
+def _rows(t: torch.Tensor):
+    """``t (..., W)`` as rows of ``W`` contiguous values: the tensor to read
+    and its row stride."""
+    W = t.shape[-1]
+    t = _packed_last(t)
+    rows = t.numel() // W if W else 0
+    if t.ndim == 1 or rows <= 1:
+        return t, W
+    # The leading dimensions must collapse into one stride.
+    stride = expect = None
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if stride is None:
+            stride = s
+        elif s != expect:
+            return t.contiguous(), W
+        expect = s * n
+    if stride < 0:
+        return t.contiguous(), W
+    return t, stride
+
+
+def _check_norm(name, x, residual, weight, eps):
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name}: rows of at least one value expected; got {tuple(x.shape)}")
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"{name}: input must be bfloat16 or float32; got {x.dtype}")
+    if residual.shape != x.shape:
+        raise ValueError(f"{name}: residual {tuple(residual.shape)} must have the input's shape {tuple(x.shape)}")
+    if residual.dtype is not x.dtype:
+        raise TypeError(f"{name}: residual must be {x.dtype} like the input; got {residual.dtype}")
+    if weight.shape != (x.shape[-1],):
+        raise ValueError(f"{name}: weight must be ({x.shape[-1]},); got {tuple(weight.shape)}")
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{name}: weight must be {x.dtype} or float32; got {weight.dtype}")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"{name}: eps must be finite and >= 0; got {eps}")
+    _one_device(name, x, residual, weight)
+    return weight.contiguous()
+
+
+def _norm_launch(name, x, residual, weight, eps, fp8):
+    w = _check_norm(name, x, residual, weight, eps)
+    W = x.shape[-1]
+    rows = x.numel() // W
+    total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    norm = torch.empty(x.shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if fp8 else None
+    (x, xs), (residual, rs) = _rows(x), _rows(residual)
+    if rows:
+        with _on(x.device):
+            st = _lib.load().avattn_add_rms_norm(
+                _ptr(x), xs, _ptr(residual), rs, _ptr(w), int(w.dtype is torch.float32), rows, W,
+                int(x.dtype is torch.float32), float(eps), _ptr(total), _ptr(norm), _ptr(scale), _stream(x.device))
+        _lib.check(st, name)
+    return norm, scale, total
+
+
+def _add_rms_norm_impl(x, residual, weight, eps):
+    norm, _, total = _norm_launch("avgen_amd.add_rms_norm", x, residual, weight, eps, False)
+    return norm, total
+
+
+def _add_rms_norm_fp8_impl(x, residual, weight, eps):
+    return _norm_launch("avgen_amd.add_rms_norm_fp8", x, residual, weight, eps, True)
+
+
+def _add_rms_norm_bwd_impl(dnorm, dsum, total, weight, eps):
+    name = "avgen_amd.add_rms_norm_bwd"
+    w = _check_norm(name, total, total, weight, eps)
+    for label, t in (("norm gradient", dnorm), ("sum gradient", dsum)):
+        if t is not None and (t.shape != total.shape or t.dtype is not total.dtype):
+            raise ValueError(f"{name}: {label} must be {total.dtype} {tuple(total.shape)}")
+    _one_device(name, dnorm, dsum, total)
+    W = total.shape[-1]
+    rows = total.numel() // W
+    dx = torch.empty(total.shape, dtype=total.dtype, device=total.device)
+    dw = torch.empty((W,), dtype=w.dtype, device=w.device)
+    (dnorm, dns), (total, hs) = _rows(dnorm), _rows(total)
+    dhs = 0
+    if dsum is not None:
+        dsum, dhs = _rows(dsum)
+    lib = _lib.load()
+    ws = _workspace(lib.avattn_add_rms_norm_bwd_workspace_size(rows, W), total.device)
+    with _on(total.device):
+        st = lib.avattn_add_rms_norm_bwd(
+            _ptr(dnorm), dns, _ptr(dsum), dhs, _ptr(total), hs, _ptr(w), int(w.dtype is torch.float32), rows, W,
+            int(total.dtype is torch.float32), float(eps), _ptr(dx), _ptr(dw), _ptr(ws), ws.numel(),
+            _stream(total.device))
+    _lib.check(st, name)
+    return dx, dw
+
+
+@torch.library.custom_op("avgen_amd::add_rms_norm", mutates_args=())
+def _add_rms_norm_op(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                     eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(norm, sum)`` of ``x + residual``; see the module docstring."""
+    return _add_rms_norm_impl(x, residual, weight, eps)
+
+
+@_add_rms_norm_op.register_fake
+def _(x, residual, weight, eps):
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+@torch.library.custom_op("avgen_amd::add_rms_norm_bwd", mutates_args=())
+def _add_rms_norm_bwd_op(dnorm: torch.Tensor, dsum: Optional[torch.Tensor], total: torch.Tensor,
+                         weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(dx, dweight)``: the gradient of both addends, and of the gain."""
+    return _add_rms_norm_bwd_impl(dnorm, dsum, total, weight, eps)
+
+
+@_add_rms_norm_bwd_op.register_fake
+def _(dnorm, dsum, total, weight, eps):
+    return total.new_empty(total.shape), weight.new_empty(weight.shape)
+
+
+@torch.library.custom_op("avgen_amd::add_rms_norm_fp8", mutates_args=())
+def _add_rms_norm_fp8_op(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                         eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(codes, scale, sum)``: the norm as e4m3 with a scale per row."""
+    return _add_rms_norm_fp8_impl(x, residual, weight, eps)
+
+
+@_add_rms_norm_fp8_op.register_fake
+def _(x, residual, weight, eps):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32),
+            x.new_empty(x.shape))
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                 eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(norm, sum)`` of ``x + residual``; differentiable."""
+    return _direct(_AddRmsNorm, _add_rms_norm_op, _add_rms_norm_impl, (x, residual, weight, eps),
+                   (x, residual, weight))
+
+
+def add_rms_norm_bwd(dnorm, dsum, total, weight, eps):
+    """``(dx, dweight)`` of ``add_rms_norm`` from its stored sum."""
+    if _grad_direct(dnorm, dsum, total, weight):
+        return _add_rms_norm_bwd_impl(dnorm, dsum, total, weight, eps)
+    return _add_rms_norm_bwd_op(dnorm, dsum, total, weight, eps)
+
+
+def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                     eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(codes, scale, sum)``: the norm as e4m3 with a scale per row; not
+    differentiable."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, residual, weight)):
+        raise RuntimeError("avgen_amd.add_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
+    return _direct(None, _add_rms_norm_fp8_op, _add_rms_norm_fp8_impl, (x, residual, weight, eps),
+                   (x, residual, weight))
+
+
+def _norm_setup(ctx, inputs, output):
+    _x, _residual, weight, ctx.eps = inputs
+    ctx.save_for_backward(output[1], weight)
+
+
+def _norm_backward(ctx, dnorm, dsum):
+    total, weight = ctx.saved_tensors
+    if dnorm is None:
+        # The sum alone was used: its gradient passes through.
+        return dsum, dsum, None, None
+    dx, dw = add_rms_norm_bwd(dnorm, dsum, total, weight, ctx.eps)
+    return dx, dx, dw, None
+
+
+torch.library.register_autograd("avgen_amd::add_rms_norm", _norm_backward, setup_context=_norm_setup)
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        result = _add_rms_norm_impl(*args)
+        ctx.set_materialize_grads(False)
+        _norm_setup(ctx, args, result)
+        return result
+
+    backward = staticmethod(_norm_backward)

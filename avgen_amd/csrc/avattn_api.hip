@@ -937,3 +937,157 @@ extern "C" int avattn_fwd_noalloc(const void* q, const void* k, const void* v, c
                   key_mask, key_mask_batch_stride, rope_cos_q, rope_sin_q, rope_batch_stride, false, nullptr,
                   nullptr, scale, out, out_strides, lse, ws, ws ? need : 0, stream);
 }
+
+// ---------------------------------------------------------------------------
+// Sequence rotation and residual RMS norm
+// ---------------------------------------------------------------------------
+
+namespace {
+
+bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int avattn_position_tables(const void* positions, int32_t positions_i64, int64_t positions_batch_stride, int32_t batch,
+                           int32_t len, int32_t pairs, const double* frequencies, double amplitude, float* cos_out,
+                           float* sin_out, avattn_stream_t stream) {
+  if (batch < 0 || len < 0 || pairs < 1 || pairs > kMaxTablePairs) return AVATTN_ERR_BAD_SHAPE;
+  if (!frequencies) return AVATTN_ERR_NULL_POINTER;
+  if (!isfinite(amplitude) || (positions_batch_stride != 0 && positions_batch_stride < len)) return AVATTN_ERR_ARGUMENT;
+  if ((int64_t)batch * len == 0) return AVATTN_OK;
+  if (!positions || !cos_out || !sin_out) return AVATTN_ERR_NULL_POINTER;
+  if (!aligned_to(positions, positions_i64 ? 8 : 4) || !aligned_to(cos_out, 4) || !aligned_to(sin_out, 4))
+    return AVATTN_ERR_LAYOUT;
+  PositionTableArgs a{};
+  a.psb = positions_batch_stride;
+  a.B = batch;
+  a.L = len;
+  a.P = pairs;
+  a.amplitude = amplitude;
+  for (int p = 0; p < pairs; ++p) {
+    if (!isfinite(frequencies[p])) return AVATTN_ERR_ARGUMENT;
+    a.freq[p] = frequencies[p];
+  }
+  a.cos_out = cos_out;
+  a.sin_out = sin_out;
+  return launch_status(launch_position_tables(a, positions, positions_i64 != 0, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int avattn_rotate(const void* q, const int64_t* q_strides, int32_t heads_q, void* q_out, const int64_t* q_out_strides,
+                  const void* k, const int64_t* k_strides, int32_t heads_k, void* k_out, const int64_t* k_out_strides,
+                  int32_t batch, int32_t len, int32_t head_dim, int32_t pairs, int32_t start, int32_t half_layout,
+                  int32_t is_f32, const float* cos_tab, const float* sin_tab, int64_t table_batch_stride,
+                  int32_t inverse, avattn_stream_t stream) {
+  if (batch < 0 || len < 0 || heads_q < 0 || heads_k < 0 || head_dim < 2 || pairs < 1 || start < 0)
+    return AVATTN_ERR_BAD_SHAPE;
+  if (head_dim > 65536 || (int64_t)start + 2 * (int64_t)pairs > head_dim) return AVATTN_ERR_BAD_SHAPE;
+  if ((int64_t)heads_q + heads_k > (1 << 24)) return AVATTN_ERR_TOO_LARGE;
+  if ((int64_t)batch * len * ((int64_t)heads_q + heads_k) == 0) return AVATTN_OK;
+  const size_t size = is_f32 ? 4 : 2;
+  if (!cos_tab || !sin_tab) return AVATTN_ERR_NULL_POINTER;
+  if (heads_q > 0 && (!q || !q_out || !q_strides || !q_out_strides)) return AVATTN_ERR_NULL_POINTER;
+  if (heads_k > 0 && (!k || !k_out || !k_strides || !k_out_strides)) return AVATTN_ERR_NULL_POINTER;
+  if ((heads_q > 0 && (!aligned_to(q, size) || !aligned_to(q_out, size))) ||
+      (heads_k > 0 && (!aligned_to(k, size) || !aligned_to(k_out, size))) || !aligned_to(cos_tab, 4) ||
+      !aligned_to(sin_tab, 4))
+    return AVATTN_ERR_LAYOUT;
+  if (table_batch_stride != 0 && table_batch_stride < (int64_t)len * pairs) return AVATTN_ERR_ARGUMENT;
+  RotateArgs a{};
+  // One tensor alone comes first.
+  const bool first = heads_q > 0;
+  a.x[0] = first ? q : k;
+  a.o[0] = first ? q_out : k_out;
+  a.H[0] = first ? heads_q : heads_k;
+  a.x[1] = k;
+  a.o[1] = k_out;
+  a.H[1] = first ? heads_k : 0;
+  for (int d = 0; d < 3; ++d) {
+    a.xs[0][d] = first ? q_strides[d] : k_strides[d];
+    a.os[0][d] = first ? q_out_strides[d] : k_out_strides[d];
+    a.xs[1][d] = a.H[1] ? k_strides[d] : 0;
+    a.os[1][d] = a.H[1] ? k_out_strides[d] : 0;
+  }
+  a.B = batch;
+  a.L = len;
+  a.D = head_dim;
+  a.P = pairs;
+  a.start = start;
+  a.ct = cos_tab;
+  a.st = sin_tab;
+  a.tsb = table_batch_stride;
+  a.inverse = inverse != 0;
+  return launch_status(launch_rotate(a, half_layout != 0, is_f32 != 0, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int avattn_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                        const void* weight, int32_t weight_is_f32, int64_t rows, int64_t width, int32_t is_f32,
+                        float eps, void* sum_out, void* norm_out, float* scale_out, avattn_stream_t stream) {
+  if (rows < 0 || width < 1) return AVATTN_ERR_BAD_SHAPE;
+  if (rows > kMaxI32 || width > kMaxI32) return AVATTN_ERR_TOO_LARGE;
+  if (!(eps >= 0.f) || !isfinite(eps) || (is_f32 && !weight_is_f32)) return AVATTN_ERR_ARGUMENT;
+  if (rows == 0) return AVATTN_OK;
+  if (!x || !residual || !weight || !sum_out || !norm_out) return AVATTN_ERR_NULL_POINTER;
+  const size_t size = is_f32 ? 4 : 2;
+  if (!aligned_to(x, size) || !aligned_to(residual, size) || !aligned_to(weight, weight_is_f32 ? 4 : 2) ||
+      !aligned_to(sum_out, size) || !aligned_to(norm_out, scale_out ? 1 : size) || !aligned_to(scale_out, 4))
+    return AVATTN_ERR_LAYOUT;
+  AddNormArgs a{};
+  a.x = x;
+  a.xs = x_row_stride;
+  a.r = residual;
+  a.rs = residual_row_stride;
+  a.w = weight;
+  a.w32 = weight_is_f32 != 0;
+  a.rows = rows;
+  a.W = width;
+  a.eps = eps;
+  a.h = sum_out;
+  a.n = norm_out;
+  a.scale = scale_out;
+  return launch_status(
+      launch_add_norm(a, is_f32 != 0, scale_out != nullptr, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t avattn_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width) {
+  if (rows < 0 || width < 1 || rows > kMaxI32 || width > kMaxI32) return 0;
+  return add_norm_bwd_workspace_bytes(rows, width);
+}
+
+int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, const void* dsum, int64_t dsum_row_stride,
+                            const void* sum, int64_t sum_row_stride, const void* weight, int32_t weight_is_f32,
+                            int64_t rows, int64_t width, int32_t is_f32, float eps, void* dx, void* dweight,
+                            void* workspace, size_t workspace_bytes, avattn_stream_t stream) {
+  if (rows < 0 || width < 1) return AVATTN_ERR_BAD_SHAPE;
+  if (rows > kMaxI32 || width > kMaxI32) return AVATTN_ERR_TOO_LARGE;
+  if (!(eps >= 0.f) || !isfinite(eps) || (is_f32 && !weight_is_f32)) return AVATTN_ERR_ARGUMENT;
+  if (!weight || !dweight) return AVATTN_ERR_NULL_POINTER;
+  const size_t size = is_f32 ? 4 : 2, wsize = weight_is_f32 ? 4 : 2;
+  if (!aligned_to(weight, wsize) || !aligned_to(dweight, wsize)) return AVATTN_ERR_LAYOUT;
+  if (rows > 0) {
+    if (!dnorm || !sum || !dx) return AVATTN_ERR_NULL_POINTER;
+    if (!aligned_to(dnorm, size) || !aligned_to(dsum, size) || !aligned_to(sum, size) || !aligned_to(dx, size))
+      return AVATTN_ERR_LAYOUT;
+    if (!workspace || workspace_bytes < add_norm_bwd_workspace_bytes(rows, width) || !aligned16(workspace))
+      return AVATTN_ERR_WORKSPACE;
+  }
+  AddNormArgs a{};
+  a.x = sum;
+  a.xs = sum_row_stride;
+  a.dn = dnorm;
+  a.dns = dnorm_row_stride;
+  a.dh = dsum;
+  a.dhs = dsum ? dsum_row_stride : 0;
+  a.w = weight;
+  a.w32 = weight_is_f32 != 0;
+  a.rows = rows;
+  a.W = width;
+  a.eps = eps;
+  a.h = dx;
+  a.part = static_cast<float*>(workspace);
+  return launch_status(
+      launch_add_norm_bwd(a, is_f32 != 0, dweight, weight_is_f32 != 0, reinterpret_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

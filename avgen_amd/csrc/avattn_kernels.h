@@ -274,6 +274,9 @@ enum KernelId : int {
   kKidDqFinish = 13,
   kKidDkdvReduce = 14,
   kKidDiag = 15,
+  kKidAddNorm = 16,
+  kKidAddNormBwd = 17,
+  kKidFwdFew = 18,
 };
 
 // Records HIP events around one launch on `stream` while timing is enabled.
@@ -355,6 +358,59 @@ hipError_t launch_qk_norm(const QkNormArgs& a, int head_dim, hipStream_t stream)
 hipError_t launch_qk_norm_bwd(const QkNormArgs& a, int head_dim, float* dw, hipStream_t stream);
 // dw[0 .. head_dim) = 0 (the gain gradient of an empty input).
 hipError_t launch_qk_norm_dw_zero(float* dw, int head_dim, hipStream_t stream);
+
+// Tables of integer positions (seq_rope.hip): position of token (b, i) at
+// b*psb + i, pair p's frequency freq[p]; cos and sin, times amplitude, to
+// (b, i, pair) contiguous.
+constexpr int kMaxTablePairs = 256;
+struct PositionTableArgs {
+  int64_t psb;
+  int B, L, P;
+  double amplitude;
+  double freq[kMaxTablePairs];
+  float* cos_out;
+  float* sin_out;
+};
+hipError_t launch_position_tables(const PositionTableArgs& a, const void* pos, bool wide, hipStream_t stream);
+
+// Rotation of part of the heads of one or two tensors (the second with H[1]
+// 0: none) with the same tables, (b, i, pair) at b*tsb + i*P + pair.  Row i
+// of head h of tensor w at b*xs[w][0] + h*xs[w][1] + i*xs[w][2] (output: os).
+struct RotateArgs {
+  const void* x[2];
+  void* o[2];
+  int64_t xs[2][3], os[2][3];
+  int H[2];
+  int B, L, D, P, start;
+  const float* ct;
+  const float* st;
+  int64_t tsb;
+  bool inverse;
+};
+hipError_t launch_rotate(const RotateArgs& a, bool half, bool f32, hipStream_t stream);
+
+// Residual addition + RMS norm (add_norm.hip).  Forward: rows of x and r, xs
+// and rs apart; h and n (e4m3 codes with scale per row, or the rows' type)
+// contiguous.  Backward: x holds the stored h, h receives dx, part the dW
+// partials (add_norm_bwd_workspace_bytes).
+struct AddNormArgs {
+  const void* x;
+  const void* r;
+  const void* w;
+  void* h;
+  void* n;
+  float* scale;
+  const void* dn;
+  const void* dh;  // null: none
+  float* part;
+  int64_t xs, rs, dns, dhs;
+  int64_t rows, W;
+  float eps;
+  bool w32;  // the gain is fp32
+};
+size_t add_norm_bwd_workspace_bytes(int64_t rows, int64_t W);
+hipError_t launch_add_norm(const AddNormArgs& a, bool f32, bool fp8, hipStream_t stream);
+hipError_t launch_add_norm_bwd(const AddNormArgs& a, bool f32, void* dw, bool dw32, hipStream_t stream);
 
 hipError_t launch_zero_rows(bf16* x, int64_t sb, int64_t sh, int64_t sl, int B, int H, int L, int D,
                             hipStream_t stream);

@@ -22,10 +22,10 @@ from __future__ import annotations
 import torch
 
 from . import attention as _attention
-from . import ops
+from . import block_ops, ops
 from .rope import RotaryTables
 
-__all__ = ["qk_norm_rope", "self_attention_core", "split_heads"]
+__all__ = ["add_rms_norm", "add_rms_norm_fp8", "qk_norm_rope", "self_attention_core", "split_heads"]
 
 
 def split_heads(projected: torch.Tensor, head_dim: int) -> torch.Tensor:
@@ -87,3 +87,28 @@ def self_attention_core(
     v = split_heads(v_proj, head_dim)
     out = _attention.attention(q, k, v, attn_mask=key_mask, enable_gqa=q.shape[1] != k.shape[1])
     return out.transpose(1, 2).flatten(2)
+
+
+def add_rms_norm(
+    x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(rms_norm(x + residual) * weight, x + residual)`` over the last
+    dimension in one pass: a block's residual addition and the norm that
+    follows it (src/avgen/models/blocks.py:173-227, layers.py:106-118).
+
+    ``x`` and ``residual`` are bf16 or float32 of one shape ``(..., width)``,
+    any width; ``weight (width,)`` in their dtype or float32.  The norm is
+    that of the unrounded fp32 sum; both results are rounded once.
+    Differentiable in all three (the addends share one gradient)."""
+    return block_ops.add_rms_norm(x, residual, weight, float(eps))
+
+
+def add_rms_norm_fp8(
+    x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`add_rms_norm` with the norm in e4m3 for an fp8 projection:
+    ``(codes, scale, x + residual)``, ``codes`` float8_e4m3fn and ``scale``
+    float32 ``(...)`` with ``norm ~ codes * scale[..., None]``; ``scale`` is the
+    row's largest magnitude / 448 (1 for a row of zeros).  For sampling: not
+    differentiable."""
+    return block_ops.add_rms_norm_fp8(x, residual, weight, float(eps))

@@ -10,21 +10,28 @@ round to bf16), and differentiable.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
 from torch import nn
 
-from . import ops
+from . import block_ops, ops
 
 __all__ = [
+    "POSITION_SCALING_MODES",
+    "PositionScaling",
     "ROPE_SCALING_MODES",
     "RoPEScaling",
     "RotaryEmbedding",
     "RotaryTables",
     "apply_rotary",
+    "build_position_tables",
     "build_rotary_tables",
     "inverse_frequencies",
+    "position_frequencies",
+    "rotate_heads",
+    "rotate_query_key",
     "rope_axis_pairs",
 ]
 
@@ -233,3 +240,146 @@ class RotaryEmbedding(nn.Module):
             f"head_dim={self.head_dim}, pairs(t,h,w)={budgets}, theta={self.theta}, "
             f"time_scale={self.time_scale}, scaling={self.scaling.mode}"
         )
+
+
+# ---------------------------------------------------------------------------
+# Token sequences: positions in one dimension, part of the head, either layout
+# (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+#: Modes of :class:`PositionScaling`.
+POSITION_SCALING_MODES: tuple[str, ...] = ("none", "linear", "ntk", "yarn")
+
+
+@dataclass(frozen=True)
+class PositionScaling:
+    """Scaling of 1D rotary frequencies for contexts ``factor`` times longer
+    than the ``original_length`` they were trained for.
+
+    With ``f_p = theta ** (-2 p / rotary_dim)``:
+
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"ntk"``: ``theta`` raised by ``factor ** (d / (d - 2))``, ``d`` the
+      rotary width;
+    * ``"yarn"`` (Peng et al., 2023): a pair that turns more than ``beta_fast``
+      times over the original length keeps its frequency, one that turns less
+      than ``beta_slow`` times has it divided by ``factor``, linearly in the
+      turns between; cos and sin are multiplied by ``attention_factor``
+      (default ``0.1 ln(factor) + 1``, 1 for factors up to 1).
+
+    Raises:
+        ValueError: unknown mode, a non-positive factor, original length or
+            attention factor, or ``beta_fast <= beta_slow``.
+    """
+
+    mode: str = "none"
+    factor: float = 1.0
+    original_length: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+
+    def __post_init__(self) -> None:
+        if self.mode not in POSITION_SCALING_MODES:
+            raise ValueError(f"mode must be one of {POSITION_SCALING_MODES}; got {self.mode!r}")
+        if not (float(self.factor) > 0.0 and math.isfinite(self.factor)):
+            raise ValueError(f"factor must be positive; got {self.factor!r}")
+        if self.mode == "yarn":
+            if not self.original_length > 0:
+                raise ValueError(f"original_length must be positive; got {self.original_length!r}")
+            if not self.beta_fast > self.beta_slow:
+                raise ValueError(f"beta_fast must exceed beta_slow; got {self.beta_fast!r} and {self.beta_slow!r}")
+            a = self.attention_factor
+            if a is not None and not (a > 0.0 and math.isfinite(a)):
+                raise ValueError(f"attention_factor must be positive; got {a!r}")
+
+
+def position_frequencies(
+    rotary_dim: int, *, theta: float = 10000.0, scaling: PositionScaling | None = None
+) -> tuple[list[float], float]:
+    """The ``rotary_dim / 2`` frequencies and the amplitude of the tables, in
+    double precision.
+
+    Raises:
+        ValueError: ``rotary_dim`` odd, below 2 or above twice
+            ``block_ops.MAX_TABLE_PAIRS``, or a non-positive ``theta``.
+    """
+    if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > 2 * block_ops.MAX_TABLE_PAIRS:
+        raise ValueError(f"rotary_dim must be even, from 2 to {2 * block_ops.MAX_TABLE_PAIRS}; got {rotary_dim!r}")
+    if not (theta > 0.0 and math.isfinite(theta)):
+        raise ValueError(f"theta must be positive; got {theta!r}")
+    plan = scaling if scaling is not None else PositionScaling()
+    if plan.mode == "ntk" and rotary_dim > 2:
+        theta = theta * plan.factor ** (rotary_dim / (rotary_dim - 2))
+    freq = [theta ** (-2.0 * p / rotary_dim) for p in range(rotary_dim // 2)]
+    if plan.mode == "linear":
+        return [f / plan.factor for f in freq], 1.0
+    if plan.mode != "yarn":
+        return freq, 1.0
+    scaled = []
+    for f in freq:
+        turns = plan.original_length * f / (2.0 * math.pi)
+        keep = min(1.0, max(0.0, (turns - plan.beta_slow) / (plan.beta_fast - plan.beta_slow)))
+        scaled.append(f * (keep + (1.0 - keep) / plan.factor))
+    if plan.attention_factor is not None:
+        return scaled, float(plan.attention_factor)
+    return scaled, 0.1 * math.log(plan.factor) + 1.0 if plan.factor > 1.0 else 1.0
+
+
+def build_position_tables(
+    positions: torch.Tensor,
+    *,
+    rotary_dim: int,
+    theta: float = 10000.0,
+    scaling: PositionScaling | None = None,
+) -> RotaryTables:
+    """Tables of a token sequence: ``positions`` int32 or int64 ``(length,)`` or
+    ``(batch, length)`` on the GPU, for :func:`rotate_heads` and
+    :func:`rotate_query_key` (and, with ``rotary_dim`` the head's width and the
+    interleaved layout, for everything that takes :class:`RotaryTables`).
+    Angles are formed and reduced in double precision: far positions lose
+    nothing.
+
+    Raises:
+        ValueError: wrong rank, or what :func:`position_frequencies` refuses.
+        TypeError: positions not int32 or int64.
+    """
+    if positions.ndim not in (1, 2):
+        raise ValueError(f"positions must be (length,) or (batch, length); got {tuple(positions.shape)}")
+    freq, amplitude = position_frequencies(rotary_dim, theta=theta, scaling=scaling)
+    cos, sin = block_ops.position_tables(positions[None] if positions.ndim == 1 else positions, freq, amplitude)
+    return RotaryTables(cos=cos, sin=sin)
+
+
+def _half_layout(layout: str) -> bool:
+    if layout not in ("interleaved", "half"):
+        raise ValueError(f"layout must be 'interleaved' or 'half'; got {layout!r}")
+    return layout == "half"
+
+
+def rotate_heads(
+    x: torch.Tensor, tables: RotaryTables, *, layout: str = "interleaved", start: int = 0
+) -> torch.Tensor:
+    """:func:`apply_rotary` on part of each head and in either pair layout:
+    channels ``[start, start + 2 * tables.pairs)`` of ``x (batch, heads,
+    length, head_dim)`` are rotated, the others copied.
+
+    ``layout``: pair ``p`` is channels ``2p, 2p + 1`` of that range
+    (``"interleaved"``) or ``p, pairs + p`` (``"half"``).  bf16 or float32, any
+    head_dim; fp32 arithmetic rounded once to x's dtype; differentiable in
+    ``x``.  Returns a new tensor.
+
+    Raises:
+        ValueError: rank, length, channels or batch that do not fit the tables,
+            or an unknown layout.
+        TypeError: dtype other than bf16 or float32.
+    """
+    return block_ops.rotate(x, tables.cos, tables.sin, int(start), _half_layout(layout), False)
+
+
+def rotate_query_key(
+    query: torch.Tensor, key: torch.Tensor, tables: RotaryTables, *, layout: str = "interleaved", start: int = 0
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`rotate_heads` of a query and a key of the same tokens (any head
+    counts) in one launch, forward and backward."""
+    return block_ops.rotate_pair(query, key, tables.cos, tables.sin, int(start), _half_layout(layout), False)

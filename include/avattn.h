@@ -864,6 +864,80 @@ int avattn_rope_apply_pair_f32(int32_t batch, int32_t head_dim,
                                float* k_out, const int64_t* k_out_strides,
                                avattn_stream_t stream);
 
+/*
+ * Sequence rotation (no reference counterpart: the reference rotates whole
+ * heads in interleaved pairs by 3D coordinates, src/avgen/models/rope.py).
+ *
+ * avattn_position_tables: cos_out / sin_out[b, i, p] = amplitude * cos / sin
+ * of positions[b * positions_batch_stride + i] * frequencies[p], float32
+ * (batch, len, pairs) contiguous; the angle in double, rounded once.
+ * positions: int64 (positions_i64) or int32 on the device, batch stride 0 =
+ * shared.  frequencies: `pairs` (at most 256) doubles in host memory.
+ *
+ * avattn_rotate: rotates channels [start, start + 2 pairs) of every head of q
+ * and k (either may have 0 heads) by the token's table row and copies the
+ * others.  Pair p is channels start + 2p, + 1 (half_layout 0) or start + p,
+ * start + pairs + p (1).  bf16, or float32 with is_f32; any strides with
+ * contiguous head_dim, any head_dim of at least 2 pairs; outputs must not
+ * overlap the inputs.  fp32 products rounded separately.  inverse: the
+ * transposed rotation (the gradient).  table_batch_stride 0 = shared.
+ */
+int avattn_position_tables(const void* positions, int32_t positions_i64,
+                           int64_t positions_batch_stride,
+                           int32_t batch, int32_t len, int32_t pairs,
+                           const double* frequencies, double amplitude,
+                           float* cos_out, float* sin_out,
+                           avattn_stream_t stream);
+
+int avattn_rotate(const void* q, const int64_t* q_strides, int32_t heads_q,
+                  void* q_out, const int64_t* q_out_strides,
+                  const void* k, const int64_t* k_strides, int32_t heads_k,
+                  void* k_out, const int64_t* k_out_strides,
+                  int32_t batch, int32_t len, int32_t head_dim,
+                  int32_t pairs, int32_t start, int32_t half_layout,
+                  int32_t is_f32,
+                  const float* cos_tab, const float* sin_tab,
+                  int64_t table_batch_stride, int32_t inverse,
+                  avattn_stream_t stream);
+
+/*
+ * Residual addition and RMS norm over rows of `width` values (the block's
+ * `hidden + branch` and the norm that follows it, src/avgen/models/blocks.py
+ * :173-227 and layers.py:106-118, in one pass):
+ *   h = x + residual,  sum_out = h,
+ *   norm_out = h / sqrt(mean(h^2) + eps) * weight
+ * in fp32 (the norm from the unrounded sum), each output rounded once.  Rows
+ * bf16, or float32 with is_f32; weight in the rows' type or float32
+ * (weight_is_f32; always for float32 rows).  Input rows their row strides
+ * apart (elements), sum_out and norm_out contiguous and not overlapping the
+ * inputs.  With scale_out (float32, one per row) norm_out holds e4m3 codes of
+ * norm / scale, scale = max|norm| / 448 of the row (1 for a row of zeros, at
+ * least 2^-126).
+ *
+ * Backward: from the stored sum and the gradients of norm_out and sum_out
+ * (dsum may be NULL), dx (the gradient of x and of residual, contiguous, rows'
+ * type) and dweight (weight's type), summed in a fixed order.  workspace:
+ * avattn_add_rms_norm_bwd_workspace_size bytes, 16-byte aligned (none for 0
+ * rows: dweight is then zeros).
+ */
+int avattn_add_rms_norm(const void* x, int64_t x_row_stride,
+                        const void* residual, int64_t residual_row_stride,
+                        const void* weight, int32_t weight_is_f32,
+                        int64_t rows, int64_t width, int32_t is_f32,
+                        float eps, void* sum_out, void* norm_out,
+                        float* scale_out, avattn_stream_t stream);
+
+size_t avattn_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width);
+
+int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
+                            const void* dsum, int64_t dsum_row_stride,
+                            const void* sum, int64_t sum_row_stride,
+                            const void* weight, int32_t weight_is_f32,
+                            int64_t rows, int64_t width, int32_t is_f32,
+                            float eps, void* dx, void* dweight,
+                            void* workspace, size_t workspace_bytes,
+                            avattn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
