@@ -280,6 +280,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_ptr, c_i64p, c_i32, c_i32, c_ptr, c_ptr, c_i64, c_ptr, c_i64p,
          c_ptr],
     ),
+    "avattn_fwd_scored_workspace_size": (c_size, [c_i32] * 7),
+    "avattn_fwd_scored": (
+        ctypes.c_int,
+        [c_ptr, c_ptr, c_ptr, c_i64p, c_i64p, c_i64p,
+         c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+         c_ptr, c_i64, c_ptr, c_ptr, c_i64,
+         c_f32, c_f32, c_ptr, c_ptr, c_i32, ctypes.c_uint32,
+         c_ptr, c_i64p, c_ptr,
+         c_ptr, c_size, c_ptr],
+    ),
+    "avattn_bwd_scored": (
+        ctypes.c_int,
+        [c_ptr] * 6 + [c_i64p] * 5 +
+        [c_i32] * 7 +
+        [c_ptr, c_i64, c_ptr, c_ptr, c_i64,
+         c_ptr, c_i64, c_i64,
+         c_f32, c_f32, c_ptr, c_ptr, c_i32,
+         c_ptr, c_i64p, c_ptr, c_i64p, c_ptr, c_i64p,
+         c_ptr, c_size, c_ptr],
+    ),
     "avattn_position_tables": (
         ctypes.c_int,
         [c_ptr, c_i32, c_i64, c_i32, c_i32, c_i32, c_ptr, ctypes.c_double, c_ptr, c_ptr, c_ptr],
@@ -325,6 +345,9 @@ BWD_REUSE_QUERY_SIDE = 1
 BWD_DQ_ACCUMULATE_F32 = 2
 BWD_STAGE_DS = 4
 BWD_DEFER_DQ = 8
+
+# avattn_fwd_scored flags (include/avattn.h).
+SCORED_SORTED_WINDOWS = 1
 
 # avattn_ring_fwd_step flags (include/avattn.h).
 RING_FIRST = 1

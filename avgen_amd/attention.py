@@ -41,7 +41,7 @@ from typing import Optional
 import torch
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
-from . import ops
+from . import ops, scored_ops
 from .rope import RotaryTables
 
 __all__ = [
@@ -50,8 +50,10 @@ __all__ = [
     "attention_backends",
     "attention_fp8",
     "device_arch",
+    "document_windows",
     "key_padding_mask",
     "rotary_attention",
+    "scored_attention",
     "sdpa_context",
     "packed_windows",
     "TemporalNeighbourhood",
@@ -594,4 +596,105 @@ def varlen_attention(
     _validate(query, key, value, 0.0, False, enable_gqa)
     lo, hi = packed_windows(cu_seqlens, query.shape[-2], device=query.device)
     out, _ = ops.flash_fwd_windowed(query, key, value, lo, hi, None, ops.default_scale(query.shape[-1]), True)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Changed scores: capped by a tanh, biased by distance
+# ---------------------------------------------------------------------------
+
+
+def document_windows(
+    cu_seqlens: torch.Tensor,
+    length: int,
+    *,
+    causal: bool = False,
+    prefix_lengths: torch.Tensor | int = 0,
+    device=None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Key windows of packed documents (``cu_seqlens`` as for
+    :func:`packed_windows`; ``[0, length]`` for a single one): int32
+    ``(length,)`` ``(lo, hi)``, both non-decreasing.
+
+    Token ``i`` of document ``s`` attends to the document's keys; with
+    ``causal`` to those up to itself and to the document's first
+    ``prefix_lengths[s]`` (a tensor ``(documents,)`` or one number for all),
+    which see each other in both directions.  Rows past the last document get
+    the empty window."""
+    lo, end = packed_windows(cu_seqlens, length, device=device)
+    if not causal:
+        return lo, end
+    dev = lo.device
+    cu = cu_seqlens.to(device=dev, dtype=torch.int64)
+    i = torch.arange(length, device=dev)
+    seen = lo + 1
+    if cu.numel() > 1:
+        prefix = torch.as_tensor(prefix_lengths, device=dev, dtype=torch.int64)
+        if prefix.ndim > 1 or (prefix.ndim == 1 and prefix.shape[0] != cu.numel() - 1):
+            raise ValueError(f"prefix_lengths must be a number or ({cu.numel() - 1},); got {tuple(prefix.shape)}")
+        seg = torch.searchsorted(cu[1:].contiguous(), i, right=True).clamp(max=cu.numel() - 2)
+        seen = lo + prefix.clamp(min=0).expand(cu.numel() - 1)[seg]
+    hi = torch.minimum(torch.maximum(i + 1, seen), end.long())
+    return lo, torch.maximum(hi, lo.long()).to(torch.int32)
+
+
+def scored_attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    *,
+    softcap: float | None = None,
+    distance_slopes: torch.Tensor | None = None,
+    query_offset: int | torch.Tensor = 0,
+    window_lo: torch.Tensor | None = None,
+    window_hi: torch.Tensor | None = None,
+    attn_mask: torch.Tensor | None = None,
+    scale: float | None = None,
+    enable_gqa: bool = False,
+    monotone: bool = False,
+) -> torch.Tensor:
+    """:func:`windowed_attention` with changed scores, in training and in
+    serving (no reference counterpart).
+
+    With ``s_ij = scale * q_i . k_j`` (``scale`` default ``1/sqrt(head_dim)``)
+    the softmax runs over ``softcap * tanh(s_ij / softcap) - distance_slopes[h]
+    * |i + query_offset - j|``, without the steps whose argument is None, of
+    the keys in ``[window_lo[.., i], window_hi[.., i])`` that ``attn_mask``
+    admits.
+
+    Args:
+        query, key, value, attn_mask, enable_gqa: as for :func:`attention`.
+        softcap: positive (bf16: up to 1,024), or None.
+        distance_slopes: float32 ``(heads,)``, any sign, no gradient (at most
+            64 query heads per kv head).
+        query_offset: position of query 0 among the keys, an int or int32
+            ``(batch,)`` on the GPU (``length - queries`` for the newest tokens
+            of a cache).
+        window_lo, window_hi: key windows as for :func:`windowed_attention`, or
+            None for every key; :func:`document_windows` builds document,
+            causal and prefix masks, ``hi = length`` bounds a cache.
+        monotone: the caller guarantees windows non-decreasing in the row;
+            spares the backward's check (a host synchronisation) and a launch
+            of the forward.  Wrong windows then give wrong values.
+
+    A row without a key returns zeros.  A key that no row of its batch entry
+    may attend contributes nothing, whatever it holds: the unused slots of a
+    cache need no clearing.  bf16 or float32, head_dim 64 or 128;
+    differentiable in query, key and value (windows non-decreasing in the
+    row).  Up to 64 query rows per kv head run on kernels that split the keys
+    over the chip and read the cache once.
+    """
+    if query.shape[-2] == 0 or key.shape[-2] == 0:
+        return torch.zeros_like(query)
+    _validate(query, key, value, 0.0, False, enable_gqa)
+    if softcap is not None and not softcap > 0.0:
+        raise ValueError(f"softcap must be positive or None; got {softcap}")
+    if distance_slopes is not None and distance_slopes.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("distance_slopes have no gradient; pass them detached")
+    mask = _as_key_mask(attn_mask, query.shape[0], query.shape[-2], key.shape[-2])
+    offsets = query_offset if isinstance(query_offset, torch.Tensor) else None
+    out, _ = scored_ops.flash_fwd_scored(
+        query, key, value, window_lo, window_hi, mask, distance_slopes, offsets,
+        ops.default_scale(query.shape[-1]) if scale is None else float(scale),
+        0.0 if softcap is None else float(softcap), 0 if offsets is not None else int(query_offset), bool(monotone))
     return out

@@ -68,7 +68,45 @@ struct F32Args {
   float* part;
   int nsplit, nparts;
   int nblocks;  // dK/dV: 128-key blocks of this pass
+  // changed scores (mode 0: none) and the forward's key hull, as in FwdArgs
+  ScoreArgs score;
+  const int* hull;
 };
+
+// The keys some row of batch b may attend: what the others hold must not
+// count (changed scores).
+struct LiveKeys {
+  int lo, hi;
+  __device__ __forceinline__ void init(const F32Args& a, const int* hull, int b) {
+    key_hull(hull, a.wlo, a.whi, a.wsb, b, a.Lq, a.Lk, lo, hi);
+  }
+  __device__ __forceinline__ bool has(const F32Args& a, int b, int key) const {
+    return key >= lo && key < hi && (a.mask == nullptr || a.mask[b * a.msb + key] != 0);
+  }
+};
+
+// A changed score in log2 units from a raw one (uniform mode); kd: the row's
+// position minus the key; f = 1 - tanh^2 (1 without a cap).  tanh to a few
+// units in the last place, small arguments too: below 0.35 its odd series to
+// x^11 (the next term is below 2^-26), above it 1 - 2 r with r = 1 / (1 +
+// e^2|x|), and then 1 - tanh^2 = 4 r (1 - r).
+__device__ __forceinline__ float changed_score(const F32Args& a, float s, float kd, float slope2, float& f) {
+  float z = s * a.c;
+  f = 1.f;
+  if (a.score.mode & kScoreCap) {
+    const float x = s * a.score.cap_x, x2 = x * x, ax = fabsf(x);
+    const float series =
+        x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -8.8632355e-3f, 2.1869488e-2f), -5.3968254e-2f), 1.3333334e-1f),
+                          -3.3333334e-1f),
+                 1.f);
+    const float r = cap_complement(ax, 2.f * kLog2e);
+    const bool small = ax < 0.35f;
+    const float t = small ? series : copysignf(fmaf(-2.f, r, 1.f), x);
+    f = small ? fmaf(-t, t, 1.f) : 4.f * r * (1.f - r);
+    z = a.score.cap2 * t;
+  }
+  return fmaf(-slope2, fabsf(kd), z);
+}
 
 // The block a workgroup takes of a grid of `total` blocks whose last nsplit
 // are split, and which part of it (-1: all).
@@ -119,12 +157,13 @@ __device__ __forceinline__ bool rows_meet_block(const F32Args& a, int lo, int hi
 }
 
 // Writes a query row from its accumulators (o[dt] register i: channel 32*dt +
-// 8*(i/4) + 4*(l/32) + i%4), maximum m and sum l over all its keys.  l > 0:
+// 8*(i/4) + 4*(l/32) + i%4), maximum m (unit: its unit in natural log) and sum
+// l over all its keys.  l > 0:
 // normal row; l == 0: no valid key (out 0, lse -inf); NaN: a NaN or +inf
 // score reached the row.
 template <int D>
 __device__ __forceinline__ void write_row_f32(const F32Args& a, const f32x16 (&o)[D / 32], float m, float l, int bh,
-                                              int row) {
+                                              int row, float unit) {
   const int hh = (threadIdx.x >> 5) & 1;
   const float nan = __builtin_nanf("");
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan);
@@ -135,7 +174,7 @@ __device__ __forceinline__ void write_row_f32(const F32Args& a, const f32x16 (&o
     for (int g = 0; g < 4; ++g)
       st4(op + 32 * dt + 8 * g + 4 * hh,
           f32x4{o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv});
-  if (hh == 0) a.lse[(int64_t)bh * a.Lq + row] = l > 0.f ? fmaf(m, a.scale, logf(l)) : (l == 0.f ? kNegInf : nan);
+  if (hh == 0) a.lse[(int64_t)bh * a.Lq + row] = l > 0.f ? fmaf(m, unit, logf(l)) : (l == 0.f ? kNegInf : nan);
 }
 
 // ---------------------------------------------------------------------------
@@ -163,7 +202,8 @@ __device__ __forceinline__ void write_row_f32(const F32Args& a, const f32x16 (&o
 // its row's window.  SPLIT: the grid has split row blocks (F32Args::nsplit);
 // without them the same code ran 0.7-1% slower ((2,20,8192,128) 10.35 against
 // 10.44 ms, (1,16,6000,64) 1,213 against 1,233 us).
-template <int D, bool WIN, bool SPLIT>
+// SCORE: changed scores (F32Args::score), from then on in log2 units.
+template <int D, bool WIN, bool SPLIT, bool SCORE = false>
 __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
   constexpr int KT = 32, ROWS = 128, PITCH = D + 4, HD = D / 2, DT = D / 32;
   constexpr int PER = KT * D / 4 / 256;  // K float4 chunks per thread and tile
@@ -198,6 +238,19 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
   float m = kNegInf, l = 0.f;
   const float* kb = a.k + b * a.ksb + hk * a.ksh;
   const float* vb = a.v + b * a.vsb + hk * a.vsh;
+  const float c = SCORE ? 1.f : a.c;  // the scores' unit in log2
+  LiveKeys live{0, 0};
+  float slope2 = 0.f;
+  int qpos = 0;
+  if constexpr (SCORE) {
+    live.init(a, a.hull, b);
+    slope2 = a.score.slopes != nullptr ? a.score.slopes[h] * kLog2e : 0.f;
+    qpos = row + a.score.query_offset(b);
+  }
+  auto loads = [&](int key) {
+    if constexpr (SCORE) return live.has(a, b, key);
+    return key < a.Lk;
+  };
 
   // Tile staging: thread tid moves K float4 chunks u = tid + 256*i (key u /
   // (D/4), channels 4*(u % (D/4)) ..) and V slots u = tid + 256*i (key u/32,
@@ -209,16 +262,16 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = tid + 256 * i, j = u / (D / 4), c4 = 4 * (u % (D / 4)), key = k0 + j;
-      pk[i] = key < a.Lk ? ld4(kb + (int64_t)key * a.ksl + c4) : f32x4{0.f, 0.f, 0.f, 0.f};
+      pk[i] = loads(key) ? ld4(kb + (int64_t)key * a.ksl + c4) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (int i = 0; i < VPER; ++i) {
       const int u = tid + 256 * i, key = k0 + u / 32;
       const float* vp = vb + (int64_t)key * a.vsl + (u % 32);
 #pragma unroll
-      for (int t = 0; t < DT; ++t) pv[i][t] = key < a.Lk ? vp[32 * t] : 0.f;
+      for (int t = 0; t < DT; ++t) pv[i][t] = loads(key) ? vp[32 * t] : 0.f;
     }
-    if (tid < KT) pbias = key_ok(a, b, k0 + tid) ? 0.f : kNegInf;
+    if (tid < KT) pbias = (SCORE ? loads(k0 + tid) : key_ok(a, b, k0 + tid)) ? 0.f : kNegInf;
   };
   auto store = [&](int buf) {
 #pragma unroll
@@ -277,7 +330,13 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
       const f32x4 bb = ld4(&bias[buf][8 * g + 4 * hh]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[4 * g + r] += bb[r];
+        if constexpr (SCORE) {
+          float f;
+          const float z = changed_score(a, s[4 * g + r], (float)(qpos - (t * KT + 8 * g + 4 * hh + r)), slope2, f);
+          s[4 * g + r] = bb[r] < 0.f ? kNegInf : z;
+        } else {
+          s[4 * g + r] += bb[r];
+        }
         if constexpr (WIN) {
           const int key = t * KT + 8 * g + 4 * hh + r;
           if (key < wl || key >= wh) s[4 * g + r] = kNegInf;
@@ -287,9 +346,9 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
     }
     mt = halves_max(mt);  // the query's other 16 keys
     // (mt - m)*c is NaN when both are -inf (no key yet: nothing to raise)
-    if (__builtin_amdgcn_ballot_w64((mt - m) * a.c > 8.f)) {
+    if (__builtin_amdgcn_ballot_w64((mt - m) * c > 8.f)) {
       const float mn = fmaxf(m, mt);
-      const float alpha = (m == kNegInf || mn == kNegInf) ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+      const float alpha = (m == kNegInf || mn == kNegInf) ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -298,11 +357,11 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
       m = mn;
     }
     // No key yet: every score is -inf (p = 0) or NaN, which must reach the sum.
-    const float mc = m == kNegInf ? 0.f : m * a.c;
+    const float mc = m == kNegInf ? 0.f : m * c;
     f32x16 p;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -mc));
+      p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -mc));
       l += p[i];
     }
     // O^T += V^T P^T: k-step j takes key 8*(j/4) + 4*hh + j%4, this lane's
@@ -337,7 +396,7 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
     if (hh == 0) slot[32 * D + l32] = m, slot[32 * D + 32 + l32] = l;
     return;
   }
-  if (valid) write_row_f32<D>(a, o, m, l, bh, row);
+  if (valid) write_row_f32<D>(a, o, m, l, bh, row, SCORE ? kLn2 : a.scale);
 }
 
 // The split row blocks: one wave per 32 rows adds the parts in order, each
@@ -352,9 +411,10 @@ __global__ __launch_bounds__(64) void fwd_f32_combine_kernel(F32Args a) {
   const float* slot = a.part + ((int64_t)sb * a.nparts * 4 + wave) * SLOT;
   f32x16 o[DT];
   float m, l;
-  combine_parts<D>(slot, 4 * SLOT, a.nparts, a.c, o, m, l);
+  const bool log2_units = a.score.mode != 0;
+  combine_parts<D>(slot, 4 * SLOT, a.nparts, log2_units ? 1.f : a.c, o, m, l);
   const int row = bid % nqb * 128 + wave * 32 + l32;
-  if (row < a.Lq) write_row_f32<D>(a, o, m, l, bid / nqb, row);
+  if (row < a.Lq) write_row_f32<D>(a, o, m, l, bid / nqb, row, log2_units ? kLn2 : a.scale);
 }
 
 // Zeros to out and -inf to lse (no keys at all).
@@ -419,12 +479,17 @@ struct Tile32 {
   using vdt = float __attribute__((ext_vector_type(DT)));
   float x[SL][DT];
   __device__ __forceinline__ void fetch(const float* base, int64_t rs, int r0, int n, int tid) {
+    fetch_if(base, rs, r0, tid, [&](int row) { return row < n; });
+  }
+  // The rows that `in` takes; zeros for the others.
+  template <class In>
+  __device__ __forceinline__ void fetch_if(const float* base, int64_t rs, int r0, int tid, In&& in) {
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
       const int v = tid + NT * i, row = r0 + v / 32;
       const float* p = base + (int64_t)row * rs + (v % 32);
 #pragma unroll
-      for (int t = 0; t < DT; ++t) x[i][t] = row < n ? p[32 * t] : 0.f;
+      for (int t = 0; t < DT; ++t) x[i][t] = in(row) ? p[32 * t] : 0.f;
     }
   }
   __device__ __forceinline__ void store(float* tile, int tid) const {
@@ -454,7 +519,9 @@ struct Tile32 {
 // windows, non-decreasing in the row: the workgroup visits the query tiles
 // holding the rows whose windows meet its keys (a contiguous range, found
 // by binary search) and P is 0 outside each row's window.
-template <int D, bool STAGE, bool WIN>
+// SCORE: changed scores; the P wave hands over P (1 - tanh^2), which is what
+// the dS wave multiplies, and keeps P for dV.
+template <int D, bool STAGE, bool WIN, bool SCORE = false>
 __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
   constexpr int QT = 32, KPB = 128, PITCH = D + 4, HD = D / 2, DT = D / 32;
   using vdt = float __attribute__((ext_vector_type(DT)));
@@ -475,12 +542,19 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
   const int group = a.Hq / a.Hkv;
   const int k0 = kb * KPB + pair * 32;  // the pair's first key
   const int key = k0 + l32;
-  const bool kvalid = key_ok(a, b, key);
+  bool kvalid = key_ok(a, b, key);
+  int qoff = 0;
+  if constexpr (SCORE) {
+    LiveKeys live;
+    live.init(a, nullptr, b);
+    kvalid = live.has(a, b, key);
+    qoff = a.score.query_offset(b);
+  }
   float kv[HD];  // K (P wave) or V (dS wave) of the lane's key, k-step order
   load_row_ksteps<D>(kv,
                      role == 0 ? a.k + b * a.ksb + hk * a.ksh + (int64_t)key * a.ksl
                                : a.v + b * a.vsb + hk * a.vsh + (int64_t)key * a.vsl,
-                     key < a.Lk, hh);
+                     SCORE ? kvalid : key < a.Lk, hh);
   f32x16 acc[DT];  // dV (P wave) or dK (dS wave)
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
@@ -551,6 +625,7 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
     const int64_t rbase = ((int64_t)b * a.Hq + h) * a.Lq;
     const float* qb = a.q + b * a.qsb + h * a.qsh;
     const float* db = a.dout + b * a.dosb + h * a.dosh;
+    const float slope2 = SCORE && a.score.slopes != nullptr ? a.score.slopes[h] * kLog2e : 0.f;
     Tile32<D> sq, sd;
     float pl2 = kPosInf, pnd = 0.f;
     int pwl = 0, pwh = 0;
@@ -602,6 +677,7 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4 L = ld4(&l2s[t & 1][8 * g + 4 * hh]);
+          f32x4 hand;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             bool in = kvalid;
@@ -609,9 +685,17 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
               const int rr = 8 * g + 4 * hh + r;
               in = in && key >= wls[t & 1][rr] && key < whs[t & 1][rr];
             }
-            w[4 * g + r] = in ? __builtin_amdgcn_exp2f(fmaf(s[4 * g + r], a.c, -L[r])) : 0.f;
+            if constexpr (SCORE) {
+              float f;
+              const float kd = (float)(t * QT + 8 * g + 4 * hh + r + qoff - key);
+              const float z = changed_score(a, s[4 * g + r], kd, slope2, f);
+              w[4 * g + r] = in ? __builtin_amdgcn_exp2f(z - L[r]) : 0.f;
+              hand[r] = in ? w[4 * g + r] * f : 0.f;
+            } else {
+              w[4 * g + r] = in ? __builtin_amdgcn_exp2f(fmaf(s[4 * g + r], a.c, -L[r])) : 0.f;
+            }
           }
-          st4(pw + 256 * g, f32x4{w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]});
+          st4(pw + 256 * g, SCORE ? hand : f32x4{w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]});
         }
         second(w, dos[t & 1]);
       }
@@ -819,7 +903,8 @@ __global__ __launch_bounds__(512) void bwd_dq_f32_kernel(F32Args a) {
 // D/32 channel blocks of K's row 16*(l/32) + j.  WIN: the workgroup stages
 // the tiles meeting its rows' windows, and a wave multiplies only the key
 // blocks its rows meet (the blocks the windowed dK/dV kernel wrote).
-template <int D, bool WIN, int NW>
+// SCORE: keys that no row may attend are taken as zeros.
+template <int D, bool WIN, int NW, bool SCORE = false>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void bwd_dq_ds_f32_kernel(F32Args a) {
   constexpr int KT = 32, ROWS = 32 * NW, PITCH = D + 4, DT = D / 32;
   using vdt = float __attribute__((ext_vector_type(DT)));
@@ -854,8 +939,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void bwd_dq_ds_f32_kernel
   const float* kb = a.k + b * a.ksb + hk * a.ksh;
   Tile32<D, 64 * NW> sk;
   f32x4 pa[4];
+  LiveKeys live{0, 0};
+  if constexpr (SCORE) live.init(a, nullptr, b);
   auto fetch = [&](int t) {
-    sk.fetch(kb, a.ksl, t * KT, a.Lk, tid);
+    if constexpr (SCORE)
+      sk.fetch_if(kb, a.ksl, t * KT, tid, [&](int key) { return live.has(a, b, key); });
+    else
+      sk.fetch(kb, a.ksl, t * KT, a.Lk, tid);
     const bool take = takes(t);
 #pragma unroll
     for (int e = 0; e < 4; ++e) pa[e] = take ? ld4(dsr + (int64_t)t * 1024 + 4 * e) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1172,15 +1262,15 @@ FwdSplit fwd_f32_split_plan(int B, int Hq, int Lq, int Lk, int D) {
   return best;
 }
 
-template <int D, bool WIN>
+template <int D, bool WIN, bool SCORE = false>
 void launch_fwd_f32(const F32Args& a, hipStream_t s) {
   const int64_t blocks = (int64_t)((a.Lq + 127) / 128) * a.B * a.Hq;
   const dim3 grid((unsigned)(blocks - a.nsplit + (int64_t)a.nsplit * a.nparts));
   if (a.nsplit == 0) {
-    hipLaunchKernelGGL((fwd_f32_kernel<D, WIN, false>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((fwd_f32_kernel<D, WIN, false, SCORE>), grid, dim3(256), 0, s, a);
     return;
   }
-  hipLaunchKernelGGL((fwd_f32_kernel<D, WIN, true>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((fwd_f32_kernel<D, WIN, true, SCORE>), grid, dim3(256), 0, s, a);
   hipLaunchKernelGGL(fwd_f32_combine_kernel<D>, dim3(4 * a.nsplit), dim3(64), 0, s, a);
 }
 
@@ -1206,27 +1296,27 @@ FwdSplit dkv_f32_split_plan(int64_t blocks, int D) {
 // (1,20,4096) 1.25 rounds 3,714 against 3,570 us, (1,10,16384) 2.5 rounds
 // 26.94 against 26.51 ms; (1,28,4096) 1.75 rounds 4,754 against 4,914 us,
 // (2,20,8192) 5 rounds 26.08 against 26.69 ms.
-template <int D, bool WIN>
+template <int D, bool WIN, bool SCORE>
 void launch_dq_ds_f32(const F32Args& a, int heads, hipStream_t s) {
   constexpr int kCus = 256;
   constexpr float kRowCost = D == 64 ? 1.09f : 1.12f;
   const int64_t n8 = (int64_t)((a.Lq + 255) / 256) * heads, n4 = (int64_t)((a.Lq + 127) / 128) * heads;
   if (0.5f * kRowCost * ((n4 + kCus - 1) / kCus) < (n8 + kCus - 1) / kCus)
-    hipLaunchKernelGGL((bwd_dq_ds_f32_kernel<D, WIN, 4>), dim3((unsigned)n4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((bwd_dq_ds_f32_kernel<D, WIN, 4, SCORE>), dim3((unsigned)n4), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((bwd_dq_ds_f32_kernel<D, WIN, 8>), dim3((unsigned)n8), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((bwd_dq_ds_f32_kernel<D, WIN, 8, SCORE>), dim3((unsigned)n8), dim3(512), 0, s, a);
 }
 
 // pairs_per_pass 0: dQ recomputes S and dP; else dS is staged for that many
 // (batch, kv head) pairs at a time.  With a.part the (single) pass's dK/dV is
-// split.
-template <int D, bool WIN>
+// split.  SCORE: with staged dS only.
+template <int D, bool WIN, bool SCORE = false>
 void launch_bwd_f32(F32Args a, int pairs_per_pass, hipStream_t s) {
   const int64_t rows = (int64_t)a.B * a.Hq * a.Lq;
   hipLaunchKernelGGL(bwd_pre_f32_kernel<D>, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, a);
   const int nkb = (a.Lk + 127) / 128;
   const int pairs = a.B * a.Hkv;
-  if (pairs_per_pass == 0) {
+  if constexpr (!SCORE) if (pairs_per_pass == 0) {
     a.pair0 = 0;
     a.nblocks = nkb * pairs;
     hipLaunchKernelGGL((bwd_dkdv_f32_kernel<D, false, WIN>), dim3((unsigned)a.nblocks), dim3(512), 0, s, a);
@@ -1242,11 +1332,11 @@ void launch_bwd_f32(F32Args a, int pairs_per_pass, hipStream_t s) {
     const FwdSplit sp = a.part ? dkv_f32_split_plan(a.nblocks, D) : FwdSplit{0, 0, 0};
     a.nsplit = sp.nsplit, a.nparts = sp.nparts;
     const dim3 grid((unsigned)(a.nblocks - a.nsplit + a.nsplit * a.nparts));
-    hipLaunchKernelGGL((bwd_dkdv_f32_kernel<D, true, WIN>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((bwd_dkdv_f32_kernel<D, true, WIN, SCORE>), grid, dim3(512), 0, s, a);
     if (a.nsplit > 0)
       hipLaunchKernelGGL(dkv_f32_reduce_kernel<D>, dim3((unsigned)(a.nsplit * (2 * 128 * (D / 4) / 256))), dim3(256), 0,
                          s, a);
-    launch_dq_ds_f32<D, WIN>(a, np * group, s);
+    launch_dq_ds_f32<D, WIN, SCORE>(a, np * group, s);
   }
 }
 
@@ -1265,6 +1355,12 @@ int check_f32_windows(const int32_t* lo, const int32_t* hi, int64_t batch_stride
 
 using namespace avattn;
 
+namespace avattn {
+
+size_t fwd_f32_split_bytes(int B, int Hq, int Lq, int Lk, int D) { return fwd_f32_split_plan(B, Hq, Lq, Lk, D).bytes; }
+
+}  // namespace avattn
+
 extern "C" {
 
 static int fwd_f32_entry(const float* q, const float* k, const float* v, const int64_t* q_strides,
@@ -1272,7 +1368,8 @@ static int fwd_f32_entry(const float* q, const float* k, const float* v, const i
                          int32_t heads_kv, int32_t len_q, int32_t len_k, int32_t head_dim, const uint8_t* key_mask,
                          int64_t key_mask_batch_stride, const int32_t* window_lo, const int32_t* window_hi,
                          int64_t window_batch_stride, float scale, float* out, const int64_t* out_strides,
-                         float* lse, avattn_stream_t stream, void* workspace = nullptr, size_t workspace_bytes = 0) {
+                         float* lse, avattn_stream_t stream, void* workspace = nullptr, size_t workspace_bytes = 0,
+                         const ScoreArgs* score = nullptr, bool sorted_windows = false) {
   int st = check_f32_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
   st = check_f32_windows(window_lo, window_hi, window_batch_stride, len_q);
@@ -1307,7 +1404,20 @@ static int fwd_f32_entry(const float* q, const float* k, const float* v, const i
     a.part = static_cast<float*>(workspace);
     a.nsplit = sp.nsplit, a.nparts = sp.nparts;
   }
-  if (window_lo) {
+  if (score) {
+    a.score = *score;
+    if (window_lo && !sorted_windows) {
+      // The caller's workspace ends with room for the hull.
+      int* hull = reinterpret_cast<int*>(static_cast<char*>(workspace) + workspace_bytes - r256((size_t)batch * 8));
+      const hipError_t e = launch_window_hull(window_lo, window_hi, window_batch_stride, batch, len_q, len_k, hull, s);
+      if (e != hipSuccess) return AVATTN_ERR_LAUNCH;
+      a.hull = hull;
+    }
+    if (head_dim == 128)
+      window_lo ? launch_fwd_f32<128, true, true>(a, s) : launch_fwd_f32<128, false, true>(a, s);
+    else
+      window_lo ? launch_fwd_f32<64, true, true>(a, s) : launch_fwd_f32<64, false, true>(a, s);
+  } else if (window_lo) {
     if (head_dim == 128)
       launch_fwd_f32<128, true>(a, s);
     else
@@ -1389,7 +1499,7 @@ static int bwd_f32_entry(const float* dout, const float* q, const float* k, cons
                          const int32_t* window_lo, const int32_t* window_hi, int64_t window_batch_stride,
                          float scale, float* dq, const int64_t* dq_strides, float* dk, const int64_t* dk_strides,
                          float* dv, const int64_t* dv_strides, void* workspace, size_t workspace_bytes,
-                         avattn_stream_t stream) {
+                         avattn_stream_t stream, const ScoreArgs* score = nullptr) {
   int st = check_f32_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
   st = check_f32_windows(window_lo, window_hi, window_batch_stride, len_q);
@@ -1467,7 +1577,14 @@ static int bwd_f32_entry(const float* dout, const float* q, const float* k, cons
     }
   }
   a.wlo = window_lo, a.whi = window_hi, a.wsb = window_batch_stride;
-  if (window_lo) {
+  if (score) {
+    if (pp == 0) return AVATTN_ERR_WORKSPACE;
+    a.score = *score;
+    if (head_dim == 128)
+      window_lo ? launch_bwd_f32<128, true, true>(a, pp, s) : launch_bwd_f32<128, false, true>(a, pp, s);
+    else
+      window_lo ? launch_bwd_f32<64, true, true>(a, pp, s) : launch_bwd_f32<64, false, true>(a, pp, s);
+  } else if (window_lo) {
     if (head_dim == 128)
       launch_bwd_f32<128, true>(a, pp, s);
     else
@@ -1649,3 +1766,28 @@ int avattn_qk_norm_rope_bwd_f32(const float* x, const int64_t* x_strides, const 
 }
 
 }  // extern "C"
+
+namespace avattn {
+
+int fwd_scored_f32(const FewArgs& c, int head_dim, float scale, bool sorted_windows, void* workspace,
+                   size_t workspace_bytes, hipStream_t stream) {
+  const int64_t qs[3] = {c.qsb, c.qsh, c.qsl}, ks[3] = {c.ksb, c.ksh, c.ksl}, vs[3] = {c.vsb, c.vsh, c.vsl},
+                os[3] = {c.osb, c.osh, c.osl};
+  return fwd_f32_entry(static_cast<const float*>(c.q), static_cast<const float*>(c.k), static_cast<const float*>(c.v),
+                       qs, ks, vs, c.B, c.Hq, c.Hkv, c.Lq, c.Lk, head_dim, c.mask, c.msb, c.wlo, c.whi, c.wsb, scale,
+                       static_cast<float*>(c.o), os, c.lse, stream, workspace, workspace_bytes, &c.score,
+                       sorted_windows);
+}
+
+int bwd_scored_f32(const BwdArgs& c, int head_dim, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  const int64_t ds[3] = {c.dosb, c.dosh, c.dosl}, qs[3] = {c.qsb, c.qsh, c.qsl}, ks[3] = {c.ksb, c.ksh, c.ksl},
+                vs[3] = {c.vsb, c.vsh, c.vsl}, os[3] = {c.osb, c.osh, c.osl}, dqs[3] = {c.dqsb, c.dqsh, c.dqsl},
+                dks[3] = {c.dksb, c.dksh, c.dksl}, dvs[3] = {c.dvsb, c.dvsh, c.dvsl};
+  auto f = [](const bf16* p) { return reinterpret_cast<const float*>(p); };
+  auto w = [](bf16* p) { return reinterpret_cast<float*>(p); };
+  return bwd_f32_entry(f(c.dout), f(c.q), f(c.k), f(c.v), f(c.out), c.lse, ds, qs, ks, vs, os, c.B, c.Hq, c.Hkv, c.Lq,
+                       c.Lk, head_dim, c.mask, c.msb, c.wlo, c.whi, c.wsb, c.scale, w(c.dq), dqs, w(c.dk), dks,
+                       w(c.dv), dvs, workspace, workspace_bytes, stream, &c.score);
+}
+
+}  // namespace avattn

@@ -1,0 +1,399 @@
+// Attention forward of few query rows per kv head against many keys (one token
+// of every sequence, a handful of drafted ones), with or without changed
+// scores: the general forward's 128- or 256-row workgroups would idle, and its
+// operand copies read and write the whole cache first.
+//
+// HBM-bound: k and v are read once, in place, by as many workgroups as fill
+// the chip.  The rows of one kv head, Lq queries of its group of heads, form
+// blocks of up to 32; the keys that a block's windows reach are split over
+// `nsplit` workgroups, and a workgroup's 32-key tiles over its 4 waves.  A wave
+// stages its own tiles (direct global->LDS loads, one tile ahead, no barrier),
+// keeps its own running maximum, sum and output, and the waves are joined
+// through LDS at the end, the workgroups by few_combine_kernel.  The products
+// are those of the general forward (S^T = K Q^T, O^T += V^T P^T on 32x32x16
+// MFMAs, P in registers); with fewer than 32 rows the matrix pipe works on
+// empty columns, for which it has time: a tile's 16 KB take longer to arrive
+// than its MFMAs to run.
+#include "avattn_device.h"
+#include "avattn_kernels.h"
+
+namespace avattn {
+
+namespace {
+
+constexpr int kWaves = 4, kTile = 32;
+
+// The state of one row over some keys.
+struct RowPart {
+  float m, l;
+};
+
+__device__ __forceinline__ float part_weight(float m, float top) {
+  return m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// A row's last steps: 1 / sum and the lse (see row_state in attn_fwd_kernel.h).
+__device__ __forceinline__ void finish_row(float m, float l, float& inv, float& lse) {
+  const float nan = __builtin_nanf("");
+  inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan);
+  lse = l > 0.f ? fmaf(m, kLn2, logf(l)) : (l == 0.f ? kNegInf : nan);
+}
+
+// Where row r of a unit's block lives: query i of head h.
+struct RowPlace {
+  int i, h;
+};
+__device__ __forceinline__ RowPlace row_place(const FewArgs& a, int hk, int r) {
+  const int group = a.Hq / a.Hkv;
+  return {r / group, hk * group + r % group};
+}
+
+// Union of the windows of a block's rows (lane l: row l % 32) and what every
+// row's window covers.
+struct BlockWindows {
+  int lo, hi;          // this lane's row
+  int glo, ghi;        // union (glo == ghi: no key)
+  int all_lo, all_hi;  // intersection over the block's rows
+};
+__device__ __forceinline__ BlockWindows block_windows(const FewArgs& a, int b, int i, bool valid) {
+  BlockWindows w{0, a.Lk, 0, 0, 0, 0};
+  if (a.wlo != nullptr && valid) {
+    w.lo = min(max(a.wlo[b * a.wsb + i], 0), a.Lk);
+    w.hi = min(max(a.whi[b * a.wsb + i], w.lo), a.Lk);
+  }
+  const bool any = valid && w.lo < w.hi;
+  int lo = any ? w.lo : 0x7fffffff, hi = any ? w.hi : 0;
+  int al = valid ? w.lo : 0, ah = valid ? w.hi : 0x7fffffff;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    lo = min(lo, __shfl_xor(lo, off));
+    hi = max(hi, __shfl_xor(hi, off));
+    al = max(al, __shfl_xor(al, off));
+    ah = min(ah, __shfl_xor(ah, off));
+  }
+  w.glo = __builtin_amdgcn_readfirstlane(min(lo, hi));
+  w.ghi = __builtin_amdgcn_readfirstlane(hi);
+  w.all_lo = __builtin_amdgcn_readfirstlane(al);
+  w.all_hi = __builtin_amdgcn_readfirstlane(ah);
+  return w;
+}
+
+// Changes one raw score (uniform mode); kd: the row's position minus the key.
+__device__ __forceinline__ float changed_score(const FewArgs& a, float s, float kd, float slope2) {
+  float z;
+  if (a.score.mode & kScoreCap)
+    z = fmaf(-2.f * a.score.cap2, cap_complement(s, a.score.cap_arg), a.score.cap2);
+  else
+    z = s * a.scale_log2;
+  return fmaf(-slope2, fabsf(kd), z);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
+  constexpr int KS = D / 16, DT = D / 32, TE = kTile * D;
+  struct Stage {
+    bf16 k[TE];  // K rows: TileLayout<D>
+    bf16 v[TE];  // V rows: TileLayout<D>
+  };
+  constexpr int kRowPitch = D + 4;  // floats per row of a wave's output at the end
+  struct Join {
+    float o[kWaves][kTile * kRowPitch];
+    float m[kWaves][kTile], l[kWaves][kTile];
+  };
+  __shared__ __attribute__((aligned(16))) union Smem {
+    Stage st[kWaves][2];
+    Join join;
+  } sm;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int prow = perm23(l32);
+  const int unit = blockIdx.x / a.nsplit, split = blockIdx.x % a.nsplit;
+  const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
+  const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
+  const int rows = min(a.Lq * (a.Hq / a.Hkv) - rb * kTile, kTile);  // of this block
+  const bool valid = l32 < rows;
+  const RowPlace rp = row_place(a, hk, rb * kTile + (valid ? l32 : 0));
+  const BlockWindows w = block_windows(a, b, rp.i, valid);
+
+  // This lane's row of Q: channels 16*ks + 8*hh + [0, 8).
+  bf16x8 qf[KS];
+  {
+    const bf16* qp = static_cast<const bf16*>(a.q) + b * a.qsb + rp.h * a.qsh + (int64_t)rp.i * a.qsl + 8 * hh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      u32x4 x = {0u, 0u, 0u, 0u};
+      if (valid) x = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
+      qf[ks] = bits_to_bf16x8(x);
+    }
+  }
+  const int qpos = rp.i + a.score.query_offset(b);
+  const float slope2 = a.score.slopes != nullptr ? a.score.slopes[rp.h] * kLog2e : 0.f;
+
+  // Tiles of this wave: the block's tiles, a range per workgroup, every
+  // fourth of it per wave.
+  const int tile0 = w.glo / kTile, ntile = w.ghi > w.glo ? (w.ghi + kTile - 1) / kTile - tile0 : 0;
+  const int t0 = tile0 + (int)((int64_t)ntile * split / a.nsplit) + wave;
+  const int t1 = tile0 + (int)((int64_t)ntile * (split + 1) / a.nsplit);
+
+  const bf16* kp = static_cast<const bf16*>(a.k) + b * a.ksb + hk * a.ksh;
+  const bf16* vp = static_cast<const bf16*>(a.v) + b * a.vsb + hk * a.vsh;
+  TileStager<kTile, D, 1> kst, vst;
+  kst.init(a.ksl, 0, lane);
+  vst.init(a.vsl, 0, lane);
+  // Rows past the last key read as zeros (or again, for strides below D).
+  auto rsrc = [&](const bf16* base, int64_t sl, int t) {
+    const int last = min(a.Lk - 1 - t * kTile, kTile - 1);
+    return make_rsrc(base + (int64_t)t * kTile * sl, (uint32_t)((last * sl + D) * 2));
+  };
+  auto stage = [&](int t, Stage& sg) {
+    kst.stage(sg.k, rsrc(kp, a.ksl, t), 0u);
+    vst.stage(sg.v, rsrc(vp, a.vsl, t), 0u);
+  };
+  // Whether key l32 of tile t is one that a row of the block may attend.
+  auto key_live = [&](int t) {
+    const int key = t * kTile + l32;
+    bool ok = key >= w.glo && key < w.ghi;
+    if (a.mask != nullptr && ok) ok = a.mask[b * a.msb + key] != 0;
+    return (int)ok;
+  };
+
+  float m = kNegInf, l = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
+
+  retire_prologue_loads();
+  int live = 0;
+  if (t0 < t1) {
+    live = key_live(t0);
+    stage(t0, sm.st[wave][0]);
+  }
+  for (int t = t0, buf = 0; t < t1; t += kWaves, buf ^= 1) {
+    Stage& sg = sm.st[wave][buf];
+    // Everything in flight belongs to this tile: its rows and its key mask.
+    wait_vmem_n<0>();
+    const uint32_t keys = (uint32_t)__builtin_amdgcn_ballot_w64(opaque(live) != 0);
+    if (t + kWaves < t1) {
+      // The other stage's reads have returned before it is filled again.
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      live = key_live(t + kWaves);
+      stage(t + kWaves, sm.st[wave][buf ^ 1]);
+    }
+    if (keys != 0xffffffffu) {
+      // What a key outside the mask and every window holds must not reach the
+      // rows through 0 * NaN.
+#pragma unroll
+      for (int i = 0; i < TE / 8 / 64; ++i) {
+        const int c = i * 64 + lane, row = c / (D / 8);
+        if (!(keys >> row & 1)) *reinterpret_cast<u32x4*>(sg.v + TileLayout<D>::off(row, 8 * (c % (D / 8)))) = u32x4{};
+      }
+    }
+    // Register 8*k2 + e of lane l: key 16*k2 + 8*hh + e of the tile, row l32.
+    f32x16 s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma32(row_operand<D>(sg.k, prow, 16 * ks + 8 * hh), qf[ks], s);
+    const float kd = (float)(qpos - (t * kTile + 8 * hh));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = changed_score(a, s[r], kd - (float)(16 * (r >> 3) + (r & 7)), slope2);
+    if (keys != 0xffffffffu || t * kTile < w.all_lo || t * kTile + kTile > w.all_hi) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = 16 * (r >> 3) + 8 * hh + (r & 7), key = t * kTile + j;
+        if (!(keys >> j & 1) || key < w.lo || key >= w.hi) s[r] = kNegInf;
+      }
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = halves_max(mx);
+    // The reference maximum moves only for a score 2^8 above it (as in the
+    // general forward); both lanes of a row agree.
+    if (mx > m + 8.f || (m == kNegInf && mx > m)) {
+      const float alpha = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
+      m = mx;
+    }
+    const float mc = m == kNegInf ? 0.f : m;
+    bf16x8 pf[2];
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2) {
+      u32x4 u;
+#pragma unroll
+      for (int e2 = 0; e2 < 4; ++e2) {
+        const float p0 = __builtin_amdgcn_exp2f(s[8 * k2 + 2 * e2] - mc);
+        const float p1 = __builtin_amdgcn_exp2f(s[8 * k2 + 2 * e2 + 1] - mc);
+        l += p0 + p1;
+        u[e2] = pack_bf16x2(p0, p1);  // the PV operand, rounded as in the general forward
+      }
+      pf[k2] = bits_to_bf16x8(u);
+    }
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const bf16x4 lo = lds_read_tr16(sg.v + tr_read_off<D>(lane, dt, 0) + 16 * k2 * D);
+        const bf16x4 hi = lds_read_tr16(sg.v + tr_read_off<D>(lane, dt, 1) + 16 * k2 * D);
+        acc[dt] = mfma32(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[k2], acc[dt]);
+      }
+  }
+
+  // Join the waves: each leaves its rows' maxima, sums and outputs.
+  l = halves_sum(l);
+  __syncthreads();  // every wave is done with its stages
+  Join& jn = sm.join;
+  if (hh == 0) jn.m[wave][l32] = m, jn.l[wave][l32] = l;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(&jn.o[wave][l32 * kRowPitch + 32 * dt + 8 * g + 4 * hh]) =
+          f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+  __syncthreads();
+  constexpr int CPR = D / 8;  // threads per row, 8 channels each
+  for (int u = tid; u < rows * CPR; u += 256) {
+    const int r = u / CPR, ch = 8 * (u % CPR);
+    float top = kNegInf;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) top = fmaxf(top, jn.m[v][r]);
+    float sum = 0.f, o[8] = {};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float wt = part_weight(jn.m[v][r], top);
+      sum = fmaf(jn.l[v][r], wt, sum);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(jn.o[v][r * kRowPitch + ch + e], wt, o[e]);
+    }
+    if (a.nsplit > 1) {
+      float* part = a.part + ((int64_t)unit * a.nsplit + split) * few_slot_floats(a.block_rows, D);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(part + r * D + ch + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+      if (ch == 0) part[a.block_rows * D + 2 * r] = top, part[a.block_rows * D + 2 * r + 1] = sum;
+    } else {
+      float inv, lse;
+      finish_row(top, sum, inv, lse);
+      const RowPlace p = row_place(a, hk, rb * kTile + r);
+      *reinterpret_cast<u32x4*>(static_cast<bf16*>(a.o) + b * a.osb + p.h * a.osh + (int64_t)p.i * a.osl + ch) =
+          u32x4{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv)};
+      if (ch == 0) a.lse[((int64_t)b * a.Hq + p.h) * a.Lq + p.i] = lse;
+    }
+  }
+}
+
+// The parts of one row, in order: a workgroup of 256 threads takes one row;
+// D / 4 threads of four channels each per part, the parts dealt out over the
+// thread groups, joined through LDS in a fixed order.
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
+  constexpr int TP = D / 4, G = 256 / TP;
+  __shared__ float so[G][D], sl[G], st[4];
+  const int unit = blockIdx.x / a.block_rows, r = blockIdx.x % a.block_rows;
+  const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
+  const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
+  if (rb * a.block_rows + r >= a.Lq * (a.Hq / a.Hkv)) return;  // the whole workgroup
+  const int64_t slot = few_slot_floats(a.block_rows, D);
+  const float* part = a.part + (int64_t)unit * a.nsplit * slot;
+  const float* ml = part + (int64_t)a.block_rows * D + 2 * r;
+  float top = kNegInf;
+  for (int p = threadIdx.x; p < a.nsplit; p += 256) top = fmaxf(top, ml[p * slot]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  if ((threadIdx.x & 63) == 0) st[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
+  const int g = threadIdx.x / TP, ch = 4 * (threadIdx.x % TP);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int p = g; p < a.nsplit; p += G) {
+    const float wt = part_weight(ml[p * slot], top);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part + p * slot + (int64_t)r * D + ch);
+    sum = fmaf(ml[p * slot + 1], wt, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], wt, o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) so[g][ch + e] = o[e];
+  if (ch == 0) sl[g] = sum;
+  __syncthreads();
+  if (g > 0) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    sum += sl[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += so[i][ch + e];
+  }
+  float inv, lse;
+  finish_row(top, sum, inv, lse);
+  const RowPlace rp = row_place(a, hk, rb * a.block_rows + r);
+  const int64_t at = b * a.osb + rp.h * a.osh + (int64_t)rp.i * a.osl + ch;
+  if constexpr (F32)
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + at) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  else
+    *reinterpret_cast<u32x2*>(static_cast<bf16*>(a.o) + at) =
+        u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+  if (ch == 0) a.lse[((int64_t)b * a.Hq + rp.h) * a.Lq + rp.i] = lse;
+}
+
+}  // namespace
+
+FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D) {
+  FewPlan p{};
+  const int64_t rows = (int64_t)Lq * (Hq / Hkv);
+  if (rows > kFewRows || Lk < 1) return p;
+  p.block_rows = (int)(rows < kTile ? rows : kTile);
+  p.row_blocks = (int)((rows + kTile - 1) / kTile);
+  const int64_t units = (int64_t)B * Hkv * p.row_blocks;
+  // Workgroups the chip holds at once: one per CU at D 128 (LDS), two at 64.
+  const int64_t slots = D == 128 ? 256 : 512;
+  // The fewest parts per unit whose rounds are shortest, each part with a tile
+  // for every wave.
+  const int most = (Lk + kWaves * kTile - 1) / (kWaves * kTile);
+  double best = 1e30;
+  for (int n = 1; n <= most && n <= 256; ++n) {
+    const double rounds = (double)((units * n + slots - 1) / slots) / n;
+    if (rounds < best * 0.95) {
+      best = rounds;
+      p.nsplit = n;
+    }
+    if (units * n >= slots) break;
+  }
+  if (units * p.nsplit > 2147483647 || units * p.block_rows > 2147483647) return FewPlan{};
+  p.bytes = p.nsplit > 1 ? (size_t)units * p.nsplit * few_slot_floats(p.block_rows, D) * sizeof(float) : 0;
+  return p;
+}
+
+hipError_t launch_few(const FewArgs& args, int D, bool f32, hipStream_t stream) {
+  FewArgs a = args;
+  const FewPlan p = few_plan(a.B, a.Hq, a.Hkv, a.Lq, a.Lk, D);
+  a.nsplit = p.nsplit;
+  a.row_blocks = p.row_blocks;
+  a.block_rows = p.block_rows;
+  const unsigned units = (unsigned)(a.B * a.Hkv * p.row_blocks);
+  {
+    LaunchTimer timer(kKidFwdFew, stream);
+    const dim3 grid(units * p.nsplit);
+    if (D == 128)
+      hipLaunchKernelGGL(attn_few_kernel<128>, grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL(attn_few_kernel<64>, grid, dim3(256), 0, stream, a);
+  }
+  if (p.nsplit > 1) {
+    LaunchTimer timer(kKidMerge, stream);
+    const dim3 grid(units * p.block_rows);
+    if (D == 128)
+      hipLaunchKernelGGL((few_combine_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((few_combine_kernel<64, false>), grid, dim3(256), 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace avattn

@@ -228,7 +228,7 @@ int fwd_impl(const void* q, const void* k, const void* v, const int64_t* q_strid
              const float* q_scale, const float* k_scale, float scale, void* out, const int64_t* out_strides,
              float* lse, void* workspace, size_t workspace_bytes, avattn_stream_t stream,
              const int32_t* window_lo = nullptr, const int32_t* window_hi = nullptr, int64_t window_batch_stride = 0,
-             const RingOpts* ring = nullptr) {
+             const RingOpts* ring = nullptr, const ScoreArgs* score = nullptr, bool sorted_windows = false) {
   int st = check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
   if (!q_strides || !k_strides || !v_strides || !out_strides) return AVATTN_ERR_NULL_POINTER;
@@ -299,6 +299,16 @@ int fwd_impl(const void* q, const void* k, const void* v, const int64_t* q_strid
     a.lse_acc = ring->lse_acc;
     a.acc_first = ring->first;
     a.acc_final = ring->last;
+  }
+  if (score) {
+    a.score = *score;
+    if (window_lo && !sorted_windows) {
+      // avattn_fwd_scored_workspace_size's room behind everything else.
+      a.hull = reinterpret_cast<int*>(ws + wl.total + split);
+      const hipError_t e =
+          launch_window_hull(window_lo, window_hi, window_batch_stride, batch, len_q, len_k, a.hull, s);
+      if (e != hipSuccess) return launch_status(e);
+    }
   }
   return launch_status(launch_fwd(a, head_dim, s));
 }
@@ -454,7 +464,7 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
                     const int64_t* dk_strides, void* dv, const int64_t* dv_strides, void* workspace,
                     size_t workspace_bytes, uint32_t flags, avattn_stream_t stream, const int32_t* window_lo,
                     const int32_t* window_hi, int64_t window_batch_stride, const RingOpts* ring = nullptr,
-                    const CompactDs* compact = nullptr) {
+                    const CompactDs* compact = nullptr, const ScoreArgs* score = nullptr) {
   int st = check_bwd_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (flags & ~(AVATTN_BWD_REUSE_QUERY_SIDE | AVATTN_BWD_DQ_ACCUMULATE_F32 | AVATTN_BWD_STAGE_DS |
                 AVATTN_BWD_DEFER_DQ))
@@ -593,6 +603,7 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
     if (kv_per_pass == a.nkv && !window_lo && split > 0 && workspace_bytes >= end + split)
       a.split_all = reinterpret_cast<float*>(ws + end);
   }
+  if (score) a.score = *score;
   return launch_status(launch_bwd(a, head_dim, kv_per_pass, s));
 }
 
@@ -1088,6 +1099,172 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, const v
   a.part = static_cast<float*>(workspace);
   return launch_status(
       launch_add_norm_bwd(a, is_f32 != 0, dweight, weight_is_f32 != 0, reinterpret_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Attention with changed scores
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// The lanes of a dK/dV wave hold one slope each.
+constexpr int kMaxSlopeGroup = 64;
+constexpr int32_t kMaxOffset = 1 << 30;
+
+// The bf16 kernels form cap tanh(s / cap) as cap - 2 cap r: off by about cap *
+// 2^-22, which up to this cap stays well below their rounding of P.
+constexpr float kMaxCapBf16 = 1024.f;
+
+int score_args(float scale, float softcap, const float* slopes, const int32_t* offsets, int32_t offset, int32_t Hq,
+               int32_t Hkv, bool f32, ScoreArgs& a) {
+  if (!(softcap >= 0.f) || !isfinite(softcap) || (!f32 && softcap > kMaxCapBf16) || offset > kMaxOffset || offset < -kMaxOffset)
+    return AVATTN_ERR_ARGUMENT;
+  if (!aligned_to(slopes, 4) || !aligned_to(offsets, 4)) return AVATTN_ERR_LAYOUT;
+  if (slopes && Hkv > 0 && Hq / Hkv > kMaxSlopeGroup) return AVATTN_ERR_TOO_LARGE;
+  a = ScoreArgs{};
+  if (softcap > 0.f) {
+    a.mode |= kScoreCap;
+    a.cap2 = softcap * kLog2e;
+    a.cap_x = scale / softcap;
+    a.cap_arg = 2.f * kLog2e * a.cap_x;
+    if (!isfinite(a.cap2) || !isfinite(a.cap_arg) || a.cap_arg == 0.f) return AVATTN_ERR_ARGUMENT;
+  }
+  // Without either the distance variants run with slope 0.
+  if (slopes || a.mode == 0) a.mode |= kScoreDistance;
+  a.slopes = slopes;
+  a.offsets = offsets;
+  a.offset = offset;
+  return AVATTN_OK;
+}
+
+bool takes_few(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool f32) {
+  return !f32 && few_plan(B, Hq, Hkv, Lq, Lk, D).nsplit > 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len_q,
+                                        int32_t len_k, int32_t head_dim, int32_t is_f32) {
+  if (check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim) != AVATTN_OK) return 0;
+  if ((int64_t)batch * heads_q * len_q == 0 || len_k == 0) return 0;
+  if (takes_few(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0))
+    return few_plan(batch, heads_q, heads_kv, len_q, len_k, head_dim).bytes;
+  const size_t hull = round256((size_t)batch * 2 * sizeof(int));
+  if (is_f32) return round256(fwd_f32_split_bytes(batch, heads_q, len_q, len_k, head_dim)) + hull;
+  return avattn_fwd_split_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, 0) + hull;
+}
+
+int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t* q_strides, const int64_t* k_strides,
+                      const int64_t* v_strides, int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len_q,
+                      int32_t len_k, int32_t head_dim, int32_t is_f32, const uint8_t* key_mask,
+                      int64_t key_mask_batch_stride, const int32_t* window_lo, const int32_t* window_hi,
+                      int64_t window_batch_stride, float scale, float softcap, const float* slopes,
+                      const int32_t* query_offsets, int32_t query_offset, uint32_t flags, void* out,
+                      const int64_t* out_strides, float* lse, void* workspace, size_t workspace_bytes,
+                      avattn_stream_t stream) {
+  int st = check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
+  if (st != AVATTN_OK) return st;
+  if (flags & ~AVATTN_SCORED_SORTED_WINDOWS) return AVATTN_ERR_ARGUMENT;
+  if (!q_strides || !k_strides || !v_strides || !out_strides) return AVATTN_ERR_NULL_POINTER;
+  if (!(scale > 0.f) || !isfinite(scale)) return AVATTN_ERR_ARGUMENT;
+  FewArgs c{};
+  st = score_args(scale, softcap, slopes, query_offsets, query_offset, heads_q, heads_kv, is_f32 != 0,
+                  c.score);
+  if (st != AVATTN_OK) return st;
+  if ((int64_t)batch * heads_q * len_q == 0) return AVATTN_OK;
+  if (len_k > 0) {
+    if (key_mask && key_mask_batch_stride != 0 && key_mask_batch_stride < len_k) return AVATTN_ERR_ARGUMENT;
+    st = check_windows(window_lo, window_hi, window_batch_stride, len_q, false);
+    if (st != AVATTN_OK) return st;
+    const size_t need = avattn_fwd_scored_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return AVATTN_ERR_WORKSPACE;
+    workspace_bytes = need;
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool sorted = (flags & AVATTN_SCORED_SORTED_WINDOWS) != 0;
+  const bool few = len_k > 0 && takes_few(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0);
+  if (!is_f32 && !few)
+    return fwd_impl(q, k, v, q_strides, k_strides, v_strides, batch, heads_q, heads_kv, len_q, len_k, head_dim,
+                    key_mask, key_mask_batch_stride, nullptr, nullptr, 0, false, nullptr, nullptr, scale, out,
+                    out_strides, lse, workspace, workspace_bytes, stream, window_lo, window_hi, window_batch_stride,
+                    nullptr, &c.score, sorted);
+  c.q = q, c.k = k, c.v = v, c.o = out;
+  c.qsb = q_strides[0], c.qsh = q_strides[1], c.qsl = q_strides[2];
+  c.ksb = k_strides[0], c.ksh = k_strides[1], c.ksl = k_strides[2];
+  c.vsb = v_strides[0], c.vsh = v_strides[1], c.vsl = v_strides[2];
+  c.osb = out_strides[0], c.osh = out_strides[1], c.osl = out_strides[2];
+  c.B = batch, c.Hq = heads_q, c.Hkv = heads_kv, c.Lq = len_q, c.Lk = len_k;
+  c.mask = key_mask, c.msb = key_mask_batch_stride;
+  c.wlo = window_lo, c.whi = window_hi, c.wsb = window_batch_stride;
+  c.scale_log2 = scale * kLog2e;
+  c.lse = lse;
+  if (!few) return fwd_scored_f32(c, head_dim, scale, sorted, workspace, workspace_bytes, s);
+  if (!q || !k || !v || !out || !lse) return AVATTN_ERR_NULL_POINTER;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return AVATTN_ERR_LAYOUT;
+  for (const int64_t* p : {q_strides, k_strides, v_strides, out_strides})
+    if (!(is_f32 ? strides_ok_f32(p) : strides_ok(p))) return AVATTN_ERR_LAYOUT;
+  // A 32-row tile of k or v lies within one 32-bit buffer range.
+  for (int64_t sl : {c.ksl, c.vsl})
+    if (sl < 0 || sl >= ((int64_t)1 << 23)) return AVATTN_ERR_LAYOUT;
+  c.part = static_cast<float*>(workspace);
+  return launch_status(launch_few(c, head_dim, is_f32 != 0, s));
+}
+
+int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                      const int64_t* dout_strides, const int64_t* q_strides, const int64_t* k_strides,
+                      const int64_t* v_strides, const int64_t* out_strides, int32_t batch, int32_t heads_q,
+                      int32_t heads_kv, int32_t len_q, int32_t len_k, int32_t head_dim, int32_t is_f32,
+                      const uint8_t* key_mask, int64_t key_mask_batch_stride, const int32_t* window_lo,
+                      const int32_t* window_hi, int64_t window_batch_stride, const int32_t* ds_table,
+                      int64_t ds_table_batch_stride, int64_t ds_units_per_head, float scale, float softcap,
+                      const float* slopes, const int32_t* query_offsets, int32_t query_offset, void* dq,
+                      const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                      const int64_t* dv_strides, void* workspace, size_t workspace_bytes, avattn_stream_t stream) {
+  ScoreArgs score;
+  if (!(scale > 0.f) || !isfinite(scale)) return AVATTN_ERR_ARGUMENT;
+  const int st = score_args(scale, softcap, slopes, query_offsets, query_offset, heads_q, heads_kv,
+                            is_f32 != 0, score);
+  if (st != AVATTN_OK) return st;
+  if (!is_f32) {
+    CompactDs c;
+    c.table = ds_table;
+    c.table_batch_stride = ds_table_batch_stride;
+    c.units_per_head = ds_units_per_head;
+    return bwd_impl(dout, q, k, v, out, lse, dout_strides, q_strides, k_strides, v_strides, out_strides, batch,
+                    heads_q, heads_kv, len_q, len_k, head_dim, key_mask, key_mask_batch_stride, scale, dq, dq_strides,
+                    dk, dk_strides, dv, dv_strides, workspace, workspace_bytes, AVATTN_BWD_STAGE_DS, stream, window_lo,
+                    window_hi, window_batch_stride, nullptr, ds_table ? &c : nullptr, &score);
+  }
+  if (ds_table) return AVATTN_ERR_ARGUMENT;
+  if (!dout_strides || !q_strides || !k_strides || !v_strides || !out_strides || !dq_strides || !dk_strides ||
+      !dv_strides)
+    return AVATTN_ERR_NULL_POINTER;
+  BwdArgs a{};
+  a.dout = static_cast<const bf16*>(dout);
+  a.q = static_cast<const bf16*>(q);
+  a.k = static_cast<const bf16*>(k);
+  a.v = static_cast<const bf16*>(v);
+  a.out = static_cast<const bf16*>(out);
+  a.lse = lse;
+  a.dosb = dout_strides[0], a.dosh = dout_strides[1], a.dosl = dout_strides[2];
+  a.qsb = q_strides[0], a.qsh = q_strides[1], a.qsl = q_strides[2];
+  a.ksb = k_strides[0], a.ksh = k_strides[1], a.ksl = k_strides[2];
+  a.vsb = v_strides[0], a.vsh = v_strides[1], a.vsl = v_strides[2];
+  a.osb = out_strides[0], a.osh = out_strides[1], a.osl = out_strides[2];
+  a.B = batch, a.Hq = heads_q, a.Hkv = heads_kv, a.Lq = len_q, a.Lk = len_k;
+  a.mask = key_mask, a.msb = key_mask_batch_stride;
+  a.wlo = window_lo, a.whi = window_hi, a.wsb = window_batch_stride;
+  a.scale = scale;
+  a.dq = static_cast<bf16*>(dq), a.dk = static_cast<bf16*>(dk), a.dv = static_cast<bf16*>(dv);
+  a.dqsb = dq_strides[0], a.dqsh = dq_strides[1], a.dqsl = dq_strides[2];
+  a.dksb = dk_strides[0], a.dksh = dk_strides[1], a.dksl = dk_strides[2];
+  a.dvsb = dv_strides[0], a.dvsh = dv_strides[1], a.dvsl = dv_strides[2];
+  a.score = score;
+  return bwd_scored_f32(a, head_dim, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -12,6 +12,42 @@ namespace avattn {
 // Mark in the sign bit of a kmax2 entry (see FwdArgs).
 constexpr uint32_t kTileSkip = 0x80000000u;
 
+// Scores changed before the softmax: z = cap tanh(s / cap) (kScoreCap), then
+// z - slopes[hq] * |position of the query - key| (kScoreDistance), s = scale
+// q.k; query i of batch b at position i + query_offset(b).  cap2 = cap *
+// log2(e); cap_x = scale / cap; cap_arg = 2 log2(e) cap_x, so that
+// exp2(cap_arg * q.k) is e^(2 s / cap).  slopes null: none (0).
+constexpr int kScoreCap = 1, kScoreDistance = 2;
+struct ScoreArgs {
+  int mode;
+  float cap2, cap_arg, cap_x;
+  const float* slopes;
+  const int* offsets;  // per batch (null: offset)
+  int offset;
+  __device__ __forceinline__ int query_offset(int b) const { return offsets ? offsets[b] : offset; }
+};
+
+// 1 / (1 + exp2(arg s)) = (1 - tanh(s / cap)) / 2, in [0, 1].
+__device__ __forceinline__ float cap_complement(float s, float arg) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * arg));
+}
+
+// The keys [lo, hi) of batch b outside which no query row's window reaches:
+// from `hull` (two ints per batch) where given, else the first row's lo and
+// the last row's hi (windows non-decreasing in the row), clamped into
+// 0 <= lo <= hi <= Lk; every key without windows.
+__device__ __forceinline__ void key_hull(const int* hull, const int* wlo, const int* whi, int64_t wsb, int b, int Lq,
+                                         int Lk, int& lo, int& hi) {
+  lo = 0, hi = Lk;
+  if (hull != nullptr) {
+    lo = hull[2 * b], hi = hull[2 * b + 1];
+  } else if (wlo != nullptr) {
+    lo = wlo[b * wsb], hi = whi[b * wsb + Lq - 1];
+  }
+  lo = min(max(lo, 0), Lk);
+  hi = min(max(hi, lo), Lk);
+}
+
 struct FwdArgs {
   const bf16* q;
   const bf16* k;
@@ -80,6 +116,11 @@ struct FwdArgs {
   // writes the rows.
   float* part;
   int nsplit, nparts;
+  // Changed scores (mode 0: none).  With them a key that no row may attend
+  // (masked, or outside every window of its batch row) is copied as zeros in
+  // k and v, so that what it holds never reaches a row; hull as in key_hull.
+  ScoreArgs score;
+  int* hull;
 };
 
 // Floats of one part of `rows` rows: the accumulators, then per 32 rows their
@@ -208,6 +249,8 @@ struct BwdArgs {
   // Slots for a split of every block (null: none; see dkv_split_plan), in
   // place of split_part.
   float* split_all;
+  // Changed scores as in FwdArgs (mode 0: none; staged dS only).
+  ScoreArgs score;
 };
 
 // Partial-sum slots of the dK/dV tail split, 256 x D floats each; the
@@ -325,6 +368,13 @@ hipError_t launch_quantize_rows(const bf16* x, int64_t sb, int64_t sh, int64_t s
 
 // Forward; the fp8 q k^T variant when a.k8 is set (a.q_scale, a.k_scale too).
 hipError_t launch_fwd(const FwdArgs& a, int head_dim, hipStream_t stream);
+// The changed-score kernels (attn_scored_fwd.hip, attn_scored_bwd.hip) of launch_fwd (its grid, in the
+// 128-row workgroups or not) and of launch_bwd's dK/dV step.
+void launch_fwd_scored(const FwdArgs& a, int head_dim, bool small, dim3 grid, hipStream_t stream);
+void launch_dkdv_scored(const BwdArgs& a, int head_dim, dim3 grid, hipStream_t stream);
+// hull[2 b], hull[2 b + 1] of key_hull, over windows in any order.
+hipError_t launch_window_hull(const int* wlo, const int* whi, int64_t wsb, int B, int Lq, int Lk, int* hull,
+                              hipStream_t stream);
 hipError_t launch_empty(bf16* o, int64_t osb, int64_t osh, int64_t osl, int B, int H, int L, int D, float* lse,
                         hipStream_t stream);
 // Backward.  With a.ds set, the (b, kv head) pairs go in passes of
@@ -358,6 +408,48 @@ hipError_t launch_qk_norm(const QkNormArgs& a, int head_dim, hipStream_t stream)
 hipError_t launch_qk_norm_bwd(const QkNormArgs& a, int head_dim, float* dw, hipStream_t stream);
 // dw[0 .. head_dim) = 0 (the gain gradient of an empty input).
 hipError_t launch_qk_norm_dw_zero(float* dw, int head_dim, hipStream_t stream);
+
+// Forward of few query rows (attn_few.hip): at most kFewRows per kv head.
+constexpr int kFewRows = 64;
+struct FewArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  int64_t qsb, qsh, qsl;
+  int64_t ksb, ksh, ksl;
+  int64_t vsb, vsh, vsl;
+  int64_t osb, osh, osl;
+  int B, Hq, Hkv, Lq, Lk;
+  const uint8_t* mask;
+  int64_t msb;
+  const int* wlo;
+  const int* whi;
+  int64_t wsb;
+  float scale_log2;
+  ScoreArgs score;
+  float* lse;
+  // Set by launch_few from few_plan: workgroups per (batch, kv head, block of
+  // rows), blocks per kv head, rows of a block; part: few_slot_floats per
+  // workgroup (nsplit > 1), outputs by row, then (maximum, sum) by row.
+  int nsplit, row_blocks, block_rows;
+  float* part;
+};
+constexpr int few_slot_floats(int rows, int D) { return rows * D + (2 * rows + 3) / 4 * 4; }
+// nsplit 0: more rows than this path takes.
+struct FewPlan {
+  int nsplit, row_blocks, block_rows;
+  size_t bytes;
+};
+FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim);
+hipError_t launch_few(const FewArgs& a, int head_dim, bool f32, hipStream_t stream);
+// The float32 kernels with changed scores (attn_f32.hip): what their C entry
+// points check, with a status code.  The forward's workspace: split parts, then
+// the hull; the backward's tensors are float behind BwdArgs' pointers.
+size_t fwd_f32_split_bytes(int B, int Hq, int Lq, int Lk, int head_dim);
+int fwd_scored_f32(const FewArgs& c, int head_dim, float scale, bool sorted_windows, void* workspace,
+                   size_t workspace_bytes, hipStream_t stream);
+int bwd_scored_f32(const BwdArgs& c, int head_dim, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 // Tables of integer positions (seq_rope.hip): position of token (b, i) at
 // b*psb + i, pair p's frequency freq[p]; cos and sin, times amplitude, to

@@ -25,6 +25,7 @@ namespace avattn {
 // produces), to `xr` (row-major, D apart) and / or `xt` (head_dim-major, Lp
 // apart; both already at the tile).  Returns the thread's share of the
 // largest squared row norm (NORM) and of "every value is finite" (FINITE).
+// Rows whose bit of `keep` is clear are copied as zeros without being read.
 struct TileScan {
   float nmax;
   bool finite;
@@ -33,7 +34,7 @@ template <int D, bool NORM>
 __device__ __forceinline__ TileScan copy_tile(const bf16* __restrict__ src, int64_t sl, int s0, int L, int Lp,
                                               bf16* __restrict__ xr, bf16* __restrict__ xt,
                                               const float* __restrict__ ct, const float* __restrict__ st,
-                                              bool check_finite, bf16* tile) {
+                                              bool check_finite, bf16* tile, uint64_t keep = ~0ull) {
   constexpr int S = 64;       // sequence rows per tile
   constexpr int CPR = D / 8;  // 16-byte chunks per row
   constexpr int LD = D + 2;   // LDS row pitch in bf16 (odd word count: column reads spread over banks)
@@ -46,7 +47,7 @@ __device__ __forceinline__ TileScan copy_tile(const bf16* __restrict__ src, int6
     const int c = tid + i * 256;
     const int row = c / CPR, ch = c % CPR;
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (s0 + row < L) {
+    if (s0 + row < L && (keep >> row & 1)) {
       v = *reinterpret_cast<const u32x4*>(src + (int64_t)(s0 + row) * sl + ch * 8);
       if (ct) {
         // Channels 8*ch .. +7 are pairs 4*ch .. +3 of row s0 + row.
@@ -121,6 +122,13 @@ __device__ __forceinline__ uint64_t attended_keys(const uint8_t* mask, int64_t m
   return __builtin_amdgcn_ballot_w64(j < Lk && (mask == nullptr || mask[b * msb + j] != 0));
 }
 
+// Those of them that some row's window reaches (see key_hull).
+__device__ __forceinline__ uint64_t reached_keys(uint64_t att, int j0, int lo, int hi) {
+  const int a = min(max(lo - j0, 0), 64), z = min(max(hi - j0, 0), 64);
+  const uint64_t below = z >= 64 ? ~0ull : (1ull << z) - 1;
+  return a >= 64 ? 0 : att & below & (~0ull << a);
+}
+
 // Key bias and flags of one 64-key tile (threads 0..63): kbias[b*Lkp + j] = 0
 // if key j is attended, else -inf; kfull[b*(Lkp/32) + t] = 1 if all 32 keys
 // of tile t are attended.
@@ -143,7 +151,8 @@ __device__ __forceinline__ void write_key_bias(uint64_t att, int b, int j0, int 
 // and the forward may leave it out.  Leaving such tiles out at both ends here
 // and in the backward took 75,600 queries x 512 text keys (one sample of 388
 // keys, one of none, 40 heads, D 128, fwd+bwd) from 7.35 to 5.59 ms.
-template <int D>
+// DROP (changed scores): keys that no row may attend are copied as zeros.
+template <int D, bool DROP>
 __global__ __launch_bounds__(256) void prep_fwd_kernel(FwdArgs a, int nk) {
   __shared__ bf16 tile[64 * (D + 2)];
   __shared__ float wmax[4];
@@ -154,13 +163,19 @@ __global__ __launch_bounds__(256) void prep_fwd_kernel(FwdArgs a, int nk) {
   const int t = u % nt, bh = u / nt;
   const int b = bh / a.Hkv, h = bh % a.Hkv;
   const int s0 = 64 * t;
+  uint64_t keep = ~0ull;
+  if constexpr (DROP) {
+    int lo, hi;
+    key_hull(a.hull, a.wlo, a.whi, a.wsb, b, a.Lq, a.Lk, lo, hi);
+    keep = reached_keys(attended_keys(a.mask, a.msb, b, s0, a.Lk), s0, lo, hi);
+  }
   if (is_k) {
     const bool unattended = a.mask != nullptr && attended_keys(a.mask, a.msb, b, s0, a.Lk) == 0;
     const float* ct = a.cos_k ? a.cos_k + b * a.rksb : nullptr;
     const float* st = a.cos_k ? a.sin_k + b * a.rksb : nullptr;
     TileScan r = copy_tile<D, true>(a.k + b * a.ksb + h * a.ksh, a.ksl, s0, a.Lk, a.Lkp,
-                                    a.kr + ((int64_t)bh * a.Lkp + s0) * D, nullptr, ct, st, unattended, tile);
-    if (unattended) r.finite = r.finite && tile_finite<D>(a.v + b * a.vsb + h * a.vsh, a.vsl, s0, a.Lk);
+                                    a.kr + ((int64_t)bh * a.Lkp + s0) * D, nullptr, ct, st, unattended, tile, keep);
+    if (unattended && !DROP) r.finite = r.finite && tile_finite<D>(a.v + b * a.vsb + h * a.vsh, a.vsl, s0, a.Lk);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) r.nmax = fmaxf(r.nmax, __shfl_xor(r.nmax, off));
     const int fin = __all(r.finite);
@@ -177,7 +192,7 @@ __global__ __launch_bounds__(256) void prep_fwd_kernel(FwdArgs a, int nk) {
   } else {
     if (h == 0) write_key_bias(attended_keys(a.mask, a.msb, b, s0, a.Lk), b, s0, a.Lkp, a.kbias, a.kfull);
     copy_tile<D, false>(a.v + b * a.vsb + h * a.vsh, a.vsl, s0, a.Lk, a.Lkp, nullptr,
-                        a.vt + (int64_t)bh * D * a.Lkp + s0, nullptr, nullptr, false, tile);
+                        a.vt + (int64_t)bh * D * a.Lkp + s0, nullptr, nullptr, false, tile, keep);
   }
 }
 
@@ -190,11 +205,11 @@ __global__ __launch_bounds__(256) void prep_fwd_kernel(FwdArgs a, int nk) {
 // dK/dV kernel needs, and the row statistics: lse2 = lse * log2(e) (+inf for
 // -inf and padded rows, whose P is then exactly 0) and ndelta =
 // -rowsum(dout * out), kStatRows rows per TPR threads.  Under a mask a row with lse
-// -inf attends nothing: its dout and out are not read.
+// -inf attends nothing: its dout and out are not read (with DROP never).
 // (One row each, its (b, h, row) by 64-bit divisions, took 485 us for 2 x 40 x
 // 75,600 rows of which half are read, against 423.)
 constexpr int kStatRows = 4;
-template <int D>
+template <int D, bool DROP>
 __global__ __launch_bounds__(256) void prep_bwd_kernel(BwdArgs a, int nk, int nq, int nd) {
   __shared__ bf16 tile[64 * (D + 2)];
   int u = blockIdx.x;
@@ -210,9 +225,15 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(BwdArgs a, int nk, int nq
     const bool rows = a.ds == nullptr;
     const int64_t row0 = ((int64_t)bh * a.Lkp + s0) * D;
     const bool scan = a.kskip != nullptr && att == 0;
+    uint64_t keep = ~0ull;
+    if constexpr (DROP) {
+      int lo, hi;
+      key_hull(nullptr, a.wlo, a.whi, a.wsb, b, a.Lq, a.Lk, lo, hi);
+      keep = reached_keys(att, s0, lo, hi);
+    }
     const TileScan r = copy_tile<D, false>(a.k + b * a.ksb + h * a.ksh, a.ksl, s0, a.Lk, a.Lkp,
                                            rows ? a.kr + row0 : nullptr, a.kt + (int64_t)bh * D * a.Lkp + s0, ct, st,
-                                           scan, tile);
+                                           scan, tile, keep);
     if (rows)
       copy_tile<D, false>(a.v + b * a.vsb + h * a.vsh, a.vsl, s0, a.Lk, a.Lkp, a.vr + row0, nullptr, nullptr,
                           nullptr, false, tile);
@@ -258,7 +279,7 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(BwdArgs a, int nk, int nq
     const int i = i0 + r * RPB;
     l[r] = i < a.Lq ? a.lse[(int64_t)bh * a.Lq + i] : kNegInf;
     x[r] = y[r] = u32x4{0u, 0u, 0u, 0u};
-    if (i < a.Lq && (a.mask == nullptr || l[r] != kNegInf)) {
+    if (i < a.Lq && ((a.mask == nullptr && !DROP) || l[r] != kNegInf)) {
       x[r] = *reinterpret_cast<const u32x4*>(dp + (int64_t)i * a.dosl);
       y[r] = *reinterpret_cast<const u32x4*>(op + (int64_t)i * a.osl);
     }
@@ -309,10 +330,14 @@ hipError_t launch_prep_fwd(const FwdArgs& a, int head_dim, hipStream_t stream) {
   const int nk = a.k8 ? 0 : (int)tiles;
   const dim3 grid((unsigned)(nk + tiles));
   LaunchTimer timer(kKidTranspose, stream);
-  if (head_dim == 128)
-    hipLaunchKernelGGL(prep_fwd_kernel<128>, grid, dim3(256), 0, stream, a, nk);
+  if (a.score.mode != 0 && head_dim == 128)
+    hipLaunchKernelGGL((prep_fwd_kernel<128, true>), grid, dim3(256), 0, stream, a, nk);
+  else if (a.score.mode != 0)
+    hipLaunchKernelGGL((prep_fwd_kernel<64, true>), grid, dim3(256), 0, stream, a, nk);
+  else if (head_dim == 128)
+    hipLaunchKernelGGL((prep_fwd_kernel<128, false>), grid, dim3(256), 0, stream, a, nk);
   else
-    hipLaunchKernelGGL(prep_fwd_kernel<64>, grid, dim3(256), 0, stream, a, nk);
+    hipLaunchKernelGGL((prep_fwd_kernel<64, false>), grid, dim3(256), 0, stream, a, nk);
   return hipGetLastError();
 }
 
@@ -328,10 +353,14 @@ hipError_t launch_prep_bwd(const BwdArgs& a, int head_dim, hipStream_t stream) {
   if (nk + nq + nd + ns > 2147483647) return hipErrorInvalidValue;
   const dim3 grid((unsigned)(nk + nq + nd + ns));
   LaunchTimer timer(kKidBwdPre, stream);
-  if (head_dim == 128)
-    hipLaunchKernelGGL(prep_bwd_kernel<128>, grid, dim3(256), 0, stream, a, (int)nk, (int)nq, (int)nd);
+  if (a.score.mode != 0 && head_dim == 128)
+    hipLaunchKernelGGL((prep_bwd_kernel<128, true>), grid, dim3(256), 0, stream, a, (int)nk, (int)nq, (int)nd);
+  else if (a.score.mode != 0)
+    hipLaunchKernelGGL((prep_bwd_kernel<64, true>), grid, dim3(256), 0, stream, a, (int)nk, (int)nq, (int)nd);
+  else if (head_dim == 128)
+    hipLaunchKernelGGL((prep_bwd_kernel<128, false>), grid, dim3(256), 0, stream, a, (int)nk, (int)nq, (int)nd);
   else
-    hipLaunchKernelGGL(prep_bwd_kernel<64>, grid, dim3(256), 0, stream, a, (int)nk, (int)nq, (int)nd);
+    hipLaunchKernelGGL((prep_bwd_kernel<64, false>), grid, dim3(256), 0, stream, a, (int)nk, (int)nq, (int)nd);
   if (a.kskip != nullptr)
     hipLaunchKernelGGL(key_hull_kernel, dim3((unsigned)(a.B * a.Hkv)), dim3(64), 0, stream, a.kskip, a.Lkp / 64,
                        a.khull);

@@ -938,6 +938,80 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
                             void* workspace, size_t workspace_bytes,
                             avattn_stream_t stream);
 
+/*
+ * Attention with changed scores (no reference counterpart: the reference's
+ * attention is F.scaled_dot_product_attention, src/avgen/models/attention.py
+ * :227-273): s = scale q.k becomes
+ *   z_ij = softcap * tanh(s_ij / softcap)          (softcap 0: s_ij; bf16:
+ *                                                   at most 1,024)
+ *          - slopes[hq] * |i + offset_b - j|       (slopes NULL: nothing)
+ * for query i at position i + offset_b (query_offsets[b] on the device, or
+ * query_offset for every batch row; within +-2^30), key j at position j, then
+ * masked by key_mask and the key windows (both may be NULL; as for avattn_fwd
+ * and avattn_fwd_windowed) and normalised.  slopes: float32 (heads_q) on the
+ * device, any sign, at most 64 query heads per kv head with them; they and the
+ * offsets get no gradient.  A row without a key: zeros and lse -inf.  A key
+ * that no row of its batch entry may attend contributes nothing, whatever its
+ * k and v hold (NaN included).  bf16 (strides multiples of 8), or float32 with
+ * is_f32 (of 4).  lse: natural log of the changed scores' sum.
+ *
+ * Up to 64 query rows per kv head (len_q * heads_q / heads_kv) run on kernels
+ * of their own, which read k and v once in place; their row strides are then
+ * below 2^23.  flags: AVATTN_SCORED_SORTED_WINDOWS, the windows are
+ * non-decreasing in the row (spares a launch; wrong values otherwise).
+ * workspace: avattn_fwd_scored_workspace_size bytes, 16-byte aligned.
+ *
+ * Backward: windows non-decreasing in the row, dS always staged.  workspace:
+ * bf16, the sizes of avattn_bwd with AVATTN_BWD_STAGE_DS
+ * (avattn_bwd_staged_workspace_size, avattn_bwd_split_workspace_size without
+ * windows), or with a ds_table (and windows) as avattn_bwd_windowed_compact;
+ * float32, avattn_bwd_f32_staged_workspace_size or
+ * avattn_bwd_f32_split_workspace_size, 256-byte aligned.
+ */
+#define AVATTN_SCORED_SORTED_WINDOWS 1u
+
+size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q,
+                                        int32_t heads_kv, int32_t len_q,
+                                        int32_t len_k, int32_t head_dim,
+                                        int32_t is_f32);
+
+int avattn_fwd_scored(const void* q, const void* k, const void* v,
+                      const int64_t* q_strides, const int64_t* k_strides,
+                      const int64_t* v_strides,
+                      int32_t batch, int32_t heads_q, int32_t heads_kv,
+                      int32_t len_q, int32_t len_k, int32_t head_dim,
+                      int32_t is_f32,
+                      const uint8_t* key_mask, int64_t key_mask_batch_stride,
+                      const int32_t* window_lo, const int32_t* window_hi,
+                      int64_t window_batch_stride,
+                      float scale, float softcap, const float* slopes,
+                      const int32_t* query_offsets, int32_t query_offset,
+                      uint32_t flags,
+                      void* out, const int64_t* out_strides, float* lse,
+                      void* workspace, size_t workspace_bytes,
+                      avattn_stream_t stream);
+
+int avattn_bwd_scored(const void* dout, const void* q, const void* k,
+                      const void* v, const void* out, const float* lse,
+                      const int64_t* dout_strides, const int64_t* q_strides,
+                      const int64_t* k_strides, const int64_t* v_strides,
+                      const int64_t* out_strides,
+                      int32_t batch, int32_t heads_q, int32_t heads_kv,
+                      int32_t len_q, int32_t len_k, int32_t head_dim,
+                      int32_t is_f32,
+                      const uint8_t* key_mask, int64_t key_mask_batch_stride,
+                      const int32_t* window_lo, const int32_t* window_hi,
+                      int64_t window_batch_stride,
+                      const int32_t* ds_table, int64_t ds_table_batch_stride,
+                      int64_t ds_units_per_head,
+                      float scale, float softcap, const float* slopes,
+                      const int32_t* query_offsets, int32_t query_offset,
+                      void* dq, const int64_t* dq_strides,
+                      void* dk, const int64_t* dk_strides,
+                      void* dv, const int64_t* dv_strides,
+                      void* workspace, size_t workspace_bytes,
+                      avattn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
