@@ -281,6 +281,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_ptr],
     ),
     "avattn_fwd_scored_workspace_size": (c_size, [c_i32] * 7),
+    "avattn_bwd_scored_workspace_size": (c_size, [c_i32] * 8),
     "avattn_fwd_scored": (
         ctypes.c_int,
         [c_ptr, c_ptr, c_ptr, c_i64p, c_i64p, c_i64p,

@@ -25,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _direct, _grad_direct, _ptr, _require_gpu, _stream, _strides3, _workspace
+from .ops import _direct, _grad_direct, _ptr, _require_gpu, _stream, _Strides3, _workspace
 
 __all__ = [
     "MAX_TABLE_PAIRS",
@@ -43,18 +43,26 @@ MAX_TABLE_PAIRS = 256
 _FLOATS = (torch.bfloat16, torch.float32)
 
 
-def _one_device(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """All tensors on one GPU."""
-    _require_gpu(name, *tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f"{name}: tensors on different devices: {sorted(map(str, devices))}")
+def _one_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """All tensors on one GPU: the GPU."""
+    device = first.device
+    if device.type != "cuda":
+        _require_gpu(name, first)
+    for t in others:
+        if t is not None and t.device != device:
+            _require_gpu(name, t)
+            raise RuntimeError(f"{name}: tensors on different devices: {device} and {t.device}")
+    return device
+
+
+_here = nullcontext()
 
 
 def _on(device: torch.device):
     """Launches on ``device``, whichever is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return nullcontext()
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
+        return _here
     return torch.cuda.device(device)
 
 
@@ -101,47 +109,56 @@ def position_tables(positions: torch.Tensor, frequencies: list[float], amplitude
 def _check_rotation(name, tensors, cos, sin, start):
     """Shapes and dtypes; the tables contiguous, with their batch stride."""
     x = tensors[0]
+    dtype, shape = x.dtype, x.shape
+    if len(shape) != 4:
+        raise ValueError(f"{name}: rotary input must be (batch, heads, length, head_dim); got {tuple(shape)}")
+    B, _, L, D = shape
     for t in tensors:
-        if t.ndim != 4:
-            raise ValueError(f"{name}: rotary input must be (batch, heads, length, head_dim); got {tuple(t.shape)}")
-        if t.dtype not in _FLOATS or t.dtype is not x.dtype:
+        if t.dtype not in _FLOATS or t.dtype is not dtype:
             raise TypeError(f"{name}: inputs must all be bfloat16 or all float32; got {t.dtype}")
-        if t.shape[0] != x.shape[0] or t.shape[2:] != x.shape[2:]:
-            raise ValueError(f"{name}: {tuple(x.shape)} and {tuple(t.shape)} differ in more than their heads")
-    if cos.ndim != 4 or cos.shape != sin.shape:
+        if t is not x:
+            s = t.shape
+            if len(s) != 4 or s[0] != B or s[2] != L or s[3] != D:
+                raise ValueError(f"{name}: {tuple(shape)} and {tuple(s)} differ in more than their heads")
+    table = cos.shape
+    if len(table) != 4 or table != sin.shape:
         raise ValueError(f"{name}: rotary tables must be (batch, 1, length, pairs) and agree")
     if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise TypeError(f"{name}: rotary tables must be float32")
-    B, _, L, D = x.shape
-    P = cos.shape[-1]
+    TB, TH, TL, P = table
     if P < 1 or start < 0 or start + 2 * P > D:
         raise ValueError(f"{name}: channels [{start}, {start + 2 * P}) do not lie in a head of {D}")
-    if cos.shape[-2] != L:
-        raise ValueError(f"{name}: sequence length {L} does not match rotary tables built for length {cos.shape[-2]}")
-    if cos.shape[0] not in (1, B) or cos.shape[1] != 1:
-        raise ValueError(f"{name}: rotary tables batch {cos.shape[0]} does not broadcast to {B}")
+    if TL != L:
+        raise ValueError(f"{name}: sequence length {L} does not match rotary tables built for length {TL}")
+    if TB not in (1, B) or TH != 1:
+        raise ValueError(f"{name}: rotary tables batch {TB} does not broadcast to {B}")
     _one_device(name, *tensors, cos, sin)
-    cos, sin = cos.contiguous(), sin.contiguous()
-    return cos, sin, (0 if cos.shape[0] == 1 else L * P)
+    return cos.contiguous(), sin.contiguous(), (0 if TB == 1 else L * P)
 
 
 def _rotate_launch(name, q, k, cos, sin, start, half, inverse):
     cos, sin, tsb = _check_rotation(name, (q,) if k is None else (q, k), cos, sin, start)
     B, H, L, D = q.shape
-    ins = [_packed_last(t) for t in (q, k) if t is not None]
     outs = []
-    for t in ins:
-        o = torch.empty_like(t, memory_format=torch.preserve_format)
-        outs.append(o if o.stride(-1) == 1 or D <= 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device))
     args = []
-    for t, o in zip(ins, outs):
-        args += [_ptr(t), _strides3(t), t.shape[1], _ptr(o), _strides3(o)]
-    if k is None:
-        args += [None, None, 0, None, None]
-    with _on(q.device):
+    for t in (q, k):
+        if t is None:
+            args += (None, None, 0, None, None)
+            continue
+        t = _packed_last(t)
+        o = torch.empty_like(t)
+        outs.append(o)
+        strides, ostrides = t.stride(), o.stride()
+        if ostrides[3] != 1 and D > 1:
+            o = outs[-1] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            ostrides = o.stride()
+        s = _Strides3(*strides[:3])
+        args += (t.data_ptr(), s, t.shape[1], o.data_ptr(), s if ostrides == strides else _Strides3(*ostrides[:3]))
+    device = q.device
+    with _on(device):
         st = _lib.load().avattn_rotate(
-            *args, B, L, D, cos.shape[-1], int(start), int(bool(half)), int(q.dtype is torch.float32),
-            _ptr(cos), _ptr(sin), tsb, int(bool(inverse)), _stream(q.device))
+            *args, B, L, D, cos.shape[-1], start, half, q.dtype is torch.float32,
+            cos.data_ptr(), sin.data_ptr(), tsb, inverse, _stream(device))
     _lib.check(st, name)
     return outs
 
@@ -250,9 +267,10 @@ def _rows(t: torch.Tensor):
     """``t (..., W)`` as rows of ``W`` contiguous values: the tensor to read
     and its row stride."""
     W = t.shape[-1]
+    if t.is_contiguous():
+        return t, W
     t = _packed_last(t)
-    rows = t.numel() // W if W else 0
-    if t.ndim == 1 or rows <= 1:
+    if t.ndim == 1 or t.numel() <= W:
         return t, W
     # The leading dimensions must collapse into one stride.
     stride = expect = None
@@ -270,18 +288,20 @@ def _rows(t: torch.Tensor):
 
 
 def _check_norm(name, x, residual, weight, eps):
-    if x.ndim < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{name}: rows of at least one value expected; got {tuple(x.shape)}")
-    if x.dtype not in _FLOATS:
-        raise TypeError(f"{name}: input must be bfloat16 or float32; got {x.dtype}")
-    if residual.shape != x.shape:
-        raise ValueError(f"{name}: residual {tuple(residual.shape)} must have the input's shape {tuple(x.shape)}")
-    if residual.dtype is not x.dtype:
-        raise TypeError(f"{name}: residual must be {x.dtype} like the input; got {residual.dtype}")
-    if weight.shape != (x.shape[-1],):
-        raise ValueError(f"{name}: weight must be ({x.shape[-1]},); got {tuple(weight.shape)}")
-    if weight.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"{name}: weight must be {x.dtype} or float32; got {weight.dtype}")
+    shape, dtype = x.shape, x.dtype
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"{name}: rows of at least one value expected; got {tuple(shape)}")
+    if dtype not in _FLOATS:
+        raise TypeError(f"{name}: input must be bfloat16 or float32; got {dtype}")
+    if residual is not x:
+        if residual.shape != shape:
+            raise ValueError(f"{name}: residual {tuple(residual.shape)} must have the input's shape {tuple(shape)}")
+        if residual.dtype is not dtype:
+            raise TypeError(f"{name}: residual must be {dtype} like the input; got {residual.dtype}")
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"{name}: weight must be ({shape[-1]},); got {tuple(weight.shape)}")
+    if weight.dtype is not dtype and weight.dtype is not torch.float32:
+        raise TypeError(f"{name}: weight must be {dtype} or float32; got {weight.dtype}")
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"{name}: eps must be finite and >= 0; got {eps}")
     _one_device(name, x, residual, weight)
@@ -290,17 +310,18 @@ def _check_norm(name, x, residual, weight, eps):
 
 def _norm_launch(name, x, residual, weight, eps, fp8):
     w = _check_norm(name, x, residual, weight, eps)
-    W = x.shape[-1]
+    shape, dtype, device = x.shape, x.dtype, x.device
+    W = shape[-1]
     rows = x.numel() // W
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    norm = torch.empty(x.shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if fp8 else None
+    total = torch.empty_like(x, memory_format=torch.contiguous_format)
+    norm = torch.empty_like(x, memory_format=torch.contiguous_format, dtype=torch.float8_e4m3fn if fp8 else dtype)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=device) if fp8 else None
     (x, xs), (residual, rs) = _rows(x), _rows(residual)
     if rows:
-        with _on(x.device):
+        with _on(device):
             st = _lib.load().avattn_add_rms_norm(
-                _ptr(x), xs, _ptr(residual), rs, _ptr(w), int(w.dtype is torch.float32), rows, W,
-                int(x.dtype is torch.float32), float(eps), _ptr(total), _ptr(norm), _ptr(scale), _stream(x.device))
+                x.data_ptr(), xs, residual.data_ptr(), rs, w.data_ptr(), w.dtype is torch.float32, rows, W,
+                dtype is torch.float32, eps, total.data_ptr(), norm.data_ptr(), _ptr(scale), _stream(device))
         _lib.check(st, name)
     return norm, scale, total
 

@@ -19,7 +19,9 @@ namespace avattn {
 
 namespace {
 
-constexpr int kMaxPartBlocks = 1024;  // dW partials of the backward
+// dW partials of the backward: one per row group in flight, four waves' rows
+// per workgroup where rows are narrow.
+constexpr int max_parts(int64_t W) { return W <= 1024 ? 4096 : 1024; }
 
 // The thread's values of a row: NV chunks of CH consecutive columns, chunk j
 // at column (j * TPR + t) * CH.
@@ -47,6 +49,22 @@ __device__ __forceinline__ void store_chunk(T* p, const float* v) {
   else
     p[0] = (T)v[0];
 }
+// A chunk as it was loaded (bf16 stays packed: half the registers), and its
+// values.
+template <class T, int CH>
+using RawChunk = u32x4;
+template <class T, int CH>
+__device__ __forceinline__ RawChunk<T, CH> read_chunk(const T* p) {
+  static_assert(CH * sizeof(T) == 16, "whole chunks");
+  return *reinterpret_cast<const u32x4*>(p);
+}
+template <class T, int CH>
+__device__ __forceinline__ float chunk_value(const RawChunk<T, CH>& r, int e) {
+  if constexpr (CH == 8)
+    return e & 1 ? bf16_hi(r[e / 2]) : bf16_lo(r[e / 2]);
+  else
+    return __uint_as_float(r[e]);
+}
 // The gain's columns: in the rows' type or fp32.
 template <class T, int CH>
 __device__ __forceinline__ void load_gain(const void* w, bool w32, int64_t col, float* v) {
@@ -69,21 +87,18 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* v) {
     p[0] = (uint8_t)pack_fp8x4(v[0], 0.f, 0.f, 0.f);
 }
 
-// Sum (or maximum) over the TPR threads of a row; every thread of the
-// workgroup calls it.  red: one float per wave.
-template <int TPR, bool MAX>
+// Sum (or maximum) over the threads of a row: a wave (WAVE) or the workgroup,
+// every thread of which calls it.  red: one float per wave.
+template <bool WAVE, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* red) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v = MAX ? fmaxf(v, __shfl_xor(v, off)) : v + __shfl_xor(v, off);
-  if constexpr (TPR > 64) {
-    constexpr int NW = TPR / 64;
-    const int wave = threadIdx.x >> 6;
+  if constexpr (!WAVE) {
     __syncthreads();  // the last reduction's values are read
-    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+    for (int i = 1; i < (int)blockDim.x / 64; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
   }
   return v;
 }
@@ -92,15 +107,16 @@ __device__ __forceinline__ float fp8_row_scale(float top) {
   return top > 0.f ? fmaxf(top / 448.f, 1.1754943508222875e-38f) : 1.f;
 }
 
-// Forward.  TPR threads per row: a wave for narrow rows (several rows per
-// workgroup), a workgroup for wide ones.
-template <class T, int CH, int TPR, int NV, bool FP8>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_norm_kernel(AddNormArgs a) {
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red[TPR / 64];
+// Forward.  A row takes a wave (narrow rows, 4 per workgroup) or a workgroup of
+// as many waves as its chunks fill (see row_shape).
+template <class T, int CH, int NV, bool WAVE, bool FP8>
+__global__ __launch_bounds__(WAVE ? 256 : 1024) void add_norm_kernel(AddNormArgs a) {
+  constexpr int RPB = WAVE ? 4 : 1;
+  __shared__ float red[16];
+  const int TPR = WAVE ? 64 : blockDim.x;
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  if (row >= a.rows) return;  // whole waves (TPR 64) or nobody
+  if (row >= a.rows) return;  // whole waves or nobody
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   const T* r = static_cast<const T*>(a.r) + row * a.rs;
   float h[NV][CH], w[NV][CH];
@@ -131,7 +147,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_norm_kernel(AddNorm
     const int64_t col = (int64_t)(j * TPR + t) * CH;
     if (col < a.W) store_chunk<T, CH>(hp + col, h[j]);
   }
-  ss = row_reduce<TPR, false>(ss, red);
+  ss = row_reduce<WAVE, false>(ss, red);
   const float rstd = 1.f / __builtin_sqrtf(ss / (float)a.W + a.eps);
   float top = 0.f;
 #pragma unroll
@@ -142,7 +158,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_norm_kernel(AddNorm
       if constexpr (FP8) top = fmaxf(top, fabsf(h[j][e]));
     }
   if constexpr (FP8) {
-    top = row_reduce<TPR, true>(top, red);
+    top = row_reduce<WAVE, true>(top, red);
     const float scale = fp8_row_scale(top), inv = 1.f / scale;
     if (t == 0) a.scale[row] = scale;
     uint8_t* np = static_cast<uint8_t*>(a.n) + row * a.W;
@@ -178,7 +194,7 @@ __global__ __launch_bounds__(256) void add_norm_any_kernel(AddNormArgs a) {
     hp[c] = (T)h;
     ss = fmaf(h, h, ss);
   }
-  ss = row_reduce<256, false>(ss, red);
+  ss = row_reduce<false, false>(ss, red);
   const float rstd = 1.f / __builtin_sqrtf(ss / (float)a.W + a.eps);
   auto norm = [&](int64_t c) {
     float w;
@@ -188,7 +204,7 @@ __global__ __launch_bounds__(256) void add_norm_any_kernel(AddNormArgs a) {
   if constexpr (FP8) {
     float top = 0.f;
     for (int64_t c = threadIdx.x; c < a.W; c += 256) top = fmaxf(top, fabsf(norm(c)));
-    top = row_reduce<256, true>(top, red);
+    top = row_reduce<false, true>(top, red);
     const float scale = fp8_row_scale(top), inv = 1.f / scale;
     if (threadIdx.x == 0) a.scale[row] = scale;
     uint8_t* np = static_cast<uint8_t*>(a.n) + row * a.W;
@@ -205,10 +221,16 @@ __global__ __launch_bounds__(256) void add_norm_any_kernel(AddNormArgs a) {
 // Backward.  Each row group walks over rows blockIdx, + gridDim, ...; its
 // threads keep their columns of w and of the dW sum in registers.  Sum of h^2
 // and of g h in one pass over the row.
-template <class T, int CH, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_norm_bwd_kernel(AddNormArgs a) {
-  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red[2][2][TPR / 64];
+// AHEAD: the next row's values are loaded before this row's sums (more
+// registers; with two chunks per thread up to 512 threads).
+// DH: a gradient of h is given.  (The loads are unconditional: behind a branch
+// the compiler would wait for them before it uses the row loaded earlier,
+// 200 us in place of 150 for 18,900 rows of 5,120.)
+template <class T, int CH, int NV, bool WAVE, bool AHEAD, bool DH>
+__global__ __launch_bounds__(WAVE ? 256 : (AHEAD && NV > 1 ? 512 : 1024)) void add_norm_bwd_kernel(AddNormArgs a) {
+  constexpr int RPB = WAVE ? 4 : 1;
+  __shared__ float red[2][2][16];
+  const int TPR = WAVE ? 64 : blockDim.x;
   const int t = threadIdx.x % TPR, rg = threadIdx.x / TPR;
   float w[NV][CH], dw[NV][CH];
 #pragma unroll
@@ -220,37 +242,55 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_norm_bwd_kernel(Add
   }
   const int64_t step = (int64_t)gridDim.x * RPB;
   int buf = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + rg; row < a.rows; row += step) {  // uniform over the row's threads
-    const T* hp = static_cast<const T*>(a.x) + row * a.xs;
-    const T* np = static_cast<const T*>(a.dn) + row * a.dns;
-    float h[NV][CH], g[NV][CH], dh[NV][CH];
+  struct Row {
+    RawChunk<T, CH> h[NV], g[NV], d[NV];
+  };
+  int64_t at[NV];       // this thread's columns, 0 past the end of the row,
+  uint32_t in[NV];      // where what is loaded is masked out
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int64_t col = (int64_t)(j * TPR + t) * CH;
+    at[j] = col < a.W ? col : 0;
+    in[j] = col < a.W ? 0xffffffffu : 0u;
+  }
+  auto load = [&](int64_t row, Row& r) {
+    row = row < a.rows ? row : a.rows - 1;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t col = (int64_t)(j * TPR + t) * CH;
-#pragma unroll
-      for (int e = 0; e < CH; ++e) h[j][e] = g[j][e] = dh[j][e] = 0.f;
-      if (col < a.W) {
-        load_chunk<T, CH>(hp + col, h[j]);
-        load_chunk<T, CH>(np + col, g[j]);
-        if (a.dh) load_chunk<T, CH>(static_cast<const T*>(a.dh) + row * a.dhs + col, dh[j]);
-      }
+      r.h[j] = read_chunk<T, CH>(static_cast<const T*>(a.x) + row * a.xs + at[j]);
+      r.g[j] = read_chunk<T, CH>(static_cast<const T*>(a.dn) + row * a.dns + at[j]);
+      if constexpr (DH) r.d[j] = read_chunk<T, CH>(static_cast<const T*>(a.dh) + row * a.dhs + at[j]);
     }
+  };
+  Row next;
+  if constexpr (AHEAD) load((int64_t)blockIdx.x * RPB + rg, next);
+  for (int64_t row = (int64_t)blockIdx.x * RPB + rg; row < a.rows; row += step) {  // uniform over the row's threads
+    Row cur;
+    if constexpr (AHEAD) {
+      cur = next;
+      load(row + step, next);
+    } else {
+      load(row, cur);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) cur.h[j] &= in[j], cur.g[j] &= in[j];
+    const auto &rh = cur.h, &rg = cur.g, &rd = cur.d;
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < CH; ++e) {
-        ss = fmaf(h[j][e], h[j][e], ss);
-        dot = fmaf(g[j][e] * w[j][e], h[j][e], dot);
+        const float h = chunk_value<T, CH>(rh[j], e);
+        ss = fmaf(h, h, ss);
+        dot = fmaf(chunk_value<T, CH>(rg[j], e) * w[j][e], h, dot);
       }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off), dot += __shfl_xor(dot, off);
-    if constexpr (TPR > 64) {
+    if constexpr (!WAVE) {
       const int wave = threadIdx.x >> 6;
       if ((threadIdx.x & 63) == 0) red[buf][0][wave] = ss, red[buf][1][wave] = dot;
       __syncthreads();
       ss = red[buf][0][0], dot = red[buf][1][0];
-#pragma unroll
       for (int i = 1; i < TPR / 64; ++i) ss += red[buf][0][i], dot += red[buf][1][i];
       buf ^= 1;  // the next row's values go elsewhere: one barrier per row
     }
@@ -260,12 +300,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_norm_bwd_kernel(Add
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t col = (int64_t)(j * TPR + t) * CH;
+      float dx[CH];
 #pragma unroll
       for (int e = 0; e < CH; ++e) {
-        dw[j][e] = fmaf(g[j][e], h[j][e] * rstd, dw[j][e]);
-        dh[j][e] += rstd * (g[j][e] * w[j][e] - h[j][e] * m);
+        const float h = chunk_value<T, CH>(rh[j], e), g = chunk_value<T, CH>(rg[j], e);
+        dw[j][e] = fmaf(g, h * rstd, dw[j][e]);
+        dx[e] = rstd * (g * w[j][e] - h * m);
+        if constexpr (DH) dx[e] += chunk_value<T, CH>(rd[j], e);
       }
-      if (col < a.W) store_chunk<T, CH>(op + col, dh[j]);
+      if (col < a.W) store_chunk<T, CH>(op + col, dx);
     }
   }
   // The workgroup's row groups one after the other, then its partial.
@@ -300,8 +343,8 @@ __global__ __launch_bounds__(256) void add_norm_bwd_any_kernel(AddNormArgs a) {
       ss = fmaf(h, h, ss);
       dot = fmaf((float)np[c] * w, h, dot);
     }
-    ss = row_reduce<256, false>(ss, red);
-    dot = row_reduce<256, false>(dot, red);
+    ss = row_reduce<false, false>(ss, red);
+    dot = row_reduce<false, false>(dot, red);
     const float rstd = 1.f / __builtin_sqrtf(ss / (float)a.W + a.eps);
     const float m = dot / (float)a.W * rstd * rstd;
     T* op = static_cast<T*>(a.h) + row * a.W;
@@ -353,64 +396,72 @@ bool chunked(const AddNormArgs& a, int size, bool bwd) {
   return ok && p % 16 == 0;
 }
 
-// Threads per row and chunks per thread for rows of `chunks` chunks: a wave
-// up to 128 chunks, 256 threads up to 1,024, then 1,024.  Few rows leave the
-// chip idle and wait for one row's latency: there a row takes 1,024 threads
-// as soon as that shortens a thread's share.
+// Threads per row and chunks per thread (nv 0: the value-by-value kernels).  A
+// wave for up to 64 chunks (forward: up to 128 of many rows); else as many
+// waves as one chunk per thread fills for few rows, whose latency counts, or up
+// to 512 chunks, two chunks per thread beyond (four for float rows past 2,048).
+// 18,900 rows of 5,120 bf16, backward: 5 waves of two chunks 161 us, 10 of one
+// 176, 4 of three 168.
 struct RowShape {
   int tpr, nv;
 };
-// (A thread of 1,024 has 128 registers: at most 16 columns.)
-RowShape row_shape(int64_t chunks, int64_t rows, int ch) {
+RowShape row_shape(int64_t chunks, int64_t rows, int ch, bool bwd) {
   if (chunks <= 64) return {64, 1};
-  if (chunks <= 128 && rows >= 1024) return {64, 2};
-  if (chunks <= 256) return {256, 1};
-  const int tpr = chunks > 1024 || rows <= 512 ? 1024 : 256;
-  const int nv = (int)((chunks + tpr - 1) / tpr);
-  if (tpr == 1024 && nv * ch > 16) return {0, 0};
-  return {tpr, tpr == 1024 && nv == 3 ? 4 : nv};
+  if (chunks <= 128 && rows >= 1024 && !bwd) return {64, 2};
+  const int nv = chunks <= 512 || (chunks <= 1024 && rows <= 512) ? 1 : (chunks <= 2048 ? 2 : 4);
+  if (chunks > 1024 * nv || nv * ch > 16) return {0, 0};
+  return {(int)((chunks + 64 * nv - 1) / (64 * nv)) * 64, nv};
 }
 
-template <class T, int TPR, int NV>
-void launch_shape(const AddNormArgs& a, int mode, int blocks, hipStream_t stream) {
-  constexpr int CH = 16 / (int)sizeof(T), RPB = TPR < 256 ? 256 / TPR : 1;
-  const dim3 block(TPR < 256 ? 256 : TPR);
+template <class T, int NV, bool WAVE>
+void launch_shape(const AddNormArgs& a, int tpr, int mode, int blocks, hipStream_t stream) {
+  constexpr int CH = 16 / (int)sizeof(T), RPB = WAVE ? 4 : 1;
+  const dim3 block(WAVE ? 256 : tpr);
   const dim3 grid(mode == 2 ? blocks : (unsigned)((a.rows + RPB - 1) / RPB));
-  if (mode == 2)
-    hipLaunchKernelGGL((add_norm_bwd_kernel<T, CH, TPR, NV>), grid, block, 0, stream, a);
-  else if (mode == 1)
-    hipLaunchKernelGGL((add_norm_kernel<T, CH, TPR, NV, true>), grid, block, 0, stream, a);
+  if (mode == 2) {
+    if constexpr (!(WAVE && NV == 2)) {
+      constexpr bool kAhead = NV <= 2;
+      const bool ahead = NV == 1 || (kAhead && tpr <= 512);
+      if (ahead && a.dh)
+        hipLaunchKernelGGL((add_norm_bwd_kernel<T, CH, NV, WAVE, kAhead, true>), grid, block, 0, stream, a);
+      else if (ahead)
+        hipLaunchKernelGGL((add_norm_bwd_kernel<T, CH, NV, WAVE, kAhead, false>), grid, block, 0, stream, a);
+      else if (a.dh)
+        hipLaunchKernelGGL((add_norm_bwd_kernel<T, CH, NV, WAVE, NV == 1, true>), grid, block, 0, stream, a);
+      else
+        hipLaunchKernelGGL((add_norm_bwd_kernel<T, CH, NV, WAVE, NV == 1, false>), grid, block, 0, stream, a);
+    }
+  } else if (mode == 1)
+    hipLaunchKernelGGL((add_norm_kernel<T, CH, NV, WAVE, true>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((add_norm_kernel<T, CH, TPR, NV, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((add_norm_kernel<T, CH, NV, WAVE, false>), grid, block, 0, stream, a);
 }
 
 // mode 0: forward, 1: forward with e4m3, 2: backward (`blocks` workgroups).
 template <class T>
 void launch_rows(const AddNormArgs& a, const RowShape& s, int mode, int blocks, hipStream_t stream) {
   if (s.tpr == 64 && s.nv == 1)
-    launch_shape<T, 64, 1>(a, mode, blocks, stream);
+    launch_shape<T, 1, true>(a, s.tpr, mode, blocks, stream);
   else if (s.tpr == 64)
-    launch_shape<T, 64, 2>(a, mode, blocks, stream);
-  else if (s.tpr == 256 && s.nv == 1)
-    launch_shape<T, 256, 1>(a, mode, blocks, stream);
-  else if (s.tpr == 256 && s.nv == 2)
-    launch_shape<T, 256, 2>(a, mode, blocks, stream);
-  else if (s.tpr == 256 && s.nv == 3)
-    launch_shape<T, 256, 3>(a, mode, blocks, stream);
-  else if (s.tpr == 256)
-    launch_shape<T, 256, 4>(a, mode, blocks, stream);
+    launch_shape<T, 2, true>(a, s.tpr, mode, blocks, stream);  // forward
   else if (s.nv == 1)
-    launch_shape<T, 1024, 1>(a, mode, blocks, stream);
+    launch_shape<T, 1, false>(a, s.tpr, mode, blocks, stream);
   else if (s.nv == 2)
-    launch_shape<T, 1024, 2>(a, mode, blocks, stream);
+    launch_shape<T, 2, false>(a, s.tpr, mode, blocks, stream);
   else if constexpr (sizeof(T) == 4)
-    launch_shape<T, 1024, 4>(a, mode, blocks, stream);
+    launch_shape<T, 4, false>(a, s.tpr, mode, blocks, stream);
 }
 
-// Workgroups of the backward and the dW partials they leave.
-int bwd_blocks(int64_t rows, int rpb) {
+// Workgroups of the backward: 16 waves on a CU with one chunk per thread, 12
+// with two, all of them resident.  More gain nothing: 37,800 rows of 2,560 in 2
+// / 3 / 4 workgroups of 5 waves per CU 157 / 155 / 186 us.
+int bwd_blocks(int64_t rows, int64_t W, const RowShape& s) {
+  const int rpb = s.tpr == 64 ? 4 : 1, waves = s.tpr <= 64 ? 4 : s.tpr / 64;
   const int64_t want = (rows + rpb - 1) / rpb;
-  return (int)(want < kMaxPartBlocks / rpb ? want : kMaxPartBlocks / rpb);
+  const int fit = (s.nv == 2 ? 12 : 16) / waves;
+  int64_t most = 256 * (fit > 0 ? fit : 1);
+  if (most > max_parts(W) / rpb) most = max_parts(W) / rpb;
+  return (int)(want < most ? want : most);
 }
 
 template <class T>
@@ -419,7 +470,7 @@ hipError_t forward(const AddNormArgs& a, bool fp8, hipStream_t stream) {
   constexpr int CH = 16 / (int)sizeof(T);
   LaunchTimer timer(kKidAddNorm, stream);
   const bool vec = chunked(a, sizeof(T), false);
-  const RowShape s = vec ? row_shape(a.W / CH, a.rows, CH) : RowShape{0, 0};
+  const RowShape s = vec ? row_shape(a.W / CH, a.rows, CH, false) : RowShape{0, 0};
   if (s.nv > 0) {
     launch_rows<T>(a, s, fp8 ? 1 : 0, 0, stream);
   } else {
@@ -439,8 +490,8 @@ hipError_t backward(const AddNormArgs& a, void* dw, bool dw32, hipStream_t strea
   if (a.rows > 0) {
     LaunchTimer timer(kKidAddNormBwd, stream);
     const bool vec = chunked(a, sizeof(T), true);
-    const RowShape s = vec ? row_shape(a.W / CH, a.rows, CH) : RowShape{0, 0};
-    const int rpb = s.tpr == 64 ? 4 : 1, blocks = bwd_blocks(a.rows, rpb);
+    const RowShape s = vec ? row_shape(a.W / CH, a.rows, CH, true) : RowShape{0, 0};
+    const int rpb = s.tpr == 64 ? 4 : 1, blocks = bwd_blocks(a.rows, a.W, s);
     nparts = blocks * rpb;
     if (s.nv > 0)
       launch_rows<T>(a, s, 2, blocks, stream);
@@ -457,7 +508,7 @@ hipError_t backward(const AddNormArgs& a, void* dw, bool dw32, hipStream_t strea
 }  // namespace
 
 size_t add_norm_bwd_workspace_bytes(int64_t rows, int64_t W) {
-  const int64_t n = rows < kMaxPartBlocks ? (rows + 3) / 4 * 4 : kMaxPartBlocks;
+  const int64_t n = rows < max_parts(W) ? (rows + 3) / 4 * 4 : max_parts(W);
   return (size_t)n * (size_t)W * sizeof(float);
 }
 

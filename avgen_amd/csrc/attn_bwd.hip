@@ -41,8 +41,9 @@ __global__ __launch_bounds__(256) void dkv_reduce_kernel(BwdArgs a) {
   const int s = (int)(u / (CQ * BK * 2));
   const int nkt = (a.Lk + BK - 1) / BK;
   const int bid = nkt * a.nkv - a.nsplit + s;
-  const int kt = bid % nkt;
-  const int bhk = a.kv0 + bid / nkt;
+  int kt = bid % nkt, pair = bid / nkt;
+  if (a.score.mode != 0 && a.wlo != nullptr && a.nsplit < nkt * a.nkv) longest_first(bid, nkt, a.nkv, kt, pair);
+  const int bhk = a.kv0 + pair;
   const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
   const int key = kt * BK + r;
   if (key >= a.Lk) return;
@@ -648,10 +649,21 @@ static int cu_count() {
 // 623 split; (2,20,40000) x 1,024 with one row empty 1,511 against 1,612).
 // Backward: (1,16,20000,128) x 256 keys 498 -> 198 us, (1,20,10000) x 128 keys
 // 255 -> 104, (1,4,4096) self-attention 171 -> 150.
-TailSplit dkv_split_plan(int64_t total, int tiles, int D) {
+// With windows (changed scores) a block's tiles are known on the device only
+// and differ: parts for two rounds of workgroups, which level out.  (1,16 / 4
+// heads,4133,64) with 2 / 3 / 4 / 5 / 6 / 8 parts of 132 blocks: five documents
+// 133 / 127 / 106 / 110 / 107 / 108 us, causal 154 / 168 / 122 / 151 / 134 / 137,
+// whole windows 381 / 280 / 298 / 263 / 283 / 273.
+TailSplit dkv_split_plan(int64_t total, int tiles, int D, bool windows) {
   constexpr int kCus = 256;
   TailSplit best{0, 0};
   if (total > kCus) return best;
+  if (windows) {
+    int p = (int)((2 * kCus + total - 1) / total);
+    if (p > 8) p = 8;
+    if (p > tiles / 8) p = tiles / 8;
+    return p > 1 ? TailSplit{(int)total, p} : best;
+  }
   const float work_us = tiles * (D == 64 ? 1.1f : 1.9f), fixed_us = 8.f;
   auto cost = [&](int p) {
     const int n = (int)total * p, rem = n % kCus;
@@ -734,7 +746,7 @@ static hipError_t launch_bwd_d(const BwdArgs& args, int kv_per_pass, hipStream_t
     TailSplit ts = p.split_part ? plan_tail_split(total, cus, kSplitSlots) : TailSplit{0, 0};
     if (p.split_all != nullptr) {
       // Every block split (the region holds the plan's parts).
-      ts = dkv_split_plan(total, (a.Lqp / 64) * (a.Hq / a.Hkv), D);
+      ts = dkv_split_plan(total, (a.Lqp / 64) * (a.Hq / a.Hkv), D, p.wlo != nullptr);
       p.split_part = p.split_all;
     }
     p.nsplit = ts.nsplit;

@@ -1284,8 +1284,16 @@ constexpr int dkv_f32_slot_floats(int D) { return 2 * 128 * D; }
 // The dK/dV split of a staged backward in one pass (one 128-key block per
 // workgroup and CU): the last round's blocks over ranges of query tiles.
 // (1,20,4096,128): 640 blocks, 2.5 rounds.
-FwdSplit dkv_f32_split_plan(int64_t blocks, int D) {
-  const TailSplit t = plan_tail_split(blocks, 256, kSplitSlots);
+// With changed scores (row_tiles > 0: the 32-row tiles of a query head) also every block of a grid of at most one round, into parts for two
+// rounds of at least 4 tiles each.
+FwdSplit dkv_f32_split_plan(int64_t blocks, int D, int64_t row_tiles = 0) {
+  TailSplit t = plan_tail_split(blocks, 256, kSplitSlots);
+  if (row_tiles > 0 && blocks <= 256) {
+    int64_t p = (512 + blocks - 1) / blocks;
+    p = p < 8 ? p : 8;
+    p = p < row_tiles / 4 ? p : row_tiles / 4;
+    if (p > 1) t = TailSplit{(int)blocks, (int)p};
+  }
   return FwdSplit{t.nsplit, t.nparts, (size_t)t.nsplit * t.nparts * dkv_f32_slot_floats(D) * sizeof(float)};
 }
 
@@ -1329,7 +1337,7 @@ void launch_bwd_f32(F32Args a, int pairs_per_pass, hipStream_t s) {
     const int np = pairs - p0 < pairs_per_pass ? pairs - p0 : pairs_per_pass;
     a.pair0 = p0;
     a.nblocks = nkb * np;
-    const FwdSplit sp = a.part ? dkv_f32_split_plan(a.nblocks, D) : FwdSplit{0, 0, 0};
+    const FwdSplit sp = a.part ? dkv_f32_split_plan(a.nblocks, D, SCORE ? (a.Lq + 31) / 32 : 0) : FwdSplit{0, 0, 0};
     a.nsplit = sp.nsplit, a.nparts = sp.nparts;
     const dim3 grid((unsigned)(a.nblocks - a.nsplit + a.nsplit * a.nparts));
     hipLaunchKernelGGL((bwd_dkdv_f32_kernel<D, true, WIN, SCORE>), grid, dim3(512), 0, s, a);
@@ -1356,6 +1364,10 @@ int check_f32_windows(const int32_t* lo, const int32_t* hi, int64_t batch_stride
 using namespace avattn;
 
 namespace avattn {
+
+size_t bwd_f32_split_bytes(int B, int Hq, int Hkv, int Lq, int Lk, int D) {
+  return dkv_f32_split_plan((int64_t)B * Hkv * ((Lk + 127) / 128), D, (Lq + 31) / 32).bytes;
+}
 
 size_t fwd_f32_split_bytes(int B, int Hq, int Lq, int Lk, int D) { return fwd_f32_split_plan(B, Hq, Lq, Lk, D).bytes; }
 
@@ -1571,7 +1583,7 @@ static int bwd_f32_entry(const float* dout, const float* q, const float* k, cons
       a.dsp = (int64_t)(per / sizeof(float));
       // One pass and room behind its dS: the parts of a split dK/dV round.
       const size_t end = off + (size_t)pairs * per;
-      const FwdSplit sp = dkv_f32_split_plan(pairs * ((len_k + 127) / 128), head_dim);
+      const FwdSplit sp = dkv_f32_split_plan(pairs * ((len_k + 127) / 128), head_dim, score ? (len_q + 31) / 32 : 0);
       if (pp == pairs && sp.nsplit > 0 && workspace_bytes >= end + sp.bytes)
         a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + end);
     }

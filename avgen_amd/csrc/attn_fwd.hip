@@ -116,7 +116,7 @@ static hipError_t launch_fwd_d(const FwdArgs& args, hipStream_t stream) {
   const bool small = !fp8 && use_small(a.B, a.Hq, a.Lq, a.Lk, D);
   const int bm = small ? 128 : 256;
   const int64_t blocks = (int64_t)((a.Lq + bm - 1) / bm) * a.B * a.Hq;
-  const FwdSplit sp = fwd_split_plan(a.B, a.Hq, a.Lq, a.Lk, D, fp8, a.wlo != nullptr);
+  const FwdSplit sp = fwd_split_plan(a.B, a.Hq, a.Lq, a.Lk, D, fp8, a.wlo != nullptr && a.score.mode == 0);
   if (a.part != nullptr) {
     a.nsplit = sp.nsplit;
     a.nparts = sp.nparts;

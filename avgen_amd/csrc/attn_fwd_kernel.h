@@ -35,6 +35,15 @@ __device__ __forceinline__ void row_state(float m, float l, float unit, float& i
   lse = l > 0.f ? fmaf(m, unit, logf(l)) : (l == 0.f ? kNegInf : nan);
 }
 
+// Row block `bid` of a call with changed scores and windows: causal and prefix
+// masks give the last rows the most keys, so the longest workgroups come
+// first, those of all the heads of an XCD before any of the next longest.
+__device__ __forceinline__ void row_block(const FwdArgs& a, int bid, int nqt, int& qt, int& bh) {
+  int rank;
+  longest_first(bid, nqt, a.B * a.Hq, rank, bh);
+  qt = nqt - 1 - rank;
+}
+
 // Writes one wave's 32 output rows row0 .. of (b, h) = bh: acc[dt][4*g + r] of
 // lane l is channel 32*dt + 8*g + 4*(l/32) + r of row l%32, times inv; lse
 // per lane row.
@@ -204,8 +213,17 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
     bid = nfull + i / a.nparts;
     part = i % a.nparts;
   }
-  const int qt = bid % nqt;
-  const int bh = bid / nqt;
+  int qt = bid % nqt, bh = bid / nqt;
+  if constexpr (SCORE && WIN) {
+    // In the order of row_block, the first parts of the split blocks before
+    // their second ones.
+    bid = blockIdx.x;
+    if (part >= 0) {
+      part = (bid - nfull) / a.nsplit;
+      bid = nfull + (bid - nfull) % a.nsplit;
+    }
+    row_block(a, bid, nqt, qt, bh);
+  }
   const int b = bh / a.Hq, h = bh % a.Hq;
   const int hk = h / (a.Hq / a.Hkv);
 
@@ -218,6 +236,9 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
   int wlo = 0, whi = a.Lkp, wlo_max = 0, whi_min = a.Lkp;
   int t0 = 0;
   int ntile = a.Lkp / BN;
+  // The tiles that meet this wave's rows (SMALL with changed scores, which
+  // leaves the others out: a wave has no part in another's work there).
+  int w_t0 = 0, w_t1 = ntile;
   if constexpr (WIN) {
     __shared__ int wred[NW][2];
     int rlo = 0x7fffffff, rhi = -1;  // range contribution (none for empty or past-the-end rows)
@@ -232,7 +253,9 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
     // The range is that of the aligned 256 rows around this workgroup's in
     // both workgroup sizes: which rows a NaN key reaches through 0 x NaN does
     // not depend on the size chosen.
-    const int urow = qt * BM / 256 * 256 + (SMALL ? tid : wave * 32 + l32);
+    // (Changed scores: those of its own rows alone, fewer tiles where documents
+    // meet.)
+    const int urow = SCORE ? qrow : qt * BM / 256 * 256 + (SMALL ? tid : wave * 32 + l32);
     if (urow < a.Lq) {
       const int ulo = min(max(a.wlo[b * a.wsb + urow], 0), a.Lk);
       const int uhi = min(max(a.whi[b * a.wsb + urow], ulo), a.Lk);
@@ -250,6 +273,10 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
     }
     wlo_max = __builtin_amdgcn_readfirstlane(mlo);
     whi_min = __builtin_amdgcn_readfirstlane(mhi);
+    if constexpr (SCORE && SMALL) {
+      w_t0 = __builtin_amdgcn_readfirstlane(rlo < rhi ? rlo / BN : 0);
+      w_t1 = __builtin_amdgcn_readfirstlane(rlo < rhi ? (rhi + BN - 1) / BN : 0);
+    }
     if (lane == 0) {
       wred[wave][0] = rlo;
       wred[wave][1] = rhi;
@@ -378,7 +405,12 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
   // The fp8 path bounds its log2-unit scores by 2^eq * |q8_row| * max_k |k8|
   // (the products of e4m3 values are exact; same margin) against a maximum
   // kept in log2 units.
-  constexpr float kBoundTau = 32.f;
+  constexpr float kBoundTau = SCORE ? 60.f : 32.f;
+  // With the cap alone the tile's scores are held as r = (1 - tanh) / 2, score
+  // cap2 - 2 cap2 r (a masked one: r infinite), one operation before exp2.
+  constexpr bool kAsComplement = SCORE == kScoreCap;
+  constexpr float kMasked = kAsComplement ? kPosInf : kNegInf;
+  const float capm2 = -2.f * a.score.cap2;
   // Distances run from this lane's query position.
   const int qpos = SCORE & kScoreDistance ? qrow + a.score.query_offset(b) : 0;
   const float slope2 = SCORE & kScoreDistance && a.score.slopes ? a.score.slopes[h] * kLog2e : 0.f;
@@ -455,6 +487,10 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
   // the log2-unit scores (fp8, where cneg holds -m_run in every register, 0
   // while m_run is -inf: the accumulator the q k^T products start from).
   float m_run = kNegInf;
+  if constexpr (kAsComplement) {
+    // Capped scores within +-2^kBoundTau of 1 need no maximum at all.
+    if (a.score.cap2 <= kBoundTau) m_run = 0.f, bounded = 1;
+  }
   f32x16 cneg = zero16();
   float l_run0 = 0.f, l_run1 = 0.f;  // this lane's share of the row sum
   f32x16 acc[DT];
@@ -580,10 +616,13 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
         for (int r = 0; r < 16; ++r) {
           float z;
           if constexpr (SCORE & kScoreCap)
-            z = fmaf(-2.f * a.score.cap2, cap_complement(s_cur[r], a.score.cap_arg), a.score.cap2);
+            z = cap_complement(s_cur[r], a.score.cap_arg);
           else
             z = s_cur[r] * a.scale_log2;
-          if constexpr (SCORE & kScoreDistance) z = fmaf(-slope2, fabsf(kd - (float)(16 * (r >> 3) + (r & 7))), z);
+          if constexpr (SCORE & kScoreDistance) {
+            if constexpr (SCORE & kScoreCap) z = fmaf(capm2, z, a.score.cap2);
+            z = fmaf(-slope2, fabsf(kd - (float)(16 * (r >> 3) + (r & 7))), z);
+          }
           s_cur[r] = z;
         }
       }
@@ -591,10 +630,21 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
         // Register 8*k2 + e holds key 64*t + 32*hf + 16*k2 + 8*hh + e.
         const int kh = BN * t + 32 * hf;
         if (kh < wlo_max || kh + 32 > whi_min) {
+          // Kept a branch: turned into selects, the compares would run for
+          // every tile (16 heads of 8,192 tokens, causal: 434 against 390 us).
+          if constexpr (SCORE != 0) {
+            __asm__ volatile("; a tile at an edge of the windows");
+            const int from = kh + 8 * hh - wlo;
+            const uint32_t span = whi - wlo;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = kh + 16 * (r >> 3) + 8 * hh + (r & 7);
-            if (key < wlo || key >= whi) s_cur[r] = kNegInf;
+            for (int r = 0; r < 16; ++r)
+              s_cur[r] = (uint32_t)(from + 16 * (r >> 3) + (r & 7)) < span ? s_cur[r] : kMasked;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int key = kh + 16 * (r >> 3) + 8 * hh + (r & 7);
+              if (key < wlo || key >= whi) s_cur[r] = kNegInf;
+            }
           }
         }
       }
@@ -605,7 +655,7 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if constexpr (SCORE != 0)
-              s_cur[4 * g + r] = bb[r] < 0.f ? kNegInf : s_cur[4 * g + r];
+              s_cur[4 * g + r] = bb[r] < 0.f ? kMasked : s_cur[4 * g + r];
             else
               s_cur[4 * g + r] += bb[r];
           }
@@ -614,8 +664,15 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
     }
     if (!bounded) {
       float mx = kNegInf;
+      if constexpr (kAsComplement) {
+        float mn = kPosInf;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(sh[0][r], sh[1][r]));
+        for (int r = 0; r < 16; ++r) mn = fminf(mn, fminf(sh[0][r], sh[1][r]));
+        mx = fmaf(capm2, mn, a.score.cap2);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(sh[0][r], sh[1][r]));
+      }
       mx = halves_max(mx);
       if (mx > m_run + tau) {
         // New reference max (both lanes of a query agree: mx is shared).
@@ -630,7 +687,9 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
       }
       bounded = __all((bound - m_run) * c <= kBoundTau);
     }
-    const float mc = (m_run == kNegInf) ? 0.f : m_run * c;
+    float mc = (m_run == kNegInf) ? 0.f : m_run * c;
+    float pc = c;  // the probabilities are exp2(pc * sh - mc)
+    if constexpr (kAsComplement) pc = capm2, mc -= a.score.cap2;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -639,8 +698,8 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
 #pragma unroll
         for (int e2 = 0; e2 < 4; ++e2) {
           const int r = 8 * k2 + 2 * e2;
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sh[hf][r], c, -mc));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sh[hf][r + 1], c, -mc));
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sh[hf][r], pc, -mc));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(sh[hf][r + 1], pc, -mc));
           if (e2 & 1)
             l_run1 += p0 + p1;
           else
@@ -722,6 +781,13 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
       barrier_lds();     // ... for every wave, and tile t - 1's stage is free
       const Stage& sg = stage_ref(bufc);
       const int tl = min(t + 1, tend - 1);
+      if constexpr (SCORE && WIN) {
+        if (t < w_t0 || t >= w_t1) {
+#pragma unroll
+          for (int i = 0; i < kStageOps; ++i) stage_op(tl, Next(), i);
+          return;
+        }
+      }
       __builtin_amdgcn_s_setprio(2);
       scores(sg, sh, loads_in(tl, Next()));
       loads_after(tl, Next(), 2 * KS);
@@ -894,14 +960,16 @@ __global__ __launch_bounds__(256) void fwd_combine_kernel(FwdArgs a, float c, fl
   const int s = u / (BM / 32), w = u % (BM / 32);
   const int nqt = (a.Lq + BM - 1) / BM;
   const int bid = nqt * a.B * a.Hq - a.nsplit + s;
-  const int row0 = bid % nqt * BM + w * 32;
+  int qt = bid % nqt, bh = bid / nqt;
+  if (a.score.mode != 0 && a.wlo != nullptr) row_block(a, bid, nqt, qt, bh);
+  const int row0 = qt * BM + w * 32;
   const float* slot = a.part + (int64_t)s * a.nparts * fwd_slot_floats(BM, D) + (int64_t)w * fwd_slot_floats(32, D);
   float m, l;
   f32x16 acc[DT];
   combine_parts<D>(slot, fwd_slot_floats(BM, D), a.nparts, c, acc, m, l);
   float inv, lse;
   row_state(m, l, unit, inv, lse);
-  write_rows<D>(a, acc, inv, lse, ep[wave], bid / nqt, row0);
+  write_rows<D>(a, acc, inv, lse, ep[wave], bh, row0);
 }
 
 }  // namespace avattn

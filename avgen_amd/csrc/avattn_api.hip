@@ -289,7 +289,8 @@ int fwd_impl(const void* q, const void* k, const void* v, const int64_t* q_strid
   a.wsb = window_batch_stride;
   // A workspace of avattn_fwd_split_workspace_size bytes holds the parts of a
   // split last round; a smaller one runs the unsplit grid.
-  const size_t split = fwd_split_plan(batch, heads_q, len_q, len_k, head_dim, fp8, window_lo != nullptr).bytes;
+  const size_t split =
+      fwd_split_plan(batch, heads_q, len_q, len_k, head_dim, fp8, window_lo != nullptr && !score).bytes;
   if (split > 0 && workspace_bytes >= wl.total + split) a.part = reinterpret_cast<float*>(ws + wl.total);
   if (ring) {
     a.cos_k = ring->cos_k;
@@ -423,9 +424,9 @@ size_t avattn_bwd_staged_workspace_size(int32_t batch, int32_t heads_q, int32_t 
 
 namespace {
 // Bytes of the parts of a dK/dV grid with every block split (0: not split).
-size_t dkv_split_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D) {
+size_t dkv_split_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool windows = false) {
   const TailSplit t = dkv_split_plan((int64_t)B * Hkv * ((Lk + 127) / 128),
-                                     (int)(transpose_padded_len(Lq) / 64 * (Hq / Hkv)), D);
+                                     (int)(transpose_padded_len(Lq) / 64 * (Hq / Hkv)), D, windows);
   return (size_t)t.nsplit * t.nparts * 256 * D * sizeof(float);
 }
 }  // namespace
@@ -596,14 +597,17 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
     kv_per_pass = (int)(((size_t)a.nkv + npass - 1) / npass);
     a.ds = reinterpret_cast<bf16*>(ws + off);
     set_hull(a, ws, wl);
-    // One pass, no windows and room behind its dS: the parts of a split of
-    // every dK/dV block.
-    const size_t split = dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim);
+    // One pass, no windows (or changed scores) and room behind its dS: the
+    // parts of a split of every dK/dV block.
+    const size_t split = dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, window_lo != nullptr);
     const size_t end = off + (size_t)a.nkv * per;
-    if (kv_per_pass == a.nkv && !window_lo && split > 0 && workspace_bytes >= end + split)
+    if (kv_per_pass == a.nkv && (!window_lo || (score && !compact)) && split > 0 && workspace_bytes >= end + split)
       a.split_all = reinterpret_cast<float*>(ws + end);
   }
-  if (score) a.score = *score;
+  if (score) {
+    a.score = *score;
+    if (score->mode & kScoreCap) a.scale *= 4.f;  // of 1 - tanh^2 (BwdArgs::score)
+  }
   return launch_status(launch_bwd(a, head_dim, kv_per_pass, s));
 }
 
@@ -1156,6 +1160,18 @@ size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t 
   const size_t hull = round256((size_t)batch * 2 * sizeof(int));
   if (is_f32) return round256(fwd_f32_split_bytes(batch, heads_q, len_q, len_k, head_dim)) + hull;
   return avattn_fwd_split_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, 0) + hull;
+}
+
+size_t avattn_bwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len_q,
+                                        int32_t len_k, int32_t head_dim, int32_t is_f32, int32_t windowed) {
+  if (check_bwd_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim) != AVATTN_OK) return 0;
+  if ((int64_t)batch * heads_q * len_q == 0 || len_k == 0) return 0;
+  const int32_t pairs = batch * heads_kv;
+  if (is_f32)
+    return avattn_bwd_f32_staged_workspace_size(batch, heads_q, heads_kv, len_q, len_k, pairs) +
+           bwd_f32_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim);
+  return avattn_bwd_staged_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, pairs) +
+         dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, windowed != 0);
 }
 
 int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t* q_strides, const int64_t* k_strides,

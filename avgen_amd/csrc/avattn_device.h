@@ -257,6 +257,22 @@ __device__ __forceinline__ int xcd_remap(int bid, int total) {
   return xcd * per + (xcd < rem ? xcd : rem) + local;
 }
 
+// Blocks of differing lengths, `per` of each of `pairs` heads, block 0 of a
+// head the longest: workgroup bid takes block `rank` of head `pair`.  Each XCD
+// keeps whole heads where they divide by 8 and runs their blocks in order of
+// rank, so that short blocks fill the end of the grid.
+__device__ __forceinline__ void longest_first(int bid, int per, int pairs, int& rank, int& pair) {
+  constexpr int kXcds = 8;
+  if (pairs % kXcds == 0) {
+    const int own = pairs / kXcds, local = bid / kXcds;
+    pair = bid % kXcds * own + local % own;
+    rank = local / own;
+  } else {
+    pair = bid % pairs;
+    rank = bid / pairs;
+  }
+}
+
 // xcd_remap for calls with a key mask: whole (batch, kv head) pairs of `per`
 // blocks still stay on one XCD, but XCD x takes pairs x, x + 8, ..., so that a
 // batch row with few attended keys leaves no XCD idle.  Needs total = pairs *

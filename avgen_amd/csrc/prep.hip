@@ -297,7 +297,8 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(BwdArgs a, int nk, int nq
     const int i = i0 + r * RPB;
     if (i < a.Lqp && c == 0) {
       a.ndelta[(int64_t)bh * a.Lqp + i] = -acc;
-      a.lse2[(int64_t)bh * a.Lqp + i] = (l[r] == kNegInf) ? kPosInf : l[r] * kLog2e;
+      a.lse2[(int64_t)bh * a.Lqp + i] =
+          (l[r] == kNegInf) ? kPosInf : (DROP ? fmaf(l[r], kLog2e, -a.score.cap2) : l[r] * kLog2e);
     }
   }
 }

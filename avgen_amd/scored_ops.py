@@ -118,19 +118,23 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
     return out, lse
 
 
-def _f32_workspace(B, Hq, Hkv, Lq, Lk, D, device) -> torch.Tensor:
-    """The float32 backward's workspace with staged dS: as many (batch, kv
-    head) pairs per pass as the budget and the allocator have, at least one."""
+def _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, windowed, device) -> torch.Tensor:
+    """The backward's workspace with (dense) staged dS: as many (batch, kv
+    head) pairs per pass as the budget and the allocator have, at least one;
+    with all of them in one pass also room for a split grid."""
     lib = _lib.load()
     total = B * Hkv
-    per = f32_ds_bytes_per_pair(Hq // Hkv, Lq, Lk)
+    per = (f32_ds_bytes_per_pair if f32 else ds_bytes_per_pair)(Hq // Hkv, Lq, Lk)
     pairs = max(1, min(total, _ds_budget(device) // per))
     pairs = -(-total // -(-total // pairs))
     while True:
-        staged = lib.avattn_bwd_f32_staged_workspace_size(B, Hq, Hkv, Lq, Lk, int(pairs))
+        if f32:
+            staged = lib.avattn_bwd_f32_staged_workspace_size(B, Hq, Hkv, Lq, Lk, int(pairs))
+        else:
+            staged = lib.avattn_bwd_staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, int(pairs))
         try:
             if pairs == total:
-                split = lib.avattn_bwd_f32_split_workspace_size(B, Hq, Hkv, Lq, Lk, D)
+                split = lib.avattn_bwd_scored_workspace_size(B, Hq, Hkv, Lq, Lk, D, int(f32), int(windowed))
                 return _one_pass_workspace(split, staged, int(pairs) * per, device)
             return _workspace(staged, device)
         except torch.OutOfMemoryError:
@@ -170,18 +174,13 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
     table, tsb, units = None, 0, 0
     if 0 in (B, Hq, Lq, Lk):
         ws = _workspace(0, q.device)
-    elif f32:
-        ws = _f32_workspace(B, Hq, Hkv, Lq, Lk, D, q.device)
-    elif lo is None:
-        ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, q.device, stage_ds=True)
+    elif (not f32 and lo is not None and B * Hkv * ds_bytes_per_pair(Hq // Hkv, Lq, Lk) > _ds_budget(q.device)
+            and not torch.cuda.is_current_stream_capturing()):
+        table, units = compact_ds_table(lo, hi, Lq, Lk)
+        tsb = 0 if table.shape[0] == 1 else table.shape[1]
+        ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, q.device, stage_ds=True, ds_units=units)
     else:
-        dense = B * Hkv * ds_bytes_per_pair(Hq // Hkv, Lq, Lk)
-        if dense > _ds_budget(q.device) and not torch.cuda.is_current_stream_capturing():
-            table, units = compact_ds_table(lo, hi, Lq, Lk)
-            tsb = 0 if table.shape[0] == 1 else table.shape[1]
-            ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, q.device, stage_ds=True, ds_units=units)
-        else:
-            ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, q.device, stage_ds=True, windows=True)
+        ws = _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, lo is not None, q.device)
     with _on(q.device):
         st = lib.avattn_bwd_scored(
             _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),

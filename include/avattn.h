@@ -962,11 +962,11 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * workspace: avattn_fwd_scored_workspace_size bytes, 16-byte aligned.
  *
  * Backward: windows non-decreasing in the row, dS always staged.  workspace:
- * bf16, the sizes of avattn_bwd with AVATTN_BWD_STAGE_DS
- * (avattn_bwd_staged_workspace_size, avattn_bwd_split_workspace_size without
- * windows), or with a ds_table (and windows) as avattn_bwd_windowed_compact;
- * float32, avattn_bwd_f32_staged_workspace_size or
- * avattn_bwd_f32_split_workspace_size, 256-byte aligned.
+ * bf16, avattn_bwd_staged_workspace_size, or with a ds_table (and windows) as
+ * avattn_bwd_windowed_compact; float32, avattn_bwd_f32_staged_workspace_size,
+ * 256-byte aligned.  With avattn_bwd_scored_workspace_size (every (batch, kv
+ * head) pair in one pass; no ds_table) the call also splits a short grid, dk
+ * and dv then being sums of fp32 parts in a fixed order.
  */
 #define AVATTN_SCORED_SORTED_WINDOWS 1u
 
@@ -974,6 +974,11 @@ size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q,
                                         int32_t heads_kv, int32_t len_q,
                                         int32_t len_k, int32_t head_dim,
                                         int32_t is_f32);
+
+size_t avattn_bwd_scored_workspace_size(int32_t batch, int32_t heads_q,
+                                        int32_t heads_kv, int32_t len_q,
+                                        int32_t len_k, int32_t head_dim,
+                                        int32_t is_f32, int32_t windowed);
 
 int avattn_fwd_scored(const void* q, const void* k, const void* v,
                       const int64_t* q_strides, const int64_t* k_strides,

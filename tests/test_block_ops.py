@@ -111,5 +111,6 @@ def test_c_entry_points_refuse():
     assert back(dw=None) == 1 and back(dn=None) == 1 and back(dx=None) == 1 and back(h=p + 1) == 5
     assert back(ws=None) == 6 and back(nb=4 * 64 * 4 - 1) == 6 and back(ws=p + 4) == 6
     assert lib.avattn_add_rms_norm_bwd_workspace_size(3, 64) == 4 * 64 * 4
-    assert lib.avattn_add_rms_norm_bwd_workspace_size(5000, 64) == 1024 * 64 * 4
+    assert lib.avattn_add_rms_norm_bwd_workspace_size(5000, 64) == 4096 * 64 * 4
+    assert lib.avattn_add_rms_norm_bwd_workspace_size(5000, 1025) == 1024 * 1025 * 4
     assert lib.avattn_add_rms_norm_bwd_workspace_size(5, 0) == 0
