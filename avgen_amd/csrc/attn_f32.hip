@@ -85,29 +85,6 @@ struct LiveKeys {
   }
 };
 
-// A changed score in log2 units from a raw one (uniform mode); kd: the row's
-// position minus the key; f = 1 - tanh^2 (1 without a cap).  tanh to a few
-// units in the last place, small arguments too: below 0.35 its odd series to
-// x^11 (the next term is below 2^-26), above it 1 - 2 r with r = 1 / (1 +
-// e^2|x|), and then 1 - tanh^2 = 4 r (1 - r).
-__device__ __forceinline__ float changed_score(const F32Args& a, float s, float kd, float slope2, float& f) {
-  float z = s * a.c;
-  f = 1.f;
-  if (a.score.mode & kScoreCap) {
-    const float x = s * a.score.cap_x, x2 = x * x, ax = fabsf(x);
-    const float series =
-        x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -8.8632355e-3f, 2.1869488e-2f), -5.3968254e-2f), 1.3333334e-1f),
-                          -3.3333334e-1f),
-                 1.f);
-    const float r = cap_complement(ax, 2.f * kLog2e);
-    const bool small = ax < 0.35f;
-    const float t = small ? series : copysignf(fmaf(-2.f, r, 1.f), x);
-    f = small ? fmaf(-t, t, 1.f) : 4.f * r * (1.f - r);
-    z = a.score.cap2 * t;
-  }
-  return fmaf(-slope2, fabsf(kd), z);
-}
-
 // The block a workgroup takes of a grid of `total` blocks whose last nsplit
 // are split, and which part of it (-1: all).
 __device__ __forceinline__ void split_block(const F32Args& a, int total, int& bid, int& part) {
@@ -332,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
       for (int r = 0; r < 4; ++r) {
         if constexpr (SCORE) {
           float f;
-          const float z = changed_score(a, s[4 * g + r], (float)(qpos - (t * KT + 8 * g + 4 * hh + r)), slope2, f);
+          const float z = changed_score_exact(a.score, s[4 * g + r], a.c, (float)(qpos - (t * KT + 8 * g + 4 * hh + r)), slope2, f);
           s[4 * g + r] = bb[r] < 0.f ? kNegInf : z;
         } else {
           s[4 * g + r] += bb[r];
@@ -688,7 +665,7 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
             if constexpr (SCORE) {
               float f;
               const float kd = (float)(t * QT + 8 * g + 4 * hh + r + qoff - key);
-              const float z = changed_score(a, s[4 * g + r], kd, slope2, f);
+              const float z = changed_score_exact(a.score, s[4 * g + r], a.c, kd, slope2, f);
               w[4 * g + r] = in ? __builtin_amdgcn_exp2f(z - L[r]) : 0.f;
               hand[r] = in ? w[4 * g + r] * f : 0.f;
             } else {

@@ -13,7 +13,8 @@
 // are those of the general forward (S^T = K Q^T, O^T += V^T P^T on 32x32x16
 // MFMAs, P in registers); with fewer than 32 rows the matrix pipe works on
 // empty columns, for which it has time: a tile's 16 KB take longer to arrive
-// than its MFMAs to run.
+// than its MFMAs to run.  One token against 205 MB of bf16 cache (D 128, 16
+// kv heads): 36 us, 5.7 TB/s, and 4 us to combine.
 #include "avattn_device.h"
 #include "avattn_kernels.h"
 
@@ -22,11 +23,6 @@ namespace avattn {
 namespace {
 
 constexpr int kWaves = 4, kTile = 32;
-
-// The state of one row over some keys.
-struct RowPart {
-  float m, l;
-};
 
 __device__ __forceinline__ float part_weight(float m, float top) {
   return m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
@@ -88,6 +84,59 @@ __device__ __forceinline__ float changed_score(const FewArgs& a, float s, float 
   return fmaf(-slope2, fabsf(kd), z);
 }
 
+// What the waves of a workgroup leave of their rows, to be joined.
+template <int D, int ROWS>
+struct Join {
+  static constexpr int kPitch = D + 4;
+  float o[kWaves][ROWS * kPitch];
+  float m[kWaves][ROWS], l[kWaves][ROWS];
+};
+
+// The waves' parts of the block's rows, in order: to the rows themselves, or to
+// the workgroup's slot.  Every thread; the waves have written jn.
+template <int D, class T, int ROWS>
+__device__ __forceinline__ void join_waves(const FewArgs& a, const Join<D, ROWS>& jn, int unit, int split, int rows) {
+  const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
+  const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
+  constexpr int CPR = D / 8;  // threads per row, 8 channels each
+  for (int u = threadIdx.x; u < rows * CPR; u += 64 * kWaves) {
+    const int r = u / CPR, ch = 8 * (u % CPR);
+    float top = kNegInf;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) top = fmaxf(top, jn.m[v][r]);
+    float sum = 0.f, o[8] = {};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float wt = part_weight(jn.m[v][r], top);
+      sum = fmaf(jn.l[v][r], wt, sum);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(jn.o[v][r * jn.kPitch + ch + e], wt, o[e]);
+    }
+    if (a.nsplit > 1) {
+      float* part = a.part + ((int64_t)unit * a.nsplit + split) * few_slot_floats(a.block_rows, D);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(part + r * D + ch + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+      if (ch == 0) part[a.block_rows * D + 2 * r] = top, part[a.block_rows * D + 2 * r + 1] = sum;
+    } else {
+      float inv, lse;
+      finish_row(top, sum, inv, lse);
+      const RowPlace p = row_place(a, hk, rb * ROWS + r);
+      T* out = static_cast<T*>(a.o) + b * a.osb + p.h * a.osh + (int64_t)p.i * a.osl + ch;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= inv;
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<u32x4*>(out) = u32x4{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
+                                               pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])};
+      } else {
+        *reinterpret_cast<f32x4*>(out) = f32x4{o[0], o[1], o[2], o[3]};
+        *reinterpret_cast<f32x4*>(out + 4) = f32x4{o[4], o[5], o[6], o[7]};
+      }
+      if (ch == 0) a.lse[((int64_t)b * a.Hq + p.h) * a.Lq + p.i] = lse;
+    }
+  }
+}
+
 template <int D>
 __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
   constexpr int KS = D / 16, DT = D / 32, TE = kTile * D;
@@ -95,14 +144,9 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
     bf16 k[TE];  // K rows: TileLayout<D>
     bf16 v[TE];  // V rows: TileLayout<D>
   };
-  constexpr int kRowPitch = D + 4;  // floats per row of a wave's output at the end
-  struct Join {
-    float o[kWaves][kTile * kRowPitch];
-    float m[kWaves][kTile], l[kWaves][kTile];
-  };
   __shared__ __attribute__((aligned(16))) union Smem {
     Stage st[kWaves][2];
-    Join join;
+    Join<D, kTile> join;
   } sm;
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -246,45 +290,178 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
   // Join the waves: each leaves its rows' maxima, sums and outputs.
   l = halves_sum(l);
   __syncthreads();  // every wave is done with its stages
-  Join& jn = sm.join;
+  auto& jn = sm.join;
   if (hh == 0) jn.m[wave][l32] = m, jn.l[wave][l32] = l;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<f32x4*>(&jn.o[wave][l32 * kRowPitch + 32 * dt + 8 * g + 4 * hh]) =
+      *reinterpret_cast<f32x4*>(&jn.o[wave][l32 * jn.kPitch + 32 * dt + 8 * g + 4 * hh]) =
           f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
   __syncthreads();
-  constexpr int CPR = D / 8;  // threads per row, 8 channels each
-  for (int u = tid; u < rows * CPR; u += 256) {
-    const int r = u / CPR, ch = 8 * (u % CPR);
-    float top = kNegInf;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) top = fmaxf(top, jn.m[v][r]);
-    float sum = 0.f, o[8] = {};
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      const float wt = part_weight(jn.m[v][r], top);
-      sum = fmaf(jn.l[v][r], wt, sum);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = fmaf(jn.o[v][r * kRowPitch + ch + e], wt, o[e]);
+  join_waves<D, bf16>(a, jn, unit, split, rows);
+}
+
+// float32, RB rows at a time on the vector ALUs (the fp32 matrix instructions
+// would multiply 32 rows whatever their number, and take longer than a tile's
+// 32 KB to arrive): 268 MB of cache in 46 us with one row per kv head, 5.8
+// TB/s, 55 us with 4; every 4 more rows read K and V again from the caches,
+// about 39 us.  Scores: lane l owns key l % 32 of the wave's tile and half
+// of the channels, K from LDS (staged as above, rows of 256 bytes), q by
+// broadcast reads.  P V: a lane owns D / 64 channels, V's rows come straight
+// from memory a tile ahead (whole rows per load), p_j by readlane.
+template <int D, int RB>
+__global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
+  constexpr int HD = D / 2, CL = D / 64, NS = D / 64;  // channels per lane in P V; 64-channel K sub-tiles
+  using vrow = std::conditional_t<CL == 2, f32x2, float>;
+  __shared__ __attribute__((aligned(16))) union Smem {
+    bf16 k[kWaves][2][NS][kTile * 128];  // 64 floats per row: TileLayout<128>
+    Join<D, RB> join;
+  } sm;
+  __shared__ __attribute__((aligned(16))) float sq[RB][D];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int unit = blockIdx.x / a.nsplit, split = blockIdx.x % a.nsplit;
+  const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
+  const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
+  const int rows = min(a.Lq * (a.Hq / a.Hkv) - rb * RB, RB);
+  const bool valid = l32 < rows;
+  const RowPlace rp = row_place(a, hk, rb * RB + (valid ? l32 : 0));
+  const BlockWindows w = block_windows(a, b, rp.i, valid);
+  // Row r's values are lane r's.
+  const int qpos = rp.i + a.score.query_offset(b);
+  const float slope2 = a.score.slopes != nullptr ? a.score.slopes[rp.h] * kLog2e : 0.f;
+  for (int u = tid; u < RB * (D / 4); u += 256) {
+    const int r = u / (D / 4), c = 4 * (u % (D / 4));
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (r < rows) {
+      const RowPlace p = row_place(a, hk, rb * RB + r);
+      x = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + b * a.qsb + p.h * a.qsh +
+                                          (int64_t)p.i * a.qsl + c);
     }
-    if (a.nsplit > 1) {
-      float* part = a.part + ((int64_t)unit * a.nsplit + split) * few_slot_floats(a.block_rows, D);
+    *reinterpret_cast<f32x4*>(&sq[r][c]) = x;
+  }
+  __syncthreads();
+
+  const int tile0 = w.glo / kTile, ntile = w.ghi > w.glo ? (w.ghi + kTile - 1) / kTile - tile0 : 0;
+  const int t0 = tile0 + (int)((int64_t)ntile * split / a.nsplit) + wave;
+  const int t1 = tile0 + (int)((int64_t)ntile * (split + 1) / a.nsplit);
+  const float* kp = static_cast<const float*>(a.k) + b * a.ksb + hk * a.ksh;
+  const float* vp = static_cast<const float*>(a.v) + b * a.vsb + hk * a.vsh + CL * lane;
+  TileStager<kTile, 128, 1> kst;  // in 2-byte units
+  kst.init(2 * a.ksl, 0, lane);
+  vrow vn[kTile];
+  auto stage = [&](int t, int buf) {
+    const int last = min(a.Lk - 1 - t * kTile, kTile - 1);
+    const float* base = kp + (int64_t)t * kTile * a.ksl;
 #pragma unroll
-      for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<f32x4*>(part + r * D + ch + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
-      if (ch == 0) part[a.block_rows * D + 2 * r] = top, part[a.block_rows * D + 2 * r + 1] = sum;
-    } else {
-      float inv, lse;
-      finish_row(top, sum, inv, lse);
-      const RowPlace p = row_place(a, hk, rb * kTile + r);
-      *reinterpret_cast<u32x4*>(static_cast<bf16*>(a.o) + b * a.osb + p.h * a.osh + (int64_t)p.i * a.osl + ch) =
-          u32x4{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
-                pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv)};
-      if (ch == 0) a.lse[((int64_t)b * a.Hq + p.h) * a.Lq + p.i] = lse;
+    for (int h = 0; h < NS; ++h)
+      kst.stage(sm.k[wave][buf][h], make_rsrc(base + 64 * h, (uint32_t)((last * a.ksl + 64) * 4)), 0u);
+#pragma unroll
+    for (int j = 0; j < kTile; ++j)  // rows past the end read the last one again: their p is 0
+      vn[j] = *reinterpret_cast<const vrow*>(vp + (int64_t)(t * kTile + min(j, last)) * a.vsl);
+  };
+  auto key_live = [&](int t) {
+    const int key = t * kTile + l32;
+    bool ok = key >= w.glo && key < w.ghi;
+    if (a.mask != nullptr && ok) ok = a.mask[b * a.msb + key] != 0;
+    return (int)ok;
+  };
+
+  float m[RB], l[RB];
+  float acc[RB][CL];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    m[r] = kNegInf, l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < CL; ++e) acc[r][e] = 0.f;
+  }
+  retire_prologue_loads();
+  int live = 0;
+  if (t0 < t1) {
+    live = key_live(t0);
+    stage(t0, 0);
+  }
+  for (int t = t0, buf = 0; t < t1; t += kWaves, buf ^= 1) {
+    wait_vmem_n<0>();  // this tile's K, V and key mask
+    const uint32_t keys = (uint32_t)__builtin_amdgcn_ballot_w64(opaque(live) != 0);
+    vrow v[kTile];
+#pragma unroll
+    for (int j = 0; j < kTile; ++j) v[j] = vn[j];
+    if (t + kWaves < t1) {
+      // The other stage's reads have returned before it is filled again.
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      live = key_live(t + kWaves);
+      stage(t + kWaves, buf ^ 1);
+    }
+    if (keys != 0xffffffffu) {
+      // (see attn_few_kernel)
+#pragma unroll
+      for (int j = 0; j < kTile; ++j)
+        if (!(keys >> j & 1)) v[j] = vrow{};
+    }
+    float s[RB] = {};
+    const bf16* kr = sm.k[wave][buf][NS == 2 ? hh : 0];
+#pragma unroll
+    for (int c = 0; c < HD / 4; ++c) {
+      const f32x4 k4 = *reinterpret_cast<const f32x4*>(kr + TileLayout<128>::off(l32, 8 * (NS == 2 ? c : hh * HD / 4 + c)));
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const f32x4 q4 = *reinterpret_cast<const f32x4*>(&sq[r][hh * HD + 4 * c]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r] = fmaf(k4[e], q4[e], s[r]);
+      }
+    }
+    const int key = t * kTile + l32;
+    const bool live_key = keys >> l32 & 1;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int lo = __builtin_amdgcn_readlane(w.lo, r), hi = __builtin_amdgcn_readlane(w.hi, r);
+      const int pos = __builtin_amdgcn_readlane(qpos, r);
+      const float sl = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(slope2), r));
+      float f;
+      float z = changed_score_exact(a.score, halves_sum(s[r]), a.scale_log2, (float)(pos - key), sl, f);
+      if (!live_key || key < lo || key >= hi) z = kNegInf;
+      if (__builtin_amdgcn_ballot_w64(z > m[r] + 8.f) != 0) {  // rare after the first tiles
+        float mx = z;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+        const float alpha = m[r] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[r] - mx);
+        l[r] *= alpha;
+#pragma unroll
+        for (int e = 0; e < CL; ++e) acc[r][e] *= alpha;
+        m[r] = mx;
+      }
+      const float p = __builtin_amdgcn_exp2f(z - (m[r] == kNegInf ? 0.f : m[r]));
+      l[r] += p;
+#pragma unroll
+      for (int j = 0; j < kTile; ++j) {
+        const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
+        if constexpr (CL == 2) {
+          acc[r][0] = fmaf(pj, v[j][0], acc[r][0]);
+          acc[r][1] = fmaf(pj, v[j][1], acc[r][1]);
+        } else {
+          acc[r][0] = fmaf(pj, v[j], acc[r][0]);
+        }
+      }
     }
   }
+
+  __syncthreads();  // every wave is done with its stages
+  auto& jn = sm.join;
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    float sum = l[r];  // both halves hold the same keys' shares
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    if (lane == 0) jn.m[wave][r] = m[r], jn.l[wave][r] = sum;
+#pragma unroll
+    for (int e = 0; e < CL; ++e) jn.o[wave][r * jn.kPitch + CL * lane + e] = acc[r][e];
+  }
+  __syncthreads();
+  join_waves<D, float>(a, jn, unit, split, rows);
 }
 
 // The parts of one row, in order: a workgroup of 256 threads takes one row;
@@ -297,6 +474,7 @@ __global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
   const int unit = blockIdx.x / a.block_rows, r = blockIdx.x % a.block_rows;
   const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
   const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
+  // (With one block of rows block_rows is their number, else a full block's.)
   if (rb * a.block_rows + r >= a.Lq * (a.Hq / a.Hkv)) return;  // the whole workgroup
   const int64_t slot = few_slot_floats(a.block_rows, D);
   const float* part = a.part + (int64_t)unit * a.nsplit * slot;
@@ -342,14 +520,34 @@ __global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
   if (ch == 0) a.lse[((int64_t)b * a.Hq + rp.h) * a.Lq + rp.i] = lse;
 }
 
+template <int D>
+void launch_few_f32(const FewArgs& a, dim3 grid, hipStream_t stream) {
+  const int rows = a.Lq * (a.Hq / a.Hkv);
+  if (rows == 1)
+    hipLaunchKernelGGL((attn_few_f32_kernel<D, 1>), grid, dim3(256), 0, stream, a);
+  else if (rows == 2)
+    hipLaunchKernelGGL((attn_few_f32_kernel<D, 2>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attn_few_f32_kernel<D, 4>), grid, dim3(256), 0, stream, a);
+}
+
 }  // namespace
 
-FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D) {
+FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D, bool f32) {
   FewPlan p{};
   const int64_t rows = (int64_t)Lq * (Hq / Hkv);
-  if (rows > kFewRows || Lk < 1) return p;
-  p.block_rows = (int)(rows < kTile ? rows : kTile);
-  p.row_blocks = (int)((rows + kTile - 1) / kTile);
+  // How many query rows are few: a block's time grows with the rows of its kv
+  // head, the general forward's with the heads.  8 sequences of 4,096 keys, 8
+  // kv heads of D 128, capped scores, this path against the general one (at
+  // one more query): bf16, 32 queries 51 / 122 us in groups of two heads,
+  // 83 / 171 of 4, 213 / 533 of 16, and 64 queries of single heads 51 / 93;
+  // float32, 16 queries 171 / 178 us of single heads, 523 / 648 in groups of
+  // 4, 1,035 / 1,242 of 8.  With fewer pairs or keys the distance grows.
+  if ((f32 ? Lq > kFewQueriesF32 : Lq > kFewQueries && rows > kFewRows) || Lk < 1) return p;
+  // Rows of a block: up to a tile's 32; float32 up to 4 (those of 8 spill).
+  const int most_rows = f32 ? 4 : kTile;
+  p.block_rows = (int)(rows < most_rows ? rows : most_rows);
+  p.row_blocks = (int)((rows + most_rows - 1) / most_rows);
   const int64_t units = (int64_t)B * Hkv * p.row_blocks;
   // Workgroups the chip holds at once: one per CU at D 128 (LDS), two at 64.
   const int64_t slots = D == 128 ? 256 : 512;
@@ -372,7 +570,7 @@ FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D) {
 
 hipError_t launch_few(const FewArgs& args, int D, bool f32, hipStream_t stream) {
   FewArgs a = args;
-  const FewPlan p = few_plan(a.B, a.Hq, a.Hkv, a.Lq, a.Lk, D);
+  const FewPlan p = few_plan(a.B, a.Hq, a.Hkv, a.Lq, a.Lk, D, f32);
   a.nsplit = p.nsplit;
   a.row_blocks = p.row_blocks;
   a.block_rows = p.block_rows;
@@ -380,7 +578,11 @@ hipError_t launch_few(const FewArgs& args, int D, bool f32, hipStream_t stream) 
   {
     LaunchTimer timer(kKidFwdFew, stream);
     const dim3 grid(units * p.nsplit);
-    if (D == 128)
+    if (f32 && D == 128)
+      launch_few_f32<128>(a, grid, stream);
+    else if (f32)
+      launch_few_f32<64>(a, grid, stream);
+    else if (D == 128)
       hipLaunchKernelGGL(attn_few_kernel<128>, grid, dim3(256), 0, stream, a);
     else
       hipLaunchKernelGGL(attn_few_kernel<64>, grid, dim3(256), 0, stream, a);
@@ -388,7 +590,11 @@ hipError_t launch_few(const FewArgs& args, int D, bool f32, hipStream_t stream) 
   if (p.nsplit > 1) {
     LaunchTimer timer(kKidMerge, stream);
     const dim3 grid(units * p.block_rows);
-    if (D == 128)
+    if (f32 && D == 128)
+      hipLaunchKernelGGL((few_combine_kernel<128, true>), grid, dim3(256), 0, stream, a);
+    else if (f32)
+      hipLaunchKernelGGL((few_combine_kernel<64, true>), grid, dim3(256), 0, stream, a);
+    else if (D == 128)
       hipLaunchKernelGGL((few_combine_kernel<128, false>), grid, dim3(256), 0, stream, a);
     else
       hipLaunchKernelGGL((few_combine_kernel<64, false>), grid, dim3(256), 0, stream, a);

@@ -1144,7 +1144,7 @@ int score_args(float scale, float softcap, const float* slopes, const int32_t* o
 }
 
 bool takes_few(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool f32) {
-  return !f32 && few_plan(B, Hq, Hkv, Lq, Lk, D).nsplit > 0;
+  return few_plan(B, Hq, Hkv, Lq, Lk, D, f32).nsplit > 0;
 }
 
 }  // namespace
@@ -1156,7 +1156,7 @@ size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t 
   if (check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim) != AVATTN_OK) return 0;
   if ((int64_t)batch * heads_q * len_q == 0 || len_k == 0) return 0;
   if (takes_few(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0))
-    return few_plan(batch, heads_q, heads_kv, len_q, len_k, head_dim).bytes;
+    return few_plan(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0).bytes;
   const size_t hull = round256((size_t)batch * 2 * sizeof(int));
   if (is_f32) return round256(fwd_f32_split_bytes(batch, heads_q, len_q, len_k, head_dim)) + hull;
   return avattn_fwd_split_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, 0) + hull;

@@ -32,6 +32,30 @@ __device__ __forceinline__ float cap_complement(float s, float arg) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * arg));
 }
 
+// The float32 kernels' changed score, in log2 units, from a raw one; kd: the row's
+// position minus the key; f = 1 - tanh^2 (1 without a cap).  tanh to a few
+// units in the last place, small arguments too: below 0.35 its odd series to
+// x^11 (the next term is below 2^-26), above it 1 - 2 r with r = 1 / (1 +
+// e^2|x|), and then 1 - tanh^2 = 4 r (1 - r).
+__device__ __forceinline__ float changed_score_exact(const ScoreArgs& a, float s, float scale_log2, float kd,
+                                                     float slope2, float& f) {
+  float z = s * scale_log2;
+  f = 1.f;
+  if (a.mode & kScoreCap) {
+    const float x = s * a.cap_x, x2 = x * x, ax = fabsf(x);
+    const float series =
+        x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -8.8632355e-3f, 2.1869488e-2f), -5.3968254e-2f), 1.3333334e-1f),
+                          -3.3333334e-1f),
+                 1.f);
+    const float r = cap_complement(ax, 2.f * kLog2e);
+    const bool small = ax < 0.35f;
+    const float t = small ? series : copysignf(fmaf(-2.f, r, 1.f), x);
+    f = small ? fmaf(-t, t, 1.f) : 4.f * r * (1.f - r);
+    z = a.cap2 * t;
+  }
+  return fmaf(-slope2, fabsf(kd), z);
+}
+
 // The keys [lo, hi) of batch b outside which no query row's window reaches:
 // from `hull` (two ints per batch) where given, else the first row's lo and
 // the last row's hi (windows non-decreasing in the row), clamped into
@@ -411,8 +435,9 @@ hipError_t launch_qk_norm_bwd(const QkNormArgs& a, int head_dim, float* dw, hipS
 // dw[0 .. head_dim) = 0 (the gain gradient of an empty input).
 hipError_t launch_qk_norm_dw_zero(float* dw, int head_dim, hipStream_t stream);
 
-// Forward of few query rows (attn_few.hip): at most kFewRows per kv head.
-constexpr int kFewRows = 64;
+// Forward of few query rows (attn_few.hip): at most kFewQueries of them, or
+// kFewRows over the group of a kv head; float32 kFewQueriesF32.
+constexpr int kFewQueries = 32, kFewRows = 64, kFewQueriesF32 = 16;
 struct FewArgs {
   const void* q;
   const void* k;
@@ -443,7 +468,7 @@ struct FewPlan {
   int nsplit, row_blocks, block_rows;
   size_t bytes;
 };
-FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim);
+FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim, bool f32);
 hipError_t launch_few(const FewArgs& a, int head_dim, bool f32, hipStream_t stream);
 // The float32 kernels with changed scores (attn_f32.hip): what their C entry
 // points check, with a status code.  The forward's workspace: split parts, then

@@ -226,6 +226,41 @@ def test_few_rows_masks(shape, kind):
     o.check(out=out.detach(), dq=grads[0], dk=grads[1], dv=grads[2])
 
 
+@pytest.mark.parametrize("kind", ["padding", "both", "documents", "none"])
+@pytest.mark.parametrize("shape", [(3, 8, 2, 2, 700, 128), (2, 4, 4, 5, 100, 64), (2, 16, 1, 1, 2000, 64),
+                                   (2, 3, 3, 3, 95, 128)])
+@pytest.mark.parametrize("score", SCORES, ids=[s[0] for s in SCORES])
+def test_few_rows_masks_float32(shape, kind, score):
+    B, Hq, Hkv, Lq, Lk, D = shape
+    q, k, v, _ = make(*shape, torch.float32, seed=9)
+    lo, hi, mask = windows(kind, B, Lq, Lk)
+    slopes = slopes_of(Hq) if score[0] in ("slopes", "both") else None
+    with torch.no_grad():
+        out = A.scored_attention(q, k, v, softcap=score[1], distance_slopes=slopes, query_offset=Lk - Lq,
+                                 window_lo=lo, window_hi=hi,
+                                 attn_mask=None if mask is None else mask[:, None, None], enable_gqa=True)
+    Oracle(q, k, v, None, score[1], slopes, Lk - Lq, lo, hi, mask).check(out=out)
+
+
+@pytest.mark.parametrize("dtype,shape", [
+    (torch.bfloat16, (1, 8, 2, 32, 300, 64)), (torch.bfloat16, (1, 8, 2, 33, 300, 64)),
+    (torch.bfloat16, (2, 2, 2, 64, 200, 128)), (torch.bfloat16, (2, 2, 2, 65, 200, 128)),
+    (torch.bfloat16, (1, 80, 2, 1, 300, 128)), (torch.float32, (1, 8, 2, 16, 300, 64)),
+    (torch.float32, (1, 8, 2, 17, 300, 64)), (torch.float32, (2, 3, 3, 16, 200, 128)),
+    (torch.float32, (2, 40, 2, 1, 200, 128)),
+], ids=str)
+def test_either_side_of_the_few_rows(dtype, shape):
+    """The largest sizes of the few-row kernels and the next ones."""
+    q, k, v, _ = make(*shape, dtype, seed=11)
+    B, Hq, Hkv, Lq, Lk, D = shape
+    lo, hi, mask = windows("both", B, Lq, Lk)
+    slopes = slopes_of(Hq)
+    with torch.no_grad():
+        out = A.scored_attention(q, k, v, softcap=20.0, distance_slopes=slopes, query_offset=Lk - Lq, window_lo=lo,
+                                 window_hi=hi, attn_mask=mask[:, None, None], enable_gqa=True)
+    Oracle(q, k, v, None, 20.0, slopes, Lk - Lq, lo, hi, mask).check(out=out)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("shape", [(2, 4, 2, 3, 300, 64), (2, 4, 2, 200, 300, 128), (1, 2, 2, 300, 1200, 128)])
 def test_windows_in_any_order(shape, dtype):
