@@ -681,14 +681,15 @@ def scored_attention(
     may attend contributes nothing, whatever it holds: the unused slots of a
     cache need no clearing.  bf16 or float32, head_dim 64 or 128;
     differentiable in query, key and value (windows non-decreasing in the
-    row).  Up to 64 query rows per kv head run on kernels that split the keys
-    over the chip and read the cache once.
+    row).  A few queries (up to 32, or 64 rows over the heads of a kv head;
+    float32 16) run on kernels that split the keys over the chip and read the
+    cache in place, without copies of it.
     """
-    if query.shape[-2] == 0 or key.shape[-2] == 0:
-        return torch.zeros_like(query)
     _validate(query, key, value, 0.0, False, enable_gqa)
     if softcap is not None and not softcap > 0.0:
         raise ValueError(f"softcap must be positive or None; got {softcap}")
+    if isinstance(query_offset, float):
+        raise TypeError(f"query_offset must be an int or an int32 tensor; got {query_offset}")
     if distance_slopes is not None and distance_slopes.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("distance_slopes have no gradient; pass them detached")
     mask = _as_key_mask(attn_mask, query.shape[0], query.shape[-2], key.shape[-2])

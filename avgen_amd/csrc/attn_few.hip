@@ -563,7 +563,10 @@ FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D, bool f32) {
     }
     if (units * n >= slots) break;
   }
-  if (units * p.nsplit > 2147483647 || units * p.block_rows > 2147483647) return FewPlan{};
+  // Grids of 256 threads each, within 2^32: past that the general path, whose
+  // grid is the smaller one.
+  constexpr int64_t kMaxGrid = (1 << 24) - 1;
+  if (units * p.nsplit > kMaxGrid || units * p.block_rows > kMaxGrid) return FewPlan{};
   p.bytes = p.nsplit > 1 ? (size_t)units * p.nsplit * few_slot_floats(p.block_rows, D) * sizeof(float) : 0;
   return p;
 }

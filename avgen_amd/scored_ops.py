@@ -161,9 +161,11 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
     if lse.shape != (B, Hq, Lq) or lse.dtype is not torch.float32:
         raise ValueError(f"{name}: logsumexp must be float32 (batch, heads, queries)")
     _one_device(name, q, dout, out, lse)
-    if lo is not None and not monotone and Lq > 1 and bool(
-            ((lo[..., 1:] < lo[..., :-1]) | (hi[..., 1:] < hi[..., :-1])).any()):
-        raise ValueError(f"{name}: the backward needs window_lo and window_hi non-decreasing along the queries")
+    if lo is not None and not monotone and Lq > 1:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{name}: a captured backward cannot check the windows' order; pass monotone=True")
+        if bool(((lo[..., 1:] < lo[..., :-1]) | (hi[..., 1:] < hi[..., :-1])).any()):
+            raise ValueError(f"{name}: the backward needs window_lo and window_hi non-decreasing along the queries")
     dout, q, k, v, out = (_ready(t) for t in (dout, q, k, v, out))
     lse = lse.contiguous()
     if f32:

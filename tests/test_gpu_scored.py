@@ -563,3 +563,32 @@ def test_document_windows():
     assert lo.tolist() == hi.tolist() == [0, 0, 0]
     with pytest.raises(ValueError):
         A.document_windows(cu, 11, causal=True, prefix_lengths=torch.tensor([3, 7]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Lq, Lk", [(3, 0), (200, 0), (0, 7)])
+def test_gradients_of_empty_sizes(Lq, Lk, dtype):
+    q, k, v, do = make(2, 4, 2, Lq, Lk, 64, dtype)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = A.scored_attention(*leaves, softcap=3.0, distance_slopes=slopes_of(4), enable_gqa=True)
+    assert not out.any()
+    for g, t in zip(torch.autograd.grad(out, leaves, do), leaves):
+        assert g.shape == t.shape and not g.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_of_broadcast_inputs(dtype):
+    """Keys shared by the batch rows and an output gradient without strides."""
+    B, Hq, Hkv, Lq, Lk, D = 3, 4, 2, 70, 90, 64
+    q, k, v, _ = make(B, Hq, Hkv, Lq, Lk, D, dtype)
+    one = [t[:1].detach().requires_grad_(True) for t in (k, v)]
+    leaves = [q.requires_grad_(True), *one]
+    out = A.scored_attention(q, *(t.expand(B, -1, -1, -1) for t in one), softcap=9.0, enable_gqa=True)
+    got = torch.autograd.grad(out.sum(), leaves)
+    o = Oracle(q.detach(), *(t.detach().expand(B, -1, -1, -1) for t in one), torch.ones_like(q), 9.0)
+    o.check(out=out.detach(), dq=got[0])
+    # Summed over the batch by three more roundings at most.
+    for name, g in (("dk", got[1]), ("dv", got[2])):
+        want, tol = getattr(o, name), getattr(o, name + "_tol")
+        bound = tol.sum(0, keepdim=True) + 3 * U[dtype] * want.abs().sum(0, keepdim=True)
+        assert bool(((g.double() - want.sum(0, keepdim=True)).abs() <= bound * 1.01 + 1e-7).all()), name
