@@ -649,21 +649,10 @@ static int cu_count() {
 // 623 split; (2,20,40000) x 1,024 with one row empty 1,511 against 1,612).
 // Backward: (1,16,20000,128) x 256 keys 498 -> 198 us, (1,20,10000) x 128 keys
 // 255 -> 104, (1,4,4096) self-attention 171 -> 150.
-// With windows (changed scores) a block's tiles are known on the device only
-// and differ: parts for two rounds of workgroups, which level out.  (1,16 / 4
-// heads,4133,64) with 2 / 3 / 4 / 5 / 6 / 8 parts of 132 blocks: five documents
-// 133 / 127 / 106 / 110 / 107 / 108 us, causal 154 / 168 / 122 / 151 / 134 / 137,
-// whole windows 381 / 280 / 298 / 263 / 283 / 273.
-TailSplit dkv_split_plan(int64_t total, int tiles, int D, bool windows) {
+TailSplit dkv_split_plan(int64_t total, int tiles, int D) {
   constexpr int kCus = 256;
   TailSplit best{0, 0};
   if (total > kCus) return best;
-  if (windows) {
-    int p = (int)((2 * kCus + total - 1) / total);
-    if (p > 8) p = 8;
-    if (p > tiles / 8) p = tiles / 8;
-    return p > 1 ? TailSplit{(int)total, p} : best;
-  }
   const float work_us = tiles * (D == 64 ? 1.1f : 1.9f), fixed_us = 8.f;
   auto cost = [&](int p) {
     const int n = (int)total * p, rem = n % kCus;
@@ -672,6 +661,37 @@ TailSplit dkv_split_plan(int64_t total, int tiles, int D, bool windows) {
   };
   float c = cost(1) - 4.f;
   for (int p = 2; p <= 8 && tiles / p >= 8; ++p) {
+    if (cost(p) < c) {
+      c = cost(p);
+      best = TailSplit{(int)total, p};
+    }
+  }
+  return best;
+}
+
+// The same with changed scores, where also grids with windows are split: a
+// block's tiles are then known on the device only and differ, so rounds after
+// the first are taken to level out.  The model was fitted to 1 to 8 parts of
+// 204 backward passes (12 to 256 blocks of 6 to 260 tiles; no windows, causal,
+// five documents; D 64 and 128): its choice is 1.1% slower than the best of
+// them on average, 13% (no windows) and 20% at most; two rounds of parts, 8
+// tiles or more each, with every window were 6.4% and 48%.  (1,16 / 4
+// heads,4133,64), 132 blocks, with 1 / 2 / 3 / 4 / 5 / 6 / 8 parts: five
+// documents 254 / 167 / 160 / 147 / 155 / 157 / 160 us, causal 416 / 263 / 283 /
+// 223 / 259 / 235 / 241, no windows 455 / 483 / 383 / 418 / 381 / 400 / 401.
+TailSplit dkv_scored_split_plan(int64_t total, int tiles, int D, bool windows) {
+  constexpr int kCus = 256;
+  TailSplit best{0, 0};
+  if (total > kCus) return best;
+  const float tile_us = D == 64 ? 1.1f : 1.55f, slot_us = D == 64 ? 0.03f : 0.048f;
+  auto cost = [&](int p) {
+    const int n = (int)total * p, rem = n % kCus;
+    float rounds = n / kCus + (rem == 0 ? 0.f : 1.f - 0.2f * (1.f - (float)rem / kCus));
+    if (windows) rounds = n > kCus ? (float)n / kCus + 0.25f : 1.f;
+    return rounds * (tiles * tile_us / p + 3.f) + (p > 1 ? 4.f + n * slot_us : 0.f);
+  };
+  float c = cost(1);
+  for (int p = 2; p <= 8 && p <= tiles; ++p) {
     if (cost(p) < c) {
       c = cost(p);
       best = TailSplit{(int)total, p};
@@ -746,7 +766,9 @@ static hipError_t launch_bwd_d(const BwdArgs& args, int kv_per_pass, hipStream_t
     TailSplit ts = p.split_part ? plan_tail_split(total, cus, kSplitSlots) : TailSplit{0, 0};
     if (p.split_all != nullptr) {
       // Every block split (the region holds the plan's parts).
-      ts = dkv_split_plan(total, (a.Lqp / 64) * (a.Hq / a.Hkv), D, p.wlo != nullptr);
+      const int tiles = (a.Lqp / 64) * (a.Hq / a.Hkv);
+      ts = p.score.mode != 0 ? dkv_scored_split_plan(total, tiles, D, p.wlo != nullptr)
+                             : dkv_split_plan(total, tiles, D);
       p.split_part = p.split_all;
     }
     p.nsplit = ts.nsplit;

@@ -963,6 +963,101 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void bwd_dq_ds_f32_kernel
 }
 
 // Zeros over a (B, H, L, D) fp32 tensor (gradients of an empty side).
+// The same with changed scores where the workgroups above are too few for the
+// chip (up to 160 of 128 rows): 32 rows per workgroup, whose 4 waves take every fourth key tile and
+// are joined through LDS, in order.  No wave shares a tile, so K comes
+// straight from memory (a row's D floats per half wave, lane l32 the D / 32
+// channels from l32 * D / 32), a tile ahead.  Backward with the kernel above
+// against this one, heads of 1,024 rows on half as many kv heads: 4 heads (32
+// workgroups above) 121 / 86 us at D 64, 201 / 137 at 128; 16 heads (128) 181 /
+// 167, 310 / 270; 32 heads (256) 266 / 287, 463 / 467.
+template <int D, bool WIN>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void bwd_dq_ds_f32_short_kernel(F32Args a) {
+  constexpr int KT = 32, NW = 4, PITCH = D + 4, DT = D / 32;
+  using vdt = float __attribute__((ext_vector_type(DT)));
+  __shared__ __attribute__((aligned(16))) float part[NW][32 * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int group = a.Hq / a.Hkv;
+  const int nrt = (a.Lq + 31) / 32;
+  const int rt = blockIdx.x % nrt, pg = blockIdx.x / nrt;
+  const int gi = pg % group, bhk = a.pair0 + pg / group;
+  const int b = bhk / a.Hkv, hk = bhk % a.Hkv, h = hk * group + gi;
+  const int r0 = rt * 32;
+  const int nkt = 4 * ((a.Lk + 127) / 128), ntile = (a.Lk + KT - 1) / KT;
+  const bool valid = r0 + l32 < a.Lq;
+  int wl = 0, wh = a.Lk, t0 = 0, t1 = ntile;
+  if constexpr (WIN) {
+    __shared__ int red[2 * NW];
+    if (valid) row_window(a, b, r0 + l32, wl, wh);
+    window_tiles<NW>(wl, wh, valid, red, t0, t1);
+  }
+  const float* dsr = a.ds + (bhk - a.pair0) * a.dsp + ((int64_t)gi * nrt + rt) * nkt * 1024 + l32 * 32 + 16 * hh;
+  const float* kb = a.k + b * a.ksb + hk * a.ksh + l32 * DT;
+  LiveKeys live;
+  live.init(a, nullptr, b);
+  f32x16 dq[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) dq[d] = zero16();
+  // Tile t of this wave: its dS (of blocks no row meets nothing was stored),
+  // K and which of the keys count.
+  f32x4 pa[4];
+  vdt kn[16];
+  int ok = 0;
+  auto fetch = [&](int t) {
+    if (WIN && !rows_meet_block(a, wl, wh, valid, t / 4)) {
+      ok = 0;
+      return;
+    }
+    ok = live.has(a, b, t * KT + l32);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pa[e] = ld4(dsr + (int64_t)t * 1024 + 4 * e);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      kn[j] = *reinterpret_cast<const vdt*>(kb + (int64_t)min(t * KT + 16 * hh + j, a.Lk - 1) * a.ksl);
+  };
+  if (t0 + wave < t1) fetch(t0 + wave);
+  for (int t = t0 + wave; t < t1; t += NW) {
+    const uint32_t keys = (uint32_t)__builtin_amdgcn_ballot_w64(ok != 0);
+    f32x4 ca[4];
+    vdt kc[16];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ca[e] = pa[e];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) kc[j] = kn[j];
+    if (t + NW < t1) fetch(t + NW);
+    if (keys == 0) continue;
+    if (keys != 0xffffffffu) {  // what the others hold must not count
+      const uint32_t half = keys >> (16 * hh);
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (!(half >> j & 1)) kc[j] = vdt{};
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        dq[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(ca[j / 4][j % 4], kc[j][d], dq[d], 0, 0, 0);
+  }
+  // dq[d] register i: row r0 + 8*(i/4) + 4*hh + i%4, channel l32*DT + d
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    vdt x;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) x[d] = dq[d][i];
+    *reinterpret_cast<vdt*>(&part[wave][(8 * (i / 4) + 4 * hh + i % 4) * PITCH + l32 * DT]) = x;
+  }
+  __syncthreads();
+  for (int u = tid; u < 32 * (D / 4); u += 64 * NW) {
+    const int r = u / (D / 4), c = 4 * (u % (D / 4));
+    if (r0 + r >= a.Lq) continue;
+    f32x4 sum = ld4(&part[0][r * PITCH + c]);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum += ld4(&part[w][r * PITCH + c]);
+    st4(a.dq + b * a.dqsb + h * a.dqsh + (int64_t)(r0 + r) * a.dqsl + c, sum * a.scale);
+  }
+}
+
 __global__ void zero_f32_kernel(float* x, int64_t sb, int64_t sh, int64_t sl, int B, int H, int L, int D) {
   const int64_t n = (int64_t)B * H * L * (D / 4);
   for (int64_t u = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; u < n; u += (int64_t)gridDim.x * blockDim.x) {
@@ -1261,14 +1356,21 @@ constexpr int dkv_f32_slot_floats(int D) { return 2 * 128 * D; }
 // The dK/dV split of a staged backward in one pass (one 128-key block per
 // workgroup and CU): the last round's blocks over ranges of query tiles.
 // (1,20,4096,128): 640 blocks, 2.5 rounds.
-// With changed scores (row_tiles > 0: the 32-row tiles of a query head) also every block of a grid of at most one round, into parts for two
-// rounds of at least 4 tiles each.
-FwdSplit dkv_f32_split_plan(int64_t blocks, int D, int64_t row_tiles = 0) {
+// With changed scores (row_tiles > 0: the 32-row tiles of a query head) also
+// every block of a grid of at most half a round, into parts that fill one
+// round, or two where windows (unequal blocks) leave 4 or more parts of more
+// than 24 tiles.  Backward with whole blocks / one round / two rounds of parts, D
+// 64: (1,8,1024) 201 / 90 / 101 us, causal 257 / 102 / 113; (1,8 on 2 heads,
+// 2048) 1,413 / 264 / 277, causal (32 tiles a part) 1,802 / 312 / 251; (1,4,
+// 2048) causal (16 tiles) 484 / 166 / 164; (1,8,2048) causal (2 parts) two rounds
+// 324 against 313.
+FwdSplit dkv_f32_split_plan(int64_t blocks, int D, int64_t row_tiles = 0, int group = 1, bool windows = false) {
   TailSplit t = plan_tail_split(blocks, 256, kSplitSlots);
   if (row_tiles > 0 && blocks <= 256) {
-    int64_t p = (512 + blocks - 1) / blocks;
-    p = p < 8 ? p : 8;
-    p = p < row_tiles / 4 ? p : row_tiles / 4;
+    int64_t p = 256 / blocks;
+    if (windows && p >= 4 && row_tiles * group > 24 * p) p = 512 / blocks;
+    p = p < 16 ? p : 16;
+    p = p < row_tiles ? p : row_tiles;
     if (p > 1) t = TailSplit{(int)blocks, (int)p};
   }
   return FwdSplit{t.nsplit, t.nparts, (size_t)t.nsplit * t.nparts * dkv_f32_slot_floats(D) * sizeof(float)};
@@ -1285,7 +1387,15 @@ template <int D, bool WIN, bool SCORE>
 void launch_dq_ds_f32(const F32Args& a, int heads, hipStream_t s) {
   constexpr int kCus = 256;
   constexpr float kRowCost = D == 64 ? 1.09f : 1.12f;
+  constexpr int64_t kShort = 160;  // bwd_dq_ds_f32_short_kernel
   const int64_t n8 = (int64_t)((a.Lq + 255) / 256) * heads, n4 = (int64_t)((a.Lq + 127) / 128) * heads;
+  if constexpr (SCORE) {
+    if (n4 <= kShort) {
+      hipLaunchKernelGGL((bwd_dq_ds_f32_short_kernel<D, WIN>), dim3((unsigned)((a.Lq + 31) / 32 * (int64_t)heads)),
+                         dim3(256), 0, s, a);
+      return;
+    }
+  }
   if (0.5f * kRowCost * ((n4 + kCus - 1) / kCus) < (n8 + kCus - 1) / kCus)
     hipLaunchKernelGGL((bwd_dq_ds_f32_kernel<D, WIN, 4, SCORE>), dim3((unsigned)n4), dim3(256), 0, s, a);
   else
@@ -1314,7 +1424,8 @@ void launch_bwd_f32(F32Args a, int pairs_per_pass, hipStream_t s) {
     const int np = pairs - p0 < pairs_per_pass ? pairs - p0 : pairs_per_pass;
     a.pair0 = p0;
     a.nblocks = nkb * np;
-    const FwdSplit sp = a.part ? dkv_f32_split_plan(a.nblocks, D, SCORE ? (a.Lq + 31) / 32 : 0) : FwdSplit{0, 0, 0};
+    const FwdSplit sp = a.part ? dkv_f32_split_plan(a.nblocks, D, SCORE ? (a.Lq + 31) / 32 : 0, group, WIN)
+                                 : FwdSplit{0, 0, 0};
     a.nsplit = sp.nsplit, a.nparts = sp.nparts;
     const dim3 grid((unsigned)(a.nblocks - a.nsplit + a.nsplit * a.nparts));
     hipLaunchKernelGGL((bwd_dkdv_f32_kernel<D, true, WIN, SCORE>), grid, dim3(512), 0, s, a);
@@ -1342,8 +1453,8 @@ using namespace avattn;
 
 namespace avattn {
 
-size_t bwd_f32_split_bytes(int B, int Hq, int Hkv, int Lq, int Lk, int D) {
-  return dkv_f32_split_plan((int64_t)B * Hkv * ((Lk + 127) / 128), D, (Lq + 31) / 32).bytes;
+size_t bwd_f32_split_bytes(int B, int Hq, int Hkv, int Lq, int Lk, int D, bool windows) {
+  return dkv_f32_split_plan((int64_t)B * Hkv * ((Lk + 127) / 128), D, (Lq + 31) / 32, Hq / Hkv, windows).bytes;
 }
 
 size_t fwd_f32_split_bytes(int B, int Hq, int Lq, int Lk, int D) { return fwd_f32_split_plan(B, Hq, Lq, Lk, D).bytes; }
@@ -1560,7 +1671,8 @@ static int bwd_f32_entry(const float* dout, const float* q, const float* k, cons
       a.dsp = (int64_t)(per / sizeof(float));
       // One pass and room behind its dS: the parts of a split dK/dV round.
       const size_t end = off + (size_t)pairs * per;
-      const FwdSplit sp = dkv_f32_split_plan(pairs * ((len_k + 127) / 128), head_dim, score ? (len_q + 31) / 32 : 0);
+      const FwdSplit sp = dkv_f32_split_plan(pairs * ((len_k + 127) / 128), head_dim, score ? (len_q + 31) / 32 : 0,
+                                             heads_q / heads_kv, window_lo != nullptr);
       if (pp == pairs && sp.nsplit > 0 && workspace_bytes >= end + sp.bytes)
         a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + end);
     }

@@ -424,9 +424,11 @@ size_t avattn_bwd_staged_workspace_size(int32_t batch, int32_t heads_q, int32_t 
 
 namespace {
 // Bytes of the parts of a dK/dV grid with every block split (0: not split).
-size_t dkv_split_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool windows = false) {
-  const TailSplit t = dkv_split_plan((int64_t)B * Hkv * ((Lk + 127) / 128),
-                                     (int)(transpose_padded_len(Lq) / 64 * (Hq / Hkv)), D, windows);
+size_t dkv_split_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool scored = false,
+                       bool windows = false) {
+  const int64_t blocks = (int64_t)B * Hkv * ((Lk + 127) / 128);
+  const int tiles = (int)(transpose_padded_len(Lq) / 64 * (Hq / Hkv));
+  const TailSplit t = scored ? dkv_scored_split_plan(blocks, tiles, D, windows) : dkv_split_plan(blocks, tiles, D);
   return (size_t)t.nsplit * t.nparts * 256 * D * sizeof(float);
 }
 }  // namespace
@@ -599,7 +601,8 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
     set_hull(a, ws, wl);
     // One pass, no windows (or changed scores) and room behind its dS: the
     // parts of a split of every dK/dV block.
-    const size_t split = dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, window_lo != nullptr);
+    const size_t split = dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, score != nullptr,
+                                         window_lo != nullptr);
     const size_t end = off + (size_t)a.nkv * per;
     if (kv_per_pass == a.nkv && (!window_lo || (score && !compact)) && split > 0 && workspace_bytes >= end + split)
       a.split_all = reinterpret_cast<float*>(ws + end);
@@ -1169,9 +1172,9 @@ size_t avattn_bwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t 
   const int32_t pairs = batch * heads_kv;
   if (is_f32)
     return avattn_bwd_f32_staged_workspace_size(batch, heads_q, heads_kv, len_q, len_k, pairs) +
-           bwd_f32_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim);
+           bwd_f32_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, windowed != 0);
   return avattn_bwd_staged_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, pairs) +
-         dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, windowed != 0);
+         dkv_split_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, true, windowed != 0);
 }
 
 int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t* q_strides, const int64_t* k_strides,

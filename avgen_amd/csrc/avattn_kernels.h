@@ -270,7 +270,7 @@ struct BwdArgs {
   // parts in order and writes dk and dv.
   float* split_part;
   int nsplit, nparts;
-  // Slots for a split of every block (null: none; see dkv_split_plan), in
+  // Slots for a split of every block (null: none; see dkv_(scored_)split_plan), in
   // place of split_part.
   float* split_all;
   // Changed scores as in FwdArgs (mode 0: none; staged dS only).  With the cap
@@ -315,7 +315,9 @@ inline TailSplit plan_tail_split(int64_t total, int cus, int max_slots) {
 
 // Split of every block of a short dK/dV grid of `total` 128-key blocks, each
 // over `tiles` 64-row query tiles (attn_bwd.hip); {0, 0}: none.
-TailSplit dkv_split_plan(int64_t total, int tiles, int D, bool windows);
+TailSplit dkv_split_plan(int64_t total, int tiles, int D);
+// The same with changed scores, with or without windows.
+TailSplit dkv_scored_split_plan(int64_t total, int tiles, int D, bool windows);
 
 // Bytes of staged dS per (b, kv head) pair: dense, or the compact layout's
 // units_per_head units per query head.
@@ -473,7 +475,7 @@ hipError_t launch_few(const FewArgs& a, int head_dim, bool f32, hipStream_t stre
 // The float32 kernels with changed scores (attn_f32.hip): what their C entry
 // points check, with a status code.  The forward's workspace: split parts, then
 // the hull; the backward's tensors are float behind BwdArgs' pointers.
-size_t bwd_f32_split_bytes(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim);
+size_t bwd_f32_split_bytes(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim, bool windows);
 size_t fwd_f32_split_bytes(int B, int Hq, int Lq, int Lk, int head_dim);
 int fwd_scored_f32(const FewArgs& c, int head_dim, float scale, bool sorted_windows, void* workspace,
                    size_t workspace_bytes, hipStream_t stream);

@@ -9,6 +9,7 @@ of that module.  bf16 and float32; differentiable in q, k and v.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -26,11 +27,10 @@ from .ops import (
     _kernel_ready,
     _normalise_mask,
     _one_pass_workspace,
-    _out_or_new,
     _ptr,
     _require_gpu,
     _stream,
-    _strides3,
+    _Strides3,
     _workspace,
     compact_ds_table,
     ds_bytes_per_pair,
@@ -88,8 +88,40 @@ def _check_scored(name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets
     return lo, hi, wsb, mask, msb, slopes, offsets
 
 
-def _ready(t: torch.Tensor) -> torch.Tensor:
-    return _f32_ready(t) if t.dtype is torch.float32 else _kernel_ready(t)
+def _laid_out(t: torch.Tensor, f32: bool):
+    """``t`` as the kernels read it, and its strides for the C call."""
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or (s0 | s1 | s2) % (4 if f32 else 8) or t.data_ptr() % 16:
+        t = _f32_ready(t) if f32 else _kernel_ready(t)
+        s0, s1, s2, _ = t.stride()
+    return t, _Strides3(s0, s1, s2)
+
+
+def _new_like(t: torch.Tensor, strides, f32: bool):
+    """An output shaped like ``t`` (whose strides are given), and its strides."""
+    o = torch.empty_like(t)
+    if o.stride() == t.stride():
+        return o, strides
+    return _laid_out(o, f32)
+
+
+# Workspace sizes: functions of a call's sizes alone.
+@lru_cache(maxsize=256)
+def _fwd_workspace_size(*sizes: int) -> int:
+    return _lib.load().avattn_fwd_scored_workspace_size(*sizes)
+
+
+@lru_cache(maxsize=256)
+def _bwd_workspace_size(*sizes: int) -> int:
+    return _lib.load().avattn_bwd_scored_workspace_size(*sizes)
+
+
+@lru_cache(maxsize=256)
+def _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs) -> int:
+    lib = _lib.load()
+    if f32:
+        return lib.avattn_bwd_f32_staged_workspace_size(B, Hq, Hkv, Lq, Lk, pairs)
+    return lib.avattn_bwd_staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, pairs)
 
 
 def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone):
@@ -99,21 +131,20 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
     B, Hq, Lq, D = q.shape
     Hkv, Lk = k.shape[1], k.shape[2]
     f32 = q.dtype is torch.float32
-    q, k, v = _ready(q), _ready(k), _ready(v)
-    k, v = (t if t.stride(2) < _MAX_ROW_STRIDE else t.contiguous() for t in (k, v))
-    out = _ready(torch.empty_like(q, memory_format=torch.preserve_format))
-    lse = torch.empty((B, Hq, Lq), device=q.device, dtype=torch.float32)
-    lib = _lib.load()
-    ws = _workspace(lib.avattn_fwd_scored_workspace_size(B, Hq, Hkv, Lq, Lk, D, int(f32)), q.device)
-    with _on(q.device):
-        st = lib.avattn_fwd_scored(
-            _ptr(q), _ptr(k), _ptr(v), _strides3(q), _strides3(k), _strides3(v),
-            B, Hq, Hkv, Lq, Lk, D, int(f32),
+    (q, qs), (k, ks), (v, vs) = _laid_out(q, f32), _laid_out(k, f32), _laid_out(v, f32)
+    if ks[2] >= _MAX_ROW_STRIDE or vs[2] >= _MAX_ROW_STRIDE:
+        (k, ks), (v, vs) = _laid_out(k.contiguous(), f32), _laid_out(v.contiguous(), f32)
+    out, os = _new_like(q, qs, f32)
+    device = q.device
+    lse = torch.empty((B, Hq, Lq), device=device, dtype=torch.float32)
+    ws = _workspace(_fwd_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32), device)
+    with _on(device):
+        st = _lib.load().avattn_fwd_scored(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, B, Hq, Hkv, Lq, Lk, D, f32,
             _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb,
-            float(scale), float(softcap), _ptr(slopes), _ptr(offsets), int(offset),
+            scale, softcap, _ptr(slopes), _ptr(offsets), offset,
             _lib.SCORED_SORTED_WINDOWS if monotone else 0,
-            _ptr(out), _strides3(out), _ptr(lse),
-            _ptr(ws), ws.numel(), _stream(q.device))
+            out.data_ptr(), os, lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
     _lib.check(st, name)
     return out, lse
 
@@ -122,20 +153,16 @@ def _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, windowed, device) -> torch.Ten
     """The backward's workspace with (dense) staged dS: as many (batch, kv
     head) pairs per pass as the budget and the allocator have, at least one;
     with all of them in one pass also room for a split grid."""
-    lib = _lib.load()
     total = B * Hkv
     per = (f32_ds_bytes_per_pair if f32 else ds_bytes_per_pair)(Hq // Hkv, Lq, Lk)
     pairs = max(1, min(total, _ds_budget(device) // per))
     pairs = -(-total // -(-total // pairs))
     while True:
-        if f32:
-            staged = lib.avattn_bwd_f32_staged_workspace_size(B, Hq, Hkv, Lq, Lk, int(pairs))
-        else:
-            staged = lib.avattn_bwd_staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, int(pairs))
+        staged = _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs)
         try:
             if pairs == total:
-                split = lib.avattn_bwd_scored_workspace_size(B, Hq, Hkv, Lq, Lk, D, int(f32), int(windowed))
-                return _one_pass_workspace(split, staged, int(pairs) * per, device)
+                split = _bwd_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, windowed)
+                return _one_pass_workspace(split, staged, pairs * per, device)
             return _workspace(staged, device)
         except torch.OutOfMemoryError:
             if pairs == 1:
@@ -166,33 +193,29 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
             raise RuntimeError(f"{name}: a captured backward cannot check the windows' order; pass monotone=True")
         if bool(((lo[..., 1:] < lo[..., :-1]) | (hi[..., 1:] < hi[..., :-1])).any()):
             raise ValueError(f"{name}: the backward needs window_lo and window_hi non-decreasing along the queries")
-    dout, q, k, v, out = (_ready(t) for t in (dout, q, k, v, out))
+    (dout, dos), (q, qs), (k, ks) = _laid_out(dout, f32), _laid_out(q, f32), _laid_out(k, f32)
+    (v, vs), (out, os) = _laid_out(v, f32), _laid_out(out, f32)
     lse = lse.contiguous()
-    if f32:
-        dq, dk, dv = (_f32_ready(torch.empty_like(t)) for t in (q, k, v))
-    else:
-        dq, dk, dv = (_out_or_new(None, t, name, "gradient") for t in (q, k, v))
-    lib = _lib.load()
+    (dq, dqs), (dk, dks), (dv, dvs) = _new_like(q, qs, f32), _new_like(k, ks, f32), _new_like(v, vs, f32)
+    device = q.device
     table, tsb, units = None, 0, 0
     if 0 in (B, Hq, Lq, Lk):
-        ws = _workspace(0, q.device)
-    elif (not f32 and lo is not None and B * Hkv * ds_bytes_per_pair(Hq // Hkv, Lq, Lk) > _ds_budget(q.device)
+        ws = _workspace(0, device)
+    elif (not f32 and lo is not None and B * Hkv * ds_bytes_per_pair(Hq // Hkv, Lq, Lk) > _ds_budget(device)
             and not torch.cuda.is_current_stream_capturing()):
         table, units = compact_ds_table(lo, hi, Lq, Lk)
         tsb = 0 if table.shape[0] == 1 else table.shape[1]
-        ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, q.device, stage_ds=True, ds_units=units)
+        ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, device, stage_ds=True, ds_units=units)
     else:
-        ws = _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, lo is not None, q.device)
-    with _on(q.device):
-        st = lib.avattn_bwd_scored(
-            _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse),
-            _strides3(dout), _strides3(q), _strides3(k), _strides3(v), _strides3(out),
-            B, Hq, Hkv, Lq, Lk, D, int(f32),
-            _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb,
-            _ptr(table), tsb, units,
-            float(scale), float(softcap), _ptr(slopes), _ptr(offsets), int(offset),
-            _ptr(dq), _strides3(dq), _ptr(dk), _strides3(dk), _ptr(dv), _strides3(dv),
-            _ptr(ws), ws.numel(), _stream(q.device))
+        ws = _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, lo is not None, device)
+    with _on(device):
+        st = _lib.load().avattn_bwd_scored(
+            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            dos, qs, ks, vs, os, B, Hq, Hkv, Lq, Lk, D, f32,
+            _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb, _ptr(table), tsb, units,
+            scale, softcap, _ptr(slopes), _ptr(offsets), offset,
+            dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dvs,
+            ws.data_ptr(), ws.numel(), _stream(device))
     _lib.check(st, name)
     return dq, dk, dv
 
