@@ -46,7 +46,8 @@ MAX_SLOPE_GROUP = 64
 #: Largest cap of bfloat16 calls (float32: any).
 MAX_SOFTCAP_BF16 = 1024.0
 
-# Largest row stride of k and v the kernels for few query rows address.
+# Bound of the row strides of k and v that the kernels for few query rows
+# address.
 _MAX_ROW_STRIDE = 1 << 23
 
 

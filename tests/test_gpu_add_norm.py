@@ -207,6 +207,24 @@ def test_gradient_of_broadcast_addend():
     assert bool(((dx.sum(0, keepdim=True) - dr).abs() <= 1e-5 * dx.abs().sum(0, keepdim=True)).all())
 
 
+@pytest.mark.parametrize("W", [8, 3])
+def test_more_rows_than_one_launch_takes(W):
+    rows = 2**21 + 5
+    x, r, w = _inputs((rows, W), torch.bfloat16)
+    with torch.no_grad():
+        n, h = layers.add_rms_norm(x, r, w)
+        codes, scale, h8 = layers.add_rms_norm_fp8(x, r, w)
+    h64 = x.double() + r.double()
+    n64, _ = _norm64(h64, w, 1e-6)
+    _check(h, h64, U[torch.bfloat16], 2.0**-24)
+    _check(n, n64, U[torch.bfloat16], slack(W))
+    assert torch.equal(h, h8)
+    back = codes.double() * scale.double()[:, None]
+    # e4m3: half a step of the value, or of the smallest step, 2^-9 of the scale.
+    bound = n64.abs() * (2.0**-4 + slack(W)) + scale.double()[:, None] * (2.0**-10 + 448 * slack(W))
+    assert bool(((back - n64).abs() <= bound).all())
+
+
 def test_no_rows():
     x = torch.empty((0, 640), device="cuda", dtype=torch.bfloat16, requires_grad=True)
     w = torch.ones(640, device="cuda", dtype=torch.bfloat16, requires_grad=True)

@@ -229,3 +229,35 @@ def test_a_captured_decoding_step():
                 assert torch.equal(a, b)
             assert torch.equal(captured.k, eager.k) and torch.equal(captured.v, eager.v)
             length += 1
+
+
+def test_a_captured_training_step():
+    """Forward and backward of the block as a graph (no eager graph of the same
+    leaves alive), replayed with new inputs and eager steps between."""
+    B, L, dtype = 2, 200, torch.bfloat16
+    w = weights(dtype)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    lo, hi = A.document_windows(torch.tensor([0, 90, 180], device="cuda"), L, causal=True, prefix_lengths=8)
+    tables = rope.build_position_tables(torch.arange(L, device="cuda") - lo, rotary_dim=ROT)
+    x, r, dn, dh = (torch.zeros(B, L, WIDTH, device="cuda", dtype=dtype) for _ in range(4))
+
+    def step():
+        leaves = {n: t.detach().requires_grad_(True) for n, t in dict(w, x=x, r=r).items()}
+        n, h = block(leaves, leaves["x"], leaves["r"], tables, lo, hi)
+        return (n.detach(), h.detach()) + torch.autograd.grad((n, h), list(leaves.values()), (dn, dh))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        for t in (x, r, dn, dh):
+            t.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)

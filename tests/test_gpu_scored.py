@@ -592,3 +592,37 @@ def test_gradients_of_broadcast_inputs(dtype):
         want, tol = getattr(o, name), getattr(o, name + "_tol")
         bound = tol.sum(0, keepdim=True) + 3 * U[dtype] * want.abs().sum(0, keepdim=True)
         assert bool(((g.double() - want.sum(0, keepdim=True)).abs() <= bound * 1.01 + 1e-7).all()), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["none", "causal", "both"])
+@pytest.mark.parametrize("shape", [(3, 32, 32, 150, 390, 64), (2, 40, 20, 200, 900, 128)])
+def test_grids_past_one_round(shape, kind, dtype):
+    """More key blocks than the chip holds at once, a last round that is split,
+    and heads that do not divide over its eighths."""
+    B, Hq, Hkv, Lq, Lk, D = shape
+    q, k, v, do = make(*shape, dtype, seed=21)
+    lo, hi, mask = windows(kind, B, Lq, Lk)
+    slopes = slopes_of(Hq)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = A.scored_attention(*leaves, softcap=12.0, distance_slopes=slopes, query_offset=Lk - Lq, window_lo=lo,
+                             window_hi=hi, attn_mask=None if mask is None else mask[:, None, None], enable_gqa=True)
+    grads = torch.autograd.grad(out, leaves, do)
+    o = Oracle(*(t.detach() for t in leaves), do, 12.0, slopes, Lk - Lq, lo, hi, mask)
+    o.check(out=out.detach(), dq=grads[0], dk=grads[1], dv=grads[2])
+
+
+@pytest.mark.parametrize("L, heads, kv", [(128, 4, 2), (384, 4, 1), (1024, 2, 1), (2048, 4, 1)])
+@pytest.mark.parametrize("kind", ["none", "causal", "documents"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_split_backward(L, heads, kv, kind, dtype):
+    """Few key blocks of many or few query tiles: parts down to a tile, and
+    empty ones."""
+    D = 64
+    q, k, v, do = make(1, heads, kv, L, L, D, dtype, seed=L)
+    lo, hi, _ = windows(kind, 1, L, L)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = A.scored_attention(*leaves, softcap=12.0, window_lo=lo, window_hi=hi, enable_gqa=True, monotone=True)
+    grads = torch.autograd.grad(out, leaves, do)
+    o = Oracle(*(t.detach() for t in leaves), do, 12.0, None, 0, lo, hi)
+    o.check(out=out.detach(), dq=grads[0], dk=grads[1], dv=grads[2])
