@@ -29,6 +29,11 @@ windows ``[lo, hi)`` that the kernels skip tiles by:
 and :func:`varlen_attention` for packed sequences (the ``cu_seqlens`` of
 src/avgen/data/packing.py:163-200); :func:`windowed_attention` takes the
 windows directly.
+
+:func:`scored_attention` (no reference counterpart) adds scores capped by a
+tanh and a bias by distance, with the windows of :func:`document_windows`
+(documents, causal rows, bidirectional prefixes) and a form for a few newest
+queries against a cache.
 """
 
 from __future__ import annotations

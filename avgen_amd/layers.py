@@ -15,6 +15,9 @@ Here the head split stays a strided view of the projection output
 and produces any such layout, writes its output in it too, so the final
 ``transpose(1, 2).flatten(2)`` is a view: no copy on either side of the
 kernel, forward or backward.
+
+:func:`add_rms_norm` is the step between two such sections: the residual
+addition with the norm that follows it, in one pass.
 """
 
 from __future__ import annotations

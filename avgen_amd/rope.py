@@ -6,6 +6,11 @@ signatures, argument meaning and exceptions.  Table construction
 HIP kernels through ``libavattn.so``; the rotation is bit-identical to the
 reference's fp32 elementwise chain (each product rounded separately, one
 round to bf16), and differentiable.
+
+Token sequences with integer positions (no reference counterpart):
+:func:`build_position_tables`, with :class:`PositionScaling` for longer
+contexts, and :func:`rotate_heads` / :func:`rotate_query_key`, which rotate
+part of each head in either pair layout.
 """
 
 from __future__ import annotations
