@@ -26,7 +26,6 @@ from .ops import (
     _grad_direct,
     _kernel_ready,
     _normalise_mask,
-    _one_pass_workspace,
     _ptr,
     _require_gpu,
     _stream,
@@ -79,14 +78,18 @@ def _check_scored(name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets
         if offsets.dtype is not torch.int32:
             raise TypeError(f"{name}: query offsets must be int32; got {offsets.dtype}")
         offsets = offsets.contiguous()
+    lo, hi, wsb, mask, msb = _masks(name, window_lo, window_hi, key_mask, B, Lq, k.shape[2])
+    _require_gpu(name, q, k, v)
+    _one_device(name, q, k, v, lo, hi, mask, slopes, offsets)
+    return lo, hi, wsb, mask, msb, slopes, offsets
+
+
+def _masks(name, window_lo, window_hi, key_mask, B, Lq, Lk):
     lo = hi = None
     wsb = 0
     if window_lo is not None or window_hi is not None:
         lo, hi, wsb = _check_windows(name, window_lo, window_hi, B, Lq)
-    mask, msb = _normalise_mask(name, key_mask, B, k.shape[2])
-    _require_gpu(name, q, k, v)
-    _one_device(name, q, k, v, lo, hi, mask, slopes, offsets)
-    return lo, hi, wsb, mask, msb, slopes, offsets
+    return (lo, hi, wsb, *_normalise_mask(name, key_mask, B, Lk))
 
 
 def _laid_out(t: torch.Tensor, f32: bool):
@@ -150,45 +153,65 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
     return out, lse
 
 
-def _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, windowed, device) -> torch.Tensor:
-    """The backward's workspace with (dense) staged dS: as many (batch, kv
-    head) pairs per pass as the budget and the allocator have, at least one;
-    with all of them in one pass also room for a split grid."""
+@lru_cache(maxsize=256)
+def _staged_plan(B, Hq, Hkv, Lq, Lk, D, f32, windowed, budget) -> tuple[int, int]:
+    """Of the backward with (dense) staged dS: its (batch, kv head) pairs per
+    pass, as many as the budget has, at least one, and its workspace's bytes:
+    with all of them in one pass also room for a split grid, if the budget
+    covers the parts."""
     total = B * Hkv
     per = (f32_ds_bytes_per_pair if f32 else ds_bytes_per_pair)(Hq // Hkv, Lq, Lk)
-    pairs = max(1, min(total, _ds_budget(device) // per))
+    pairs = max(1, min(total, budget // per))
     pairs = -(-total // -(-total // pairs))
+    staged = _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs)
+    if pairs == total:
+        split = _bwd_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, windowed)
+        if pairs * per + split - staged <= budget:
+            return pairs, split
+    return pairs, staged
+
+
+def _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, windowed, device) -> torch.Tensor:
+    """The workspace of :func:`_staged_plan`; where the allocator has not got
+    it, without the room for a split grid, then in passes of half the pairs."""
+    pairs, nbytes = _staged_plan(B, Hq, Hkv, Lq, Lk, D, f32, windowed, _ds_budget(device))
     while True:
-        staged = _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs)
         try:
-            if pairs == total:
-                split = _bwd_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, windowed)
-                return _one_pass_workspace(split, staged, pairs * per, device)
-            return _workspace(staged, device)
+            return _workspace(nbytes, device)
         except torch.OutOfMemoryError:
-            if pairs == 1:
-                raise
-            pairs = (pairs + 1) // 2
+            staged = _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs)
+            if staged >= nbytes:
+                if pairs == 1:
+                    raise
+                pairs = (pairs + 1) // 2
+                staged = _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs)
+            nbytes = staged
 
 
 def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
-              monotone):
+              monotone, from_forward=False):
     """``monotone``: the caller guarantees windows non-decreasing in the row
     (otherwise checked here, one host synchronisation).  With windows dS is
     staged densely where all of it fits the budget (no synchronisation), else
-    compactly (one, for its size)."""
+    compactly (one, for its size).  ``from_forward``: the arguments passed the
+    forward's checks (the backward of a small call is bound by this function,
+    at half speed on autograd's own thread)."""
     name = "avgen_amd.flash_bwd_scored"
-    lo, hi, wsb, mask, msb, slopes, offsets = _check_scored(
-        name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset)
     B, Hq, Lq, D = q.shape
     Hkv, Lk = k.shape[1], k.shape[2]
     f32 = q.dtype is torch.float32
-    for label, t in (("grad_out", dout), ("out", out)):
-        if t.shape != q.shape or t.dtype is not q.dtype:
-            raise ValueError(f"{name}: {label} must be {q.dtype} {tuple(q.shape)}")
-    if lse.shape != (B, Hq, Lq) or lse.dtype is not torch.float32:
-        raise ValueError(f"{name}: logsumexp must be float32 (batch, heads, queries)")
-    _one_device(name, q, dout, out, lse)
+    if from_forward:
+        lo, hi, wsb, mask, msb = _masks(name, window_lo, window_hi, key_mask, B, Lq, Lk)
+        slopes, offsets = (None if t is None else t.contiguous() for t in (slopes, offsets))
+    else:
+        lo, hi, wsb, mask, msb, slopes, offsets = _check_scored(
+            name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset)
+        for label, t in (("grad_out", dout), ("out", out)):
+            if t.shape != q.shape or t.dtype is not q.dtype:
+                raise ValueError(f"{name}: {label} must be {q.dtype} {tuple(q.shape)}")
+        if lse.shape != (B, Hq, Lq) or lse.dtype is not torch.float32:
+            raise ValueError(f"{name}: logsumexp must be float32 (batch, heads, queries)")
+    _one_device(name, q, k, v, dout, out, lse, lo, hi, mask, slopes, offsets)
     if lo is not None and not monotone and Lq > 1:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{name}: a captured backward cannot check the windows' order; pass monotone=True")
@@ -302,4 +325,12 @@ class _FlashFwdScored(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, _dlse):
-        return (None,) * 12 if dout is None else _backward(ctx, dout, None)
+        if dout is None:
+            return (None,) * 12
+        if not _grad_direct(dout):
+            return _backward(ctx, dout, None)
+        # The forward was a plain call: so is this one.
+        q, k, v, out, lse, lo, hi, mask, slopes, offsets = ctx.saved_tensors
+        grads = _bwd_impl(dout, q, k, v, out, lse, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap, ctx.offset,
+                          ctx.monotone, True)
+        return (*grads,) + (None,) * 9
