@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import math
 from contextlib import nullcontext
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -138,7 +139,12 @@ def _check_rotation(name, tensors, cos, sin, start):
 
 def _rotate_launch(name, q, k, cos, sin, start, half, inverse):
     cos, sin, tsb = _check_rotation(name, (q,) if k is None else (q, k), cos, sin, start)
-    B, H, L, D = q.shape
+    return _rotate_run(name, q, k, cos, sin, tsb, start, half, inverse)
+
+
+def _rotate_run(name, q, k, cos, sin, tsb, start, half, inverse):
+    """The rotation of checked arguments."""
+    B, _, L, D = q.shape
     outs = []
     args = []
     for t in (q, k):
@@ -237,14 +243,24 @@ torch.library.register_autograd("avgen_amd::rotate", _rotate_backward, setup_con
 torch.library.register_autograd("avgen_amd::rotate_pair", _rotate_pair_backward, setup_context=_rotate_pair_setup)
 
 
+# Plain eager calls.  Their backward, a plain call itself, takes the arguments
+# that the forward has checked: small calls are bound by this Python, which runs
+# at half speed on autograd's own thread.
 class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *args):
         result = _rotate_impl(*args)
+        ctx.set_materialize_grads(False)
         _rotate_setup(ctx, args, result)
         return result
 
-    backward = staticmethod(_rotate_backward)
+    @staticmethod
+    def backward(ctx, grad):
+        if grad is None:
+            return (None,) * 6
+        if not _grad_direct(grad):
+            return _rotate_backward(ctx, grad)
+        return _rotate_grads(ctx, "avgen_amd.rotate", grad)[0], None, None, None, None, None
 
 
 class _RotatePair(torch.autograd.Function):
@@ -255,7 +271,18 @@ class _RotatePair(torch.autograd.Function):
         _rotate_pair_setup(ctx, args, result)
         return result
 
-    backward = staticmethod(_rotate_pair_backward)
+    @staticmethod
+    def backward(ctx, gq, gk):
+        if gq is None or gk is None or not _grad_direct(gq, gk):
+            return _rotate_pair_backward(ctx, gq, gk)
+        return (*_rotate_grads(ctx, "avgen_amd.rotate_pair", gq, gk), None, None, None, None, None)
+
+
+def _rotate_grads(ctx, name, gq, gk=None):
+    cos, sin = ctx.saved_tensors
+    cos, sin = cos.contiguous(), sin.contiguous()
+    tsb = 0 if cos.shape[0] == 1 else cos.shape[2] * cos.shape[3]
+    return _rotate_run(name, gq, gk, cos, sin, tsb, ctx.start, ctx.half, not ctx.inverse)
 
 
 # ---------------------------------------------------------------------------
@@ -335,6 +362,11 @@ def _add_rms_norm_fp8_impl(x, residual, weight, eps):
     return _norm_launch("avgen_amd.add_rms_norm_fp8", x, residual, weight, eps, True)
 
 
+@lru_cache(maxsize=256)
+def _norm_workspace_size(rows: int, width: int) -> int:
+    return _lib.load().avattn_add_rms_norm_bwd_workspace_size(rows, width)
+
+
 def _add_rms_norm_bwd_impl(dnorm, dsum, total, weight, eps):
     name = "avgen_amd.add_rms_norm_bwd"
     w = _check_norm(name, total, total, weight, eps)
@@ -342,6 +374,11 @@ def _add_rms_norm_bwd_impl(dnorm, dsum, total, weight, eps):
         if t is not None and (t.shape != total.shape or t.dtype is not total.dtype):
             raise ValueError(f"{name}: {label} must be {total.dtype} {tuple(total.shape)}")
     _one_device(name, dnorm, dsum, total)
+    return _add_rms_norm_bwd_run(name, dnorm, dsum, total, w, eps)
+
+
+def _add_rms_norm_bwd_run(name, dnorm, dsum, total, w, eps):
+    """The backward of checked arguments."""
     W = total.shape[-1]
     rows = total.numel() // W
     dx = torch.empty(total.shape, dtype=total.dtype, device=total.device)
@@ -350,13 +387,13 @@ def _add_rms_norm_bwd_impl(dnorm, dsum, total, weight, eps):
     dhs = 0
     if dsum is not None:
         dsum, dhs = _rows(dsum)
-    lib = _lib.load()
-    ws = _workspace(lib.avattn_add_rms_norm_bwd_workspace_size(rows, W), total.device)
-    with _on(total.device):
-        st = lib.avattn_add_rms_norm_bwd(
-            _ptr(dnorm), dns, _ptr(dsum), dhs, _ptr(total), hs, _ptr(w), int(w.dtype is torch.float32), rows, W,
-            int(total.dtype is torch.float32), float(eps), _ptr(dx), _ptr(dw), _ptr(ws), ws.numel(),
-            _stream(total.device))
+    device = total.device
+    ws = _workspace(_norm_workspace_size(rows, W), device)
+    with _on(device):
+        st = _lib.load().avattn_add_rms_norm_bwd(
+            dnorm.data_ptr(), dns, _ptr(dsum), dhs, total.data_ptr(), hs, w.data_ptr(), w.dtype is torch.float32,
+            rows, W, total.dtype is torch.float32, eps, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(),
+            _stream(device))
     _lib.check(st, name)
     return dx, dw
 
@@ -447,4 +484,10 @@ class _AddRmsNorm(torch.autograd.Function):
         _norm_setup(ctx, args, result)
         return result
 
-    backward = staticmethod(_norm_backward)
+    @staticmethod
+    def backward(ctx, dnorm, dsum):
+        if dnorm is None or not _grad_direct(dnorm, dsum):
+            return _norm_backward(ctx, dnorm, dsum)
+        total, weight = ctx.saved_tensors
+        dx, dw = _add_rms_norm_bwd_run("avgen_amd.add_rms_norm_bwd", dnorm, dsum, total, weight.contiguous(), ctx.eps)
+        return dx, dx, dw, None

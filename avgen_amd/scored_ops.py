@@ -17,6 +17,7 @@ import torch
 from . import _lib
 from .block_ops import _on, _one_device
 from .ops import (
+    SUPPORTED_HEAD_DIMS,
     _alloc_bwd_workspace,
     _check_qkv,
     _check_windows,
@@ -27,7 +28,6 @@ from .ops import (
     _kernel_ready,
     _normalise_mask,
     _ptr,
-    _require_gpu,
     _stream,
     _Strides3,
     _workspace,
@@ -45,6 +45,8 @@ MAX_SLOPE_GROUP = 64
 #: Largest cap of bfloat16 calls (float32: any).
 MAX_SOFTCAP_BF16 = 1024.0
 
+_DTYPES = (torch.bfloat16, torch.float32)
+
 # Bound of the row strides of k and v that the kernels for few query rows
 # address.
 _MAX_ROW_STRIDE = 1 << 23
@@ -53,13 +55,17 @@ _MAX_ROW_STRIDE = 1 << 23
 def _check_scored(name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset):
     """The arguments both directions share: (lo, hi, window stride, mask, mask
     stride, slopes, offsets)."""
-    _check_qkv(name, q, k, v, allow_f32=True)
-    B, Hq, Lq, _ = q.shape
+    shape, kshape, dtype = q.shape, k.shape, q.dtype
+    if not (len(shape) == 4 and len(kshape) == 4 and kshape == v.shape and shape[0] == kshape[0]
+            and shape[3] == kshape[3] and shape[3] in SUPPORTED_HEAD_DIMS and kshape[1] and shape[1] % kshape[1] == 0
+            and dtype in _DTYPES and k.dtype is dtype and v.dtype is dtype):
+        _check_qkv(name, q, k, v, allow_f32=True)  # says what is wrong
+    B, Hq, Lq, _ = shape
     if not (math.isfinite(scale) and scale > 0.0):
         raise ValueError(f"{name}: scale must be positive and finite; got {scale}")
     if not (math.isfinite(softcap) and softcap >= 0.0):
         raise ValueError(f"{name}: softcap must be finite and >= 0 (0: none); got {softcap}")
-    if q.dtype is torch.bfloat16 and softcap > MAX_SOFTCAP_BF16:
+    if dtype is torch.bfloat16 and softcap > MAX_SOFTCAP_BF16:
         raise ValueError(f"{name}: softcap {softcap} exceeds {MAX_SOFTCAP_BF16} (bfloat16)")
     if abs(offset) > MAX_OFFSET:
         raise ValueError(f"{name}: query offset {offset} exceeds {MAX_OFFSET}")
@@ -68,9 +74,9 @@ def _check_scored(name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets
             raise ValueError(f"{name}: slopes must have one entry per query head ({Hq},); got {tuple(slopes.shape)}")
         if slopes.dtype is not torch.float32:
             raise TypeError(f"{name}: slopes must be float32; got {slopes.dtype}")
-        if Hq // k.shape[1] > MAX_SLOPE_GROUP:
+        if Hq // kshape[1] > MAX_SLOPE_GROUP:
             raise ValueError(f"{name}: slopes take at most {MAX_SLOPE_GROUP} query heads per key head; got "
-                             f"{Hq // k.shape[1]}")
+                             f"{Hq // kshape[1]}")
         slopes = slopes.contiguous()
     if offsets is not None:
         if offsets.shape != (B,):
@@ -78,8 +84,7 @@ def _check_scored(name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets
         if offsets.dtype is not torch.int32:
             raise TypeError(f"{name}: query offsets must be int32; got {offsets.dtype}")
         offsets = offsets.contiguous()
-    lo, hi, wsb, mask, msb = _masks(name, window_lo, window_hi, key_mask, B, Lq, k.shape[2])
-    _require_gpu(name, q, k, v)
+    lo, hi, wsb, mask, msb = _masks(name, window_lo, window_hi, key_mask, B, Lq, kshape[2])
     _one_device(name, q, k, v, lo, hi, mask, slopes, offsets)
     return lo, hi, wsb, mask, msb, slopes, offsets
 

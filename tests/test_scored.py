@@ -72,7 +72,6 @@ def test_refusals(call, error):
 ])
 def test_backward_refusals(change, error, monkeypatch):
     # Past the device checks, which on a CPU tensor would come first.
-    monkeypatch.setattr(scored_ops, "_require_gpu", lambda *a: None)
     monkeypatch.setattr(scored_ops, "_one_device", lambda *a: None)
     t = {"dout": Q, "out": Q, "lse": torch.zeros(2, 4, 5), **change}
     with pytest.raises(error):
@@ -86,7 +85,6 @@ def test_backward_refusals(change, error, monkeypatch):
     (torch.tensor([[0, 0, 0, 0, 0], [0, 0, 2, 1, 3]], dtype=torch.int32), HI.expand(2, -1)),
 ])
 def test_backward_refuses_windows_out_of_order(lo, hi, capturing, error, match, monkeypatch):
-    monkeypatch.setattr(scored_ops, "_require_gpu", lambda *a: None)
     monkeypatch.setattr(scored_ops, "_one_device", lambda *a: None)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
     with pytest.raises(error, match=match):
