@@ -432,10 +432,12 @@ __global__ __launch_bounds__(512, 1) void bwd_dq_kernel(BwdArgs a) {
 // windows are staged, and a wave multiplies only those that meet its own
 // 32 rows' windows (the dK/dV kernel wrote the dS of exactly those: a
 // group's window union lies inside its 64-row tile's).
-template <int D, int BK, int NSTG, bool WIN, bool CT>
-__global__ __launch_bounds__(512, 1) void bwd_dq_ds_kernel(BwdArgs a) {
+// NW: waves (32 rows each) per workgroup; 4 for short grids of changed scores
+// (launch_dq_ds_d), two workgroups per CU.  The bits are the same.
+template <int D, int BK, int NSTG, bool WIN, bool CT, int NW = 8>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void bwd_dq_ds_kernel(BwdArgs a) {
   static_assert(!CT || WIN, "the compact dS layout (BwdArgs::ds_tab) is for windows");
-  constexpr int NW = 8, DT = D / 32;
+  constexpr int DT = D / 32;
   static_assert(BK == 32 || BK == 64, "stage of 32 or 64 keys");
   struct Stage {
     bf16 kt[D * BK];             // K^T: D rows of BK keys, TileLayout<BK>
@@ -453,8 +455,19 @@ __global__ __launch_bounds__(512, 1) void bwd_dq_ds_kernel(BwdArgs a) {
   const int nqb = (nqg + NW - 1) / NW;
   const int total = nqb * a.nkv * group;
   const int bid = xcd_remap_pairs(blockIdx.x, total, nqb * group, a.mask != nullptr);
-  const int qb = bid % nqb;
-  const int bq_rel = bid / nqb;             // (b, hq) within the pass
+  int qb = bid % nqb;
+  int bq_rel = bid / nqb;                   // (b, hq) within the pass
+  if constexpr (WIN) {
+    // Changed scores (causal and prefix masks): the row blocks with the most
+    // keys first, from whichever end the windows are wider (batch row 0 stands
+    // for all: any order is right).  (2,20,2304,128) with a prefix of 512: 76 ->
+    // 64 us.
+    if (a.score.mode != 0) {
+      longest_first(blockIdx.x, nqb, a.nkv * group, qb, bq_rel);
+      const int n = min(NW * 32, a.Lq);
+      if (a.whi[a.Lq - 1] - a.wlo[a.Lq - n] >= a.whi[n - 1] - a.wlo[0]) qb = nqb - 1 - qb;
+    }
+  }
   const int bq = a.kv0 * group + bq_rel;    // b*Hq + hq
   const int b = bq / a.Hq, h = bq % a.Hq;
   const int hk = h / group;
@@ -711,7 +724,20 @@ static void launch_dq_ds_d(const BwdArgs& a, hipStream_t stream) {
   // partial last round is not split as the dK/dV one is: this kernel is
   // bound by HBM, and the last round's workgroups share all of it (measured:
   // no gain at c3).
-  if (a.wlo && a.ds_tab)
+  // With changed scores, grids of few rounds in workgroups of 128 rows: more of
+  // them share a CU's latency, but K is staged twice as often.  Backward in 256
+  // against 128 rows, D 128: causal (1,4,1024) 16 workgroups of 256 rows 53.0 /
+  // 47.8 us, (1,16,2048) 128 115.8 / 105.4, (1,16 on 4 heads,4133) 272 299 / 286,
+  // (1,40,2304) 360 243.1 / 241.4 (with a prefix of 512 dQ alone 64 / 67), (1,16
+  // on 8 heads,8192) 512 856 / 881; no windows (1,2,16384) 128 849 / 796,
+  // (1,20,2304) 180 212 / 216, (1,8,8192) 256 795 / 818.
+  if (a.score.mode != 0 && !a.ds_tab && grid.x <= (a.wlo ? 300 : 160)) {
+    const dim3 short_grid((a.Lqp / 32 + 3) / 4 * a.nkv * group);
+    if (a.wlo)
+      hipLaunchKernelGGL((bwd_dq_ds_kernel<D, 64, 3, true, false, 4>), short_grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((bwd_dq_ds_kernel<D, 64, 3, false, false, 4>), short_grid, dim3(256), 0, stream, a);
+  } else if (a.wlo && a.ds_tab)
     hipLaunchKernelGGL((bwd_dq_ds_kernel<D, 64, 3, true, true>), grid, dim3(512), 0, stream, a);
   else if (a.wlo)
     hipLaunchKernelGGL((bwd_dq_ds_kernel<D, 64, 3, true, false>), grid, dim3(512), 0, stream, a);
