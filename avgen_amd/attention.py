@@ -687,8 +687,8 @@ def scored_attention(
     cache need no clearing.  bf16 or float32, head_dim 64 or 128;
     differentiable in query, key and value (windows non-decreasing in the
     row).  A few queries (up to 32, or 64 rows over the heads of a kv head;
-    float32 16) run on kernels that split the keys over the chip and read the
-    cache in place, without copies of it.
+    float32 16) and small calls run on kernels that split the keys over the
+    chip and read them in place, without copies.
     """
     _validate(query, key, value, 0.0, False, enable_gqa)
     if softcap is not None and not softcap > 0.0:

@@ -1,7 +1,7 @@
 // Attention forward of few query rows per kv head against many keys (one token
-// of every sequence, a handful of drafted ones), with or without changed
-// scores: the general forward's 128- or 256-row workgroups would idle, and its
-// operand copies read and write the whole cache first.
+// of every sequence, a handful of drafted ones), and of small calls, with or
+// without changed scores: the general forward's 128- or 256-row workgroups
+// would idle, and its operand copies read and write the whole cache first.
 //
 // HBM-bound: k and v are read once, in place, by as many workgroups as fill
 // the chip.  The rows of one kv head, Lq queries of its group of heads, form
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
 // float32, RB rows at a time on the vector ALUs (the fp32 matrix instructions
 // would multiply 32 rows whatever their number, and take longer than a tile's
 // 32 KB to arrive): 268 MB of cache in 46 us with one row per kv head, 5.8
-// TB/s, 55 us with 4; every 4 more rows read K and V again from the caches,
+// TB/s, 54 us with 4; every 4 more rows read K and V again from the caches,
 // about 39 us.  Scores: lane l owns key l % 32 of the wave's tile and half
 // of the channels, K from LDS (staged as above, rows of 256 bytes), q by
 // broadcast reads.  P V: a lane owns D / 64 channels, V's rows come straight
@@ -464,6 +464,24 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
   join_waves<D, float>(a, jn, unit, split, rows);
 }
 
+// A row from its joined parts.
+template <int D, bool F32>
+__device__ __forceinline__ void write_joined(const FewArgs& a, int unit, int r, float top, float sum, const f32x4& o,
+                                             int ch) {
+  const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
+  const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
+  float inv, lse;
+  finish_row(top, sum, inv, lse);
+  const RowPlace rp = row_place(a, hk, rb * a.block_rows + r);
+  const int64_t at = b * a.osb + rp.h * a.osh + (int64_t)rp.i * a.osl + ch;
+  if constexpr (F32)
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + at) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  else
+    *reinterpret_cast<u32x2*>(static_cast<bf16*>(a.o) + at) =
+        u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+  if (ch == 0) a.lse[((int64_t)b * a.Hq + rp.h) * a.Lq + rp.i] = lse;
+}
+
 // The parts of one row, in order: a workgroup of 256 threads takes one row;
 // D / 4 threads of four channels each per part, the parts dealt out over the
 // thread groups, joined through LDS in a fixed order.
@@ -472,10 +490,8 @@ __global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
   constexpr int TP = D / 4, G = 256 / TP;
   __shared__ float so[G][D], sl[G], st[4];
   const int unit = blockIdx.x / a.block_rows, r = blockIdx.x % a.block_rows;
-  const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
-  const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
   // (With one block of rows block_rows is their number, else a full block's.)
-  if (rb * a.block_rows + r >= a.Lq * (a.Hq / a.Hkv)) return;  // the whole workgroup
+  if (unit % a.row_blocks * a.block_rows + r >= a.Lq * (a.Hq / a.Hkv)) return;  // the whole workgroup
   const int64_t slot = few_slot_floats(a.block_rows, D);
   const float* part = a.part + (int64_t)unit * a.nsplit * slot;
   const float* ml = part + (int64_t)a.block_rows * D + 2 * r;
@@ -508,16 +524,58 @@ __global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += so[i][ch + e];
   }
-  float inv, lse;
-  finish_row(top, sum, inv, lse);
-  const RowPlace rp = row_place(a, hk, rb * a.block_rows + r);
-  const int64_t at = b * a.osb + rp.h * a.osh + (int64_t)rp.i * a.osl + ch;
-  if constexpr (F32)
-    *reinterpret_cast<f32x4*>(static_cast<float*>(a.o) + at) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  write_joined<D, F32>(a, unit, r, top, sum, o, ch);
+}
+
+// The same for up to kFewParts parts of many rows: D / 4 threads join a row
+// by themselves, in order.
+constexpr int kFewParts = 4;
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void few_combine_rows_kernel(FewArgs a) {
+  constexpr int TP = D / 4;
+  const int64_t u = (int64_t)blockIdx.x * (256 / TP) + threadIdx.x / TP;
+  const int ch = 4 * (threadIdx.x % TP);
+  const int64_t unit = u / a.block_rows;
+  const int r = (int)(u - unit * a.block_rows);
+  if (unit >= (int64_t)a.B * a.Hkv * a.row_blocks ||
+      (int)(unit % a.row_blocks) * a.block_rows + r >= a.Lq * (a.Hq / a.Hkv))
+    return;
+  const int64_t slot = few_slot_floats(a.block_rows, D);
+  const float* part = a.part + unit * a.nsplit * slot;
+  const float* ml = part + (int64_t)a.block_rows * D + 2 * r;
+  f32x4 x[kFewParts];
+  float m[kFewParts], l[kFewParts];
+#pragma unroll
+  for (int p = 0; p < kFewParts; ++p) {
+    const int64_t at = min(p, a.nsplit - 1) * slot;  // (a part again, left out below)
+    x[p] = *reinterpret_cast<const f32x4*>(part + at + (int64_t)r * D + ch);
+    m[p] = ml[at];
+    l[p] = ml[at + 1];
+  }
+  float top = m[0];
+#pragma unroll
+  for (int p = 1; p < kFewParts; ++p) top = fmaxf(top, m[p]);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < kFewParts; ++p) {
+    if (p >= a.nsplit) break;
+    const float wt = part_weight(m[p], top);
+    sum = fmaf(l[p], wt, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[p][e], wt, o[e]);
+  }
+  write_joined<D, F32>(a, (int)unit, r, top, sum, o, ch);
+}
+
+template <int D, bool F32>
+void launch_combine(const FewArgs& a, unsigned units, hipStream_t stream) {
+  const unsigned rows = units * (unsigned)a.block_rows;
+  if (a.nsplit <= kFewParts)
+    hipLaunchKernelGGL((few_combine_rows_kernel<D, F32>), dim3((rows + 1024 / D - 1) / (1024 / D)), dim3(256), 0, stream,
+                       a);
   else
-    *reinterpret_cast<u32x2*>(static_cast<bf16*>(a.o) + at) =
-        u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-  if (ch == 0) a.lse[((int64_t)b * a.Hq + rp.h) * a.Lq + rp.i] = lse;
+    hipLaunchKernelGGL((few_combine_kernel<D, F32>), dim3(rows), dim3(256), 0, stream, a);
 }
 
 template <int D>
@@ -536,32 +594,48 @@ void launch_few_f32(const FewArgs& a, dim3 grid, hipStream_t stream) {
 FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D, bool f32) {
   FewPlan p{};
   const int64_t rows = (int64_t)Lq * (Hq / Hkv);
-  // How many query rows are few: a block's time grows with the rows of its kv
-  // head, the general forward's with the heads.  8 sequences of 4,096 keys, 8
-  // kv heads of D 128, capped scores, this path against the general one (at
-  // one more query): bf16, 32 queries 51 / 122 us in groups of two heads,
-  // 83 / 171 of 4, 213 / 533 of 16, and 64 queries of single heads 51 / 93;
-  // float32, 16 queries 171 / 178 us of single heads, 523 / 648 in groups of
-  // 4, 1,035 / 1,242 of 8.  With fewer pairs or keys the distance grows.
-  if ((f32 ? Lq > kFewQueriesF32 : Lq > kFewQueries && rows > kFewRows) || Lk < 1) return p;
+  if (Lk < 1) return p;
   // Rows of a block: up to a tile's 32; float32 up to 4 (those of 8 spill).
   const int most_rows = f32 ? 4 : kTile;
   p.block_rows = (int)(rows < most_rows ? rows : most_rows);
-  p.row_blocks = (int)((rows + most_rows - 1) / most_rows);
-  const int64_t units = (int64_t)B * Hkv * p.row_blocks;
+  const int64_t units = (int64_t)B * Hkv * ((rows + most_rows - 1) / most_rows);
   // Workgroups the chip holds at once: one per CU at D 128 (LDS), two at 64.
   const int64_t slots = D == 128 ? 256 : 512;
-  // The fewest parts per unit whose rounds are shortest, each part with a tile
-  // for every wave.
-  const int most = (Lk + kWaves * kTile - 1) / (kWaves * kTile);
-  double best = 1e30;
+  // How many query rows are few.  Few queries: a block's time grows with the
+  // rows of its kv head, the general forward's with the heads.  8 sequences of
+  // 4,096 keys, 8 kv heads of D 128, capped scores, this path against the
+  // general one (at one more query): bf16, 32 queries 51 / 122 us in groups of
+  // two heads, 83 / 171 of 4, 213 / 533 of 16, and 64 queries of single heads
+  // 51 / 93; float32, 16 queries 171 / 178 us of single heads, 523 / 648 in
+  // groups of 4, 1,035 / 1,242 of 8.
+  const bool few_queries = f32 ? Lq <= kFewQueriesF32 : Lq <= kFewQueries || rows <= kFewRows;
+  // Small calls, whose blocks the chip holds at once (of long keys, a part of
+  // it): the general forward's workgroups are fewer and longer, and its copies
+  // a launch.  D 128: (1,4,128) 8 / 13 us, (1,4,1024) 18 / 31, (1,4,2048) 32 /
+  // 41, (1,8 on 2 heads,2048) 512 blocks 60 / 72 (not taken), (2,8,1024) 512 36
+  // / 34; (1,8 on 2 heads,128) x 8,192 keys 24 / 55, (1,32 on 8 heads,256) x
+  // 4,096 256 blocks 56 / 52.  float32: (1,4,256) 256 blocks 16 / 32, (1,4,512)
+  // 512 46 / 35, (1,8 on 2 heads,64) x 2,048 44 / 60, twice the heads 73 / 63.
+  const bool few_blocks = f32 ? units <= (Lk <= 512 ? slots : slots / 2) : units <= (Lk <= 2048 ? slots : slots / 4);
+  if (!few_queries && !few_blocks) return FewPlan{};
+  p.row_blocks = (int)((rows + most_rows - 1) / most_rows);
+  // Parts of a block's keys, each with a tile for every wave: rounds of
+  // workgroups at the measured times of a wave's tile (with one and with two
+  // workgroups on a CU) against the combination's launch and traffic.
+  const int tiles = (Lk + kTile - 1) / kTile, most = (tiles + kWaves - 1) / kWaves;
+  const float one = f32 ? (D == 128 ? 4.3f : 2.7f) : (D == 128 ? 1.55f : 1.4f);
+  const float two = f32 ? (D == 128 ? 4.3f : 4.4f) : (D == 128 ? 1.55f : 1.75f);
+  float best = 3e38f;
   for (int n = 1; n <= most && n <= 256; ++n) {
-    const double rounds = (double)((units * n + slots - 1) / slots) / n;
-    if (rounds < best * 0.95) {
-      best = rounds;
+    const int64_t wgs = units * n;
+    const int turns = (tiles + kWaves * n - 1) / (kWaves * n);
+    const float cost = (float)((wgs + slots - 1) / slots) * (turns * (wgs <= 256 ? one : two) + 4.5f) +
+                       (n > 1 ? 4.f + (float)wgs * p.block_rows * D * 1.1e-6f : 0.f);
+    if (cost < best) {
+      best = cost;
       p.nsplit = n;
     }
-    if (units * n >= slots) break;
+    if (wgs >= slots) break;
   }
   // Grids of 256 threads each, within 2^32: past that the general path, whose
   // grid is the smaller one.
@@ -592,15 +666,14 @@ hipError_t launch_few(const FewArgs& args, int D, bool f32, hipStream_t stream) 
   }
   if (p.nsplit > 1) {
     LaunchTimer timer(kKidMerge, stream);
-    const dim3 grid(units * p.block_rows);
     if (f32 && D == 128)
-      hipLaunchKernelGGL((few_combine_kernel<128, true>), grid, dim3(256), 0, stream, a);
+      launch_combine<128, true>(a, units, stream);
     else if (f32)
-      hipLaunchKernelGGL((few_combine_kernel<64, true>), grid, dim3(256), 0, stream, a);
+      launch_combine<64, true>(a, units, stream);
     else if (D == 128)
-      hipLaunchKernelGGL((few_combine_kernel<128, false>), grid, dim3(256), 0, stream, a);
+      launch_combine<128, false>(a, units, stream);
     else
-      hipLaunchKernelGGL((few_combine_kernel<64, false>), grid, dim3(256), 0, stream, a);
+      launch_combine<64, false>(a, units, stream);
   }
   return hipGetLastError();
 }

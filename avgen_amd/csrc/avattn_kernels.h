@@ -438,7 +438,8 @@ hipError_t launch_qk_norm_bwd(const QkNormArgs& a, int head_dim, float* dw, hipS
 hipError_t launch_qk_norm_dw_zero(float* dw, int head_dim, hipStream_t stream);
 
 // Forward of few query rows (attn_few.hip): at most kFewQueries of them, or
-// kFewRows over the group of a kv head; float32 kFewQueriesF32.
+// kFewRows over the group of a kv head; float32 kFewQueriesF32; and small calls
+// (few_plan).
 constexpr int kFewQueries = 32, kFewRows = 64, kFewQueriesF32 = 16;
 struct FewArgs {
   const void* q;

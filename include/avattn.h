@@ -956,8 +956,8 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * is_f32 (of 4).  lse: natural log of the changed scores' sum.
  *
  * A few queries (up to 32, or up to 64 rows len_q * heads_q / heads_kv; float32
- * up to 16) run on kernels of their own, which read k and v in place; their row
- * strides are then below 2^23.  flags: AVATTN_SCORED_SORTED_WINDOWS, the windows are
+ * up to 16) and small calls run on kernels of their own, which read k and v in
+ * place; the row strides of k and v are then below 2^23 (AVATTN_ERR_LAYOUT).  flags: AVATTN_SCORED_SORTED_WINDOWS, the windows are
  * non-decreasing in the row (spares a launch; wrong values otherwise).
  * workspace: avattn_fwd_scored_workspace_size bytes, 16-byte aligned.
  *

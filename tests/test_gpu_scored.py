@@ -156,9 +156,15 @@ SHAPES = [
     (2, 4, 2, 70, 130, 64),
     (2, 6, 6, 65, 65, 128),
     (1, 8, 2, 257, 300, 128),
-    (1, 4, 4, 400, 1100, 128),   # 256-row workgroups
+    (1, 4, 4, 400, 1100, 128),
     (1, 2, 1, 1000, 1025, 64),
     (1, 12, 3, 513, 513, 128),
+    # More row blocks than the few-row kernels take:
+    (2, 16, 16, 300, 333, 128),
+    (1, 36, 18, 515, 520, 64),
+    (1, 8, 8, 400, 2100, 128),
+    (1, 4, 4, 1000, 2500, 128),  # 256-row workgroups
+    (1, 12, 6, 700, 2300, 64),
 ]
 SCORES = [("cap", 20.0), ("slopes", None), ("both", 5.0), ("none", None)]
 MASKS = ["none", "causal", "sliding", "documents", "padding", "both"]
@@ -248,6 +254,11 @@ def test_few_rows_masks_float32(shape, kind, score):
     (torch.bfloat16, (1, 80, 2, 1, 300, 128)), (torch.float32, (1, 8, 2, 16, 300, 64)),
     (torch.float32, (1, 8, 2, 17, 300, 64)), (torch.float32, (2, 3, 3, 16, 200, 128)),
     (torch.float32, (2, 40, 2, 1, 200, 128)),
+    (torch.bfloat16, (1, 64, 64, 256, 256, 64)), (torch.bfloat16, (1, 64, 64, 257, 256, 64)),
+    (torch.bfloat16, (1, 32, 32, 256, 200, 128)), (torch.bfloat16, (1, 32, 32, 257, 200, 128)),
+    (torch.bfloat16, (1, 8, 8, 256, 2049, 128)), (torch.bfloat16, (1, 8, 8, 257, 2049, 128)),
+    (torch.float32, (1, 8, 8, 256, 512, 64)), (torch.float32, (1, 8, 8, 260, 512, 64)),
+    (torch.float32, (1, 8, 8, 128, 513, 64)), (torch.float32, (1, 8, 8, 132, 513, 64)),
 ], ids=str)
 def test_either_side_of_the_few_rows(dtype, shape):
     """The largest sizes of the few-row kernels and the next ones."""
@@ -262,7 +273,8 @@ def test_either_side_of_the_few_rows(dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("shape", [(2, 4, 2, 3, 300, 64), (2, 4, 2, 200, 300, 128), (1, 2, 2, 300, 1200, 128)])
+@pytest.mark.parametrize("shape", [(2, 4, 2, 3, 300, 64), (2, 4, 2, 200, 300, 128), (1, 2, 2, 300, 1200, 128),
+                                   (2, 72, 36, 200, 300, 64), (1, 16, 16, 1000, 1200, 128)])
 def test_windows_in_any_order(shape, dtype):
     """Forward only: windows that are not sorted, wider and narrower, empty,
     reversed or out of range (clamped)."""
@@ -279,10 +291,10 @@ def test_windows_in_any_order(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("Lq", [2, 300])
+@pytest.mark.parametrize("Lq, Hq, Hkv", [(2, 4, 2), (300, 4, 2), (300, 40, 20)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_what_unattended_keys_hold_never_counts(Lq, bad, dtype):
-    B, Hq, Hkv, Lk, D = 2, 4, 2, 310, 128
+def test_what_unattended_keys_hold_never_counts(Lq, Hq, Hkv, bad, dtype):
+    B, Lk, D = 2, 310, 128
     q, k, v, do = make(B, Hq, Hkv, Lq, Lk, D, dtype)
     mask = torch.rand((B, Lk), device="cuda") > 0.4
     mask[1, 200:] = False
@@ -308,34 +320,35 @@ def test_what_unattended_keys_hold_never_counts(Lq, bad, dtype):
             assert not t[dead[:, None].expand(B, Hkv, Lk)].any()
 
 
-@pytest.mark.parametrize("Lq", [1, 200])
-def test_garbage_in_queries_without_keys(Lq):
-    q, k, v, _ = make(1, 4, 2, Lq, 200, 64, torch.bfloat16)
+@pytest.mark.parametrize("Lq, heads", [(1, 4), (200, 4), (200, 160)])
+def test_garbage_in_queries_without_keys(Lq, heads):
+    q, k, v, _ = make(1, heads, heads // 2, Lq, 200, 64, torch.bfloat16)
     lo = torch.zeros(Lq, device="cuda", dtype=torch.int32)
     hi = torch.full_like(lo, 150)
     hi[Lq // 2:] = 0
     q[:, :, Lq // 2:] = float("nan")
-    for kw in (dict(softcap=9.0), dict(distance_slopes=slopes_of(4))):
+    for kw in (dict(softcap=9.0), dict(distance_slopes=slopes_of(heads))):
         out = A.scored_attention(q, k, v, window_lo=lo, window_hi=hi, enable_gqa=True, **kw)
         assert not out[:, :, Lq // 2:].any() and out.isfinite().all()
 
 
-def test_nan_key_reaches_the_rows_that_attend_it():
-    q, k, v, _ = make(1, 2, 2, 64, 64, 64, torch.bfloat16)
+@pytest.mark.parametrize("heads", [2, 264])
+def test_nan_key_reaches_the_rows_that_attend_it(heads):
+    q, k, v, _ = make(1, heads, heads, 64, 64, 64, torch.bfloat16)
     k[0, 0, 10] = float("nan")
     lo, hi, _ = windows("causal", 1, 64, 64)
     out = A.scored_attention(q, k, v, softcap=9.0, window_lo=lo, window_hi=hi)
-    assert out[0, 0, 10:].isnan().all() and out[0, 1].isfinite().all()
+    assert out[0, 0, 10:].isnan().all() and out[0, 1:].isfinite().all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("Lq", [3, 130])
+@pytest.mark.parametrize("Lq, Hq, Hkv", [(3, 4, 2), (130, 4, 2), (130, 128, 64)])
 @pytest.mark.parametrize("kw", [dict(cap=0.5), dict(cap=50.0, spread=40.0), dict(slope=30.0), dict(slope=-0.5),
                                 dict(slope=-3.0, cap=4.0), dict(cap=1e4), dict(slope=0.0)], ids=str)
-def test_extreme_scores(Lq, kw, dtype):
+def test_extreme_scores(Lq, Hq, Hkv, kw, dtype):
     """Caps far below and above the scores, scores far beyond the cap, slopes
     that leave one key and slopes that favour the farthest."""
-    B, Hq, Hkv, Lk, D = 1, 4, 2, 200, 64
+    B, Lk, D = 1, 200, 64
     q, k, v, do = make(B, Hq, Hkv, Lq, Lk, D, dtype, 11)
     q = (q.float() * kw.get("spread", 1.0)).to(dtype)
     slopes = None if "slope" not in kw else torch.full((Hq,), kw["slope"], device="cuda")
@@ -352,14 +365,16 @@ def test_extreme_scores(Lq, kw, dtype):
     o.check(out=out.detach(), dq=grads[0], dk=grads[1], dv=grads[2])
 
 
-def test_infinite_scores_with_a_cap_are_the_cap():
+@pytest.mark.parametrize("heads", [1, 180])
+def test_infinite_scores_with_a_cap_are_the_cap(heads):
     q = torch.full((1, 1, 70, 64), 3e38, device="cuda")
     k = torch.randn((1, 1, 70, 64), device="cuda").sign() * torch.ones((1, 1, 70, 1), device="cuda")
     k[:, :, ::2] = 1.0
     k[:, :, 1::2] = -1.0
     v = torch.randn((1, 1, 70, 64), device="cuda")
     for dtype in (torch.float32, torch.bfloat16):
-        out = A.scored_attention(q.to(dtype), k.to(dtype), v.to(dtype), softcap=2.0)
+        out = A.scored_attention(*(t.to(dtype).expand(1, heads, 70, 64) for t in (q, k, v)), softcap=2.0)
+        assert bool((out == out[:, :1]).all())
         w = torch.where(torch.arange(70, device="cuda") % 2 == 0, 2.0, -2.0).double().softmax(0)
         want = (w[:, None] * v.to(dtype)[0, 0].double()).sum(0)
         size = (w[:, None] * v[0, 0].double().abs()).sum(0)
@@ -392,11 +407,11 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("Lq", [2, 150])
-def test_layouts(Lq, dtype):
+@pytest.mark.parametrize("Lq, Hq, Hkv", [(2, 4, 2), (150, 4, 2), (150, 56, 28)])
+def test_layouts(Lq, Hq, Hkv, dtype):
     """Contiguous, (B, L, H, D) views, keys shared by expansion, slices of a
     cache, unaligned rows: the same values."""
-    B, Hq, Hkv, Lk, D = 2, 4, 2, 150, 64
+    B, Lk, D = 2, 150, 64
     q, k, v, _ = make(B, Hq, Hkv, Lq, Lk, D, dtype)
     base = A.scored_attention(q.contiguous(), k.contiguous(), v.contiguous(), softcap=7.0, enable_gqa=True)
     assert torch.equal(A.scored_attention(q, k, v, softcap=7.0, enable_gqa=True), base)
@@ -466,8 +481,9 @@ def test_staging_in_passes_and_compactly(dtype, monkeypatch):
             ops.set_ds_budget(None)
 
 
-def test_repeatable_on_any_stream():
-    q, k, v, do = make(1, 8, 2, 700, 700, 128, torch.bfloat16)
+@pytest.mark.parametrize("heads", [8, 16])
+def test_repeatable_on_any_stream(heads):
+    q, k, v, do = make(1, heads, heads // 4, 700, 700, 128, torch.bfloat16)
     lo, hi, _ = windows("causal", 1, 700, 700)
     leaves = [t.requires_grad_(True) for t in (q, k, v)]
 
@@ -487,12 +503,13 @@ def test_repeatable_on_any_stream():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize("heads", [4, 64])
+def test_captured_and_replayed(heads):
     """Two graphs, replayed in turn with eager calls between them."""
     L = 300
-    q, k, v, do = make(1, 4, 2, L, L, 64, torch.bfloat16)
+    q, k, v, do = make(1, heads, heads // 2, L, L, 64, torch.bfloat16)
     lo, hi, _ = windows("causal", 1, L, L)
-    slopes = slopes_of(4)
+    slopes = slopes_of(heads)
     scale = 0.125
     end = torch.full((1, 1), 200, device="cuda", dtype=torch.int32)
 

@@ -121,12 +121,12 @@ cpu_only = pytest.mark.skipif(torch.cuda.is_available(), reason="fake-pointer va
 
 @cpu_only
 @pytest.mark.parametrize("f32", [0, 1])
-@pytest.mark.parametrize("Lq", [1, 200])  # the few-row kernels and the others
+@pytest.mark.parametrize("Lq", [1, 5000])  # the few-row kernels and the others
 def test_c_entry_points_refuse(f32, Lq):
     lib = _lib.load()
     p, s = 4096, _lib.i64_array([64, 64, 64])
     odd = _lib.i64_array([64, 64, 66])
-    Lk = 300
+    Lk = 5000
 
     def fwd(q=p, k=p, v=p, qs=s, ks=s, vs=s, B=1, Hq=4, Hkv=2, Lq=Lq, Lk=Lk, D=64, mask=None, msb=0, lo=None, hi=None,
             wsb=0, scale=0.125, cap=10.0, slopes=None, offs=None, off=0, flags=0, out=p, os=s, lse=p, ws=p, nb=1 << 40):
