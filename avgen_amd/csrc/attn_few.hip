@@ -645,9 +645,8 @@ FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int D, bool f32) {
   return p;
 }
 
-hipError_t launch_few(const FewArgs& args, int D, bool f32, hipStream_t stream) {
+hipError_t launch_few(const FewArgs& args, const FewPlan& p, int D, bool f32, hipStream_t stream) {
   FewArgs a = args;
-  const FewPlan p = few_plan(a.B, a.Hq, a.Hkv, a.Lq, a.Lk, D, f32);
   a.nsplit = p.nsplit;
   a.row_blocks = p.row_blocks;
   a.block_rows = p.block_rows;

@@ -1146,8 +1146,11 @@ int score_args(float scale, float softcap, const float* slopes, const int32_t* o
   return AVATTN_OK;
 }
 
-bool takes_few(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool f32) {
-  return few_plan(B, Hq, Hkv, Lq, Lk, D, f32).nsplit > 0;
+// The forward's workspace where the few-row kernels do not take the call.
+size_t fwd_scored_general_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D, bool f32) {
+  const size_t hull = round256((size_t)B * 2 * sizeof(int));
+  if (f32) return round256(fwd_f32_split_bytes(B, Hq, Lq, Lk, D)) + hull;
+  return avattn_fwd_split_workspace_size(B, Hq, Hkv, Lq, Lk, D, 0) + hull;
 }
 
 }  // namespace
@@ -1158,11 +1161,9 @@ size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t 
                                         int32_t len_k, int32_t head_dim, int32_t is_f32) {
   if (check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim) != AVATTN_OK) return 0;
   if ((int64_t)batch * heads_q * len_q == 0 || len_k == 0) return 0;
-  if (takes_few(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0))
-    return few_plan(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0).bytes;
-  const size_t hull = round256((size_t)batch * 2 * sizeof(int));
-  if (is_f32) return round256(fwd_f32_split_bytes(batch, heads_q, len_q, len_k, head_dim)) + hull;
-  return avattn_fwd_split_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, 0) + hull;
+  const FewPlan few = few_plan(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0);
+  return few.nsplit > 0 ? few.bytes
+                        : fwd_scored_general_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0);
 }
 
 size_t avattn_bwd_scored_workspace_size(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len_q,
@@ -1195,17 +1196,21 @@ int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t
                   c.score);
   if (st != AVATTN_OK) return st;
   if ((int64_t)batch * heads_q * len_q == 0) return AVATTN_OK;
+  FewPlan plan{};
   if (len_k > 0) {
     if (key_mask && key_mask_batch_stride != 0 && key_mask_batch_stride < len_k) return AVATTN_ERR_ARGUMENT;
     st = check_windows(window_lo, window_hi, window_batch_stride, len_q, false);
     if (st != AVATTN_OK) return st;
-    const size_t need = avattn_fwd_scored_workspace_size(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32);
+    plan = few_plan(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0);
+    const size_t need = plan.nsplit > 0 ? plan.bytes
+                                        : fwd_scored_general_bytes(batch, heads_q, heads_kv, len_q, len_k, head_dim,
+                                                                   is_f32 != 0);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return AVATTN_ERR_WORKSPACE;
     workspace_bytes = need;
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool sorted = (flags & AVATTN_SCORED_SORTED_WINDOWS) != 0;
-  const bool few = len_k > 0 && takes_few(batch, heads_q, heads_kv, len_q, len_k, head_dim, is_f32 != 0);
+  const bool few = plan.nsplit > 0;
   if (!is_f32 && !few)
     return fwd_impl(q, k, v, q_strides, k_strides, v_strides, batch, heads_q, heads_kv, len_q, len_k, head_dim,
                     key_mask, key_mask_batch_stride, nullptr, nullptr, 0, false, nullptr, nullptr, scale, out,
@@ -1230,7 +1235,7 @@ int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t
   for (int64_t sl : {c.ksl, c.vsl})
     if (sl < 0 || sl >= ((int64_t)1 << 23)) return AVATTN_ERR_LAYOUT;
   c.part = static_cast<float*>(workspace);
-  return launch_status(launch_few(c, head_dim, is_f32 != 0, s));
+  return launch_status(launch_few(c, plan, head_dim, is_f32 != 0, s));
 }
 
 int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,

@@ -472,7 +472,7 @@ struct FewPlan {
   size_t bytes;
 };
 FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim, bool f32);
-hipError_t launch_few(const FewArgs& a, int head_dim, bool f32, hipStream_t stream);
+hipError_t launch_few(const FewArgs& a, const FewPlan& plan, int head_dim, bool f32, hipStream_t stream);
 // The float32 kernels with changed scores (attn_f32.hip): what their C entry
 // points check, with a status code.  The forward's workspace: split parts, then
 // the hull; the backward's tensors are float behind BwdArgs' pointers.
