@@ -682,9 +682,10 @@ def scored_attention(
             spares the backward's check (a host synchronisation) and a launch
             of the forward.  Wrong windows then give wrong values.
 
-    A row without a key returns zeros.  A key that no row of its batch entry
-    may attend contributes nothing, whatever it holds: the unused slots of a
-    cache need no clearing.  bf16 or float32, head_dim 64 or 128;
+    A row without a key returns zeros.  A key that ``attn_mask`` excludes or
+    that lies outside ``[window_lo.min(), window_hi.max())`` over the rows of
+    its batch entry contributes nothing, whatever it holds: the unused slots of
+    a cache need no clearing.  bf16 or float32, head_dim 64 or 128;
     differentiable in query, key and value (windows non-decreasing in the
     row).  A few queries (up to 32, or 64 rows over the heads of a kv head;
     float32 16) and small calls run on kernels that split the keys over the

@@ -140,9 +140,9 @@ struct FwdArgs {
   // writes the rows.
   float* part;
   int nsplit, nparts;
-  // Changed scores (mode 0: none).  With them a key that no row may attend
-  // (masked, or outside every window of its batch row) is copied as zeros in
-  // k and v, so that what it holds never reaches a row; hull as in key_hull.
+  // Changed scores (mode 0: none).  With them a key that is masked or outside
+  // the hull of its batch row's windows is copied as zeros in k and v, so that
+  // what it holds never reaches a row; hull as in key_hull.
   ScoreArgs score;
   int* hull;
 };

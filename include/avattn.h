@@ -951,8 +951,8 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * and avattn_fwd_windowed) and normalised.  slopes: float32 (heads_q) on the
  * device, any sign, at most 64 query heads per kv head with them; they and the
  * offsets get no gradient.  A row without a key: zeros and lse -inf.  A key
- * that no row of its batch entry may attend contributes nothing, whatever its
- * k and v hold (NaN included).  bf16 (strides multiples of 8), or float32 with
+ * that key_mask excludes, or outside [smallest window_lo, largest window_hi) of
+ * its batch row, contributes nothing, whatever its k and v hold (NaN included).  bf16 (strides multiples of 8), or float32 with
  * is_f32 (of 4).  lse: natural log of the changed scores' sum.
  *
  * A few queries (up to 32, or up to 64 rows len_q * heads_q / heads_kv; float32
