@@ -357,7 +357,8 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
   // of dS as four 16-byte stores per lane (group g = 2*sub + k2: the lane's
   // key, its 8 consecutive rows), each instruction 1 KB contiguous in unit
   // `sub`, in the first slot of each group's dK^T MFMAs.
-  const uint32_t ds_keep = STAGE && (SCORE ? live : key_valid()) ? 0xffffffffu : 0u;  // dS of masked / past-the-end keys is stored as 0
+  // dS of masked / past-the-end keys is stored as 0.
+  const uint32_t ds_keep = STAGE && (SCORE ? live : key_valid()) ? 0xffffffffu : 0u;
   const uint32_t ds_voff = DsUnit::store_offset(kw * 32 + l32, lane, 0, 0, 0);
 
   const float c = a.scale_log2;

@@ -309,7 +309,8 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
       for (int r = 0; r < 4; ++r) {
         if constexpr (SCORE) {
           float f;
-          const float z = changed_score_exact(a.score, s[4 * g + r], a.c, (float)(qpos - (t * KT + 8 * g + 4 * hh + r)), slope2, f);
+          const float kd = (float)(qpos - (t * KT + 8 * g + 4 * hh + r));
+          const float z = changed_score_exact(a.score, s[4 * g + r], a.c, kd, slope2, f);
           s[4 * g + r] = bb[r] < 0.f ? kNegInf : z;
         } else {
           s[4 * g + r] += bb[r];
@@ -962,11 +963,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void bwd_dq_ds_f32_kernel
   }
 }
 
-// Zeros over a (B, H, L, D) fp32 tensor (gradients of an empty side).
 // The same with changed scores where the workgroups above are too few for the
-// chip (up to 160 of 128 rows): 32 rows per workgroup, whose 4 waves take every fourth key tile and
-// are joined through LDS, in order.  No wave shares a tile, so K comes
-// straight from memory (a row's D floats per half wave, lane l32 the D / 32
+// chip (up to 160 of 128 rows): 32 rows per workgroup, whose 4 waves take
+// every fourth key tile and are joined through LDS, in order.  No wave shares
+// a tile, so K comes straight from memory (a row's D floats per half wave, lane l32 the D / 32
 // channels from l32 * D / 32), a tile ahead.  Backward with the kernel above
 // against this one, heads of 1,024 rows on half as many kv heads: 4 heads (32
 // workgroups above) 121 / 86 us at D 64, 201 / 137 at 128; 16 heads (128) 181 /
@@ -1058,6 +1058,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void bwd_dq_ds_f32_short_kern
   }
 }
 
+// Zeros over a (B, H, L, D) fp32 tensor (gradients of an empty side).
 __global__ void zero_f32_kernel(float* x, int64_t sb, int64_t sh, int64_t sl, int B, int H, int L, int D) {
   const int64_t n = (int64_t)B * H * L * (D / 4);
   for (int64_t u = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; u < n; u += (int64_t)gridDim.x * blockDim.x) {

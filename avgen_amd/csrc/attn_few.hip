@@ -406,7 +406,8 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
     const bf16* kr = sm.k[wave][buf][NS == 2 ? hh : 0];
 #pragma unroll
     for (int c = 0; c < HD / 4; ++c) {
-      const f32x4 k4 = *reinterpret_cast<const f32x4*>(kr + TileLayout<128>::off(l32, 8 * (NS == 2 ? c : hh * HD / 4 + c)));
+      const int chunk = NS == 2 ? c : hh * HD / 4 + c;
+      const f32x4 k4 = *reinterpret_cast<const f32x4*>(kr + TileLayout<128>::off(l32, 8 * chunk));
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
         const f32x4 q4 = *reinterpret_cast<const f32x4*>(&sq[r][hh * HD + 4 * c]);
@@ -572,8 +573,8 @@ template <int D, bool F32>
 void launch_combine(const FewArgs& a, unsigned units, hipStream_t stream) {
   const unsigned rows = units * (unsigned)a.block_rows;
   if (a.nsplit <= kFewParts)
-    hipLaunchKernelGGL((few_combine_rows_kernel<D, F32>), dim3((rows + 1024 / D - 1) / (1024 / D)), dim3(256), 0, stream,
-                       a);
+    hipLaunchKernelGGL((few_combine_rows_kernel<D, F32>), dim3((rows + 1024 / D - 1) / (1024 / D)), dim3(256), 0,
+                       stream, a);
   else
     hipLaunchKernelGGL((few_combine_kernel<D, F32>), dim3(rows), dim3(256), 0, stream, a);
 }

@@ -1126,7 +1126,8 @@ constexpr float kMaxCapBf16 = 1024.f;
 
 int score_args(float scale, float softcap, const float* slopes, const int32_t* offsets, int32_t offset, int32_t Hq,
                int32_t Hkv, bool f32, ScoreArgs& a) {
-  if (!(softcap >= 0.f) || !isfinite(softcap) || (!f32 && softcap > kMaxCapBf16) || offset > kMaxOffset || offset < -kMaxOffset)
+  if (!(softcap >= 0.f) || !isfinite(softcap) || (!f32 && softcap > kMaxCapBf16) || offset > kMaxOffset ||
+      offset < -kMaxOffset)
     return AVATTN_ERR_ARGUMENT;
   if (!aligned_to(slopes, 4) || !aligned_to(offsets, 4)) return AVATTN_ERR_LAYOUT;
   if (slopes && Hkv > 0 && Hq / Hkv > kMaxSlopeGroup) return AVATTN_ERR_TOO_LARGE;

@@ -396,8 +396,9 @@ hipError_t launch_quantize_rows(const bf16* x, int64_t sb, int64_t sh, int64_t s
 
 // Forward; the fp8 q k^T variant when a.k8 is set (a.q_scale, a.k_scale too).
 hipError_t launch_fwd(const FwdArgs& a, int head_dim, hipStream_t stream);
-// The changed-score kernels (attn_scored_fwd.hip, attn_scored_bwd.hip) of launch_fwd (its grid, in the
-// 128-row workgroups or not) and of launch_bwd's dK/dV step.
+// The changed-score kernels (attn_scored_fwd.hip, attn_scored_bwd.hip) of
+// launch_fwd (its grid, in the 128-row workgroups or not) and of launch_bwd's
+// dK/dV step.
 void launch_fwd_scored(const FwdArgs& a, int head_dim, bool small, dim3 grid, hipStream_t stream);
 void launch_dkdv_scored(const BwdArgs& a, int head_dim, dim3 grid, hipStream_t stream);
 // hull[2 b], hull[2 b + 1] of key_hull, over windows in any order.

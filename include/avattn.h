@@ -952,13 +952,15 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * device, any sign, at most 64 query heads per kv head with them; they and the
  * offsets get no gradient.  A row without a key: zeros and lse -inf.  A key
  * that key_mask excludes, or outside [smallest window_lo, largest window_hi) of
- * its batch row, contributes nothing, whatever its k and v hold (NaN included).  bf16 (strides multiples of 8), or float32 with
- * is_f32 (of 4).  lse: natural log of the changed scores' sum.
+ * its batch row, contributes nothing, whatever its k and v hold (NaN
+ * included).  bf16 (strides multiples of 8), or float32 with is_f32 (of 4).
+ * lse: natural log of the changed scores' sum.
  *
  * A few queries (up to 32, or up to 64 rows len_q * heads_q / heads_kv; float32
  * up to 16) and small calls run on kernels of their own, which read k and v in
- * place; the row strides of k and v are then below 2^23 (AVATTN_ERR_LAYOUT).  flags: AVATTN_SCORED_SORTED_WINDOWS, the windows are
- * non-decreasing in the row (spares a launch; wrong values otherwise).
+ * place; the row strides of k and v are then below 2^23 (AVATTN_ERR_LAYOUT).
+ * flags: AVATTN_SCORED_SORTED_WINDOWS, the windows are non-decreasing in the row
+ * (spares a launch; wrong values otherwise).
  * workspace: avattn_fwd_scored_workspace_size bytes, 16-byte aligned.
  *
  * Backward: windows non-decreasing in the row, dS always staged.  workspace:
