@@ -301,6 +301,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_ptr, c_i64p, c_ptr, c_i64p, c_ptr, c_i64p,
          c_ptr, c_size, c_ptr],
     ),
+    "avattn_bwd_scored_row_lse": (
+        ctypes.c_int,
+        [c_ptr] * 6 + [c_i64p] * 5 +
+        [c_i32] * 7 +
+        [c_ptr, c_i64, c_ptr, c_ptr, c_i64,
+         c_ptr, c_i64, c_i64,
+         c_f32, c_f32, c_ptr, c_ptr, c_i32,
+         c_ptr, c_i64p, c_ptr, c_i64p, c_ptr, c_i64p,
+         c_ptr, c_size, c_ptr],
+    ),
     "avattn_position_tables": (
         ctypes.c_int,
         [c_ptr, c_i32, c_i64, c_i32, c_i32, c_i32, c_ptr, ctypes.c_double, c_ptr, c_ptr, c_ptr],
@@ -349,6 +359,7 @@ BWD_DEFER_DQ = 8
 
 # avattn_fwd_scored flags (include/avattn.h).
 SCORED_SORTED_WINDOWS = 1
+SCORED_ROW_LSE = 4
 
 # avattn_ring_fwd_step flags (include/avattn.h).
 RING_FIRST = 1

@@ -682,6 +682,10 @@ def scored_attention(
             spares the backward's check (a host synchronisation) and a launch
             of the forward.  Wrong windows then give wrong values.
 
+    Distances cost the scores no bits, however far the queries lie from the
+    keys and whichever end of many keys a slope favours (exact integers up to
+    2^24 keys).
+
     A row without a key returns zeros.  A key that ``attn_mask`` excludes or
     that lies outside ``[window_lo.min(), window_hi.max())`` over the rows of
     its batch entry contributes nothing, whatever it holds: the unused slots of

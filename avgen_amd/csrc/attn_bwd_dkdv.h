@@ -47,6 +47,13 @@ namespace avattn {
 // bf16 like P) and keep P itself for dV, so the exchange stays one value per
 // score and the dS waves do not change.  A score outside its row's window gets
 // lse2 = +inf (P = 0 whatever the capped score is).
+// Distances are measured as BiasRef says.  A tile's rows mostly have their pos
+// among their keys in steps of one per row, or in steps of none (all of them
+// behind their last key, or before their first); with a slope < 0 the bias is
+// that of the distance from the far end of a row's keys, which moves by none or
+// two per row where the wave's keys lie on one side of pos.  Such tiles share
+// one form of the bias; in the others (`far`) each score's goes into its lse2
+// before its softmax step.
 template <int D, bool MASK, bool STAGE, bool WIN, bool CT, int SCORE = 0>
 __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
   static_assert(!SCORE || (STAGE && !MASK), "changed scores with staged dS only");
@@ -201,6 +208,8 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
   // Row statistics of the lane's rows 8*hh + ...: lse2 at sb, ndelta and
   // the windows at the offsets below.
   const uint32_t sb = opaque(lds_addr(&sm.rs[0].lse2[0]) + 32 * hh);
+  // The lane's row's window (SCORE with a bias).
+  const uint32_t wb = SCORE & kScoreDistance && WIN ? opaque(lds_addr(&sm.rs[0].wlo[0]) + 4 * lane) : 0u;
   constexpr uint32_t kNdlOff = BQ * 4, kWloOff = 2 * BQ * 4, kWhiOff = kWloOff + sizeof(sm.rs[0].wlo);
   static_assert(offsetof(RowStage, ndl) - offsetof(RowStage, lse2) == kNdlOff &&
                     offsetof(RowStage, wlo) - offsetof(RowStage, lse2) == kWloOff &&
@@ -362,12 +371,17 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
   const uint32_t ds_voff = DsUnit::store_offset(kw * 32 + l32, lane, 0, 0, 0);
 
   const float c = a.scale_log2;
-  // Distance bias: lane g holds the slope of the group's query head g.
+  // Distance bias: lane g holds the slope of the group's query head g; the hull
+  // of the attended keys (BiasRef).
   float slope_of = 0.f;
-  int qoff = 0;
+  int qoff = 0, hull_lo = 0, hull_hi = a.Lk;
   if constexpr (SCORE & kScoreDistance) {
     slope_of = a.score.slopes && lane < group ? a.score.slopes[hk * group + lane] * kLog2e : 0.f;
     qoff = __builtin_amdgcn_readfirstlane(a.score.query_offset(b));
+    if (masked && a.score.slopes) {
+      hull_lo = 64 * load_const_i32(a.khull, 2 * bhk);
+      hull_hi = min(64 * load_const_i32(a.khull, 2 * bhk + 1), a.Lk);
+    }
   }
 
   // The loop bodies below are explicitly software-pipelined: each "slot" is
@@ -403,10 +417,66 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
       l2[q8 >> 2][(q8 >> 1) & 1][q8 & 1] =
           lds_ld<f32x4>(sb + u * kRS + 4 * (32 * (q8 >> 2) + 16 * ((q8 >> 1) & 1) + 4 * (q8 & 1)));
     };
+    // The bias as the fast path has it: near2 (|slope2|; 0: far) times the
+    // distance of the lane's key from a point that moves by `step` per row (kd:
+    // from that of row 0 of the lane's first eight in this tile).
+    float kd = 0.f, slope2 = 0.f, step = 1.f, near2 = 0.f;
+    bool far = false;
+    int rlo = 0, rhi = 0;  // lane l: the window of row l of the tile
+    if constexpr (SCORE & kScoreDistance && WIN)
+      rlo = lds_ld<int>(wb + u * kRS), rhi = lds_ld<int>(wb + u * kRS + (kWhiOff - kWloOff));
     __builtin_amdgcn_sched_barrier(0);
 
     f32x16 s[2] = {zero16(), zero16()};
     bf16x8 pb[2][2];
+    // Row l's keys: its window, clamped, within the hull.
+    auto keys_of = [&](int lo, int hi, int& wl, int& wh) {
+      wl = min(max(lo, hull_lo), a.Lk);
+      wh = max(min(hi, hull_hi), wl);
+    };
+    auto place_bias = [&]() {
+      if constexpr (SCORE & kScoreDistance) {
+        slope2 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(slope_of), tile_head(it)));
+        const int r0 = tile_idx(it) * BQ, p0 = r0 + qoff;  // row 0 and its position
+        int wl = hull_lo, wh = hull_hi;
+        bool plain = !(slope2 < 0.f);  // every row's position is among its keys
+        if constexpr (WIN) {
+          keys_of(rlo, rhi, wl, wh);
+          const bool out = wl < wh && (uint32_t)(p0 + lane - wl) >= (uint32_t)(wh - wl);
+          plain = plain && __builtin_amdgcn_ballot_w64(out) == 0;
+        } else {
+          plain = plain && p0 >= wl && p0 + min(BQ, a.Lq - r0) <= wh;
+        }
+        kd = (float)(p0 + 8 * hh - key);
+        near2 = slope2;
+        if (__builtin_expect(!plain, 0)) {
+          const bool alive = wl < wh && (WIN || r0 + lane < a.Lq);
+          const uint64_t rows = __builtin_amdgcn_ballot_w64(alive);
+          const int f = rows != 0 ? __builtin_ctzll(rows) : 0;
+          auto all = [&](bool x) { return (rows & ~__builtin_amdgcn_ballot_w64(x)) == 0; };
+          const bool neg = slope2 < 0.f;
+          const BiasRef br = bias_ref(p0 + lane, wl, wh, neg);
+          int e = br.pos;
+          if (neg) {
+            // From the side of the row's pos on which its keys of this wave lie:
+            // ref - |pos - j| = |pos -+ ref - j|.
+            const int k0 = kt * BK + kw * 32;
+            const bool left = all(min(wh - 1, k0 + 31) <= br.pos), right = all(max(wl, k0) >= br.pos);
+            e += left ? -br.ref : br.ref;
+            far = !left && !right;
+          }
+          const int e0 = __builtin_amdgcn_readlane(e, f), n = lane - f;
+          int st = 1;
+          if (!all(e - e0 == n)) {
+            st = all(e == e0) ? 0 : 2;
+            far = far || (st == 2 && !all(e - e0 == 2 * n));
+          }
+          step = (float)st;
+          kd = (float)(e0 + st * (8 * hh - f) - key);
+          near2 = far ? 0.f : fabsf(slope2);
+        }
+      }
+    };
     u32x4 up[2][2];
     // WIN: a tile outside [w_ia, w_ib) masks the scores of a row half per
     // (row, key) before its softmax steps: one wave-uniform branch per half,
@@ -442,12 +512,28 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
     };
     // Softmax step (sub, k2, e2): two probabilities, packed; the last step
     // of a (sub, k2) hands its 16 bytes to the partner wave.
-    // Distance of the lane's key from row 0 of its first eight in this tile.
-    float kd = 0.f, slope2 = 0.f;
-    if constexpr (SCORE & kScoreDistance) {
-      kd = (float)(tile_idx(it) * BQ + 8 * hh + qoff - key);
-      slope2 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(slope_of), tile_head(it)));
-    }
+    auto far_sub = [&](int sub) {
+      if constexpr (SCORE & kScoreDistance) {
+        if (__builtin_expect(far, 0)) {
+          // Lane l has row l's bias; each lane fetches those of its rows.
+          int wl = hull_lo, wh = hull_hi;
+          if constexpr (WIN)
+            keys_of(lds_ld<int>(wb + u * kRS), lds_ld<int>(wb + u * kRS + (kWhiOff - kWloOff)), wl, wh);
+          const BiasRef br = bias_ref(tile_idx(it) * BQ + lane + qoff, wl, wh, slope2 < 0.f);
+          const int pos = __float_as_int((float)(br.pos - kt * BK)), ref = __float_as_int((float)br.ref);
+          const float kf = (float)(kw * 32 + l32);
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int from = 4 * (32 * sub + 16 * k2 + 8 * hh + e);
+              const float d = fabsf(__int_as_float(__builtin_amdgcn_ds_bpermute(from, pos)) - kf) -
+                              __int_as_float(__builtin_amdgcn_ds_bpermute(from, ref));
+              l2[sub][k2][e >> 2][e & 3] = fmaf(slope2, d, l2[sub][k2][e >> 2][e & 3]);
+            }
+        }
+      }
+    };
     u32x4 ux;  // SCORE: P (1 - tanh^2) of one (sub, k2)
     auto smx = [&](int sub, int k2, int e2) {
       const int e = 2 * e2;
@@ -469,7 +555,7 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
             z = fmaf(z, c, -lv[(e & 3) + i]);
           }
           if constexpr (SCORE & kScoreDistance)
-            z = fmaf(-slope2, fabsf(kd + (float)(32 * sub + 16 * k2 + e + i)), z);
+            z = fmaf(-near2, fabsf(fmaf(step, (float)(32 * sub + 16 * k2 + e + i), kd)), z);
           p[i] = __builtin_amdgcn_exp2f(z);
         }
         up[sub][k2][e2] = pack_bf16x2(p[0], p[1]);
@@ -497,9 +583,10 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
       s[sub] = mfma32(qa[j % kRA], kv[ks], s[sub]);
       if (j + kRA < NS) qa[j % kRA] = qop(j + kRA);
       if (j >= 1 && j <= 8) l2_read(j - 1);
+      if (j == 2) place_bias();
       if (j >= kLo) {
         const int n = NS - kLo;
-        if (j == kLo) mask_sub(0);
+        if (j == kLo) far_sub(0), mask_sub(0);
         for (int st = (j - kLo) * 8 / n; st < (j - kLo + 1) * 8 / n; ++st) smx(0, st >> 2, st & 3);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -507,10 +594,12 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
 #pragma unroll
     for (int q8 = NS - 1; q8 < 8; ++q8) l2_read(q8);  // what the loop had no slot for
     if (kLo >= NS) {
+      far_sub(0);
       mask_sub(0);
 #pragma unroll
       for (int st = 0; st < 8; ++st) smx(0, st >> 2, st & 3);
     }
+    far_sub(1);
     mask_sub(1);
 #pragma unroll
     for (int st = 0; st < 8; ++st) smx(1, st >> 2, st & 3);

@@ -71,6 +71,8 @@ struct F32Args {
   // changed scores (mode 0: none) and the forward's key hull, as in FwdArgs
   ScoreArgs score;
   const int* hull;
+  float* row_lse;    // forward (null: not wanted)
+  bool shifted_lse;  // backward: lse_in holds FwdArgs' lse, else its row_lse
 };
 
 // The keys some row of batch b may attend: what the others hold must not
@@ -107,6 +109,14 @@ __device__ __forceinline__ void row_window(const F32Args& a, int b, int r, int& 
   hi = min(max(a.whi[i], lo), a.Lk);
 }
 
+// What limits a row's keys [lo, hi) besides its window (rows_hull), a row per
+// lane at position p; with a bias.
+__device__ __forceinline__ void bias_hull(const F32Args& a, float slope, int b, int p, int lo, int hi, int& hull_lo,
+                                          int& hull_hi) {
+  rows_hull(a.score.slopes != nullptr && a.mask != nullptr ? a.mask + b * a.msb : nullptr, a.Lk, slope, p, lo, hi,
+            hull_lo, hull_hi);
+}
+
 // The 32-key tiles [t0, t1) meeting the union of the non-empty windows held
 // by the lanes of a workgroup's NW waves (every thread calls it: it holds a
 // barrier; red: 2*NW ints of LDS).
@@ -137,10 +147,10 @@ __device__ __forceinline__ bool rows_meet_block(const F32Args& a, int lo, int hi
 // 8*(i/4) + 4*(l/32) + i%4), maximum m (unit: its unit in natural log) and sum
 // l over all its keys.  l > 0:
 // normal row; l == 0: no valid key (out 0, lse -inf); NaN: a NaN or +inf
-// score reached the row.
+// score reached the row.  slope, distance: of a biased row (BiasRef).
 template <int D>
 __device__ __forceinline__ void write_row_f32(const F32Args& a, const f32x16 (&o)[D / 32], float m, float l, int bh,
-                                              int row, float unit) {
+                                              int row, float unit, float slope = 0.f, uint32_t distance = 0) {
   const int hh = (threadIdx.x >> 5) & 1;
   const float nan = __builtin_nanf("");
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : nan);
@@ -151,7 +161,11 @@ __device__ __forceinline__ void write_row_f32(const F32Args& a, const f32x16 (&o
     for (int g = 0; g < 4; ++g)
       st4(op + 32 * dt + 8 * g + 4 * hh,
           f32x4{o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv});
-  if (hh == 0) a.lse[(int64_t)bh * a.Lq + row] = l > 0.f ? fmaf(m, unit, logf(l)) : (l == 0.f ? kNegInf : nan);
+  if (hh == 0) {
+    const float lse = l > 0.f ? fmaf(m, unit, logf(l)) : (l == 0.f ? kNegInf : nan);
+    a.lse[(int64_t)bh * a.Lq + row] = distance != 0 ? lse_of_scores(lse, slope, distance) : lse;
+    if (a.row_lse != nullptr) a.row_lse[(int64_t)bh * a.Lq + row] = lse;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -217,13 +231,12 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
   const float* vb = a.v + b * a.vsb + hk * a.vsh;
   const float c = SCORE ? 1.f : a.c;  // the scores' unit in log2
   LiveKeys live{0, 0};
-  float slope2 = 0.f;
-  int qpos = 0;
+  float slope = 0.f;
   if constexpr (SCORE) {
     live.init(a, a.hull, b);
-    slope2 = a.score.slopes != nullptr ? a.score.slopes[h] * kLog2e : 0.f;
-    qpos = row + a.score.query_offset(b);
+    slope = a.score.slopes != nullptr ? a.score.slopes[h] : 0.f;
   }
+  const float slope2 = slope * kLog2e;
   auto loads = [&](int key) {
     if constexpr (SCORE) return live.has(a, b, key);
     return key < a.Lk;
@@ -273,6 +286,14 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
     if (valid) row_window(a, b, row, wl, wh);
     window_tiles<4>(wl, wh, valid, red, t0, ntile);
   }
+  BiasRef rb{0, 0};
+  if constexpr (SCORE) {
+    int lo = wl, hi = wh, hull_lo, hull_hi;
+    const int p = row + a.score.query_offset(b);
+    bias_hull(a, slope, b, p, lo, hi, hull_lo, hull_hi);
+    within_hull(hull_lo, hull_hi, lo, hi);
+    rb = bias_ref(p, lo, hi, slope < 0.f);
+  }
   if (SPLIT && part >= 0) {  // this part's share of the tiles (possibly none)
     const int n = ntile - t0;
     ntile = t0 + n * (part + 1) / a.nparts;
@@ -302,6 +323,7 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
     }
     // register i: key 8*(i/4) + 4*hh + i%4 of the tile, query l32
     float mt = kNegInf;
+    const float kd = (float)(rb.pos - (t * KT + 4 * hh)), ref = (float)rb.ref;  // (SCORE)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 bb = ld4(&bias[buf][8 * g + 4 * hh]);
@@ -309,8 +331,8 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
       for (int r = 0; r < 4; ++r) {
         if constexpr (SCORE) {
           float f;
-          const float kd = (float)(qpos - (t * KT + 8 * g + 4 * hh + r));
-          const float z = changed_score_exact(a.score, s[4 * g + r], a.c, kd, slope2, f);
+          const float d = fabsf(kd - (float)(8 * g + r)) - ref;
+          const float z = changed_score_exact(a.score, s[4 * g + r], a.c, d, slope2, f);
           s[4 * g + r] = bb[r] < 0.f ? kNegInf : z;
         } else {
           s[4 * g + r] += bb[r];
@@ -374,7 +396,11 @@ __global__ __launch_bounds__(256, 2) void fwd_f32_kernel(F32Args a) {
     if (hh == 0) slot[32 * D + l32] = m, slot[32 * D + 32 + l32] = l;
     return;
   }
-  if (valid) write_row_f32<D>(a, o, m, l, bh, row, SCORE ? kLn2 : a.scale);
+  if constexpr (SCORE) {
+    if (valid) write_row_f32<D>(a, o, m, l, bh, row, kLn2, slope, bias_distance(row + a.score.query_offset(b), rb));
+  } else {
+    if (valid) write_row_f32<D>(a, o, m, l, bh, row, a.scale);
+  }
 }
 
 // The split row blocks: one wave per 32 rows adds the parts in order, each
@@ -391,8 +417,19 @@ __global__ __launch_bounds__(64) void fwd_f32_combine_kernel(F32Args a) {
   float m, l;
   const bool log2_units = a.score.mode != 0;
   combine_parts<D>(slot, 4 * SLOT, a.nparts, log2_units ? 1.f : a.c, o, m, l);
-  const int row = bid % nqb * 128 + wave * 32 + l32;
-  if (row < a.Lq) write_row_f32<D>(a, o, m, l, bid / nqb, row, log2_units ? kLn2 : a.scale);
+  const int row = bid % nqb * 128 + wave * 32 + l32, bh = bid / nqb;
+  float slope = 0.f;
+  uint32_t distance = 0;
+  if (a.score.slopes != nullptr) {
+    const int b = bh / a.Hq, p = row + a.score.query_offset(b);
+    slope = a.score.slopes[bh % a.Hq];
+    int lo = 0, hi = a.Lk, hull_lo, hull_hi;
+    if (a.wlo != nullptr) row_window(a, b, min(row, a.Lq - 1), lo, hi);
+    bias_hull(a, slope, b, p, lo, hi, hull_lo, hull_hi);
+    within_hull(hull_lo, hull_hi, lo, hi);
+    distance = bias_distance(p, bias_ref(p, lo, hi, slope < 0.f));
+  }
+  if (row < a.Lq) write_row_f32<D>(a, o, m, l, bh, row, log2_units ? kLn2 : a.scale, slope, distance);
 }
 
 // Zeros to out and -inf to lse (no keys at all).
@@ -431,6 +468,25 @@ __global__ __launch_bounds__(256) void bwd_pre_f32_kernel(F32Args a) {
   a.ndelta[r] = -acc;
   const float l = a.lse_in[r];
   a.lse2[r] = l == kNegInf ? kPosInf : l * kLog2e;
+}
+
+// lse2 from the lse of biased scores (F32Args::shifted_lse): what BiasRef
+// leaves out goes back in.  One wave per 64 rows of a head.
+__global__ __launch_bounds__(64) void shift_lse2_f32_kernel(F32Args a) {
+  const int nb = (a.Lq + 63) / 64;
+  const int bh = blockIdx.x / nb, i = blockIdx.x % nb * 64 + threadIdx.x;
+  const int b = bh / a.Hq;
+  const float slope = a.score.slopes[bh % a.Hq];
+  int hull_lo, hull_hi, lo = 0, hi = a.Lk;
+  if (a.wlo != nullptr) row_window(a, b, min(i, a.Lq - 1), lo, hi);
+  const int p = i + a.score.query_offset(b);
+  bias_hull(a, slope, b, p, lo, hi, hull_lo, hull_hi);
+  if (i >= a.Lq) return;
+  within_hull(hull_lo, hull_hi, lo, hi);
+  const int64_t r = (int64_t)bh * a.Lq + i;
+  const float l = a.lse_in[r];
+  if (l != kNegInf)
+    a.lse2[r] = lse_from_scores(l, slope, bias_distance(p, bias_ref(p, lo, hi, slope < 0.f))) * kLog2e;
 }
 
 
@@ -509,6 +565,9 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
   __shared__ __attribute__((aligned(16))) float nds[3][QT];
   __shared__ __attribute__((aligned(16))) float px[2][4][16 * 64];
   __shared__ __attribute__((aligned(16))) int wls[WIN ? 2 : 1][QT], whs[WIN ? 2 : 1][QT];
+  // The rows' BiasRef (pos from the block's first key).
+  __shared__ __attribute__((aligned(16))) float bps[SCORE ? 2 : 1][SCORE ? QT : 4];
+  __shared__ __attribute__((aligned(16))) float brs[SCORE ? 2 : 1][SCORE ? QT : 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   const int pair = wave & 3, role = wave >> 2;  // role 0: P wave, 1: dS wave
@@ -521,12 +580,24 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
   const int k0 = kb * KPB + pair * 32;  // the pair's first key
   const int key = k0 + l32;
   bool kvalid = key_ok(a, b, key);
-  int qoff = 0;
+  int qoff = 0, hull_lo = 0, hull_hi = a.Lk;  // hull of the attended keys (BiasRef)
   if constexpr (SCORE) {
     LiveKeys live;
     live.init(a, nullptr, b);
     kvalid = live.has(a, b, key);
     qoff = a.score.query_offset(b);
+    if (a.mask != nullptr && a.score.slopes != nullptr) {
+      __shared__ int hred[8][2];
+      int lo, hi;
+      attended_share(a.mask + b * a.msb, a.Lk, tid, 512, lo, hi);
+      if (lane == 0) hred[wave][0] = lo, hred[wave][1] = hi;
+      __syncthreads();
+      hull_lo = 0x7fffffff, hull_hi = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) hull_lo = min(hull_lo, hred[w][0]), hull_hi = max(hull_hi, hred[w][1]);
+      hull_lo = __builtin_amdgcn_readfirstlane(hull_lo);
+      hull_hi = __builtin_amdgcn_readfirstlane(hull_hi);
+    }
   }
   float kv[HD];  // K (P wave) or V (dS wave) of the lane's key, k-step order
   load_row_ksteps<D>(kv,
@@ -603,7 +674,7 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
     const int64_t rbase = ((int64_t)b * a.Hq + h) * a.Lq;
     const float* qb = a.q + b * a.qsb + h * a.qsh;
     const float* db = a.dout + b * a.dosb + h * a.dosh;
-    const float slope2 = SCORE && a.score.slopes != nullptr ? a.score.slopes[h] * kLog2e : 0.f;
+    const float slope = SCORE && a.score.slopes != nullptr ? a.score.slopes[h] : 0.f, slope2 = slope * kLog2e;
     Tile32<D> sq, sd;
     float pl2 = kPosInf, pnd = 0.f;
     int pwl = 0, pwh = 0;
@@ -625,6 +696,12 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
       if (tid < QT) {
         l2s[u & 1][tid] = pl2, nds[u % 3][tid] = pnd;
         if constexpr (WIN) wls[u & 1][tid] = pwl, whs[u & 1][tid] = pwh;
+        if constexpr (SCORE) {
+          int lo = WIN ? pwl : 0, hi = WIN ? pwh : a.Lk;
+          within_hull(hull_lo, hull_hi, lo, hi);
+          const BiasRef br = bias_ref(u * QT + tid + qoff, lo, hi, slope < 0.f);
+          bps[u & 1][tid] = (float)(br.pos - kb * KPB), brs[u & 1][tid] = (float)br.ref;
+        }
       }
     };
     __syncthreads();  // the previous head's last tiles are consumed
@@ -655,7 +732,11 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4 L = ld4(&l2s[t & 1][8 * g + 4 * hh]);
-          f32x4 hand;
+          f32x4 hand, pos = {0.f, 0.f, 0.f, 0.f}, ref = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (SCORE) {
+            pos = ld4(&bps[t & 1][8 * g + 4 * hh]);
+            if (slope < 0.f) ref = ld4(&brs[t & 1][8 * g + 4 * hh]);
+          }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             bool in = kvalid;
@@ -665,8 +746,8 @@ __global__ __launch_bounds__(512) void bwd_dkdv_f32_kernel(F32Args a) {
             }
             if constexpr (SCORE) {
               float f;
-              const float kd = (float)(t * QT + 8 * g + 4 * hh + r + qoff - key);
-              const float z = changed_score_exact(a.score, s[4 * g + r], a.c, kd, slope2, f);
+              const float d = fabsf(pos[r] - (float)(pair * 32 + l32)) - ref[r];
+              const float z = changed_score_exact(a.score, s[4 * g + r], a.c, d, slope2, f);
               w[4 * g + r] = in ? __builtin_amdgcn_exp2f(z - L[r]) : 0.f;
               hand[r] = in ? w[4 * g + r] * f : 0.f;
             } else {
@@ -1410,6 +1491,9 @@ template <int D, bool WIN, bool SCORE = false>
 void launch_bwd_f32(F32Args a, int pairs_per_pass, hipStream_t s) {
   const int64_t rows = (int64_t)a.B * a.Hq * a.Lq;
   hipLaunchKernelGGL(bwd_pre_f32_kernel<D>, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, a);
+  if (SCORE && a.shifted_lse && a.score.slopes != nullptr)
+    hipLaunchKernelGGL(shift_lse2_f32_kernel, dim3((unsigned)((int64_t)a.B * a.Hq * ((a.Lq + 63) / 64))), dim3(64), 0,
+                       s, a);
   const int nkb = (a.Lk + 127) / 128;
   const int pairs = a.B * a.Hkv;
   if constexpr (!SCORE) if (pairs_per_pass == 0) {
@@ -1470,7 +1554,7 @@ static int fwd_f32_entry(const float* q, const float* k, const float* v, const i
                          int64_t key_mask_batch_stride, const int32_t* window_lo, const int32_t* window_hi,
                          int64_t window_batch_stride, float scale, float* out, const int64_t* out_strides,
                          float* lse, avattn_stream_t stream, void* workspace = nullptr, size_t workspace_bytes = 0,
-                         const ScoreArgs* score = nullptr, bool sorted_windows = false) {
+                         const ScoreArgs* score = nullptr, bool sorted_windows = false, float* row_lse = nullptr) {
   int st = check_f32_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
   st = check_f32_windows(window_lo, window_hi, window_batch_stride, len_q);
@@ -1507,6 +1591,7 @@ static int fwd_f32_entry(const float* q, const float* k, const float* v, const i
   }
   if (score) {
     a.score = *score;
+    a.row_lse = row_lse;
     if (window_lo && !sorted_windows) {
       // The caller's workspace ends with room for the hull.
       int* hull = reinterpret_cast<int*>(static_cast<char*>(workspace) + workspace_bytes - r256((size_t)batch * 8));
@@ -1600,7 +1685,7 @@ static int bwd_f32_entry(const float* dout, const float* q, const float* k, cons
                          const int32_t* window_lo, const int32_t* window_hi, int64_t window_batch_stride,
                          float scale, float* dq, const int64_t* dq_strides, float* dk, const int64_t* dk_strides,
                          float* dv, const int64_t* dv_strides, void* workspace, size_t workspace_bytes,
-                         avattn_stream_t stream, const ScoreArgs* score = nullptr) {
+                         avattn_stream_t stream, const ScoreArgs* score = nullptr, bool shifted_lse = false) {
   int st = check_f32_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
   st = check_f32_windows(window_lo, window_hi, window_batch_stride, len_q);
@@ -1682,6 +1767,7 @@ static int bwd_f32_entry(const float* dout, const float* q, const float* k, cons
   if (score) {
     if (pp == 0) return AVATTN_ERR_WORKSPACE;
     a.score = *score;
+    a.shifted_lse = shifted_lse;
     if (head_dim == 128)
       window_lo ? launch_bwd_f32<128, true, true>(a, pp, s) : launch_bwd_f32<128, false, true>(a, pp, s);
     else
@@ -1878,7 +1964,7 @@ int fwd_scored_f32(const FewArgs& c, int head_dim, float scale, bool sorted_wind
   return fwd_f32_entry(static_cast<const float*>(c.q), static_cast<const float*>(c.k), static_cast<const float*>(c.v),
                        qs, ks, vs, c.B, c.Hq, c.Hkv, c.Lq, c.Lk, head_dim, c.mask, c.msb, c.wlo, c.whi, c.wsb, scale,
                        static_cast<float*>(c.o), os, c.lse, stream, workspace, workspace_bytes, &c.score,
-                       sorted_windows);
+                       sorted_windows, c.row_lse);
 }
 
 int bwd_scored_f32(const BwdArgs& c, int head_dim, void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -1889,7 +1975,7 @@ int bwd_scored_f32(const BwdArgs& c, int head_dim, void* workspace, size_t works
   auto w = [](bf16* p) { return reinterpret_cast<float*>(p); };
   return bwd_f32_entry(f(c.dout), f(c.q), f(c.k), f(c.v), f(c.out), c.lse, ds, qs, ks, vs, os, c.B, c.Hq, c.Hkv, c.Lq,
                        c.Lk, head_dim, c.mask, c.msb, c.wlo, c.whi, c.wsb, c.scale, w(c.dq), dqs, w(c.dk), dks,
-                       w(c.dv), dvs, workspace, workspace_bytes, stream, &c.score);
+                       w(c.dv), dvs, workspace, workspace_bytes, stream, &c.score, c.shifted_lse);
 }
 
 }  // namespace avattn

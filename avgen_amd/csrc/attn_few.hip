@@ -74,14 +74,41 @@ __device__ __forceinline__ BlockWindows block_windows(const FewArgs& a, int b, i
   return w;
 }
 
-// Changes one raw score (uniform mode); kd: the row's position minus the key.
-__device__ __forceinline__ float changed_score(const FewArgs& a, float s, float kd, float slope2) {
+// The bias of this lane's row (its clamped window in w; all of the wave).
+struct RowBias {
+  BiasRef at;
+  float slope, slope2;
+  uint32_t distance;
+  __device__ __forceinline__ void init(const FewArgs& a, const BlockWindows& w, int b, const RowPlace& rp) {
+    at = {0, 0}, slope = slope2 = 0.f, distance = 0;
+    if (!(a.score.mode & kScoreDistance)) return;
+    slope = a.score.slopes != nullptr ? a.score.slopes[rp.h] : 0.f;
+    slope2 = slope * kLog2e;
+    int lo = w.lo, hi = w.hi, hull_lo, hull_hi;
+    const int p = rp.i + a.score.query_offset(b);
+    rows_hull(a.score.slopes != nullptr && a.mask != nullptr ? a.mask + b * a.msb : nullptr, a.Lk, slope, p, lo, hi,
+              hull_lo, hull_hi);
+    within_hull(hull_lo, hull_hi, lo, hi);
+    at = bias_ref(p, lo, hi, slope < 0.f);
+    distance = bias_distance(p, at);
+  }
+};
+
+// A row's logsumexp from that of its computed scores, to both arrays.
+__device__ __forceinline__ void store_lse(const FewArgs& a, int b, const RowPlace& p, float lse, uint32_t distance) {
+  const int64_t at = ((int64_t)b * a.Hq + p.h) * a.Lq + p.i;
+  a.lse[at] = a.score.slopes != nullptr ? lse_of_scores(lse, a.score.slopes[p.h], distance) : lse;
+  if (a.row_lse != nullptr) a.row_lse[at] = lse;
+}
+
+// Changes one raw score (uniform mode); kd: the row's pos minus the key.
+__device__ __forceinline__ float changed_score(const FewArgs& a, float s, float kd, float ref, float slope2) {
   float z;
   if (a.score.mode & kScoreCap)
     z = fmaf(-2.f * a.score.cap2, cap_complement(s, a.score.cap_arg), a.score.cap2);
   else
     z = s * a.scale_log2;
-  return fmaf(-slope2, fabsf(kd), z);
+  return fmaf(-slope2, fabsf(kd) - ref, z);
 }
 
 // What the waves of a workgroup leave of their rows, to be joined.
@@ -90,6 +117,7 @@ struct Join {
   static constexpr int kPitch = D + 4;
   float o[kWaves][ROWS * kPitch];
   float m[kWaves][ROWS], l[kWaves][ROWS];
+  uint32_t distance[ROWS];  // bias_distance (wave 0 writes it)
 };
 
 // The waves' parts of the block's rows, in order: to the rows themselves, or to
@@ -117,7 +145,10 @@ __device__ __forceinline__ void join_waves(const FewArgs& a, const Join<D, ROWS>
 #pragma unroll
       for (int e = 0; e < 8; e += 4)
         *reinterpret_cast<f32x4*>(part + r * D + ch + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
-      if (ch == 0) part[a.block_rows * D + 2 * r] = top, part[a.block_rows * D + 2 * r + 1] = sum;
+      if (ch == 0) {
+        float* ml = part + a.block_rows * D + 3 * r;
+        ml[0] = top, ml[1] = sum, ml[2] = __uint_as_float(jn.distance[r]);
+      }
     } else {
       float inv, lse;
       finish_row(top, sum, inv, lse);
@@ -132,7 +163,7 @@ __device__ __forceinline__ void join_waves(const FewArgs& a, const Join<D, ROWS>
         *reinterpret_cast<f32x4*>(out) = f32x4{o[0], o[1], o[2], o[3]};
         *reinterpret_cast<f32x4*>(out + 4) = f32x4{o[4], o[5], o[6], o[7]};
       }
-      if (ch == 0) a.lse[((int64_t)b * a.Hq + p.h) * a.Lq + p.i] = lse;
+      if (ch == 0) store_lse(a, b, p, lse, jn.distance[r]);
     }
   }
 }
@@ -172,8 +203,10 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
       qf[ks] = bits_to_bf16x8(x);
     }
   }
-  const int qpos = rp.i + a.score.query_offset(b);
-  const float slope2 = a.score.slopes != nullptr ? a.score.slopes[rp.h] * kLog2e : 0.f;
+  RowBias rbias;
+  rbias.init(a, w, b, rp);
+  const int qpos = rbias.at.pos;
+  const float slope2 = rbias.slope2, ref = (float)rbias.at.ref;
 
   // Tiles of this wave: the block's tiles, a range per workgroup, every
   // fourth of it per wave.
@@ -240,7 +273,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
     for (int ks = 0; ks < KS; ++ks) s = mfma32(row_operand<D>(sg.k, prow, 16 * ks + 8 * hh), qf[ks], s);
     const float kd = (float)(qpos - (t * kTile + 8 * hh));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = changed_score(a, s[r], kd - (float)(16 * (r >> 3) + (r & 7)), slope2);
+    for (int r = 0; r < 16; ++r) s[r] = changed_score(a, s[r], kd - (float)(16 * (r >> 3) + (r & 7)), ref, slope2);
     if (keys != 0xffffffffu || t * kTile < w.all_lo || t * kTile + kTile > w.all_hi) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -291,7 +324,10 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
   l = halves_sum(l);
   __syncthreads();  // every wave is done with its stages
   auto& jn = sm.join;
-  if (hh == 0) jn.m[wave][l32] = m, jn.l[wave][l32] = l;
+  if (hh == 0) {
+    jn.m[wave][l32] = m, jn.l[wave][l32] = l;
+    if (wave == 0) jn.distance[l32] = rbias.distance;
+  }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -319,6 +355,7 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
     Join<D, RB> join;
   } sm;
   __shared__ __attribute__((aligned(16))) float sq[RB][D];
+  __shared__ float sneg[RB][2];  // the rows' slopes < 0, negated, and BiasRef::ref
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -331,8 +368,14 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
   const RowPlace rp = row_place(a, hk, rb * RB + (valid ? l32 : 0));
   const BlockWindows w = block_windows(a, b, rp.i, valid);
   // Row r's values are lane r's.
-  const int qpos = rp.i + a.score.query_offset(b);
-  const float slope2 = a.score.slopes != nullptr ? a.score.slopes[rp.h] * kLog2e : 0.f;
+  RowBias rbias;
+  rbias.init(a, w, b, rp);
+  const int qpos = rbias.at.pos;
+  const float slope2 = fmaxf(rbias.slope2, 0.f);
+  // A slope < 0: its bias is added in a step of its own (with a reference to
+  // subtract in the other slopes' code 4 rows took 59 us in place of 55).
+  if (wave == 0 && lane < RB) sneg[lane][0] = fmaxf(-rbias.slope2, 0.f), sneg[lane][1] = (float)rbias.at.ref;
+  const bool farthest = __builtin_amdgcn_ballot_w64(rbias.slope2 < 0.f) != 0;
   for (int u = tid; u < RB * (D / 4); u += 256) {
     const int r = u / (D / 4), c = 4 * (u % (D / 4));
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -423,7 +466,12 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
       const int pos = __builtin_amdgcn_readlane(qpos, r);
       const float sl = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(slope2), r));
       float f;
-      float z = changed_score_exact(a.score, halves_sum(s[r]), a.scale_log2, (float)(pos - key), sl, f);
+      const float d = fabsf((float)(pos - key));
+      float z = changed_score_exact(a.score, halves_sum(s[r]), a.scale_log2, d, sl, f);
+      if (farthest) {
+        __asm__ volatile("; a negative slope");
+        z = fmaf(sneg[r][0], d - sneg[r][1], z);
+      }
       if (!live_key || key < lo || key >= hi) z = kNegInf;
       if (__builtin_amdgcn_ballot_w64(z > m[r] + 8.f) != 0) {  // rare after the first tiles
         float mx = z;
@@ -458,6 +506,7 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     if (lane == 0) jn.m[wave][r] = m[r], jn.l[wave][r] = sum;
+    if (wave == 0 && lane == r) jn.distance[r] = rbias.distance;
 #pragma unroll
     for (int e = 0; e < CL; ++e) jn.o[wave][r * jn.kPitch + CL * lane + e] = acc[r][e];
   }
@@ -467,8 +516,8 @@ __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
 
 // A row from its joined parts.
 template <int D, bool F32>
-__device__ __forceinline__ void write_joined(const FewArgs& a, int unit, int r, float top, float sum, const f32x4& o,
-                                             int ch) {
+__device__ __forceinline__ void write_joined(const FewArgs& a, int unit, int r, float top, float sum,
+                                             uint32_t distance, const f32x4& o, int ch) {
   const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
   const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
   float inv, lse;
@@ -480,7 +529,7 @@ __device__ __forceinline__ void write_joined(const FewArgs& a, int unit, int r, 
   else
     *reinterpret_cast<u32x2*>(static_cast<bf16*>(a.o) + at) =
         u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-  if (ch == 0) a.lse[((int64_t)b * a.Hq + rp.h) * a.Lq + rp.i] = lse;
+  if (ch == 0) store_lse(a, b, rp, lse, distance);
 }
 
 // The parts of one row, in order: a workgroup of 256 threads takes one row;
@@ -495,7 +544,7 @@ __global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
   if (unit % a.row_blocks * a.block_rows + r >= a.Lq * (a.Hq / a.Hkv)) return;  // the whole workgroup
   const int64_t slot = few_slot_floats(a.block_rows, D);
   const float* part = a.part + (int64_t)unit * a.nsplit * slot;
-  const float* ml = part + (int64_t)a.block_rows * D + 2 * r;
+  const float* ml = part + (int64_t)a.block_rows * D + 3 * r;
   float top = kNegInf;
   for (int p = threadIdx.x; p < a.nsplit; p += 256) top = fmaxf(top, ml[p * slot]);
 #pragma unroll
@@ -525,7 +574,7 @@ __global__ __launch_bounds__(256) void few_combine_kernel(FewArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += so[i][ch + e];
   }
-  write_joined<D, F32>(a, unit, r, top, sum, o, ch);
+  write_joined<D, F32>(a, unit, r, top, sum, __float_as_uint(ml[2]), o, ch);
 }
 
 // The same for up to kFewParts parts of many rows: D / 4 threads join a row
@@ -543,7 +592,7 @@ __global__ __launch_bounds__(256) void few_combine_rows_kernel(FewArgs a) {
     return;
   const int64_t slot = few_slot_floats(a.block_rows, D);
   const float* part = a.part + unit * a.nsplit * slot;
-  const float* ml = part + (int64_t)a.block_rows * D + 2 * r;
+  const float* ml = part + (int64_t)a.block_rows * D + 3 * r;
   f32x4 x[kFewParts];
   float m[kFewParts], l[kFewParts];
 #pragma unroll
@@ -566,7 +615,7 @@ __global__ __launch_bounds__(256) void few_combine_rows_kernel(FewArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(x[p][e], wt, o[e]);
   }
-  write_joined<D, F32>(a, (int)unit, r, top, sum, o, ch);
+  write_joined<D, F32>(a, (int)unit, r, top, sum, __float_as_uint(ml[2]), o, ch);
 }
 
 template <int D, bool F32>

@@ -44,18 +44,26 @@ __device__ __forceinline__ void row_block(const FwdArgs& a, int bid, int nqt, in
   qt = nqt - 1 - rank;
 }
 
+// What limits a row's keys [lo, hi) besides its window (rows_hull), a row per
+// lane at position p; with a bias.
+__device__ __forceinline__ void bias_hull(const FwdArgs& a, float slope, int b, int p, int lo, int hi, int& hull_lo,
+                                          int& hull_hi) {
+  rows_hull(a.score.slopes != nullptr && a.mask != nullptr ? a.mask + b * a.msb : nullptr, a.Lk, slope, p, lo, hi,
+            hull_lo, hull_hi);
+}
+
 // Writes one wave's 32 output rows row0 .. of (b, h) = bh: acc[dt][4*g + r] of
 // lane l is channel 32*dt + 8*g + 4*(l/32) + r of row l%32, times inv; lse
-// per lane row.
+// per lane row.  BIAS: of scores with a bias, moved by slope * distance.
 // The output leaves through LDS (ep: 32*D elements nothing else
 // uses), so that each store instruction covers whole rows: in the C
 // layout a lane holds 4 consecutive channels, and a store would touch 32
 // rows for 16 bytes each (with few keys per row that cost more than the
 // products: 75,600 queries x 512 keys, fwd+bwd, 5.59 -> 5.29 ms with
 // the dQ kernel's, (2,20,3600,128) forward 331 -> 326 us).
-template <int D>
+template <int D, bool BIAS = false>
 __device__ __forceinline__ void write_rows(const FwdArgs& a, const f32x16 (&acc)[D / 32], float inv, float lse,
-                                           bf16* ep, int bh, int row0) {
+                                           bf16* ep, int bh, int row0, float slope = 0.f, uint32_t distance = 0) {
   constexpr int DT = D / 32;
   const int lane = threadIdx.x & 63;
   const int l32 = lane & 31, hh = lane >> 5;
@@ -74,7 +82,12 @@ __device__ __forceinline__ void write_rows(const FwdArgs& a, const f32x16 (&acc)
   const int er = lane / kCpr, ec = 8 * (lane % kCpr);
   bf16* op = a.o + b * a.osb + h * a.osh + ec;
   if (a.o_acc == nullptr) {
-    if (qvalid && hh == 0) a.lse[(int64_t)bh * a.Lq + row0 + l32] = lse;
+    if (qvalid && hh == 0) {
+      const int64_t at = (int64_t)bh * a.Lq + row0 + l32;
+      a.lse[at] = BIAS ? lse_of_scores(lse, slope, distance) : lse;
+      if constexpr (BIAS)
+        if (a.row_lse != nullptr) a.row_lse[at] = lse;
+    }
 #pragma unroll
     for (int i = 0; i < 32 / kRpi; ++i) {
       const int r = i * kRpi + er;
@@ -162,14 +175,17 @@ __device__ __forceinline__ void write_rows(const FwdArgs& a, const f32x16 (&acc)
 // score outside its row's window to -inf (before the key bias and softmax).
 //
 // SCORE (kScoreCap, kScoreDistance or both; FwdArgs::score): each raw score
-// becomes cap tanh(s / cap) and / or loses slope |distance|, in log2 units,
-// before the masks.  tanh(x) = 1 - 2 / (1 + e^2x) is one exp2 and one
-// reciprocal, whose 2^-23 relative errors leave the score within cap * 2^-22;
-// the softmax then runs in log2 units, its score bound capped too.  These
-// transcendentals make the VALU phase the longer one: per score 7 operations
-// of which 3 transcendental with the cap, against 4 and 1 without.
+// becomes cap tanh(s / cap) and / or loses slope |distance| (measured as BiasRef
+// says), in log2 units, before the masks.  tanh(x) = 1 - 2 / (1 + e^2x) is one
+// exp2 and one reciprocal, whose 2^-23 relative errors leave the score within
+// cap * 2^-22; the softmax then runs in log2 units, its score bound capped too.
+// These transcendentals make the VALU phase the longer one: per score 7
+// operations of which 3 transcendental with the cap, against 4 and 1 without.
+// (D 64 is held to the registers of three workgroups a CU; a bias without
+// windows would take three more: 219 -> 230 us for 32 heads of 4,096 tokens.)
 template <int D, bool ROPE, bool FP8, bool WIN, bool SMALL, int SCORE = 0>
-__global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? (D == 64 && SCORE ? 3 : 2) : 1)
+void attn_fwd_kernel(FwdArgs a) {
   static_assert(!SCORE || (!ROPE && !FP8), "score changes on rotated bf16 operands only");
   static_assert(!(ROPE && FP8), "the fp8 variant takes rotated q");
   static_assert(!(WIN && FP8), "windows on the bf16 path only");
@@ -411,9 +427,26 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
   constexpr bool kAsComplement = SCORE == kScoreCap;
   constexpr float kMasked = kAsComplement ? kPosInf : kNegInf;
   const float capm2 = -2.f * a.score.cap2;
-  // Distances run from this lane's query position.
-  const int qpos = SCORE & kScoreDistance ? qrow + a.score.query_offset(b) : 0;
-  const float slope2 = SCORE & kScoreDistance && a.score.slopes ? a.score.slopes[h] * kLog2e : 0.f;
+  // Distances run from this lane's row's pos (BiasRef).
+  const float slope = SCORE & kScoreDistance && a.score.slopes ? a.score.slopes[h] : 0.f;
+  const bool farthest = slope < 0.f;
+  // |slope| in log2 units (uniform, but formed by a vector instruction).
+  const float near2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fabsf(slope * kLog2e))));
+  // The row's bias is |slope| times the distance from a point (BiasRef): its pos
+  // with a slope >= 0; else the far end of its keys as ref - |pos - j| = |pos -+
+  // ref - j| has it, for keys to the left and to the right of pos.
+  int from_left = 0, from_right = 0, hull_lo = 0, hull_hi = 0;
+  auto row_bias = [&](int p) __attribute__((always_inline)) {
+    int lo = WIN ? wlo : 0, hi = WIN ? min(whi, a.Lk) : a.Lk;
+    within_hull(hull_lo, hull_hi, lo, hi);
+    return bias_ref(p, lo, hi, farthest);
+  };
+  if constexpr (SCORE & kScoreDistance) {
+    const int p = qrow + a.score.query_offset(b);
+    bias_hull(a, slope, b, p, WIN ? wlo : 0, WIN ? min(whi, a.Lk) : a.Lk, hull_lo, hull_hi);
+    const BiasRef r = row_bias(p);
+    from_left = r.pos - r.ref, from_right = r.pos + r.ref;
+  }
   float bound = kPosInf;
   if constexpr (FP8) {
     if (a.kmax2 != nullptr) {
@@ -456,9 +489,7 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
       if constexpr (SCORE != 0) {
         bound *= a.scale_log2;
         if constexpr (SCORE & kScoreCap) bound = fminf(bound, a.score.cap2);
-        // A negative slope raises scores by up to its largest distance.
-        if constexpr (SCORE & kScoreDistance)
-          bound += fmaxf(-slope2, 0.f) * (float)max(abs(qpos), abs(qpos - a.Lk));
+        // (A bias raises no score.)
       }
       if constexpr (!WIN) {
         if (a.mask != nullptr) {
@@ -611,7 +642,11 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
       f32x16& s_cur = sh[hf];
       if constexpr (SCORE != 0) {
         // Register 8*k2 + e holds key 64*t + 32*hf + 16*k2 + 8*hh + e.
-        const float kd = (float)(qpos - (BN * t + 32 * hf + 8 * hh));
+        float kd = 0.f;
+        if constexpr (SCORE & kScoreDistance) {
+          const int k0 = BN * t + 32 * hf + 8 * hh;
+          kd = (float)((2 * (k0 + 23) <= from_left + from_right ? from_left : from_right) - k0);
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           float z;
@@ -621,7 +656,7 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
             z = s_cur[r] * a.scale_log2;
           if constexpr (SCORE & kScoreDistance) {
             if constexpr (SCORE & kScoreCap) z = fmaf(capm2, z, a.score.cap2);
-            z = fmaf(-slope2, fabsf(kd - (float)(16 * (r >> 3) + (r & 7))), z);
+            z = fmaf(-near2, fabsf(kd - (float)(16 * (r >> 3) + (r & 7))), z);
           }
           s_cur[r] = z;
         }
@@ -658,6 +693,24 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
               s_cur[4 * g + r] = bb[r] < 0.f ? kMasked : s_cur[4 * g + r];
             else
               s_cur[4 * g + r] += bb[r];
+          }
+        }
+      }
+    }
+    if constexpr (SCORE & kScoreDistance) {
+      // Keys of a half tile on both sides of a row's pos, with a slope < 0:
+      // those on the left were taken for ones on the right.  (They lie nearest to
+      // pos, so that what the larger bias rounded off weighs nothing.)
+      if (farthest) {
+        const int k0 = BN * t + 8 * hh, pos = (from_left + from_right) >> 1;
+        if (__builtin_amdgcn_ballot_w64(k0 < pos && k0 + 55 > pos) != 0) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const int kh = k0 + 32 * hf;
+            const float kd = kh + 23 <= pos ? 0.f : (float)(pos - kh);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)  // (-inf stays)
+              sh[hf][r] = fmaf(2.f * near2, fmaxf(kd - (float)(16 * (r >> 3) + (r & 7)), 0.f), sh[hf][r]);
           }
         }
       }
@@ -945,7 +998,13 @@ __global__ __launch_bounds__(SMALL ? 256 : 512, SMALL ? 2 : 1) void attn_fwd_ker
     ep = wave < 4 ? est.k : est.vt;
   }
   static_assert(sizeof(st0.k) >= 32 * D * sizeof(bf16), "a wave's output rows fit a K stage");
-  write_rows<D>(a, acc, inv, lse, ep, bh, qt * BM + wave * 32);
+  if constexpr (SCORE & kScoreDistance) {
+    const int p = qrow + a.score.query_offset(b);
+    const uint32_t distance = bias_distance(p, row_bias(p));
+    write_rows<D, true>(a, acc, inv, lse, ep, bh, qt * BM + wave * 32, slope, distance);
+  } else {
+    write_rows<D>(a, acc, inv, lse, ep, bh, qt * BM + wave * 32);
+  }
 }
 
 // The split row blocks (FwdArgs::nsplit): one wave per 32 rows adds the
@@ -969,7 +1028,23 @@ __global__ __launch_bounds__(256) void fwd_combine_kernel(FwdArgs a, float c, fl
   combine_parts<D>(slot, fwd_slot_floats(BM, D), a.nparts, c, acc, m, l);
   float inv, lse;
   row_state(m, l, unit, inv, lse);
-  write_rows<D>(a, acc, inv, lse, ep[wave], bh, row0);
+  if (a.score.slopes != nullptr) {
+    const int b = bh / a.Hq, row = min(row0 + (int)(threadIdx.x & 31), a.Lq - 1);
+    const float slope = a.score.slopes[bh % a.Hq];
+    int lo = 0, hi = a.Lk;
+    if (a.wlo != nullptr) {
+      lo = min(max(a.wlo[b * a.wsb + row], 0), a.Lk);
+      hi = min(max(a.whi[b * a.wsb + row], lo), a.Lk);
+    }
+    const int p = row + a.score.query_offset(b);
+    int hull_lo, hull_hi;
+    bias_hull(a, slope, b, p, lo, hi, hull_lo, hull_hi);
+    within_hull(hull_lo, hull_hi, lo, hi);
+    const uint32_t distance = bias_distance(p, bias_ref(p, lo, hi, slope < 0.f));
+    write_rows<D, true>(a, acc, inv, lse, ep[wave], bh, row0, slope, distance);
+  } else {
+    write_rows<D>(a, acc, inv, lse, ep[wave], bh, row0);
+  }
 }
 
 }  // namespace avattn

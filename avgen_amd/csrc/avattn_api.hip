@@ -137,9 +137,10 @@ BwdWorkspace bwd_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32
 
 // BwdArgs::khull and kskip of a backward with staged dS and no windows: they
 // take the place of the K row copy, which only the recomputing dQ kernel
-// reads (8 KB or more per 64-key tile, against 12 bytes).
+// reads (8 KB or more per 64-key tile, against 12 bytes).  With windows only
+// where a mask limits the keys of a bias (BiasRef).
 void set_hull(BwdArgs& a, char* ws, const BwdWorkspace& w) {
-  if (a.wlo) return;
+  if (a.wlo && !(a.mask && a.score.slopes)) return;
   a.khull = reinterpret_cast<int*>(ws + w.kr);
   a.kskip = a.mask ? a.khull + 2 * (size_t)a.nkv : nullptr;
 }
@@ -228,7 +229,8 @@ int fwd_impl(const void* q, const void* k, const void* v, const int64_t* q_strid
              const float* q_scale, const float* k_scale, float scale, void* out, const int64_t* out_strides,
              float* lse, void* workspace, size_t workspace_bytes, avattn_stream_t stream,
              const int32_t* window_lo = nullptr, const int32_t* window_hi = nullptr, int64_t window_batch_stride = 0,
-             const RingOpts* ring = nullptr, const ScoreArgs* score = nullptr, bool sorted_windows = false) {
+             const RingOpts* ring = nullptr, const ScoreArgs* score = nullptr, bool sorted_windows = false,
+             float* row_lse = nullptr) {
   int st = check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
   if (!q_strides || !k_strides || !v_strides || !out_strides) return AVATTN_ERR_NULL_POINTER;
@@ -303,6 +305,7 @@ int fwd_impl(const void* q, const void* k, const void* v, const int64_t* q_strid
   }
   if (score) {
     a.score = *score;
+    a.row_lse = row_lse;
     if (window_lo && !sorted_windows) {
       // avattn_fwd_scored_workspace_size's room behind everything else.
       a.hull = reinterpret_cast<int*>(ws + wl.total + split);
@@ -467,7 +470,7 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
                     const int64_t* dk_strides, void* dv, const int64_t* dv_strides, void* workspace,
                     size_t workspace_bytes, uint32_t flags, avattn_stream_t stream, const int32_t* window_lo,
                     const int32_t* window_hi, int64_t window_batch_stride, const RingOpts* ring = nullptr,
-                    const CompactDs* compact = nullptr, const ScoreArgs* score = nullptr) {
+                    const CompactDs* compact = nullptr, const ScoreArgs* score = nullptr, bool shifted_lse = false) {
   int st = check_bwd_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (flags & ~(AVATTN_BWD_REUSE_QUERY_SIDE | AVATTN_BWD_DQ_ACCUMULATE_F32 | AVATTN_BWD_STAGE_DS |
                 AVATTN_BWD_DEFER_DQ))
@@ -544,6 +547,11 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
   a.msb = key_mask_batch_stride;
   a.scale = scale;
   a.scale_log2 = scale * kLog2e;
+  if (score) {
+    a.score = *score;
+    a.shifted_lse = shifted_lse;
+    if (score->mode & kScoreCap) a.scale *= 4.f;  // of 1 - tanh^2 (BwdArgs::score)
+  }
   a.dq = dq_f32 ? nullptr : static_cast<bf16*>(dq);
   a.dq_acc = dq_f32 ? static_cast<float*>(dq) : nullptr;
   a.reuse_q = (flags & AVATTN_BWD_REUSE_QUERY_SIDE) != 0;
@@ -606,10 +614,6 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
     const size_t end = off + (size_t)a.nkv * per;
     if (kv_per_pass == a.nkv && (!window_lo || (score && !compact)) && split > 0 && workspace_bytes >= end + split)
       a.split_all = reinterpret_cast<float*>(ws + end);
-  }
-  if (score) {
-    a.score = *score;
-    if (score->mode & kScoreCap) a.scale *= 4.f;  // of 1 - tanh^2 (BwdArgs::score)
   }
   return launch_status(launch_bwd(a, head_dim, kv_per_pass, s));
 }
@@ -1189,7 +1193,9 @@ int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t
                       avattn_stream_t stream) {
   int st = check_dims(batch, heads_q, heads_kv, len_q, len_k, head_dim);
   if (st != AVATTN_OK) return st;
-  if (flags & ~AVATTN_SCORED_SORTED_WINDOWS) return AVATTN_ERR_ARGUMENT;
+  if (flags & ~(AVATTN_SCORED_SORTED_WINDOWS | AVATTN_SCORED_ROW_LSE)) return AVATTN_ERR_ARGUMENT;
+  const bool rows = (flags & AVATTN_SCORED_ROW_LSE) != 0;
+  if (rows && !slopes) return AVATTN_ERR_ARGUMENT;
   if (!q_strides || !k_strides || !v_strides || !out_strides) return AVATTN_ERR_NULL_POINTER;
   if (!(scale > 0.f) || !isfinite(scale)) return AVATTN_ERR_ARGUMENT;
   FewArgs c{};
@@ -1212,11 +1218,19 @@ int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool sorted = (flags & AVATTN_SCORED_SORTED_WINDOWS) != 0;
   const bool few = plan.nsplit > 0;
+  float* const row_lse = rows && lse ? lse + (int64_t)batch * heads_q * len_q : nullptr;
+  if (rows && len_k == 0) {  // no key: both halves alike
+    st = avattn_fwd_scored(q, k, v, q_strides, k_strides, v_strides, batch, heads_q, heads_kv, len_q, len_k, head_dim,
+                           is_f32, key_mask, key_mask_batch_stride, window_lo, window_hi, window_batch_stride, scale,
+                           softcap, slopes, query_offsets, query_offset, flags & ~AVATTN_SCORED_ROW_LSE, out,
+                           out_strides, row_lse, workspace, workspace_bytes, stream);
+    if (st != AVATTN_OK) return st;
+  }
   if (!is_f32 && !few)
     return fwd_impl(q, k, v, q_strides, k_strides, v_strides, batch, heads_q, heads_kv, len_q, len_k, head_dim,
                     key_mask, key_mask_batch_stride, nullptr, nullptr, 0, false, nullptr, nullptr, scale, out,
                     out_strides, lse, workspace, workspace_bytes, stream, window_lo, window_hi, window_batch_stride,
-                    nullptr, &c.score, sorted);
+                    nullptr, &c.score, sorted, row_lse);
   c.q = q, c.k = k, c.v = v, c.o = out;
   c.qsb = q_strides[0], c.qsh = q_strides[1], c.qsl = q_strides[2];
   c.ksb = k_strides[0], c.ksh = k_strides[1], c.ksl = k_strides[2];
@@ -1227,6 +1241,7 @@ int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t
   c.wlo = window_lo, c.whi = window_hi, c.wsb = window_batch_stride;
   c.scale_log2 = scale * kLog2e;
   c.lse = lse;
+  c.row_lse = row_lse;
   if (!few) return fwd_scored_f32(c, head_dim, scale, sorted, workspace, workspace_bytes, s);
   if (!q || !k || !v || !out || !lse) return AVATTN_ERR_NULL_POINTER;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return AVATTN_ERR_LAYOUT;
@@ -1239,7 +1254,11 @@ int avattn_fwd_scored(const void* q, const void* k, const void* v, const int64_t
   return launch_status(launch_few(c, plan, head_dim, is_f32 != 0, s));
 }
 
-int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+}  // extern "C"
+
+// shifted_lse: lse is the forward's lse (BwdArgs::shifted_lse), else its
+// row_lse.
+static int bwd_scored(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                       const int64_t* dout_strides, const int64_t* q_strides, const int64_t* k_strides,
                       const int64_t* v_strides, const int64_t* out_strides, int32_t batch, int32_t heads_q,
                       int32_t heads_kv, int32_t len_q, int32_t len_k, int32_t head_dim, int32_t is_f32,
@@ -1248,7 +1267,8 @@ int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void
                       int64_t ds_table_batch_stride, int64_t ds_units_per_head, float scale, float softcap,
                       const float* slopes, const int32_t* query_offsets, int32_t query_offset, void* dq,
                       const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
-                      const int64_t* dv_strides, void* workspace, size_t workspace_bytes, avattn_stream_t stream) {
+                      const int64_t* dv_strides, void* workspace, size_t workspace_bytes, avattn_stream_t stream,
+                      bool shifted_lse) {
   ScoreArgs score;
   if (!(scale > 0.f) || !isfinite(scale)) return AVATTN_ERR_ARGUMENT;
   const int st = score_args(scale, softcap, slopes, query_offsets, query_offset, heads_q, heads_kv,
@@ -1262,7 +1282,7 @@ int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void
     return bwd_impl(dout, q, k, v, out, lse, dout_strides, q_strides, k_strides, v_strides, out_strides, batch,
                     heads_q, heads_kv, len_q, len_k, head_dim, key_mask, key_mask_batch_stride, scale, dq, dq_strides,
                     dk, dk_strides, dv, dv_strides, workspace, workspace_bytes, AVATTN_BWD_STAGE_DS, stream, window_lo,
-                    window_hi, window_batch_stride, nullptr, ds_table ? &c : nullptr, &score);
+                    window_hi, window_batch_stride, nullptr, ds_table ? &c : nullptr, &score, shifted_lse);
   }
   if (ds_table) return AVATTN_ERR_ARGUMENT;
   if (!dout_strides || !q_strides || !k_strides || !v_strides || !out_strides || !dq_strides || !dk_strides ||
@@ -1289,7 +1309,45 @@ int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void
   a.dksb = dk_strides[0], a.dksh = dk_strides[1], a.dksl = dk_strides[2];
   a.dvsb = dv_strides[0], a.dvsh = dv_strides[1], a.dvsl = dv_strides[2];
   a.score = score;
+  a.shifted_lse = shifted_lse;
   return bwd_scored_f32(a, head_dim, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" {
+
+int avattn_bwd_scored(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                      const int64_t* dout_strides, const int64_t* q_strides, const int64_t* k_strides,
+                      const int64_t* v_strides, const int64_t* out_strides, int32_t batch, int32_t heads_q,
+                      int32_t heads_kv, int32_t len_q, int32_t len_k, int32_t head_dim, int32_t is_f32,
+                      const uint8_t* key_mask, int64_t key_mask_batch_stride, const int32_t* window_lo,
+                      const int32_t* window_hi, int64_t window_batch_stride, const int32_t* ds_table,
+                      int64_t ds_table_batch_stride, int64_t ds_units_per_head, float scale, float softcap,
+                      const float* slopes, const int32_t* query_offsets, int32_t query_offset, void* dq,
+                      const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                      const int64_t* dv_strides, void* workspace, size_t workspace_bytes, avattn_stream_t stream) {
+  return bwd_scored(dout, q, k, v, out, lse, dout_strides, q_strides, k_strides, v_strides, out_strides, batch, heads_q,
+                    heads_kv, len_q, len_k, head_dim, is_f32, key_mask, key_mask_batch_stride, window_lo, window_hi,
+                    window_batch_stride, ds_table, ds_table_batch_stride, ds_units_per_head, scale, softcap, slopes,
+                    query_offsets, query_offset, dq, dq_strides, dk, dk_strides, dv, dv_strides, workspace,
+                    workspace_bytes, stream, true);
+}
+
+int avattn_bwd_scored_row_lse(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                              const float* row_lse, const int64_t* dout_strides, const int64_t* q_strides,
+                              const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
+                              int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len_q, int32_t len_k,
+                              int32_t head_dim, int32_t is_f32, const uint8_t* key_mask, int64_t key_mask_batch_stride,
+                              const int32_t* window_lo, const int32_t* window_hi, int64_t window_batch_stride,
+                              const int32_t* ds_table, int64_t ds_table_batch_stride, int64_t ds_units_per_head,
+                              float scale, float softcap, const float* slopes, const int32_t* query_offsets,
+                              int32_t query_offset, void* dq, const int64_t* dq_strides, void* dk,
+                              const int64_t* dk_strides, void* dv, const int64_t* dv_strides, void* workspace,
+                              size_t workspace_bytes, avattn_stream_t stream) {
+  return bwd_scored(dout, q, k, v, out, row_lse, dout_strides, q_strides, k_strides, v_strides, out_strides, batch,
+                    heads_q, heads_kv, len_q, len_k, head_dim, is_f32, key_mask, key_mask_batch_stride, window_lo,
+                    window_hi, window_batch_stride, ds_table, ds_table_batch_stride, ds_units_per_head, scale, softcap,
+                    slopes, query_offsets, query_offset, dq, dq_strides, dk, dk_strides, dv, dv_strides, workspace,
+                    workspace_bytes, stream, false);
 }
 
 }  // extern "C"

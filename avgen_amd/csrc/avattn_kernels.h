@@ -13,9 +13,9 @@ namespace avattn {
 constexpr uint32_t kTileSkip = 0x80000000u;
 
 // Scores changed before the softmax: z = cap tanh(s / cap) (kScoreCap), then
-// z - slopes[hq] * |position of the query - key| (kScoreDistance), s = scale
-// q.k; query i of batch b at position i + query_offset(b).  cap2 = cap *
-// log2(e); cap_x = scale / cap; cap_arg = 2 log2(e) cap_x, so that
+// z - slopes[hq] * |position of the query - key| (kScoreDistance, see BiasRef),
+// s = scale q.k; query i of batch b at position i + query_offset(b).  cap2 = cap
+// * log2(e); cap_x = scale / cap; cap_arg = 2 log2(e) cap_x, so that
 // exp2(cap_arg * q.k) is e^(2 s / cap).  slopes null: none (0).
 constexpr int kScoreCap = 1, kScoreDistance = 2;
 struct ScoreArgs {
@@ -27,17 +27,84 @@ struct ScoreArgs {
   __device__ __forceinline__ int query_offset(int b) const { return offsets ? offsets[b] : offset; }
 };
 
+// The bias of a row is measured from that of the key it favours most, since in
+// fp32 slope * distance rounds the scores away long before the distances end (a
+// query 2^20 behind its keys, slope 1/2: scores in steps of 1/16).  With the
+// row's position p and its keys [lo, hi), pos is p moved into them, so that
+// |p - j| = |p - pos| + |pos - j| for every key j; what is subtracted from a
+// score is slope (|pos - j| - ref) >= 0, with ref 0 for a slope >= 0 (the nearest
+// key has no bias) and pos's largest distance for one below (the farthest has
+// none).  Integers until the difference is formed.  slope (|p - pos| + ref) is
+// the constant that this leaves out: it moves the row's logsumexp, nothing else
+// (bias_distance: the bracket).
+// Keys: the row's window (every key without windows), with a key mask those of
+// them between the first and the last 64-key tile with an attended key.
+struct BiasRef {
+  int pos, ref;
+};
+__device__ __forceinline__ BiasRef bias_ref(int p, int lo, int hi, bool farthest) {
+  const int last = max(hi - 1, lo), pos = min(max(p, lo), last);
+  return {pos, farthest ? max(pos - lo, last - pos) : 0};
+}
+__device__ __forceinline__ uint32_t bias_distance(int p, const BiasRef& r) {
+  return (p < r.pos ? (uint32_t)r.pos - (uint32_t)p : (uint32_t)p - (uint32_t)r.pos) + (uint32_t)r.ref;
+}
+// The logsumexp of a row's scores from that of what the kernels compute, and
+// back.
+__device__ __forceinline__ float lse_of_scores(float lse, float slope, uint32_t distance) {
+  return (float)((double)lse - (double)slope * (double)distance);
+}
+__device__ __forceinline__ float lse_from_scores(float lse, float slope, uint32_t distance) {
+  return (float)((double)lse + (double)slope * (double)distance);
+}
+
+// The keys [lo, hi) from the first to the last 64-key tile with an attended key of
+// a mask over n keys, as a wave of a group of `threads` sees it whose threads
+// look at every threads-th key (none: lo large, hi 0).
+__device__ __forceinline__ void attended_share(const uint8_t* mask, int n, int thread, int threads, int& lo, int& hi) {
+  constexpr int U = 16;  // loads in flight
+  lo = 0x7fffffff, hi = 0;
+  for (int j0 = thread; j0 < n; j0 += U * threads) {
+    uint8_t v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = j0 + u * threads < n ? mask[j0 + u * threads] : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v[u] != 0) lo = min(lo, j0 + u * threads), hi = j0 + u * threads + 1;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
+  lo = __builtin_amdgcn_readfirstlane(lo) & ~63;
+  hi = min((__builtin_amdgcn_readfirstlane(hi) + 63) & ~63, n);
+}
+// A row's keys [lo, hi) without those outside that hull.
+__device__ __forceinline__ void within_hull(int hull_lo, int hull_hi, int& lo, int& hi) {
+  lo = max(lo, min(hull_lo, hull_hi));
+  hi = max(min(hi, hull_hi), lo);
+}
+// The hull (0, n: not needed, it would change no row) for the rows of a wave, a
+// row per lane at position p with keys [lo, hi): looked for where a slope is
+// negative or a row's pos is masked.  The whole wave calls it.
+__device__ __forceinline__ void rows_hull(const uint8_t* mask, int n, float slope, int p, int lo, int hi, int& hull_lo,
+                                          int& hull_hi) {
+  hull_lo = 0, hull_hi = n;
+  if (mask == nullptr) return;
+  const bool look = slope < 0.f || (lo < hi && mask[bias_ref(p, lo, hi, false).pos] == 0);
+  if (__builtin_amdgcn_ballot_w64(look) == 0) return;
+  attended_share(mask, n, threadIdx.x & 63, 64, hull_lo, hull_hi);
+}
+
 // 1 / (1 + exp2(arg s)) = (1 - tanh(s / cap)) / 2, in [0, 1].
 __device__ __forceinline__ float cap_complement(float s, float arg) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * arg));
 }
 
-// The float32 kernels' changed score, in log2 units, from a raw one; kd: the row's
-// position minus the key; f = 1 - tanh^2 (1 without a cap).  tanh to a few
+// The float32 kernels' changed score, in log2 units, from a raw one; d: the key's
+// distance from the row's pos, less its ref (BiasRef); f = 1 - tanh^2 (1 without a cap).  tanh to a few
 // units in the last place, small arguments too: below 0.35 its odd series to
 // x^11 (the next term is below 2^-26), above it 1 - 2 r with r = 1 / (1 +
 // e^2|x|), and then 1 - tanh^2 = 4 r (1 - r).
-__device__ __forceinline__ float changed_score_exact(const ScoreArgs& a, float s, float scale_log2, float kd,
+__device__ __forceinline__ float changed_score_exact(const ScoreArgs& a, float s, float scale_log2, float d,
                                                      float slope2, float& f) {
   float z = s * scale_log2;
   f = 1.f;
@@ -53,7 +120,7 @@ __device__ __forceinline__ float changed_score_exact(const ScoreArgs& a, float s
     f = small ? fmaf(-t, t, 1.f) : 4.f * r * (1.f - r);
     z = a.cap2 * t;
   }
-  return fmaf(-slope2, fabsf(kd), z);
+  return fmaf(-slope2, d, z);
 }
 
 // The keys [lo, hi) of batch b outside which no query row's window reaches:
@@ -143,8 +210,11 @@ struct FwdArgs {
   // Changed scores (mode 0: none).  With them a key that is masked or outside
   // the hull of its batch row's windows is copied as zeros in k and v, so that
   // what it holds never reaches a row; hull as in key_hull.
+  // lse is that of the changed scores; row_lse (null: not wanted) that
+  // of what the kernels compute (BiasRef), which the backward starts from.
   ScoreArgs score;
   int* hull;
+  float* row_lse;
 };
 
 // Floats of one part of `rows` rows: the accumulators, then per 32 rows their
@@ -207,8 +277,9 @@ struct BwdArgs {
   // Staged dS without windows: khull[2 p], khull[2 p + 1] bound the 64-key
   // tiles of pair p = b*Hkv + hk that can contribute; outside them no key is
   // attended and k is finite, so dS is exactly 0 there: the dK/dV kernel does
-  // not form it, the dQ kernel does not read it.  kskip: per (p, tile), the
-  // marks it is made from (null without a mask).
+  // not form it, the dQ kernel does not read it.  (With windows, a mask and a
+  // bias: the tiles with an attended key, for BiasRef alone.)  kskip: per (p,
+  // tile), the marks it is made from (null without a mask).
   int* khull;
   int* kskip;
   // dq as an fp32 accumulator (dq_acc += this chunk's dq; dq is then null),
@@ -273,10 +344,12 @@ struct BwdArgs {
   // Slots for a split of every block (null: none; see dkv_(scored_)split_plan), in
   // place of split_part.
   float* split_all;
-  // Changed scores as in FwdArgs (mode 0: none; staged dS only).  With the cap
-  // lse2 holds lse * log2(e) - cap2, the staged dS a quarter of it, and scale 4
-  // times the softmax scale (scale_log2 stays).
+  // Changed scores as in FwdArgs (mode 0: none; staged dS only).  lse is its
+  // row_lse, or with shifted_lse its lse.  With the cap lse2 holds that times
+  // log2(e) - cap2, the staged dS a quarter of it, and scale 4 times the softmax
+  // scale (scale_log2 stays).
   ScoreArgs score;
+  bool shifted_lse;
 };
 
 // Partial-sum slots of the dK/dV tail split, 256 x D floats each; the
@@ -460,13 +533,15 @@ struct FewArgs {
   float scale_log2;
   ScoreArgs score;
   float* lse;
+  float* row_lse;  // as in FwdArgs
   // Set by launch_few from few_plan: workgroups per (batch, kv head, block of
   // rows), blocks per kv head, rows of a block; part: few_slot_floats per
-  // workgroup (nsplit > 1), outputs by row, then (maximum, sum) by row.
+  // workgroup (nsplit > 1), outputs by row, then (maximum, sum, bias_distance)
+  // by row.
   int nsplit, row_blocks, block_rows;
   float* part;
 };
-constexpr int few_slot_floats(int rows, int D) { return rows * D + (2 * rows + 3) / 4 * 4; }
+constexpr int few_slot_floats(int rows, int D) { return rows * D + (3 * rows + 3) / 4 * 4; }
 // nsplit 0: more rows than this path takes.
 struct FewPlan {
   int nsplit, row_blocks, block_rows;

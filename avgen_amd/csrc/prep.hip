@@ -284,6 +284,25 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(BwdArgs a, int nk, int nq
       y[r] = *reinterpret_cast<const u32x4*>(op + (int64_t)i * a.osl);
     }
   }
+  if constexpr (DROP) {
+    // The lse of the scores: what BiasRef leaves out goes back in.
+    if (a.shifted_lse && a.score.slopes != nullptr) {
+      const float slope = a.score.slopes[h];
+      int hull_lo = 0, hull_hi = a.Lk;
+      if (a.mask != nullptr) attended_share(a.mask + b * a.msb, a.Lk, threadIdx.x & 63, 64, hull_lo, hull_hi);
+#pragma unroll
+      for (int r = 0; r < kStatRows; ++r) {
+        const int i = min(i0 + r * RPB, a.Lq - 1), p = i + a.score.query_offset(b);
+        int lo = 0, hi = a.Lk;
+        if (a.wlo != nullptr) {
+          lo = min(max(a.wlo[b * a.wsb + i], 0), a.Lk);
+          hi = min(max(a.whi[b * a.wsb + i], lo), a.Lk);
+        }
+        within_hull(hull_lo, hull_hi, lo, hi);
+        l[r] = lse_from_scores(l[r], slope, bias_distance(p, bias_ref(p, lo, hi, slope < 0.f)));
+      }
+    }
+  }
 #pragma unroll
   for (int r = 0; r < kStatRows; ++r) {
     float acc = 0.f;

@@ -4,6 +4,11 @@
 ``flash_fwd(_windowed)`` of :mod:`avgen_amd.ops` with ``softcap``, ``slopes`` and
 the queries' offset; checks, strides, workspaces, streams and errors are those
 of that module.  bf16 and float32; differentiable in q, k and v.
+
+With slopes the backward starts from ``row_lse``, the logsumexp without the
+constant ``slope * distance`` that the kernels leave out of a row's scores
+(``avattn_fwd_scored``): ``lse`` holds that only as float32 does.
+``flash_fwd_scored_rows`` is ``flash_fwd_scored`` with it as a third result.
 """
 
 from __future__ import annotations
@@ -133,7 +138,10 @@ def _staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32, pairs) -> int:
     return lib.avattn_bwd_staged_workspace_size(B, Hq, Hkv, Lq, Lk, D, pairs)
 
 
-def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone):
+def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone,
+              rows=False):
+    """``(out, lse)``; with ``rows`` ``(out, lse, row_lse)``, ``row_lse`` being
+    ``lse`` itself without slopes."""
     name = "avgen_amd.flash_fwd_scored"
     lo, hi, wsb, mask, msb, slopes, offsets = _check_scored(
         name, q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset)
@@ -145,17 +153,21 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
         (k, ks), (v, vs) = _laid_out(k.contiguous(), f32), _laid_out(v.contiguous(), f32)
     out, os = _new_like(q, qs, f32)
     device = q.device
-    lse = torch.empty((B, Hq, Lq), device=device, dtype=torch.float32)
+    row_lse = lse = torch.empty((B, Hq, Lq) if slopes is None or not rows else (2, B, Hq, Lq), device=device,
+                                dtype=torch.float32)
+    flags = _lib.SCORED_SORTED_WINDOWS if monotone else 0
+    if lse.ndim == 4:
+        flags |= _lib.SCORED_ROW_LSE
+        lse, row_lse = lse[0], lse[1]
     ws = _workspace(_fwd_workspace_size(B, Hq, Hkv, Lq, Lk, D, f32), device)
     with _on(device):
         st = _lib.load().avattn_fwd_scored(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, B, Hq, Hkv, Lq, Lk, D, f32,
             _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb,
-            scale, softcap, _ptr(slopes), _ptr(offsets), offset,
-            _lib.SCORED_SORTED_WINDOWS if monotone else 0,
+            scale, softcap, _ptr(slopes), _ptr(offsets), offset, flags,
             out.data_ptr(), os, lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
     _lib.check(st, name)
-    return out, lse
+    return (out, lse, row_lse) if rows else (out, lse)
 
 
 @lru_cache(maxsize=256)
@@ -194,8 +206,8 @@ def _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, windowed, device) -> torch.Ten
 
 
 def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
-              monotone, from_forward=False):
-    """``monotone``: the caller guarantees windows non-decreasing in the row
+              monotone, row_lse=None, from_forward=False):
+    """``row_lse`` (see the module docstring): in place of ``lse``.  ``monotone``: the caller guarantees windows non-decreasing in the row
     (otherwise checked here, one host synchronisation).  With windows dS is
     staged densely where all of it fits the budget (no synchronisation), else
     compactly (one, for its size).  ``from_forward``: the arguments passed the
@@ -214,9 +226,10 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
         for label, t in (("grad_out", dout), ("out", out)):
             if t.shape != q.shape or t.dtype is not q.dtype:
                 raise ValueError(f"{name}: {label} must be {q.dtype} {tuple(q.shape)}")
-        if lse.shape != (B, Hq, Lq) or lse.dtype is not torch.float32:
-            raise ValueError(f"{name}: logsumexp must be float32 (batch, heads, queries)")
-    _one_device(name, q, k, v, dout, out, lse, lo, hi, mask, slopes, offsets)
+        for t in (lse, row_lse):
+            if t is not None and (t.shape != (B, Hq, Lq) or t.dtype is not torch.float32):
+                raise ValueError(f"{name}: logsumexp must be float32 (batch, heads, queries)")
+    _one_device(name, q, k, v, dout, out, lse, row_lse, lo, hi, mask, slopes, offsets)
     if lo is not None and not monotone and Lq > 1:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{name}: a captured backward cannot check the windows' order; pass monotone=True")
@@ -224,7 +237,7 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
             raise ValueError(f"{name}: the backward needs window_lo and window_hi non-decreasing along the queries")
     (dout, dos), (q, qs), (k, ks) = _laid_out(dout, f32), _laid_out(q, f32), _laid_out(k, f32)
     (v, vs), (out, os) = _laid_out(v, f32), _laid_out(out, f32)
-    lse = lse.contiguous()
+    stat = (lse if row_lse is None else row_lse).contiguous()
     (dq, dqs), (dk, dks), (dv, dvs) = _new_like(q, qs, f32), _new_like(k, ks, f32), _new_like(v, vs, f32)
     device = q.device
     table, tsb, units = None, 0, 0
@@ -237,9 +250,10 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
         ws = _alloc_bwd_workspace(B, Hq, Hkv, Lq, Lk, D, device, stage_ds=True, ds_units=units)
     else:
         ws = _staged_workspace(B, Hq, Hkv, Lq, Lk, D, f32, lo is not None, device)
+    lib = _lib.load()
     with _on(device):
-        st = _lib.load().avattn_bwd_scored(
-            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        st = (lib.avattn_bwd_scored if row_lse is None else lib.avattn_bwd_scored_row_lse)(
+            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stat.data_ptr(),
             dos, qs, ks, vs, os, B, Hq, Hkv, Lq, Lk, D, f32,
             _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb, _ptr(table), tsb, units,
             scale, softcap, _ptr(slopes), _ptr(offsets), offset,
@@ -264,22 +278,44 @@ def _(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, 
     return torch.empty_like(q), q.new_empty((q.shape[0], q.shape[1], q.shape[2]), dtype=torch.float32)
 
 
+@torch.library.custom_op("avgen_amd::flash_fwd_scored_rows", mutates_args=())
+def _fwd_rows_op(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window_lo: Optional[torch.Tensor],
+    window_hi: Optional[torch.Tensor], key_mask: Optional[torch.Tensor], slopes: torch.Tensor,
+    offsets: Optional[torch.Tensor], scale: float, softcap: float, offset: int, monotone: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``flash_fwd_scored`` with slopes: ``(out, lse, row_lse)``."""
+    out, lse, row_lse = _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
+                                  monotone, True)
+    return out, lse.clone(), row_lse.clone()  # an op's results share no memory
+
+
+@_fwd_rows_op.register_fake
+def _(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone=False):
+    row = (q.shape[0], q.shape[1], q.shape[2])
+    return torch.empty_like(q), q.new_empty(row, dtype=torch.float32), q.new_empty(row, dtype=torch.float32)
+
+
 @torch.library.custom_op("avgen_amd::flash_bwd_scored", mutates_args=())
 def _bwd_op(
     dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
     window_lo: Optional[torch.Tensor], window_hi: Optional[torch.Tensor], key_mask: Optional[torch.Tensor],
     slopes: Optional[torch.Tensor], offsets: Optional[torch.Tensor], scale: float, softcap: float, offset: int,
-    monotone: bool = False,
+    monotone: bool = False, row_lse: Optional[torch.Tensor] = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Backward of ``flash_fwd_scored``: ``(dq, dk, dv)``."""
     return _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
-                     monotone)
+                     monotone, row_lse)
 
 
 @_bwd_op.register_fake
 def _(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
-      monotone=False):
+      monotone=False, row_lse=None):
     return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+
+
+def _fwd_of_rows(*args):
+    return _fwd_rows_op(*args)[:2]
 
 
 def flash_fwd_scored(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
@@ -288,54 +324,62 @@ def flash_fwd_scored(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, s
     softcap)`` (0: none), lose ``slopes[h] |i + offset - j|`` (None: nothing;
     ``offsets`` int32 per batch row in place of ``offset``) and are masked by
     key windows and ``key_mask`` (each may be None): ``(out, lse)``."""
-    return _direct(_FlashFwdScored, _fwd_op, _fwd_impl,
+    return _direct(_FlashFwdScored, _fwd_op if slopes is None else _fwd_of_rows, _fwd_impl,
                    (q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone),
                    (q, k, v, window_lo, window_hi, key_mask, slopes, offsets))
 
 
 def flash_bwd_scored(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset,
-                     monotone=False):
+                     monotone=False, row_lse=None):
     """``(dq, dk, dv)`` of :func:`flash_fwd_scored` (windows non-decreasing in
-    the row; checked unless ``monotone``)."""
-    args = (dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone)
-    if _grad_direct(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets):
+    the row; checked unless ``monotone``).  With slopes and without ``row_lse``
+    (of ``flash_fwd_scored_rows``) probabilities are as exact as ``lse``: off by
+    up to ``|lse| 2^-24`` relatively."""
+    args = (dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, scale, softcap, offset, monotone,
+            row_lse)
+    if _grad_direct(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, offsets, row_lse):
         return _bwd_impl(*args)
     return _bwd_op(*args)
 
 
 def _setup(ctx, inputs, output):
     q, k, v, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap, ctx.offset, ctx.monotone = inputs
-    out, lse = output
-    ctx.save_for_backward(q, k, v, out, lse, lo, hi, mask, slopes, offsets)
-    ctx.mark_non_differentiable(lse)
+    out, lse, *rows = output
+    ctx.save_for_backward(q, k, v, out, rows[0] if rows else lse, lo, hi, mask, slopes, offsets)
+    ctx.has_rows = bool(rows)
+    ctx.mark_non_differentiable(lse, *rows)
 
 
-def _backward(ctx, dout, _dlse):
-    q, k, v, out, lse, lo, hi, mask, slopes, offsets = ctx.saved_tensors
-    grads = flash_bwd_scored(dout, q, k, v, out, lse, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap,
-                             ctx.offset, ctx.monotone)
+def _backward(ctx, dout, *_):
+    q, k, v, out, stat, lo, hi, mask, slopes, offsets = ctx.saved_tensors
+    grads = flash_bwd_scored(dout, q, k, v, out, stat, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap,
+                             ctx.offset, ctx.monotone, stat if ctx.has_rows else None)
     return (*grads,) + (None,) * 9
 
 
 torch.library.register_autograd("avgen_amd::flash_fwd_scored", _backward, setup_context=_setup)
+torch.library.register_autograd("avgen_amd::flash_fwd_scored_rows", _backward, setup_context=_setup)
 
 
 class _FlashFwdScored(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *args):
-        result = _fwd_impl(*args)
+        out, lse, row_lse = _fwd_impl(*args, True)
         ctx.set_materialize_grads(False)
-        _setup(ctx, args, result)
-        return result
+        q, k, v, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap, ctx.offset, ctx.monotone = args
+        ctx.save_for_backward(q, k, v, out, row_lse, lo, hi, mask, slopes, offsets)
+        ctx.has_rows = True
+        ctx.mark_non_differentiable(lse)
+        return out, lse
 
     @staticmethod
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 12
         if not _grad_direct(dout):
-            return _backward(ctx, dout, None)
+            return _backward(ctx, dout)
         # The forward was a plain call: so is this one.
-        q, k, v, out, lse, lo, hi, mask, slopes, offsets = ctx.saved_tensors
-        grads = _bwd_impl(dout, q, k, v, out, lse, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap, ctx.offset,
-                          ctx.monotone, True)
+        q, k, v, out, stat, lo, hi, mask, slopes, offsets = ctx.saved_tensors
+        grads = _bwd_impl(dout, q, k, v, out, stat, lo, hi, mask, slopes, offsets, ctx.scale, ctx.softcap, ctx.offset,
+                          ctx.monotone, stat, True)
         return (*grads,) + (None,) * 9

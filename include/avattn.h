@@ -956,6 +956,17 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * included).  bf16 (strides multiples of 8), or float32 with is_f32 (of 4).
  * lse: natural log of the changed scores' sum.
  *
+ * Precision of the bias: the kernels measure a row's distances from that of the
+ * key it favours most, its nearest one with a slope >= 0, its farthest one with
+ * a slope below, so that neither a far position nor a long cache costs the
+ * scores bits (exact integers up to 2^24 keys).  Its keys are those of its
+ * window; with a slope below 0 also between the first and the last key that
+ * key_mask attends.  What that leaves out of the row's scores, slopes[hq] times
+ * that distance, is in lse, which holds it as float32 does.  With
+ * AVATTN_SCORED_ROW_LSE (and slopes; else AVATTN_ERR_ARGUMENT) lse has room for
+ * 2 x batch * heads_q * len_q floats, and the second half receives the same
+ * without it, for avattn_bwd_scored_row_lse.
+ *
  * A few queries (up to 32, or up to 64 rows len_q * heads_q / heads_kv; float32
  * up to 16) and small calls run on kernels of their own, which read k and v in
  * place; the row strides of k and v are then below 2^23 (AVATTN_ERR_LAYOUT).
@@ -969,8 +980,12 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * 256-byte aligned.  With avattn_bwd_scored_workspace_size (every (batch, kv
  * head) pair in one pass; no ds_table) the call also splits a short grid, dk
  * and dv then being sums of fp32 parts in a fixed order.
+ * avattn_bwd_scored takes the forward's lse (with slopes as exact as float32
+ * holds it: probabilities are off by up to |lse| 2^-24 relatively),
+ * avattn_bwd_scored_row_lse its second half.  Without slopes the two are one.
  */
 #define AVATTN_SCORED_SORTED_WINDOWS 1u
+#define AVATTN_SCORED_ROW_LSE 4u
 
 size_t avattn_fwd_scored_workspace_size(int32_t batch, int32_t heads_q,
                                         int32_t heads_kv, int32_t len_q,
@@ -1018,6 +1033,29 @@ int avattn_bwd_scored(const void* dout, const void* q, const void* k,
                       void* dv, const int64_t* dv_strides,
                       void* workspace, size_t workspace_bytes,
                       avattn_stream_t stream);
+
+int avattn_bwd_scored_row_lse(const void* dout, const void* q,
+                              const void* k, const void* v, const void* out,
+                              const float* row_lse,
+                              const int64_t* dout_strides,
+                              const int64_t* q_strides,
+                              const int64_t* k_strides, const int64_t* v_strides,
+                              const int64_t* out_strides,
+                              int32_t batch, int32_t heads_q, int32_t heads_kv,
+                              int32_t len_q, int32_t len_k, int32_t head_dim,
+                              int32_t is_f32,
+                              const uint8_t* key_mask, int64_t key_mask_batch_stride,
+                              const int32_t* window_lo, const int32_t* window_hi,
+                              int64_t window_batch_stride,
+                              const int32_t* ds_table, int64_t ds_table_batch_stride,
+                              int64_t ds_units_per_head,
+                              float scale, float softcap, const float* slopes,
+                              const int32_t* query_offsets, int32_t query_offset,
+                              void* dq, const int64_t* dq_strides,
+                              void* dk, const int64_t* dk_strides,
+                              void* dv, const int64_t* dv_strides,
+                              void* workspace, size_t workspace_bytes,
+                              avattn_stream_t stream);
 
 #ifdef __cplusplus
 }

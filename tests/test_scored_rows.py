@@ -1,0 +1,48 @@
+"""The row statistic of biased scores without a GPU: refusals of the C entry
+points and of the backward."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from avgen_amd import _lib, scored_ops
+
+B16 = torch.bfloat16
+cpu_only = pytest.mark.skipif(torch.cuda.is_available(), reason="fake-pointer validation tests run only without a GPU")
+
+
+@cpu_only
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("Lq", [1, 5000])
+def test_c_entry_points_refuse(f32, Lq):
+    lib = _lib.load()
+    p, s, odd = 4096, _lib.i64_array([64, 64, 64]), _lib.i64_array([64, 64, 66])
+    Lk = 5000
+
+    def fwd(slopes=p, flags=4, B=1, lse=p):
+        return lib.avattn_fwd_scored(p, p, p, s, s, s, B, 4, 2, Lq, Lk, 64, f32, None, 0, None, None, 0, 0.125, 10.0,
+                                     slopes, None, 0, flags, p, s, lse, p, 1 << 40, None)
+
+    assert _lib.SCORED_ROW_LSE == 4
+    assert fwd(slopes=None) == 9 and fwd(flags=8) == 9 and fwd(flags=2) == 9
+    assert fwd(lse=None) == 1
+    assert fwd(B=0) == 0 and fwd(B=0, flags=5) == 0
+
+    def bwd(lse=p, dqs=s, ws=p, scale=0.125, B=1, slopes=p):
+        return lib.avattn_bwd_scored_row_lse(p, p, p, p, p, lse, s, s, s, s, s, B, 4, 2, Lq, Lk, 64, f32, None, 0, None,
+                                             None, 0, None, 0, 0, scale, 10.0, slopes, None, 0, p, dqs, p, s, p, s, ws,
+                                             1 << 40, None)
+
+    assert bwd(lse=None) == 1 and bwd(dqs=None) == 1 and bwd(dqs=odd) == 5 and bwd(ws=None) == 6
+    assert bwd(scale=0.0) == 9 and bwd(slopes=p + 2) == 5
+    assert bwd(B=0) == 0 and bwd(B=-1) == 2
+
+
+@pytest.mark.parametrize("row_lse", [torch.zeros(2, 4, 4), torch.zeros(2, 4, 5, dtype=B16), torch.zeros(2, 2, 5)])
+def test_backward_refuses_another_row_statistic(row_lse, monkeypatch):
+    monkeypatch.setattr(scored_ops, "_one_device", lambda *a: None)
+    q, k = torch.zeros(2, 4, 5, 64, dtype=B16), torch.zeros(2, 2, 7, 64, dtype=B16)
+    with pytest.raises(ValueError, match="logsumexp"):
+        scored_ops._bwd_impl(q, q, k, k, q, torch.zeros(2, 4, 5), None, None, None, torch.ones(4), None, 0.125, 5.0, 0,
+                             False, row_lse)
