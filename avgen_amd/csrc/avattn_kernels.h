@@ -581,6 +581,7 @@ struct RotateArgs {
   int64_t xs[2][3], os[2][3];
   int H[2];
   int B, L, D, P, start;
+  int64_t first;  // the launch's first token (b * L + i), set by launch_rotate
   const float* ct;
   const float* st;
   int64_t tsb;

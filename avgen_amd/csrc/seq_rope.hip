@@ -128,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   if (g >= groups) return;
   const int heads = a.H[0] + a.H[1];
   const int tpb = max(1, groups / heads);
-  const int64_t tok = (int64_t)blockIdx.x * tpb + (tpb > 1 ? g / heads : 0);
+  const int64_t tok = a.first + (int64_t)blockIdx.x * tpb + (tpb > 1 ? g / heads : 0);
   if (tok >= (int64_t)a.B * a.L || (tpb > 1 && g >= tpb * heads)) return;
   const int h0 = tpb > 1 ? g % heads : g, hstep = tpb > 1 ? heads : groups;
   const int b = (int)(tok / a.L), i = (int)(tok - (int64_t)b * a.L);
@@ -245,18 +245,25 @@ hipError_t rotate(const RotateArgs& a, bool half, hipStream_t stream) {
   const int heads = a.H[0] + a.H[1];
   const int tpb = groups / heads > 1 ? groups / heads : 1;
   const int64_t blocks = ((int64_t)a.B * a.L + tpb - 1) / tpb;
-  if (blocks > (1 << 24) - 1) return hipErrorInvalidValue;  // threads of a grid: below 2^32
   LaunchTimer timer(kKidRopeApply, stream);
-  const dim3 grid((unsigned)blocks), block(kThreads);
-  if (half && vec)
-    hipLaunchKernelGGL((rotate_kernel<T, true, true>), grid, block, 0, stream, a);
-  else if (half)
-    hipLaunchKernelGGL((rotate_kernel<T, true, false>), grid, block, 0, stream, a);
-  else if (vec)
-    hipLaunchKernelGGL((rotate_kernel<T, false, true>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((rotate_kernel<T, false, false>), grid, block, 0, stream, a);
-  return hipGetLastError();
+  // Any number of tokens: the threads of a grid stay below 2^32.
+  constexpr int64_t kMost = 1 << 23;
+  for (int64_t done = 0; done < blocks; done += kMost) {
+    RotateArgs r = a;
+    r.first = done * tpb;
+    const dim3 grid((unsigned)(blocks - done < kMost ? blocks - done : kMost)), block(kThreads);
+    if (half && vec)
+      hipLaunchKernelGGL((rotate_kernel<T, true, true>), grid, block, 0, stream, r);
+    else if (half)
+      hipLaunchKernelGGL((rotate_kernel<T, true, false>), grid, block, 0, stream, r);
+    else if (vec)
+      hipLaunchKernelGGL((rotate_kernel<T, false, true>), grid, block, 0, stream, r);
+    else
+      hipLaunchKernelGGL((rotate_kernel<T, false, false>), grid, block, 0, stream, r);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace

@@ -878,9 +878,10 @@ int avattn_rope_apply_pair_f32(int32_t batch, int32_t head_dim,
  * and k (either may have 0 heads) by the token's table row and copies the
  * others.  Pair p is channels start + 2p, + 1 (half_layout 0) or start + p,
  * start + pairs + p (1).  bf16, or float32 with is_f32; any strides with
- * contiguous head_dim, any head_dim of at least 2 pairs; outputs must not
- * overlap the inputs.  fp32 products rounded separately.  inverse: the
- * transposed rotation (the gradient).  table_batch_stride 0 = shared.
+ * contiguous head_dim, any head_dim of at least 2 pairs (up to 65,536), any
+ * number of tokens, up to 2^24 heads; outputs must not overlap the inputs.
+ * fp32 products rounded separately.  inverse: the transposed rotation (the
+ * gradient).  table_batch_stride 0 = shared.
  */
 int avattn_position_tables(const void* positions, int32_t positions_i64,
                            int64_t positions_batch_stride,
