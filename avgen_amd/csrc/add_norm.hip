@@ -366,21 +366,24 @@ __global__ __launch_bounds__(256) void add_norm_dw_kernel(const float* __restric
                                                           void* dw, bool dw32) {
   __shared__ float red[8][32];
   const int c = threadIdx.x % 32, g = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * 32 + c;
-  float s = 0.f;
-  if (col < W) {
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < W; c0 += (int64_t)gridDim.x * 32) {
+    const int64_t col = c0 + c;
+    float s = 0.f;
+    if (col < W) {
 #pragma unroll 8
-    for (int p = g; p < nparts; p += 8) s += part[p * W + col];
-  }
-  red[g][c] = s;
-  __syncthreads();
-  if (g == 0 && col < W) {
+      for (int p = g; p < nparts; p += 8) s += part[p * W + col];
+    }
+    __syncthreads();  // the last columns' sums are read
+    red[g][c] = s;
+    __syncthreads();
+    if (g == 0 && col < W) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][c];
-    if (dw32)
-      static_cast<float*>(dw)[col] = s;
-    else
-      static_cast<bf16*>(dw)[col] = (bf16)s;
+      for (int i = 1; i < 8; ++i) s += red[i][c];
+      if (dw32)
+        static_cast<float*>(dw)[col] = s;
+      else
+        static_cast<bf16*>(dw)[col] = (bf16)s;
+    }
   }
 }
 
@@ -519,8 +522,9 @@ hipError_t backward(const AddNormArgs& a, void* dw, bool dw32, hipStream_t strea
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(add_norm_dw_kernel, dim3((unsigned)((a.W + 31) / 32)), dim3(256), 0, stream, a.part, nparts, a.W,
-                     dw, dw32);
+  const int64_t groups = (a.W + 31) / 32;
+  hipLaunchKernelGGL(add_norm_dw_kernel, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(256), 0, stream,
+                     a.part, nparts, a.W, dw, dw32);
   return hipGetLastError();
 }
 

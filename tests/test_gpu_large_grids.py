@@ -1,11 +1,12 @@
-"""Rotation of more tokens than one launch can hold."""
+"""Rotation of more tokens, and residual norm over wider rows, than one launch
+of a thread group each can hold."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from avgen_amd import rope
+from avgen_amd import layers, rope
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +45,25 @@ def test_tables_of_many_tokens_in_the_rotation():
     c, s = tables.cos[..., 0], tables.sin[..., 0]
     assert torch.equal(out[..., 0], (c - s).bfloat16()) and torch.equal(out[..., 1], (s + c).bfloat16())
     assert not out[..., 2:].any()
+
+
+def test_residual_norm_backward_of_wide_rows():
+    """One row of 2^29 + 8 values: more columns than the threads of a launch."""
+    W = (1 << 29) + 8
+    x = torch.zeros((1, W), device="cuda", dtype=torch.bfloat16)
+    x[0, ::3] = 1.0
+    r = torch.zeros((1, 1), device="cuda", dtype=torch.bfloat16).expand(1, W)
+    w = torch.ones(W, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    n, h = layers.add_rms_norm(x, r, w)
+    dn = torch.zeros((1, W), device="cuda", dtype=torch.bfloat16)
+    dn[0, 0] = 1.0
+    dn[0, -1] = 4.0  # W - 1 = 3 m: a value of 1
+    dn[0, -2] = 2.0  # a value of 0
+    (dw,) = torch.autograd.grad(n, (w,), dn)
+    # Every third value is 1: rstd = sqrt(W / ceil(W / 3)) = sqrt(3) to 1e-8.
+    assert (W - 1) % 3 == 0
+    want = torch.tensor([3.0**0.5, 0.0, 0.0, 4 * 3.0**0.5])
+    got = torch.stack([dw[0], dw[1], dw[-2], dw[-1]]).float().cpu()
+    # A bf16 rounding of the gradient, and sums of 2^29 / 3 ones in float32 partial sums.
+    assert bool(((got - want).abs() <= (2.0**-8 + 2.0**-12) * want).all())
+    assert int((dw != 0).sum()) == 2
