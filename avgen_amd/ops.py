@@ -84,7 +84,12 @@ _Strides3 = ctypes.c_int64 * 3
 
 
 def _strides3(t: torch.Tensor) -> ctypes.Array:
-    return _Strides3(*t.stride()[:3])
+    """Batch, head and row strides for a C call, which wants them in units of up
+    to 8 elements: those of sizes of one, which nothing steps by, are rounded up."""
+    s0, s1, s2, _ = t.stride()
+    if (s0 | s1 | s2) % 8:
+        s0, s1, s2 = (-(-s // 8) * 8 if n == 1 else s for s, n in zip((s0, s1, s2), t.shape))
+    return _Strides3(s0, s1, s2)
 
 
 # Plain eager calls go straight to an autograd function (or, without grad, to

@@ -35,6 +35,7 @@ from .ops import (
     _ptr,
     _stream,
     _Strides3,
+    _strides3,
     _workspace,
     compact_ds_table,
     ds_bytes_per_pair,
@@ -107,7 +108,7 @@ def _laid_out(t: torch.Tensor, f32: bool):
     s0, s1, s2, s3 = t.stride()
     if s3 != 1 or (s0 | s1 | s2) % (4 if f32 else 8) or t.data_ptr() % 16:
         t = _f32_ready(t) if f32 else _kernel_ready(t)
-        s0, s1, s2, _ = t.stride()
+        return t, _strides3(t)
     return t, _Strides3(s0, s1, s2)
 
 

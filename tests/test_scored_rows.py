@@ -46,3 +46,19 @@ def test_backward_refuses_another_row_statistic(row_lse, monkeypatch):
     with pytest.raises(ValueError, match="logsumexp"):
         scored_ops._bwd_impl(q, q, k, k, q, torch.zeros(2, 4, 5), None, None, None, torch.ones(4), None, 0.125, 5.0, 0,
                              False, row_lse)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_strides_of_sizes_of_one_are_rounded(f32):
+    """What the C entry points would refuse in a size that is stepped by, they
+    get in whole units where the size is one."""
+    t = torch.zeros(100_000, dtype=torch.float32 if f32 else B16)
+    one = t.as_strided((1, 3, 5, 64), (12_345, 320, 64, 1))
+    laid, strides = scored_ops._laid_out(one, f32)
+    assert laid.data_ptr() == one.data_ptr() and list(strides) == [12_352, 320, 64]
+    one = t.as_strided((2, 1, 1, 64), (640, 77, 67, 1))
+    laid, strides = scored_ops._laid_out(one, f32)
+    assert laid.data_ptr() == one.data_ptr() and list(strides) == [640, 80, 72]
+    two = t.as_strided((2, 3, 5, 64), (12_345, 320, 64, 1))
+    laid, strides = scored_ops._laid_out(two, f32)
+    assert laid.data_ptr() != two.data_ptr() and list(strides) == [960, 320, 64]
