@@ -147,11 +147,13 @@ def _rotate_run(name, q, k, cos, sin, tsb, start, half, inverse):
     B, _, L, D = q.shape
     outs = []
     args = []
+    read = []  # held until the launch: copies among them belong to nobody else
     for t in (q, k):
         if t is None:
             args += (None, None, 0, None, None)
             continue
         t = _packed_last(t)
+        read.append(t)
         o = torch.empty_like(t)
         outs.append(o)
         strides, ostrides = t.stride(), o.stride()
