@@ -146,28 +146,35 @@ def _rotate_run(name, q, k, cos, sin, tsb, start, half, inverse):
     """The rotation of checked arguments."""
     B, _, L, D = q.shape
     outs = []
+    written = []
     args = []
     read = []  # held until the launch: copies among them belong to nobody else
     for t in (q, k):
         if t is None:
             args += (None, None, 0, None, None)
             continue
+        # The layout that the op promises; written elsewhere and copied where
+        # its channels are not next to each other.
+        o = w = torch.empty_like(t)
+        outs.append(o)
         t = _packed_last(t)
         read.append(t)
-        o = torch.empty_like(t)
-        outs.append(o)
-        strides, ostrides = t.stride(), o.stride()
-        if ostrides[3] != 1 and D > 1:
-            o = outs[-1] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            ostrides = o.stride()
+        strides, wstrides = t.stride(), o.stride()
+        if wstrides[3] != 1 and D > 1:
+            w = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            wstrides = w.stride()
+        written.append(w)
         s = _Strides3(*strides[:3])
-        args += (t.data_ptr(), s, t.shape[1], o.data_ptr(), s if ostrides == strides else _Strides3(*ostrides[:3]))
+        args += (t.data_ptr(), s, t.shape[1], w.data_ptr(), s if wstrides == strides else _Strides3(*wstrides[:3]))
     device = q.device
     with _on(device):
         st = _lib.load().avattn_rotate(
             *args, B, L, D, cos.shape[-1], start, half, q.dtype is torch.float32,
             cos.data_ptr(), sin.data_ptr(), tsb, inverse, _stream(device))
     _lib.check(st, name)
+    for o, w in zip(outs, written):
+        if w is not o:
+            o.copy_(w)
     return outs
 
 

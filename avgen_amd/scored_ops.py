@@ -112,12 +112,24 @@ def _laid_out(t: torch.Tensor, f32: bool):
     return t, _Strides3(s0, s1, s2)
 
 
-def _new_like(t: torch.Tensor, strides, f32: bool):
-    """An output shaped like ``t`` (whose strides are given), and its strides."""
+def _new_like(t: torch.Tensor, laid: torch.Tensor, strides, f32: bool):
+    """An output in the layout that the op promises, ``empty_like`` of its input
+    ``t`` (read as ``laid``, with these strides): the output, what the kernels
+    write (the output, or where they cannot write its layout a tensor to copy from,
+    see :func:`_deliver`), and its strides for the C call."""
     o = torch.empty_like(t)
-    if o.stride() == t.stride():
-        return o, strides
-    return _laid_out(o, f32)
+    if t is laid and o.stride() == t.stride():
+        return o, o, strides
+    written, strides = _laid_out(o, f32)
+    return o, written, strides
+
+
+def _deliver(*outputs):
+    """The outputs of ``(output, written, strides)`` triples, as written."""
+    for o, written, _ in outputs:
+        if written is not o:
+            o.copy_(written)
+    return tuple(o for o, _, _ in outputs)
 
 
 # Workspace sizes: functions of a call's sizes alone.
@@ -149,10 +161,11 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
     B, Hq, Lq, D = q.shape
     Hkv, Lk = k.shape[1], k.shape[2]
     f32 = q.dtype is torch.float32
+    given = q
     (q, qs), (k, ks), (v, vs) = _laid_out(q, f32), _laid_out(k, f32), _laid_out(v, f32)
     if ks[2] >= _MAX_ROW_STRIDE or vs[2] >= _MAX_ROW_STRIDE:
         (k, ks), (v, vs) = _laid_out(k.contiguous(), f32), _laid_out(v.contiguous(), f32)
-    out, os = _new_like(q, qs, f32)
+    o = _new_like(given, q, qs, f32)
     device = q.device
     row_lse = lse = torch.empty((B, Hq, Lq) if slopes is None or not rows else (2, B, Hq, Lq), device=device,
                                 dtype=torch.float32)
@@ -166,8 +179,9 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
             q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, B, Hq, Hkv, Lq, Lk, D, f32,
             _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb,
             scale, softcap, _ptr(slopes), _ptr(offsets), offset, flags,
-            out.data_ptr(), os, lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
+            o[1].data_ptr(), o[2], lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
     _lib.check(st, name)
+    (out,) = _deliver(o)
     return (out, lse, row_lse) if rows else (out, lse)
 
 
@@ -236,10 +250,11 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
             raise RuntimeError(f"{name}: a captured backward cannot check the windows' order; pass monotone=True")
         if bool(((lo[..., 1:] < lo[..., :-1]) | (hi[..., 1:] < hi[..., :-1])).any()):
             raise ValueError(f"{name}: the backward needs window_lo and window_hi non-decreasing along the queries")
+    given = (q, k, v)
     (dout, dos), (q, qs), (k, ks) = _laid_out(dout, f32), _laid_out(q, f32), _laid_out(k, f32)
     (v, vs), (out, os) = _laid_out(v, f32), _laid_out(out, f32)
     stat = (lse if row_lse is None else row_lse).contiguous()
-    (dq, dqs), (dk, dks), (dv, dvs) = _new_like(q, qs, f32), _new_like(k, ks, f32), _new_like(v, vs, f32)
+    dq, dk, dv = (_new_like(*t, f32) for t in zip(given, (q, k, v), (qs, ks, vs)))
     device = q.device
     table, tsb, units = None, 0, 0
     if 0 in (B, Hq, Lq, Lk):
@@ -258,10 +273,10 @@ def _bwd_impl(dout, q, k, v, out, lse, window_lo, window_hi, key_mask, slopes, o
             dos, qs, ks, vs, os, B, Hq, Hkv, Lq, Lk, D, f32,
             _ptr(mask), msb, _ptr(lo), _ptr(hi), wsb, _ptr(table), tsb, units,
             scale, softcap, _ptr(slopes), _ptr(offsets), offset,
-            dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dvs,
+            dq[1].data_ptr(), dq[2], dk[1].data_ptr(), dk[2], dv[1].data_ptr(), dv[2],
             ws.data_ptr(), ws.numel(), _stream(device))
     _lib.check(st, name)
-    return dq, dk, dv
+    return _deliver(dq, dk, dv)
 
 
 @torch.library.custom_op("avgen_amd::flash_fwd_scored", mutates_args=())
