@@ -446,6 +446,7 @@ KERNEL_IDS = {
     "add_rms_norm": 16,
     "add_rms_norm_bwd": 17,
     "attn_fwd_few": 18,
+    "window_hull": 19,
 }
 
 

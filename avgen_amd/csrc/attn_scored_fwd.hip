@@ -64,7 +64,7 @@ void launch_fwd_scored(const FwdArgs& a, int head_dim, bool small, dim3 grid, hi
 
 hipError_t launch_window_hull(const int* wlo, const int* whi, int64_t wsb, int B, int Lq, int Lk, int* hull,
                               hipStream_t stream) {
-  LaunchTimer timer(kKidTranspose, stream);
+  LaunchTimer timer(kKidWindowHull, stream);
   hipLaunchKernelGGL(window_hull_kernel, dim3((unsigned)B), dim3(1024), 0, stream, wlo, whi, wsb, Lq, Lk, hull);
   return hipGetLastError();
 }

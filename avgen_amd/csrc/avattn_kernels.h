@@ -421,6 +421,7 @@ enum KernelId : int {
   kKidAddNorm = 16,
   kKidAddNormBwd = 17,
   kKidFwdFew = 18,
+  kKidWindowHull = 19,
 };
 
 // Records HIP events around one launch on `stream` while timing is enabled.

@@ -657,7 +657,9 @@ int avattn_qk_norm_rope_bwd(const void* x, const int64_t* x_strides,
  * fp8 forward's e4m3 k copy), 8 fp8 forward, 9 fp8 absmax scales,
  * 10 dQ from staged dS, 11 q/k norm + rotation, 12 its backward,
  * 13 the ring dq finish (avattn_ring_dq_finish), 14 the sum of the
- * partial results of split dK/dV workgroups, 15 avattn_diag_dq_partials.
+ * partial results of split dK/dV workgroups, 15 avattn_diag_dq_partials,
+ * 16 residual norm, 17 its backward (without the gain's reduction),
+ * 18 forward of few query rows, 19 the range of unsorted key windows.
  * avattn_timing_begin creates `capacity` event pairs (call it outside any
  * timed or captured region); launches beyond capacity are not recorded and
  * make avattn_timing_read return AVATTN_ERR_WORKSPACE.
