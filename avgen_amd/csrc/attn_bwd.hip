@@ -433,7 +433,8 @@ __global__ __launch_bounds__(512, 1) void bwd_dq_kernel(BwdArgs a) {
 // 32 rows' windows (the dK/dV kernel wrote the dS of exactly those: a
 // group's window union lies inside its 64-row tile's).
 // NW: waves (32 rows each) per workgroup; 4 for short grids of changed scores
-// (launch_dq_ds_d), two workgroups per CU.  The bits are the same.
+// (launch_dq_ds_d).  By their LDS two of those fit a CU at D 64 (72 KB each), one
+// at D 128 (96 KB).  The bits are the same.
 template <int D, int BK, int NSTG, bool WIN, bool CT, int NW = 8>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void bwd_dq_ds_kernel(BwdArgs a) {
   static_assert(!CT || WIN, "the compact dS layout (BwdArgs::ds_tab) is for windows");
@@ -724,13 +725,13 @@ static void launch_dq_ds_d(const BwdArgs& a, hipStream_t stream) {
   // partial last round is not split as the dK/dV one is: this kernel is
   // bound by HBM, and the last round's workgroups share all of it (measured:
   // no gain at c3).
-  // With changed scores, grids of few rounds in workgroups of 128 rows: more of
-  // them share a CU's latency, but K is staged twice as often.  Backward in 256
-  // against 128 rows, D 128: causal (1,4,1024) 16 workgroups of 256 rows 53.0 /
-  // 47.8 us, (1,16,2048) 128 115.8 / 105.4, (1,16 on 4 heads,4133) 272 299 / 286,
-  // (1,40,2304) 360 243.1 / 241.4 (with a prefix of 512 dQ alone 64 / 67), (1,16
-  // on 8 heads,8192) 512 856 / 881; no windows (1,2,16384) 128 849 / 796,
-  // (1,20,2304) 180 212 / 216, (1,8,8192) 256 795 / 818.
+  // With changed scores, short grids in workgroups of 128 rows: twice as many
+  // spread over CUs that would idle (and at D 64 two share a CU), but K is staged
+  // twice as often.  Backward in 256 against 128 rows, D 128: causal (1,4,1024)
+  // 16 workgroups of 256 rows 53.0 / 47.8 us, (1,16,2048) 128 115.8 / 105.4, (1,16
+  // on 4 heads,4133) 272 299 / 286, (1,40,2304) 360 243.1 / 241.4 (with a prefix of
+  // 512 dQ alone 64 / 67), (1,16 on 8 heads,8192) 512 856 / 881; no windows
+  // (1,2,16384) 128 849 / 796, (1,20,2304) 180 212 / 216, (1,8,8192) 256 795 / 818.
   if (a.score.mode != 0 && !a.ds_tab && grid.x <= (a.wlo ? 300 : 160)) {
     const dim3 short_grid((a.Lqp / 32 + 3) / 4 * a.nkv * group);
     if (a.wlo)
