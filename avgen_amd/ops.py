@@ -225,7 +225,8 @@ def _kernel_ready(t: torch.Tensor) -> torch.Tensor:
     ok = s3 == 1 and t.data_ptr() % 16 == 0
     if ok and (s0 | s1 | s2) % 8:
         ok = all(s % 8 == 0 or n == 1 for s, n in zip((s0, s1, s2), t.shape[:3]))
-    return t if ok else t.contiguous()
+    # (A copy always: contiguous() returns contiguous rows as they are, aligned or not.)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _normalise_mask(name: str, key_mask: Optional[torch.Tensor], batch: int, len_k: int):
@@ -318,7 +319,8 @@ def _f32_ready(t: torch.Tensor) -> torch.Tensor:
     ok = s3 == 1 and t.data_ptr() % 16 == 0
     if ok and (s0 | s1 | s2) % 4:
         ok = all(s % 4 == 0 or n == 1 for s, n in zip((s0, s1, s2), t.shape[:3]))
-    return t if ok else t.contiguous()
+    # (A copy always: contiguous() returns contiguous rows as they are, aligned or not.)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _fwd_f32_impl(name, q, k, v, key_mask, rope_cos, rope_sin, scale):

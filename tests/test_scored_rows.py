@@ -3,10 +3,12 @@ points and of the backward."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from avgen_amd import _lib, scored_ops
+from avgen_amd import _lib, ops, scored_ops
 
 B16 = torch.bfloat16
 cpu_only = pytest.mark.skipif(torch.cuda.is_available(), reason="fake-pointer validation tests run only without a GPU")
@@ -62,3 +64,16 @@ def test_strides_of_sizes_of_one_are_rounded(f32):
     two = t.as_strided((2, 3, 5, 64), (12_345, 320, 64, 1))
     laid, strides = scored_ops._laid_out(two, f32)
     assert laid.data_ptr() != two.data_ptr() and list(strides) == [960, 320, 64]
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_unaligned_rows_are_copied(f32):
+    """Also where they are contiguous, one row of one head among them."""
+    dtype = torch.float32 if f32 else B16
+    ready = ops._f32_ready if f32 else ops._kernel_ready
+    flat = torch.arange(3000, dtype=torch.float32).to(dtype)
+    for shape in ((2, 3, 5, 64), (1, 1, 1, 64)):
+        t = flat[1:1 + math.prod(shape)].view(shape)
+        assert t.is_contiguous() and t.data_ptr() % 16 != 0
+        for got in (ready(t), scored_ops._laid_out(t, f32)[0]):
+            assert got.data_ptr() % 16 == 0 and torch.equal(got, t)
