@@ -534,6 +534,9 @@ __global__ __launch_bounds__(512, 1) void bwd_dkdv_kernel(BwdArgs a) {
         }
       }
     };
+    // P and, capped, P (1 - tanh^2) are rounded to bf16 here, as the operands
+    // of dV's products and the factors of dS; everything before is fp32.  (The
+    // fp32 matrix instructions run at an eighth of the rate.)
     u32x4 ux;  // SCORE: P (1 - tanh^2) of one (sub, k2)
     auto smx = [&](int sub, int k2, int e2) {
       const int e = 2 * e2;

@@ -338,14 +338,15 @@ __global__ __launch_bounds__(256) void attn_few_kernel(FewArgs a) {
   join_waves<D, bf16>(a, jn, unit, split, rows);
 }
 
-// float32, RB rows at a time on the vector ALUs (the fp32 matrix instructions
-// would multiply 32 rows whatever their number, and take longer than a tile's
-// 32 KB to arrive): 268 MB of cache in 46 us with one row per kv head, 5.8
-// TB/s, 54 us with 4; every 4 more rows read K and V again from the caches,
-// about 39 us.  Scores: lane l owns key l % 32 of the wave's tile and half
-// of the channels, K from LDS (staged as above, rows of 256 bytes), q by
-// broadcast reads.  P V: a lane owns D / 64 channels, V's rows come straight
-// from memory a tile ahead (whole rows per load), p_j by readlane.
+// float32, RB rows at a time on the vector ALUs: 268 MB of cache in 41 us with
+// one row per kv head, 6.5 TB/s (part of it from the last-level cache), 52 us
+// with 4, and 4 us to combine; every 4 more rows read K and V again, about 38
+// us.  (The fp32 matrix instructions, which this kernel does not use, would
+// multiply 32 rows whatever their number: 4.3 GFLOP, 28 us beside these loads.)
+// Scores: lane l owns key l % 32 of the wave's tile and half of the channels, K
+// from LDS (staged as above, rows of 256 bytes), q by broadcast reads.  P V: a
+// lane owns D / 64 channels, V's rows come straight from memory a tile ahead
+// (whole rows per load), p_j by readlane.
 template <int D, int RB>
 __global__ __launch_bounds__(256) void attn_few_f32_kernel(FewArgs a) {
   constexpr int HD = D / 2, CL = D / 64, NS = D / 64;  // channels per lane in P V; 64-channel K sub-tiles

@@ -8,11 +8,14 @@
 //            y0 = x0 c - x1 s,  y1 = x0 s + x1 c     (s -> -s: the transpose)
 //            interleaved: x0, x1 at start + 2p, + 1; half: at start + p,
 //            start + P + p; the other channels are copied.
-// Both are HBM-bound: the rotation reads and writes every value once; the
-// tables are read once per token, not once per head.  2 x 4,096 tokens of 80
+// The rotation is HBM-bound: it reads and writes every value once; the tables
+// are read once per token, not once per head.  2 x 4,096 tokens of 80
 // heads of 128 bf16, half of each rotated: 73 us (4.6 TB/s); 65,537 tokens of
-// 20 heads, all of it: 154 us (4.6 TB/s), their tables 21 us (1.6 TB/s: the
-// double arithmetic); 16 tokens of 40 heads 4 us.
+// 20 heads, all of it: 150 us (4.5 TB/s), their tables 20 us (1.7 TB/s: the
+// vector ALUs are busy in every cycle, with about 119 instructions an entry,
+// 31 of them in double and 36 of the two index divisions); 16 tokens of 40
+// heads 4 us.  Value by value (VEC false), 2 x 4,096 tokens of 80 heads of 80,
+// 20 pairs in half layout, 97 us, where the interleaved layout's chunks take 33.
 #include "avattn_device.h"
 #include "avattn_kernels.h"
 

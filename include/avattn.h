@@ -963,8 +963,8 @@ int avattn_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
  * key it favours most, its nearest one with a slope >= 0, its farthest one with
  * a slope below, so that neither a far position nor a long cache costs the
  * scores bits (exact integers up to 2^24 keys).  Its keys are those of its
- * window; with a slope below 0 also between the first and the last key that
- * key_mask attends.  What that leaves out of the row's scores, slopes[hq] times
+ * window from the first to the last 64 keys with one that key_mask attends.
+ * What that leaves out of the row's scores, slopes[hq] times
  * that distance, is in lse, which holds it as float32 does.  With
  * AVATTN_SCORED_ROW_LSE (and slopes; else AVATTN_ERR_ARGUMENT) lse has room for
  * 2 x batch * heads_q * len_q floats, and the second half receives the same
