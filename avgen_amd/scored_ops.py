@@ -164,7 +164,7 @@ def _fwd_impl(q, k, v, window_lo, window_hi, key_mask, slopes, offsets, scale, s
     given = q
     (q, qs), (k, ks), (v, vs) = _laid_out(q, f32), _laid_out(k, f32), _laid_out(v, f32)
     if ks[2] >= _MAX_ROW_STRIDE or vs[2] >= _MAX_ROW_STRIDE:
-        (k, ks), (v, vs) = _laid_out(k.contiguous(), f32), _laid_out(v.contiguous(), f32)
+        (k, ks), (v, vs) = (_laid_out(t.clone(memory_format=torch.contiguous_format), f32) for t in (k, v))
     o = _new_like(given, q, qs, f32)
     device = q.device
     row_lse = lse = torch.empty((B, Hq, Lq) if slopes is None or not rows else (2, B, Hq, Lq), device=device,

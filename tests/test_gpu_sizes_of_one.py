@@ -45,6 +45,20 @@ def test_strides_of_sizes_of_one(Lq, heads, dtype):
 
 
 @pytest.mark.parametrize("dtype", [B16, F32])
+def test_one_key_of_any_row_stride(dtype):
+    """The one row of k and v of rows that lie far apart."""
+    q, k, v, do = (normal((1, 4, n, 64), dtype, s) for s, n in enumerate((3, 1, 1, 3)))
+    results = []
+    for far in (False, True):
+        a = [odd(t, 2, 1 << 24) if far else t for t in (k, v)]
+        leaves = [t.detach().requires_grad_(True) for t in (q, *a)]
+        out = A.scored_attention(*leaves, softcap=5.0)
+        results.append((out,) + torch.autograd.grad(out, leaves, do))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [B16, F32])
 def test_strides_of_sizes_of_one_in_plain_attention(dtype):
     q, k, v, do = (normal((1, 4, 90, 64), dtype, s) for s in range(4))
     results = []
