@@ -11,17 +11,21 @@ interfaces:
 * :mod:`avgen_amd.rope` — 3D RoPE tables and rotation (``avgen.models.rope``),
   and the rotation of token sequences by integer positions;
 * :mod:`avgen_amd.layers` — a block's q/k norm with rotation, and its residual
-  addition with the RMS norm behind it (also to e4m3);
+  addition with the RMS norm behind it (also to e4m3, or gated and modulated);
+* :mod:`avgen_amd.cache` — a paged key/value cache for serving, bf16 or e4m3:
+  ``append_paged`` (rotating on the way) and ``paged_attention``;
 * :mod:`avgen_amd.ring` — ring local step, LSE merger, emulated ring;
 * :mod:`avgen_amd.context` — contiguous context-parallel shard rules;
-* :mod:`avgen_amd.ops`, :mod:`avgen_amd.scored_ops`, :mod:`avgen_amd.block_ops`
-  — the ``torch.library`` ops over the C ABI.
+* :mod:`avgen_amd.ops`, :mod:`avgen_amd.scored_ops`, :mod:`avgen_amd.block_ops`,
+  :mod:`avgen_amd.gated_ops`, :mod:`avgen_amd.cache_ops` — the ``torch.library``
+  ops over the C ABI.
 """
 
-from . import attention, block_ops, context, layers, ops, ring, rope, scored_ops
+from . import attention, block_ops, cache, cache_ops, context, gated_ops, layers, ops, ring, rope, scored_ops
 from .attention import attention as attention_fn
 from .attention import document_windows, key_padding_mask, rotary_attention, scored_attention
-from .layers import add_rms_norm, add_rms_norm_fp8
+from .cache import PagedCache, append_paged, paged_attention
+from .layers import add_rms_norm, add_rms_norm_fp8, gated_add_rms_norm
 from .ring import SDPAMerger, flash_attention_backward_op, flash_attention_op, ring_attention
 from .rope import (
     PositionScaling,
@@ -36,25 +40,32 @@ from .rope import (
 )
 
 __all__ = [
+    "PagedCache",
     "PositionScaling",
     "RotaryEmbedding",
     "RotaryTables",
     "SDPAMerger",
     "add_rms_norm",
     "add_rms_norm_fp8",
+    "append_paged",
     "apply_rotary",
     "attention",
     "attention_fn",
     "block_ops",
     "build_position_tables",
     "build_rotary_tables",
+    "cache",
+    "cache_ops",
     "context",
     "document_windows",
     "flash_attention_backward_op",
     "flash_attention_op",
+    "gated_add_rms_norm",
+    "gated_ops",
     "key_padding_mask",
     "layers",
     "ops",
+    "paged_attention",
     "ring",
     "ring_attention",
     "rope",

@@ -333,6 +333,41 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i32, c_i64, c_i64, c_i32, c_f32, c_ptr, c_ptr,
          c_ptr, c_size, c_ptr],
     ),
+    "avattn_append_paged": (
+        ctypes.c_int,
+        [c_ptr, c_i64p, c_ptr, c_i64p, c_ptr, c_i64p, c_i32, c_ptr, c_i64p,
+         c_i32, c_i32, c_i32, c_i32,
+         c_ptr, c_ptr, c_i64, c_i32, c_i32, c_i32,
+         c_ptr, c_i64, c_i32, c_ptr, c_ptr,
+         c_ptr, c_i64p, c_ptr, c_i64p, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_i32,
+         c_ptr],
+    ),
+    "avattn_page_values": (
+        ctypes.c_int,
+        [c_ptr, c_i64p, c_ptr, c_i64, c_ptr, c_ptr, c_i64p, c_ptr, c_i64, c_ptr, c_i32, c_i32, c_i32, c_i32, c_ptr],
+    ),
+    "avattn_paged_attention_workspace_size": (c_size, [c_i32] * 9),
+    "avattn_paged_attention": (
+        ctypes.c_int,
+        [c_ptr, c_i64p, c_i32, c_i32, c_i32, c_i32, c_i32,
+         c_ptr, c_i64, c_i32, c_ptr, c_ptr,
+         c_ptr, c_i64p, c_ptr, c_i64p, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_i32,
+         c_i32, c_f32, c_f32, c_ptr,
+         c_ptr, c_i64p, c_ptr, c_ptr, c_size, c_ptr],
+    ),
+    "avattn_gated_add_rms_norm": (
+        ctypes.c_int,
+        [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32,
+         c_i64, c_i64, c_i64, c_i32, c_f32, c_f32, c_ptr, c_ptr, c_ptr],
+    ),
+    "avattn_gated_add_rms_norm_bwd_workspace_size": (c_size, [c_i64, c_i64, c_i64, c_i32]),
+    "avattn_gated_add_rms_norm_bwd": (
+        ctypes.c_int,
+        [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64,
+         c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32,
+         c_i64, c_i64, c_i64, c_i32, c_f32, c_f32,
+         c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr],
+    ),
 }
 
 # Status codes (include/avattn.h).
@@ -447,6 +482,12 @@ KERNEL_IDS = {
     "add_rms_norm_bwd": 17,
     "attn_fwd_few": 18,
     "window_hull": 19,
+    "append_paged": 20,
+    "page_values": 21,
+    "attn_fwd_paged": 22,
+    "prep_paged": 23,
+    "gated_add_rms_norm": 24,
+    "gated_add_rms_norm_bwd": 25,
 }
 
 

@@ -18,8 +18,7 @@
 // 18,900 rows of 5,120 bf16: forward 125 us (6.2 TB/s), backward 160 + 6 (4.8
 // TB/s), 9,450 of float32 125 and 154 + 5; 37,800 rows of 2,560 to e4m3 120 us
 // (5.6 TB/s); 8 rows of 5,120 4 us.
-#include "avattn_device.h"
-#include "avattn_kernels.h"
+#include "norm_parts.h"
 
 namespace avattn {
 
@@ -29,60 +28,6 @@ namespace {
 // per workgroup where rows are narrow.
 constexpr int max_parts(int64_t W) { return W <= 1024 ? 4096 : 1024; }
 
-// The thread's values of a row: NV chunks of CH consecutive columns, chunk j
-// at column (j * TPR + t) * CH.
-template <class T, int CH>
-__device__ __forceinline__ void load_chunk(const T* p, float* v) {
-  if constexpr (CH == 8) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
-  } else if constexpr (CH == 4) {
-    const f32x4 w = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = w[i];
-  } else {
-    v[0] = (float)p[0];
-  }
-}
-template <class T, int CH>
-__device__ __forceinline__ void store_chunk(T* p, const float* v) {
-  if constexpr (CH == 8)
-    *reinterpret_cast<u32x4*>(p) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                         pack_bf16x2(v[6], v[7])};
-  else if constexpr (CH == 4)
-    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-  else
-    p[0] = (T)v[0];
-}
-// A chunk as it was loaded (bf16 stays packed: half the registers), and its
-// values.
-template <class T, int CH>
-using RawChunk = u32x4;
-template <class T, int CH>
-__device__ __forceinline__ RawChunk<T, CH> read_chunk(const T* p) {
-  static_assert(CH * sizeof(T) == 16, "whole chunks");
-  return *reinterpret_cast<const u32x4*>(p);
-}
-template <class T, int CH>
-__device__ __forceinline__ float chunk_value(const RawChunk<T, CH>& r, int e) {
-  if constexpr (CH == 8)
-    return e & 1 ? bf16_hi(r[e / 2]) : bf16_lo(r[e / 2]);
-  else
-    return __uint_as_float(r[e]);
-}
-// The gain's columns: in the rows' type or fp32.
-template <class T, int CH>
-__device__ __forceinline__ void load_gain(const void* w, bool w32, int64_t col, float* v) {
-  if constexpr (sizeof(T) == 4) {
-    load_chunk<float, CH>(static_cast<const float*>(w) + col, v);
-  } else if (!w32) {
-    load_chunk<T, CH>(static_cast<const T*>(w) + col, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) v[i] = static_cast<const float*>(w)[col + i];
-  }
-}
 template <int CH>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float* v) {
   if constexpr (CH == 8)
@@ -91,22 +36,6 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* v) {
     *reinterpret_cast<uint32_t*>(p) = pack_fp8x4(v[0], v[1], v[2], v[3]);
   else
     p[0] = (uint8_t)pack_fp8x4(v[0], 0.f, 0.f, 0.f);
-}
-
-// Sum (or maximum) over the threads of a row: a wave (WAVE) or the workgroup,
-// every thread of which calls it.  red: one float per wave.
-template <bool WAVE, bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float* red) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = MAX ? fmaxf(v, __shfl_xor(v, off)) : v + __shfl_xor(v, off);
-  if constexpr (!WAVE) {
-    __syncthreads();  // the last reduction's values are read
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-    for (int i = 1; i < (int)blockDim.x / 64; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
-  }
-  return v;
 }
 
 __device__ __forceinline__ float fp8_row_scale(float top) {

@@ -107,7 +107,7 @@ template <int D>
 static hipError_t launch_fwd_d(const FwdArgs& args, hipStream_t stream) {
   FwdArgs a = args;
   const bool fp8 = a.k8 != nullptr;
-  hipError_t e = launch_prep_fwd(a, D, stream);
+  hipError_t e = a.paged ? launch_prep_paged(a, D, stream) : launch_prep_fwd(a, D, stream);
   if (e == hipSuccess && fp8) {
     LaunchTimer timer(kKidTranspose, stream);
     e = launch_quantize_rows(a.k, a.ksb, a.ksh, a.ksl, a.B, a.Hkv, a.Lk, D, a.k_scale, a.k8, a.kmax2, stream);

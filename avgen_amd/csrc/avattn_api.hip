@@ -1351,3 +1351,324 @@ int avattn_bwd_scored_row_lse(const void* dout, const void* q, const void* k, co
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// A cache of pages
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// The pool, its strides and the block table that the entry points share.
+int page_args(const void* kp, const int64_t* k_strides, const void* vp, const int64_t* v_strides, const int8_t* ke,
+              int64_t kes, const int8_t* ve, int64_t ves, int32_t pages, int32_t page_size, int32_t heads,
+              int32_t head_dim, int& shift) {
+  if (pages < 0 || heads < 1) return AVATTN_ERR_BAD_SHAPE;
+  if (head_dim != 64 && head_dim != 128) return AVATTN_ERR_HEAD_DIM;
+  shift = kMinPageShift;
+  while (shift <= kMaxPageShift && page_size != 1 << shift) ++shift;
+  if (shift > kMaxPageShift) return AVATTN_ERR_BAD_SHAPE;
+  if (!k_strides || !v_strides) return AVATTN_ERR_NULL_POINTER;
+  if ((ke == nullptr) != (ve == nullptr)) return AVATTN_ERR_ARGUMENT;
+  if (pages == 0) return AVATTN_OK;
+  if (!kp || !vp) return AVATTN_ERR_NULL_POINTER;
+  const int64_t unit = ke ? 16 : 8;  // elements of 16 bytes
+  if (!aligned16(kp) || !aligned16(vp)) return AVATTN_ERR_LAYOUT;
+  for (const int64_t* s : {k_strides, v_strides})
+    if (s[0] % unit != 0 || s[1] % unit != 0 || s[0] < 0 || s[1] < 0) return AVATTN_ERR_LAYOUT;
+  if (ke && (kes < 0 || ves < 0)) return AVATTN_ERR_LAYOUT;
+  return AVATTN_OK;
+}
+
+int table_args(const int32_t* table, int64_t stride, int32_t blocks, const int32_t* lengths, const int32_t* counts,
+               int32_t batch) {
+  if (blocks < 0) return AVATTN_ERR_BAD_SHAPE;
+  if (batch == 0) return AVATTN_OK;
+  if ((blocks > 0 && !table) || !lengths) return AVATTN_ERR_NULL_POINTER;
+  if (!aligned_to(table, 4) || !aligned_to(lengths, 4) || !aligned_to(counts, 4)) return AVATTN_ERR_LAYOUT;
+  if (batch > 1 && stride < blocks && stride != 0) return AVATTN_ERR_ARGUMENT;
+  return AVATTN_OK;
+}
+
+struct PagedWorkspace {
+  size_t windows, offsets, total;
+};
+PagedWorkspace paged_general_workspace(int32_t B, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D) {
+  PagedWorkspace w;
+  w.windows = round256(fwd_workspace(B, Hkv, Lk, D).total);
+  w.offsets = w.windows + round256((size_t)B * Lq * 2 * sizeof(int));
+  w.total = w.offsets + round256((size_t)B * sizeof(int));
+  return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+int avattn_append_paged(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                        const void* q, const int64_t* q_strides, int32_t heads_q, void* q_out,
+                        const int64_t* q_out_strides, int32_t batch, int32_t heads_kv, int32_t len, int32_t head_dim,
+                        const float* cos_tab, const float* sin_tab, int64_t table_batch_stride, int32_t pairs,
+                        int32_t start, int32_t half_layout, const int32_t* block_table, int64_t block_table_stride,
+                        int32_t blocks, const int32_t* lengths, const int32_t* counts, void* key_pages,
+                        const int64_t* key_page_strides, void* value_pages, const int64_t* value_page_strides,
+                        int8_t* key_exponents, int64_t key_exponent_stride, int8_t* value_exponents,
+                        int64_t value_exponent_stride, int32_t pages, int32_t page_size, avattn_stream_t stream) {
+  if (batch < 0 || len < 0 || heads_q < 0 || heads_kv < 1) return AVATTN_ERR_BAD_SHAPE;
+  AppendArgs a{};
+  int st = page_args(key_pages, key_page_strides, value_pages, value_page_strides, key_exponents, key_exponent_stride,
+                     value_exponents, value_exponent_stride, pages, page_size, heads_kv, head_dim, a.pages.shift);
+  if (st != AVATTN_OK) return st;
+  st = table_args(block_table, block_table_stride, blocks, lengths, counts, batch);
+  if (st != AVATTN_OK) return st;
+  if ((cos_tab == nullptr) != (sin_tab == nullptr)) return AVATTN_ERR_ARGUMENT;
+  if (cos_tab) {
+    if (pairs < 1 || start < 0 || (int64_t)start + 2 * (int64_t)pairs > head_dim) return AVATTN_ERR_BAD_SHAPE;
+    if (!aligned_to(cos_tab, 4) || !aligned_to(sin_tab, 4)) return AVATTN_ERR_LAYOUT;
+    if (table_batch_stride != 0 && table_batch_stride < (int64_t)len * pairs) return AVATTN_ERR_ARGUMENT;
+  }
+  if ((int64_t)batch * len == 0) return AVATTN_OK;
+  if (!k || !v || !k_strides || !v_strides) return AVATTN_ERR_NULL_POINTER;
+  if (!aligned_to(k, 2) || !aligned_to(v, 2)) return AVATTN_ERR_LAYOUT;
+  const bool has_q = heads_q > 0;
+  if (has_q && (!q || !q_out || !q_strides || !q_out_strides)) return AVATTN_ERR_NULL_POINTER;
+  if (has_q && (!aligned_to(q, 2) || !aligned_to(q_out, 2))) return AVATTN_ERR_LAYOUT;
+  a.k = static_cast<const bf16*>(k);
+  a.v = static_cast<const bf16*>(v);
+  a.ksb = k_strides[0], a.ksh = k_strides[1], a.ksl = k_strides[2];
+  a.vsb = v_strides[0], a.vsh = v_strides[1], a.vsl = v_strides[2];
+  if (has_q) {
+    a.q = static_cast<const bf16*>(q);
+    a.q_out = static_cast<bf16*>(q_out);
+    a.qsb = q_strides[0], a.qsh = q_strides[1], a.qsl = q_strides[2];
+    a.osb = q_out_strides[0], a.osh = q_out_strides[1], a.osl = q_out_strides[2];
+  }
+  a.B = batch, a.Hq = heads_q, a.Hkv = heads_kv, a.L = len;
+  a.rot.cos = cos_tab, a.rot.sin = sin_tab, a.rot.tsb = table_batch_stride;
+  a.rot.pairs = pairs, a.rot.start = start, a.rot.half = half_layout != 0;
+  a.pages.table = block_table, a.pages.tsb = block_table_stride, a.pages.blocks = blocks, a.pages.pages = pages;
+  a.lengths = lengths, a.counts = counts;
+  a.kp = key_pages, a.vp = value_pages;
+  a.kps = key_page_strides[0], a.kph = key_page_strides[1];
+  a.vps = value_page_strides[0], a.vph = value_page_strides[1];
+  a.ke = key_exponents, a.kes = key_exponent_stride;
+  a.ve = value_exponents, a.ves = value_exponent_stride;
+  if (!append_fits(a, head_dim)) return AVATTN_ERR_TOO_LARGE;
+  return launch_status(launch_append(a, head_dim, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int avattn_page_values(const void* key_pages, const int64_t* key_page_strides, const int8_t* key_exponents,
+                       int64_t key_exponent_stride, void* key_out, const void* value_pages,
+                       const int64_t* value_page_strides, const int8_t* value_exponents,
+                       int64_t value_exponent_stride, void* value_out, int32_t pages, int32_t heads,
+                       int32_t page_size, int32_t head_dim, avattn_stream_t stream) {
+  PageValuesArgs a{};
+  const int st = page_args(key_pages, key_page_strides, value_pages, value_page_strides, key_exponents,
+                           key_exponent_stride, value_exponents, value_exponent_stride, pages, page_size, heads,
+                           head_dim, a.shift);
+  if (st != AVATTN_OK) return st;
+  if (pages == 0) return AVATTN_OK;
+  if (!key_exponents || !key_out || !value_out) return AVATTN_ERR_NULL_POINTER;
+  if (!aligned16(key_out) || !aligned16(value_out)) return AVATTN_ERR_LAYOUT;
+  a.codes[0] = static_cast<const uint8_t*>(key_pages), a.codes[1] = static_cast<const uint8_t*>(value_pages);
+  a.exponent[0] = key_exponents, a.exponent[1] = value_exponents;
+  a.ps[0] = key_page_strides[0], a.hs[0] = key_page_strides[1], a.es[0] = key_exponent_stride;
+  a.ps[1] = value_page_strides[0], a.hs[1] = value_page_strides[1], a.es[1] = value_exponent_stride;
+  a.out[0] = static_cast<bf16*>(key_out), a.out[1] = static_cast<bf16*>(value_out);
+  a.pages = pages, a.H = heads, a.D = head_dim;
+  return launch_status(launch_page_values(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t avattn_paged_attention_workspace_size(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len_q,
+                                             int32_t head_dim, int32_t blocks, int32_t page_size, int32_t window,
+                                             int32_t is_e4m3) {
+  if (blocks < 0 || page_size < 1 || (int64_t)blocks * page_size > kMaxI32) return 0;
+  const int32_t cap = blocks * page_size;
+  if (check_dims(batch, heads_q, heads_kv, len_q, cap, head_dim) != AVATTN_OK) return 0;
+  if ((int64_t)batch * heads_q * len_q == 0 || cap == 0) return 0;
+  const FewPlan few = paged_plan(batch, heads_q, heads_kv, len_q, cap, window, head_dim, is_e4m3 != 0);
+  return few.nsplit > 0 ? few.bytes : paged_general_workspace(batch, heads_kv, len_q, cap, head_dim).total;
+}
+
+int avattn_paged_attention(const void* q, const int64_t* q_strides, int32_t batch, int32_t heads_q, int32_t heads_kv,
+                           int32_t len_q, int32_t head_dim, const int32_t* block_table, int64_t block_table_stride,
+                           int32_t blocks, const int32_t* lengths, const int32_t* counts, const void* key_pages,
+                           const int64_t* key_page_strides, const void* value_pages,
+                           const int64_t* value_page_strides, const int8_t* key_exponents,
+                           int64_t key_exponent_stride, const int8_t* value_exponents, int64_t value_exponent_stride,
+                           int32_t pages, int32_t page_size, int32_t window, float scale, float softcap,
+                           const float* slopes, void* out, const int64_t* out_strides, float* lse, void* workspace,
+                           size_t workspace_bytes, avattn_stream_t stream) {
+  PagedArgs p{};
+  int st = page_args(key_pages, key_page_strides, value_pages, value_page_strides, key_exponents, key_exponent_stride,
+                     value_exponents, value_exponent_stride, pages, page_size, heads_kv, head_dim, p.pages.shift);
+  if (st != AVATTN_OK) return st;
+  st = table_args(block_table, block_table_stride, blocks, lengths, counts, batch);
+  if (st != AVATTN_OK) return st;
+  if ((int64_t)blocks * page_size > kMaxI32) return AVATTN_ERR_TOO_LARGE;
+  const int32_t cap = pages > 0 ? blocks * page_size : 0;
+  st = check_dims(batch, heads_q, heads_kv, len_q, cap, head_dim);
+  if (st != AVATTN_OK) return st;
+  if (!q_strides || !out_strides) return AVATTN_ERR_NULL_POINTER;
+  if (window < 0 || !(scale > 0.f) || !isfinite(scale)) return AVATTN_ERR_ARGUMENT;
+  FewArgs& c = p.few;
+  st = score_args(scale, softcap, slopes, nullptr, 0, heads_q, heads_kv, false, c.score);
+  if (st != AVATTN_OK) return st;
+  if ((int64_t)batch * heads_q * len_q == 0) return AVATTN_OK;
+  if (!q || !out || !lse) return AVATTN_ERR_NULL_POINTER;
+  if (!aligned16(q) || !aligned16(out) || !strides_ok(q_strides) || !strides_ok(out_strides))
+    return AVATTN_ERR_LAYOUT;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (cap == 0)
+    return launch_status(launch_empty(static_cast<bf16*>(out), out_strides[0], out_strides[1], out_strides[2], batch,
+                                      heads_q, len_q, head_dim, lse, s));
+  const FewPlan plan = paged_plan(batch, heads_q, heads_kv, len_q, cap, window, head_dim, key_exponents != nullptr);
+  const PagedWorkspace wl = paged_general_workspace(batch, heads_kv, len_q, cap, head_dim);
+  const size_t need = plan.nsplit > 0 ? plan.bytes : wl.total;
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return AVATTN_ERR_WORKSPACE;
+  c.q = q, c.o = out;
+  c.qsb = q_strides[0], c.qsh = q_strides[1], c.qsl = q_strides[2];
+  c.osb = out_strides[0], c.osh = out_strides[1], c.osl = out_strides[2];
+  c.B = batch, c.Hq = heads_q, c.Hkv = heads_kv, c.Lq = len_q, c.Lk = cap;
+  c.scale_log2 = scale * kLog2e;
+  c.lse = lse;
+  p.pages.table = block_table, p.pages.tsb = block_table_stride, p.pages.blocks = blocks, p.pages.pages = pages;
+  p.lengths = lengths, p.counts = counts, p.window = window;
+  p.kp = key_pages, p.vp = value_pages;
+  p.kps = key_page_strides[0], p.kph = key_page_strides[1];
+  p.vps = value_page_strides[0], p.vph = value_page_strides[1];
+  p.ke = key_exponents, p.kes = key_exponent_stride;
+  p.ve = value_exponents, p.ves = value_exponent_stride;
+  if (plan.nsplit > 0) {
+    c.part = static_cast<float*>(workspace);
+    return launch_status(launch_paged_few(p, plan, head_dim, s));
+  }
+  FwdArgs a{};
+  a.q = static_cast<const bf16*>(q);
+  a.qsb = c.qsb, a.qsh = c.qsh, a.qsl = c.qsl;
+  a.B = batch, a.Hq = heads_q, a.Hkv = heads_kv, a.Lq = len_q, a.Lk = cap;
+  a.scale = scale;
+  a.scale_log2 = c.scale_log2;
+  a.o = static_cast<bf16*>(out);
+  a.osb = c.osb, a.osh = c.osh, a.osl = c.osl;
+  a.lse = lse;
+  char* ws = static_cast<char*>(workspace);
+  const FwdWorkspace w = fwd_workspace(batch, heads_kv, cap, head_dim);
+  a.kr = reinterpret_cast<bf16*>(ws + w.kr);
+  a.vt = reinterpret_cast<bf16*>(ws + w.vt);
+  a.kbias = reinterpret_cast<float*>(ws + w.kbias);
+  a.kfull = reinterpret_cast<int*>(ws + w.kfull);
+  a.kmax2 = reinterpret_cast<uint32_t*>(ws + w.kmax2);
+  a.Lkp = (int)transpose_padded_len(cap);
+  a.wlo = reinterpret_cast<int*>(ws + wl.windows);
+  a.whi = a.wlo + (int64_t)batch * len_q;
+  a.wsb = len_q;
+  if (2 * (int64_t)batch * heads_kv * (a.Lkp / 64) + ((int64_t)batch * len_q + 255) / 256 >= (int64_t)1 << 24)
+    return AVATTN_ERR_TOO_LARGE;  // the preparation's grid
+  // Neither cap nor bias: the plain forward with windows.
+  if (softcap > 0.f || slopes) a.score = c.score;
+  if (slopes) a.score.offsets = reinterpret_cast<int*>(ws + wl.offsets);
+  a.paged = &p;
+  return launch_status(launch_fwd(a, head_dim, s));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Gated residual step with its norms
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// Sizes, vectors and their strides, for both directions.
+int gated_args(const void* w, int32_t w32, const void* p, int32_t p32, const void* g, int64_t gs, const void* s,
+               int64_t ss, const void* t, int64_t ts, int32_t m32, int64_t rows, int64_t width, int64_t group_rows,
+               int32_t is_f32, float alpha, float eps, GatedNormArgs& a) {
+  if (rows < 0 || width < 1 || group_rows < 1) return AVATTN_ERR_BAD_SHAPE;
+  if (rows > kMaxI32 || width > kMaxI32) return AVATTN_ERR_TOO_LARGE;
+  if (rows % group_rows != 0) return AVATTN_ERR_BAD_SHAPE;
+  if (!(eps >= 0.f) || !isfinite(eps) || !isfinite(alpha)) return AVATTN_ERR_ARGUMENT;
+  if (is_f32 && ((w && !w32) || (p && !p32) || ((g || s || t) && !m32))) return AVATTN_ERR_ARGUMENT;
+  if (!aligned_to(w, w32 ? 4 : 2) || !aligned_to(p, p32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  for (const void* q : {g, s, t})
+    if (!aligned_to(q, m32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  a.w = w, a.p = p, a.g = g, a.s = s, a.t = t;
+  a.gs = g ? gs : 0, a.ss = s ? ss : 0, a.ts = t ? ts : 0;
+  a.w32 = w32 != 0, a.p32 = p32 != 0, a.m32 = m32 != 0;
+  a.rows = rows, a.W = width, a.R = group_rows;
+  a.alpha = alpha, a.eps = eps;
+  return AVATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int avattn_gated_add_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                              const void* weight, int32_t weight_is_f32, const void* post_weight,
+                              int32_t post_weight_is_f32, const void* gate, int64_t gate_stride, const void* scale,
+                              int64_t scale_stride, const void* shift, int64_t shift_stride,
+                              int32_t modulation_is_f32, int64_t rows, int64_t width, int64_t group_rows,
+                              int32_t is_f32, float residual_scale, float eps, void* sum_out, void* norm_out,
+                              avattn_stream_t stream) {
+  GatedNormArgs a{};
+  const int st = gated_args(weight, weight_is_f32, post_weight, post_weight_is_f32, gate, gate_stride, scale,
+                            scale_stride, shift, shift_stride, modulation_is_f32, rows, width, group_rows, is_f32,
+                            residual_scale, eps, a);
+  if (st != AVATTN_OK) return st;
+  if (rows == 0) return AVATTN_OK;
+  if (!x || !residual || !sum_out || !norm_out) return AVATTN_ERR_NULL_POINTER;
+  for (const void* q : {x, residual, (const void*)sum_out, (const void*)norm_out})
+    if (!aligned_to(q, is_f32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  a.x = x, a.xs = x_row_stride;
+  a.r = residual, a.rs = residual_row_stride;
+  a.h = sum_out, a.n = norm_out;
+  return launch_status(launch_gated_norm(a, is_f32 != 0, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t avattn_gated_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width, int64_t group_rows,
+                                                    int32_t modulated) {
+  if (rows < 1 || width < 1 || group_rows < 1 || rows > kMaxI32 || width > kMaxI32) return 0;
+  return gated_norm_bwd_workspace_bytes(rows, group_rows, width, modulated != 0);
+}
+
+int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, const void* dsum,
+                                  int64_t dsum_row_stride, const void* x, int64_t x_row_stride, const void* sum,
+                                  int64_t sum_row_stride, const void* weight, int32_t weight_is_f32,
+                                  const void* post_weight, int32_t post_weight_is_f32, const void* gate,
+                                  int64_t gate_stride, const void* scale, int64_t scale_stride, const void* shift,
+                                  int64_t shift_stride, int32_t modulation_is_f32, int64_t rows, int64_t width,
+                                  int64_t group_rows, int32_t is_f32, float residual_scale, float eps, void* dx,
+                                  void* dresidual, void* dweight, void* dpost_weight, void* dgate, void* dscale,
+                                  void* dshift, void* workspace, size_t workspace_bytes, avattn_stream_t stream) {
+  GatedNormArgs a{};
+  const int st = gated_args(weight, weight_is_f32, post_weight, post_weight_is_f32, gate, gate_stride, scale,
+                            scale_stride, shift, shift_stride, modulation_is_f32, rows, width, group_rows, is_f32,
+                            residual_scale, eps, a);
+  if (st != AVATTN_OK) return st;
+  if ((dweight && !weight) || (dpost_weight && !post_weight) || (dgate && !gate) || (dscale && !scale) ||
+      (dshift && !shift))
+    return AVATTN_ERR_ARGUMENT;
+  if (rows == 0) return AVATTN_ERR_BAD_SHAPE;  // its sums are zeros: the caller's to write
+  const bool whole = gate || post_weight;      // dx is not the sum's gradient
+  if (!dnorm || !sum || !dx || (whole && !x)) return AVATTN_ERR_NULL_POINTER;
+  if (!dresidual && (whole || residual_scale != 1.f)) return AVATTN_ERR_NULL_POINTER;
+  for (const void* q : {dnorm, dsum, x, sum, (const void*)dx, (const void*)dresidual})
+    if (!aligned_to(q, is_f32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  if (!aligned_to(dweight, weight_is_f32 ? 4 : 2) || !aligned_to(dpost_weight, post_weight_is_f32 ? 4 : 2))
+    return AVATTN_ERR_LAYOUT;
+  for (const void* q : {dgate, dscale, dshift})
+    if (!aligned_to(q, modulation_is_f32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  if (!workspace || !aligned16(workspace) ||
+      workspace_bytes < gated_norm_bwd_workspace_bytes(rows, group_rows, width, gate || scale || shift))
+    return AVATTN_ERR_WORKSPACE;
+  a.dn = dnorm, a.dns = dnorm_row_stride;
+  a.dh = dsum, a.dhs = dsum ? dsum_row_stride : 0;
+  a.x = whole ? x : nullptr, a.xs = whole ? x_row_stride : 0;
+  a.hin = sum, a.hs = sum_row_stride;
+  a.dx = dx, a.dr = dresidual;
+  a.dw = dweight, a.dp = dpost_weight, a.dg = dgate, a.ds = dscale, a.dt = dshift;
+  a.part = static_cast<float*>(workspace);
+  return launch_status(launch_gated_norm_bwd(a, is_f32 != 0, reinterpret_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -139,6 +139,8 @@ __device__ __forceinline__ void key_hull(const int* hull, const int* wlo, const 
   hi = min(max(hi, lo), Lk);
 }
 
+struct PagedArgs;
+
 struct FwdArgs {
   const bf16* q;
   const bf16* k;
@@ -215,6 +217,9 @@ struct FwdArgs {
   ScoreArgs score;
   int* hull;
   float* row_lse;
+  // Keys and values in pages (null: k and v): the copies are made from them, and
+  // wlo and whi (here also an output of the preparation) from the lengths.
+  const PagedArgs* paged;
 };
 
 // Floats of one part of `rows` rows: the accumulators, then per 32 rows their
@@ -422,6 +427,12 @@ enum KernelId : int {
   kKidAddNormBwd = 17,
   kKidFwdFew = 18,
   kKidWindowHull = 19,
+  kKidAppend = 20,
+  kKidPageValues = 21,
+  kKidFwdPaged = 22,
+  kKidPrepPaged = 23,
+  kKidGatedNorm = 24,
+  kKidGatedNormBwd = 25,
 };
 
 // Records HIP events around one launch on `stream` while timing is enabled.
@@ -445,6 +456,8 @@ inline int64_t transpose_padded_len(int64_t L) { return (L + 63) / 64 * 64; }
 // The forward's preparation (FwdArgs::kr, vt, kbias, kfull, kmax2; with k8
 // set everything but the K copy and kmax2).
 hipError_t launch_prep_fwd(const FwdArgs& a, int head_dim, hipStream_t stream);
+// The same from pages (a.paged; with bias a.score.offsets is written too).
+hipError_t launch_prep_paged(const FwdArgs& a, int head_dim, hipStream_t stream);
 // The backward's (BwdArgs::kt, kbias, kfull, khull, the row copies it needs
 // and, unless a.reuse_q, lse2 and ndelta; a.qt and a.dt must be set).
 hipError_t launch_prep_bwd(const BwdArgs& a, int head_dim, hipStream_t stream);
@@ -550,6 +563,90 @@ struct FewPlan {
 };
 FewPlan few_plan(int B, int Hq, int Hkv, int Lq, int Lk, int head_dim, bool f32);
 hipError_t launch_few(const FewArgs& a, const FewPlan& plan, int head_dim, bool f32, hipStream_t stream);
+// The second step of a split bf16 call: joins the parts of a.row_blocks blocks
+// of a.block_rows rows of every (batch, kv head).
+void launch_few_combine(const FewArgs& a, int head_dim, hipStream_t stream);
+
+// A cache of pages (paged_append.hip, attn_paged.hip): slot s of head h of page
+// p at p*kps + h*kph + s*head_dim (values: vps, vph), 1 << shift slots; bf16, or
+// e4m3 codes with the exponent of (p, h) at p*kes + h (values: ves).  Token t of
+// sequence b is in slot t % page of page table[b*tsb + t / page], t / page <
+// blocks; an entry outside [0, pages) names no page.
+constexpr int kMinPageShift = 4, kMaxPageShift = 8;
+// Exponents written: code * 2^e is then a normal bf16 number, or zero.
+constexpr int kMinCodeExponent = -110, kMaxCodeExponent = 119;
+struct PageTable {
+  const int* table;
+  int64_t tsb;
+  int blocks, pages, shift;
+  // The page of a sequence's block, -1 for none.
+  __device__ __forceinline__ int page(int b, int64_t block) const {
+    if (block < 0 || block >= blocks) return -1;
+    const int p = table[b * tsb + block];
+    return p >= 0 && p < pages ? p : -1;
+  }
+};
+// The rotation of rotate_kernel for rows of 16-channel items; cos null: none.
+struct AppendRotation {
+  const float* cos;
+  const float* sin;
+  int64_t tsb;
+  int pairs, start;
+  bool half;
+};
+struct AppendArgs {
+  const bf16* k;
+  const bf16* v;
+  const bf16* q;  // null: none
+  bf16* q_out;
+  int64_t ksb, ksh, ksl, vsb, vsh, vsl, qsb, qsh, qsl, osb, osh, osl;
+  int B, Hq, Hkv, L;
+  AppendRotation rot;
+  PageTable pages;
+  const int* lengths;
+  const int* counts;  // null: L
+  void* kp;
+  void* vp;
+  int64_t kps, kph, vps, vph;
+  int8_t* ke;  // null: bf16 pages
+  int8_t* ve;
+  int64_t kes, ves;
+  int nblocks;  // blocks that L tokens may touch (set by launch_append)
+};
+bool append_fits(const AppendArgs& a, int head_dim);
+hipError_t launch_append(const AppendArgs& a, int head_dim, hipStream_t stream);
+// bf16 values of all pages, (page, head, slot, channel) contiguous, of keys [0]
+// and values [1].
+struct PageValuesArgs {
+  const uint8_t* codes[2];
+  const int8_t* exponent[2];
+  int64_t ps[2], hs[2], es[2];
+  bf16* out[2];
+  int pages, H, D, shift;
+};
+hipError_t launch_page_values(const PageValuesArgs& a, hipStream_t stream);
+
+// Attention over pages (attn_paged.hip).  few: q, o, lse, their strides and
+// sizes, scale and scores (k, v, masks and windows unused); few.Lk is blocks <<
+// shift.  Query i < counts[b] (null: Lq) is at position p = lengths[b] -
+// counts[b] + i and sees keys (p - window, p] (window 0: from 0 on).
+struct PagedArgs {
+  FewArgs few;
+  PageTable pages;
+  const int* lengths;
+  const int* counts;
+  int window;
+  const void* kp;
+  const void* vp;
+  int64_t kps, kph, vps, vph;
+  const int8_t* ke;  // null: bf16 pages
+  const int8_t* ve;
+  int64_t kes, ves;
+};
+// nsplit > 0: the few-row kernel, `bytes` of parts; else the general forward on
+// bf16 copies of the pages (its workspace, then the windows).
+FewPlan paged_plan(int B, int Hq, int Hkv, int Lq, int64_t cap, int window, int head_dim, bool fp8);
+hipError_t launch_paged_few(const PagedArgs& a, const FewPlan& plan, int head_dim, hipStream_t stream);
 // The float32 kernels with changed scores (attn_f32.hip): what their C entry
 // points check, with a status code.  The forward's workspace: split parts, then
 // the hull; the backward's tensors are float behind BwdArgs' pointers.
@@ -612,6 +709,46 @@ struct AddNormArgs {
 size_t add_norm_bwd_workspace_bytes(int64_t rows, int64_t W);
 hipError_t launch_add_norm(const AddNormArgs& a, bool f32, bool fp8, hipStream_t stream);
 hipError_t launch_add_norm_bwd(const AddNormArgs& a, bool f32, void* dw, bool dw32, hipStream_t stream);
+
+// The gated residual step with its norms (gated_norm.hip, which has the
+// formulas).  Rows of x, r (forward) and hin, dn, dh (backward) their strides
+// apart; h, n, dx and dr contiguous.  w and p: (W), null for none; g, s, t: a row
+// for each group of R rows, gs, ss and ts apart (0: shared), null for none.
+// Backward: x null without g and p, dh null for none, dr null where it is dx;
+// ds, dt, dg (a contiguous row per group), dw and dp null where not wanted.
+struct GatedNormArgs {
+  const void* x;
+  const void* r;
+  int64_t xs, rs;
+  const void* w;
+  const void* p;
+  const void* g;
+  const void* s;
+  const void* t;
+  int64_t gs, ss, ts;
+  bool w32, p32, m32;  // fp32 in place of the rows' type
+  int64_t rows, W, R;
+  float alpha, eps;
+  void* h;
+  void* n;
+  const void* hin;
+  const void* dn;
+  const void* dh;
+  int64_t hs, dns, dhs;
+  void* dx;
+  void* dr;
+  void* dg;
+  void* ds;
+  void* dt;
+  void* dw;
+  void* dp;
+  float* part;
+  int64_t first;      // a launch's first worker, and workers of a group, each with
+  int64_t per_group;  // every per_group-th of its rows (set by the launchers)
+};
+size_t gated_norm_bwd_workspace_bytes(int64_t rows, int64_t R, int64_t W, bool modulated);
+hipError_t launch_gated_norm(const GatedNormArgs& a, bool f32, hipStream_t stream);
+hipError_t launch_gated_norm_bwd(const GatedNormArgs& a, bool f32, hipStream_t stream);
 
 hipError_t launch_zero_rows(bf16* x, int64_t sb, int64_t sh, int64_t sl, int B, int H, int L, int D,
                             hipStream_t stream);

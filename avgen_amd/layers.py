@@ -17,7 +17,8 @@ and produces any such layout, writes its output in it too, so the final
 kernel, forward or backward.
 
 :func:`add_rms_norm` is the step between two such sections: the residual
-addition with the norm that follows it, in one pass.
+addition with the norm that follows it, in one pass; :func:`gated_add_rms_norm`
+is the same with a gate, a norm behind the section and a modulated norm.
 """
 
 from __future__ import annotations
@@ -25,10 +26,17 @@ from __future__ import annotations
 import torch
 
 from . import attention as _attention
-from . import block_ops, ops
+from . import block_ops, gated_ops, ops
 from .rope import RotaryTables
 
-__all__ = ["add_rms_norm", "add_rms_norm_fp8", "qk_norm_rope", "self_attention_core", "split_heads"]
+__all__ = [
+    "add_rms_norm",
+    "add_rms_norm_fp8",
+    "gated_add_rms_norm",
+    "qk_norm_rope",
+    "self_attention_core",
+    "split_heads",
+]
 
 
 def split_heads(projected: torch.Tensor, head_dim: int) -> torch.Tensor:
@@ -115,3 +123,65 @@ def add_rms_norm_fp8(
     row's largest magnitude / 448 (1 for a row of zeros).  For sampling: not
     differentiable."""
     return block_ops.add_rms_norm_fp8(x, residual, weight, float(eps))
+
+
+def _one_modulation(shape, *given):
+    """gate, scale and shift with one shape: a row for each group of consecutive
+    rows of ``shape``."""
+    first = next((t for t in given if t is not None), None)
+    if first is None:
+        return given
+    lead = tuple(shape[:-1])
+    groups = 0  # leading sizes of x that some of them has a row for each of
+    for t in given:
+        if t is None:
+            continue
+        if t.ndim < 1 or t.ndim > len(shape) or t.shape[-1] != shape[-1]:
+            raise ValueError(f"gate, scale and shift must broadcast to {tuple(shape)}; got {tuple(t.shape)}")
+        skip = len(shape) - t.ndim
+        for d, n in enumerate(t.shape[:-1], skip):
+            if n != 1 and n != lead[d]:
+                raise ValueError(f"gate, scale and shift must broadcast to {tuple(shape)}; got {tuple(t.shape)}")
+            if n != 1:
+                groups = max(groups, d + 1)
+    want = lead[:groups] + (1,) * (len(lead) - groups) + (shape[-1],)
+    return tuple(t if t is None or t.shape == want or (groups == 0 and t.numel() == shape[-1] and
+                                                       t.shape == first.shape)
+                 else t.expand(want) for t in given)
+
+
+def gated_add_rms_norm(
+    x: torch.Tensor,
+    residual: torch.Tensor,
+    weight: torch.Tensor | None = None,
+    *,
+    gate: torch.Tensor | None = None,
+    scale: torch.Tensor | None = None,
+    shift: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    residual_scale: float = 1.0,
+    eps: float = 1e-6,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The step between two sections of a block in one pass: with ``h =
+    residual_scale * residual + gate * y``, ``y`` being ``x`` or with
+    ``post_weight`` ``rms_norm(x) * post_weight``, returns ``(rms_norm(h) *
+    weight * (1 + scale) + shift, h)`` (src/avgen/models/blocks.py:173-227: the
+    gated residual addition of one branch and the modulated norm of the next).
+
+    ``x`` and ``residual`` are bf16 or float32 of one shape ``(..., width)``, any
+    width.  ``weight`` and ``post_weight`` ``(width,)``, in their dtype or
+    float32; ``gate``, ``scale`` and ``shift`` broadcast to them, for instance
+    ``(width,)``, ``(batch, 1, width)`` (pieces of a modulation's projection, read
+    in place) or ``(batch, seq, width)``, all in their dtype or all float32.
+    What is None leaves its step out.  The norm is that of the unrounded fp32
+    ``h``; both results are rounded once.  Differentiable in every tensor; the
+    backward starts from the stored ``h``.
+
+    Raises:
+        ValueError: shapes that do not fit, a negative eps.
+        TypeError: other types.
+        RuntimeError: a tensor not on the GPU, or not on the same one.
+    """
+    gate, scale, shift = _one_modulation(x.shape, gate, scale, shift)
+    return gated_ops.gated_add_rms_norm(x, residual, weight, post_weight, gate, scale, shift, float(residual_scale),
+                                        float(eps))

@@ -659,7 +659,10 @@ int avattn_qk_norm_rope_bwd(const void* x, const int64_t* x_strides,
  * 13 the ring dq finish (avattn_ring_dq_finish), 14 the sum of the
  * partial results of split dK/dV workgroups, 15 avattn_diag_dq_partials,
  * 16 residual norm, 17 its backward (without the gain's reduction),
- * 18 forward of few query rows, 19 the range of unsorted key windows.
+ * 18 forward of few query rows, 19 the range of unsorted key windows,
+ * 20 append to pages, 21 values of pages, 22 few query rows over pages,
+ * 23 operand copies from pages, 24 gated residual norm, 25 its backward
+ * (without the sums' reduction).
  * avattn_timing_begin creates `capacity` event pairs (call it outside any
  * timed or captured region); launches beyond capacity are not recorded and
  * make avattn_timing_read return AVATTN_ERR_WORKSPACE.
@@ -1059,6 +1062,158 @@ int avattn_bwd_scored_row_lse(const void* dout, const void* q,
                               void* dv, const int64_t* dv_strides,
                               void* workspace, size_t workspace_bytes,
                               avattn_stream_t stream);
+
+/*
+ * A cache of keys and values in pages (no reference counterpart: the reference
+ * samples whole clips).  A pool holds `pages` pages of page_size slots (a power
+ * of two, 16 to 256) for every kv head: slot s of head h of page p is head_dim
+ * contiguous values at p * strides[0] + h * strides[1] + s * head_dim
+ * (key_page_strides, value_page_strides; elements; whole 16-byte units, as the
+ * pools' addresses).  bf16, or e4m3 codes with an int8 exponent for each page and head at
+ * p * exponent_stride + h: a value is code * 2^exponent (exponents of -126 and
+ * more; append writes -110 to 119).  Exponents NULL: bf16.
+ * Token t of sequence b is in slot t % page_size of page block_table[b *
+ * block_table_stride + t / page_size], `blocks` entries a sequence; an entry
+ * outside [0, pages) names no page.  lengths[b] counts the sequence's tokens, the
+ * call's included, of which counts[b] (NULL: len) are real: token i is at position
+ * lengths[b] - counts[b] + i.  All of these are device data (int32).
+ *
+ * avattn_append_paged: writes the bf16 keys and values of i < counts[b] to their
+ * slots, the keys rotated as by avattn_rotate (cos_tab NULL: not; a product
+ * rounded separately, a result once) and writes q rotated to q_out (heads_q 0:
+ * no q).  Every row of q is written, whatever counts says.  A token before
+ * position 0, behind the table or without a page is left out, and no other
+ * slot changes its code.  e4m3: the exponent of a page and head becomes the least e with 448 *
+ * 2^e >= the largest finite magnitude among its new tokens, but not below its
+ * present one where earlier tokens of the sequence are in the page; if that
+ * raises it, their codes become e4m3(code * 2^(old - e)).  Codes are rounded to
+ * nearest even; what is not finite becomes NaN.  No page may be written for two
+ * sequences of a call.
+ *
+ * avattn_page_values: bf16 values of all pages of an e4m3 pool, contiguous
+ * (pages, heads, page_size, head_dim).
+ *
+ * avattn_paged_attention: bf16 queries against the pages: query i < counts[b] at
+ * position p sees the keys max(0, p - window + 1) .. p (window 0: 0 .. p) that
+ * have a page, with scores changed as by avattn_fwd_scored (softcap 0, slopes
+ * NULL: not) and distances p - key.  Rows without a key, and i >= counts[b], are
+ * zeros with lse -inf.  What a key outside a sequence's rows' windows holds
+ * never counts.  workspace: avattn_paged_attention_workspace_size bytes,
+ * 16-byte aligned; it follows from blocks * page_size, not from the lengths.
+ * Errors: AVATTN_ERR_TOO_LARGE for 2^31 slots a sequence or more, or where
+ * avattn_fwd has it.
+ */
+int avattn_append_paged(const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides,
+                        const void* q, const int64_t* q_strides, int32_t heads_q,
+                        void* q_out, const int64_t* q_out_strides,
+                        int32_t batch, int32_t heads_kv, int32_t len,
+                        int32_t head_dim,
+                        const float* cos_tab, const float* sin_tab,
+                        int64_t table_batch_stride, int32_t pairs,
+                        int32_t start, int32_t half_layout,
+                        const int32_t* block_table, int64_t block_table_stride,
+                        int32_t blocks, const int32_t* lengths,
+                        const int32_t* counts,
+                        void* key_pages, const int64_t* key_page_strides,
+                        void* value_pages, const int64_t* value_page_strides,
+                        int8_t* key_exponents, int64_t key_exponent_stride,
+                        int8_t* value_exponents, int64_t value_exponent_stride,
+                        int32_t pages, int32_t page_size,
+                        avattn_stream_t stream);
+
+int avattn_page_values(const void* key_pages, const int64_t* key_page_strides,
+                       const int8_t* key_exponents, int64_t key_exponent_stride,
+                       void* key_out,
+                       const void* value_pages, const int64_t* value_page_strides,
+                       const int8_t* value_exponents,
+                       int64_t value_exponent_stride, void* value_out,
+                       int32_t pages, int32_t heads, int32_t page_size,
+                       int32_t head_dim, avattn_stream_t stream);
+
+size_t avattn_paged_attention_workspace_size(int32_t batch, int32_t heads_q,
+                                             int32_t heads_kv, int32_t len_q,
+                                             int32_t head_dim, int32_t blocks,
+                                             int32_t page_size, int32_t window,
+                                             int32_t is_e4m3);
+
+int avattn_paged_attention(const void* q, const int64_t* q_strides,
+                           int32_t batch, int32_t heads_q, int32_t heads_kv,
+                           int32_t len_q, int32_t head_dim,
+                           const int32_t* block_table,
+                           int64_t block_table_stride, int32_t blocks,
+                           const int32_t* lengths, const int32_t* counts,
+                           const void* key_pages, const int64_t* key_page_strides,
+                           const void* value_pages,
+                           const int64_t* value_page_strides,
+                           const int8_t* key_exponents,
+                           int64_t key_exponent_stride,
+                           const int8_t* value_exponents,
+                           int64_t value_exponent_stride,
+                           int32_t pages, int32_t page_size, int32_t window,
+                           float scale, float softcap, const float* slopes,
+                           void* out, const int64_t* out_strides, float* lse,
+                           void* workspace, size_t workspace_bytes,
+                           avattn_stream_t stream);
+
+/*
+ * The step between two sections of a block (src/avgen/models/blocks.py:173-227:
+ * the gated residual addition and the modulated norm behind it), over rows of
+ * `width` values:
+ *   y = x / sqrt(mean(x^2) + eps) * post_weight     (post_weight NULL: y = x)
+ *   h = residual_scale * residual + gate * y,  sum_out = h,
+ *   norm_out = h / sqrt(mean(h^2) + eps) * weight * (1 + scale) + shift
+ * in fp32 (the norm from the unrounded h), each output rounded once.  Rows bf16,
+ * or float32 with is_f32; x and residual rows their strides apart (elements),
+ * outputs contiguous and not overlapping the inputs.  weight, post_weight
+ * (width) and gate, scale, shift (a row for each of the consecutive groups of
+ * group_rows rows, which divide `rows`; their strides apart, 0: one row) in the
+ * rows' type or float32 (always float32 for float32 rows); each may be NULL.
+ *
+ * Backward: from x (may be NULL without gate and post_weight), the stored sum and
+ * the gradients of norm_out and sum_out (dsum may be NULL): dx and dresidual
+ * (contiguous, rows' type; dresidual NULL where it equals dx: no gate, no
+ * post_weight, residual_scale 1), and where not NULL dweight, dpost_weight,
+ * dgate, dscale, dshift (contiguous rows, one per group, the vectors' types),
+ * summed in a fixed order.  workspace: avattn_gated_add_rms_norm_bwd_workspace_size
+ * bytes (modulated: any of gate, scale, shift), 16-byte aligned.  Needs a row.
+ */
+int avattn_gated_add_rms_norm(const void* x, int64_t x_row_stride,
+                              const void* residual, int64_t residual_row_stride,
+                              const void* weight, int32_t weight_is_f32,
+                              const void* post_weight, int32_t post_weight_is_f32,
+                              const void* gate, int64_t gate_stride,
+                              const void* scale, int64_t scale_stride,
+                              const void* shift, int64_t shift_stride,
+                              int32_t modulation_is_f32,
+                              int64_t rows, int64_t width, int64_t group_rows,
+                              int32_t is_f32, float residual_scale, float eps,
+                              void* sum_out, void* norm_out,
+                              avattn_stream_t stream);
+
+size_t avattn_gated_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width,
+                                                    int64_t group_rows,
+                                                    int32_t modulated);
+
+int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
+                                  const void* dsum, int64_t dsum_row_stride,
+                                  const void* x, int64_t x_row_stride,
+                                  const void* sum, int64_t sum_row_stride,
+                                  const void* weight, int32_t weight_is_f32,
+                                  const void* post_weight,
+                                  int32_t post_weight_is_f32,
+                                  const void* gate, int64_t gate_stride,
+                                  const void* scale, int64_t scale_stride,
+                                  const void* shift, int64_t shift_stride,
+                                  int32_t modulation_is_f32,
+                                  int64_t rows, int64_t width,
+                                  int64_t group_rows, int32_t is_f32,
+                                  float residual_scale, float eps,
+                                  void* dx, void* dresidual, void* dweight,
+                                  void* dpost_weight, void* dgate, void* dscale,
+                                  void* dshift,
+                                  void* workspace, size_t workspace_bytes,
+                                  avattn_stream_t stream);
 
 #ifdef __cplusplus
 }
