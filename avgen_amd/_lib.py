@@ -358,12 +358,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "avattn_gated_add_rms_norm": (
         ctypes.c_int,
         [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32,
-         c_i64, c_i64, c_i64, c_i32, c_f32, c_f32, c_ptr, c_ptr, c_ptr],
+         c_i64, c_i64, c_i64, c_i32, c_f32, c_f32, c_ptr, c_ptr, c_ptr, c_ptr],
     ),
     "avattn_gated_add_rms_norm_bwd_workspace_size": (c_size, [c_i64, c_i64, c_i64, c_i32]),
     "avattn_gated_add_rms_norm_bwd": (
         ctypes.c_int,
-        [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64,
+        [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr,
          c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32,
          c_i64, c_i64, c_i64, c_i32, c_f32, c_f32,
          c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr],

@@ -51,8 +51,11 @@ class PagedCache:
 
     def __post_init__(self) -> None:
         tensors = (self.key, self.value, self.key_exponent, self.value_exponent)
-        cache_ops.check_pool("PagedCache", *tensors)
+        plan = cache_ops.check_pool("PagedCache", *tensors)
         _one_device("PagedCache", *tensors)
+        # The pool's strides, where its tensors are ordinary ones: calls then look
+        # at their other arguments only.
+        object.__setattr__(self, "_plan", plan if ops._plain_eager(*tensors) else None)
 
     @classmethod
     def empty(
@@ -142,7 +145,7 @@ def append_paged(
         rotated = None
     out = cache_ops.append_paged(key, value, query if tables is not None else None, cos, sin, int(start), half,
                                  block_table, lengths, counts, cache.key, cache.value, cache.key_exponent,
-                                 cache.value_exponent)
+                                 cache.value_exponent, cache._plan)
     return out if rotated is None else rotated
 
 
@@ -193,5 +196,5 @@ def paged_attention(
         query, cache.key, cache.value, cache.key_exponent, cache.value_exponent, block_table, lengths, counts,
         distance_slopes, 0 if window is None else int(window),
         ops.default_scale(query.shape[-1]) if scale is None else float(scale),
-        0.0 if softcap is None else float(softcap))
+        0.0 if softcap is None else float(softcap), cache._plan, rows=False)
     return out

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .block_ops import _on, _one_device, _packed_last
-from .ops import SUPPORTED_HEAD_DIMS, _direct, _ptr, _stream, _Strides3, _workspace
+from .ops import SUPPORTED_HEAD_DIMS, _direct, _plain_eager, _ptr, _stream, _Strides3, _workspace
 from .scored_ops import MAX_SLOPE_GROUP, MAX_SOFTCAP_BF16, _deliver, _laid_out, _new_like
 
 __all__ = ["MAX_WINDOW", "PAGE_SIZES", "append_paged", "page_values", "paged_attention"]
@@ -85,17 +85,25 @@ def _pool_plan(key, value, key_exponent, value_exponent):
 
 
 def check_pool(name, key, value, key_exponent, value_exponent):
-    """Refuses a pool that the kernels cannot take (but for its device); its C arguments (key, strides,
-    value, strides, exponents, stride, exponents, stride)."""
+    """Refuses a pool that the kernels cannot take (but for its device); its
+    strides."""
     try:
-        (ks, kes), (vs, ves) = _pool_plan(*(None if t is None else (t.shape, t.stride(), t.dtype)
-                                            for t in (key, value, key_exponent, value_exponent)))
+        plan = _pool_plan(*(None if t is None else (t.shape, t.stride(), t.dtype)
+                            for t in (key, value, key_exponent, value_exponent)))
     except (ValueError, TypeError) as e:
         raise type(e)(f"{name}: {e}") from None
-    kp, vp = key.data_ptr(), value.data_ptr()
-    if (kp | vp) % 16:
+    if (key.data_ptr() | value.data_ptr()) % 16:
         raise ValueError(f"{name}: pools must begin at multiples of 16 bytes")
-    return kp, ks, vp, vs, _ptr(key_exponent), kes, _ptr(value_exponent), ves
+    return plan
+
+
+def _pool_args(plan, key, value, key_exponent, value_exponent):
+    """The C arguments of a pool with these strides: (key, strides, value, strides,
+    exponents, stride, exponents, stride)."""
+    (ks, kes), (vs, ves) = plan
+    if key_exponent is None:
+        return key.data_ptr(), ks, value.data_ptr(), vs, None, 0, None, 0
+    return key.data_ptr(), ks, value.data_ptr(), vs, key_exponent.data_ptr(), kes, value_exponent.data_ptr(), ves
 
 
 def _check_tables(name, B, block_table, lengths, counts):
@@ -125,9 +133,11 @@ def _check_tables(name, B, block_table, lengths, counts):
 
 
 def _append_impl(k, v, query, cos, sin, start, half, block_table, lengths, counts, key_pages, value_pages,
-                 key_exponent, value_exponent):
+                 key_exponent, value_exponent, plan=None):
     name = "avgen_amd.append_paged"
-    pool = check_pool(name, key_pages, value_pages, key_exponent, value_exponent)
+    pool = (key_pages, value_pages, key_exponent, value_exponent)
+    if plan is None:
+        plan = check_pool(name, *pool)
     pages, heads, page, D = key_pages.shape
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError(f"{name}: key and value must be (batch, heads, length, head_dim) and agree; got "
@@ -159,8 +169,7 @@ def _append_impl(k, v, query, cos, sin, start, half, block_table, lengths, count
         cos, sin = cos.contiguous(), sin.contiguous()
         tsb = 0 if TB == 1 else L * pairs
     block_table, bts, lengths, counts = _check_tables(name, B, block_table, lengths, counts)
-    device = _one_device(name, k, v, query, cos, sin, block_table, lengths, counts, key_pages, value_pages, key_exponent,
-                         value_exponent)
+    device = _one_device(name, k, v, query, cos, sin, block_table, lengths, counts, *pool)
     k, v = _packed_last(k), _packed_last(v)
     out = written = torch.empty_like(query) if query is not None else None
     q_args = (None, None, 0, None, None)
@@ -175,7 +184,7 @@ def _append_impl(k, v, query, cos, sin, start, half, block_table, lengths, count
             k.data_ptr(), _Strides3(*k.stride()[:3]), v.data_ptr(), _Strides3(*v.stride()[:3]), *q_args,
             B, H, L, D, _ptr(cos), _ptr(sin), tsb, pairs, start, half,
             block_table.data_ptr(), bts, block_table.shape[1], lengths.data_ptr(), _ptr(counts),
-            *pool, pages, page, _stream(device))
+            *_pool_args(plan, *pool), pages, page, _stream(device))
     _lib.check(st, name)
     if written is not out:
         out.copy_(written)
@@ -206,20 +215,22 @@ def _no_gradient(name, *tensors) -> None:
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
-def _append_plain(*args):
-    out = _append_impl(*args)
-    torch.autograd.graph.increment_version([t for t in args[-4:] if t is not None])
-    return out
-
-
 def append_paged(k, v, query, cos, sin, start: int, half: bool, block_table, lengths, counts, key_pages, value_pages,
-                 key_exponent, value_exponent):
-    """Writes keys and values to their pages; the rotated query, None for none."""
-    args = (k, v, query, cos, sin, start, half, block_table, lengths, counts, key_pages, value_pages, key_exponent,
-            value_exponent)
-    tensors = args[:5] + args[7:]
-    _no_gradient("avgen_amd.append_paged", *tensors)
-    out = _direct(None, _append_op, _append_plain, args, tensors)
+                 key_exponent, value_exponent, plan=None):
+    """Writes keys and values to their pages; the rotated query, None for none.
+    ``plan``: that of the pool's :func:`check_pool`, its tensors being
+    :func:`avgen_amd.ops._plain_eager`'s."""
+    name = "avgen_amd.append_paged"
+    pool = (key_pages, value_pages, key_exponent, value_exponent)
+    args = (k, v, query, cos, sin, start, half, block_table, lengths, counts, *pool)
+    _no_gradient(name, k, v, query, cos, sin, key_pages, value_pages)
+    given = (k, v, query, cos, sin, block_table, lengths, counts)
+    if _plain_eager(*given) if plan is not None else _plain_eager(*given, *pool):
+        out = _append_impl(*args, plan)
+        # (As the op does for what it writes.)
+        torch.autograd.graph.increment_version(pool[:2] if key_exponent is None else pool)
+        return out
+    out = _append_op(*args)
     return None if query is None else out
 
 
@@ -230,12 +241,15 @@ def append_paged(k, v, query, cos, sin, start: int, half: bool, block_table, len
 
 def _values_impl(key_pages, value_pages, key_exponent, value_exponent):
     name = "avgen_amd.page_values"
-    kp, kps, vp, vps, ke, kes, ve, ves = check_pool(name, key_pages, value_pages, key_exponent, value_exponent)
+    pool = (key_pages, value_pages, key_exponent, value_exponent)
+    plan = check_pool(name, *pool)
     if key_exponent is None:
         raise ValueError(f"{name}: the pages hold bfloat16 values as they are")
     pages, heads, page, D = key_pages.shape
-    device = _one_device(name, key_pages, value_pages, key_exponent, value_exponent)
-    key, value = (torch.empty(key_pages.shape, dtype=_BF16, device=device) for _ in range(2))
+    device = _one_device(name, *pool)
+    key = torch.empty(key_pages.shape, dtype=_BF16, device=device)
+    value = torch.empty(key_pages.shape, dtype=_BF16, device=device)
+    kp, kps, vp, vps, ke, kes, ve, ves = _pool_args(plan, *pool)
     with _on(device):
         st = _lib.load().avattn_page_values(kp, kps, ke, kes, key.data_ptr(), vp, vps, ve, ves, value.data_ptr(),
                                             pages, heads, page, D, _stream(device))
@@ -272,9 +286,12 @@ def _attention_workspace_size(*sizes: int) -> int:
 
 
 def _attention_impl(q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes,
-                    window, scale, softcap):
+                    window, scale, softcap, plan=None, rows=True):
+    """``(out, lse)``; without ``rows`` the lse is scratch, and None."""
     name = "avgen_amd.paged_attention"
-    pool = check_pool(name, key_pages, value_pages, key_exponent, value_exponent)
+    pool = (key_pages, value_pages, key_exponent, value_exponent)
+    if plan is None:
+        plan = check_pool(name, *pool)
     pages, Hkv, page, D = key_pages.shape
     if q.ndim != 4 or q.shape[3] != D:
         raise ValueError(f"{name}: query must be (batch, heads, length, {D}); got {tuple(q.shape)}")
@@ -298,19 +315,26 @@ def _attention_impl(q, key_pages, value_pages, key_exponent, value_exponent, blo
             raise ValueError(f"{name}: slopes take at most {MAX_SLOPE_GROUP} query heads per key head; got {Hq // Hkv}")
         slopes = slopes.contiguous()
     block_table, bts, lengths, counts = _check_tables(name, B, block_table, lengths, counts)
-    device = _one_device(name, q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes)
+    device = _one_device(name, q, *pool, block_table, lengths, counts, slopes)
     given = q
     q, qs = _laid_out(q, False)
     o = _new_like(given, q, qs, False)
-    lse = torch.empty((B, Hq, Lq), device=device, dtype=torch.float32)
     blocks = block_table.shape[1]
-    ws = _workspace(_attention_workspace_size(B, Hq, Hkv, Lq, D, blocks, page, window, key_exponent is not None),
-                    device)
+    need = _attention_workspace_size(B, Hq, Hkv, Lq, D, blocks, page, window, key_exponent is not None)
+    lse = None
+    if rows:
+        lse = torch.empty((B, Hq, Lq), device=device, dtype=torch.float32)
+        ws = _workspace(need, device)
+        at, lse_at = ws.data_ptr(), lse.data_ptr()
+    else:
+        ws = _workspace(need + 4 * B * Hq * Lq, device)  # what is needed is whole 16 bytes
+        at = ws.data_ptr()
+        lse_at = at + need
     with _on(device):
         st = _lib.load().avattn_paged_attention(
             q.data_ptr(), qs, B, Hq, Hkv, Lq, D, block_table.data_ptr(), bts, blocks, lengths.data_ptr(), _ptr(counts),
-            *pool, pages, page, window, scale, softcap, _ptr(slopes),
-            o[1].data_ptr(), o[2], lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
+            *_pool_args(plan, *pool), pages, page, window, scale, softcap, _ptr(slopes),
+            o[1].data_ptr(), o[2], lse_at, at, max(need, 256) if rows else need, _stream(device))
     _lib.check(st, name)
     return _deliver(o)[0], lse
 
@@ -333,9 +357,12 @@ def _(q, key_pages, value_pages, key_exponent, value_exponent, block_table, leng
 
 
 def paged_attention(q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes,
-                    window: int, scale: float, softcap: float) -> tuple[torch.Tensor, torch.Tensor]:
-    """Attention of the newest tokens over pages: ``(out, lse)``."""
+                    window: int, scale: float, softcap: float, plan=None, rows: bool = True):
+    """Attention of the newest tokens over pages: ``(out, lse)``.  ``plan`` as for
+    :func:`append_paged`; without ``rows`` the lse may be None."""
     args = (q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes, window,
             scale, softcap)
-    _no_gradient("avgen_amd.paged_attention", *args[:9])
-    return _direct(None, _attention_op, _attention_impl, args, args[:9])
+    _no_gradient("avgen_amd.paged_attention", q, key_pages, value_pages, slopes)
+    if _plain_eager(q, block_table, lengths, counts, slopes, *(args[1:5] if plan is None else ())):
+        return _attention_impl(*args, plan, rows)
+    return _attention_op(*args)

@@ -1609,7 +1609,7 @@ int avattn_gated_add_rms_norm(const void* x, int64_t x_row_stride, const void* r
                               int64_t scale_stride, const void* shift, int64_t shift_stride,
                               int32_t modulation_is_f32, int64_t rows, int64_t width, int64_t group_rows,
                               int32_t is_f32, float residual_scale, float eps, void* sum_out, void* norm_out,
-                              avattn_stream_t stream) {
+                              float* stats_out, avattn_stream_t stream) {
   GatedNormArgs a{};
   const int st = gated_args(weight, weight_is_f32, post_weight, post_weight_is_f32, gate, gate_stride, scale,
                             scale_stride, shift, shift_stride, modulation_is_f32, rows, width, group_rows, is_f32,
@@ -1619,9 +1619,11 @@ int avattn_gated_add_rms_norm(const void* x, int64_t x_row_stride, const void* r
   if (!x || !residual || !sum_out || !norm_out) return AVATTN_ERR_NULL_POINTER;
   for (const void* q : {x, residual, (const void*)sum_out, (const void*)norm_out})
     if (!aligned_to(q, is_f32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  if (!aligned_to(stats_out, 8)) return AVATTN_ERR_LAYOUT;
   a.x = x, a.xs = x_row_stride;
   a.r = residual, a.rs = residual_row_stride;
   a.h = sum_out, a.n = norm_out;
+  a.stats = stats_out;
   return launch_status(launch_gated_norm(a, is_f32 != 0, reinterpret_cast<hipStream_t>(stream)));
 }
 
@@ -1632,9 +1634,9 @@ size_t avattn_gated_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width,
 }
 
 int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, const void* dsum,
-                                  int64_t dsum_row_stride, const void* x, int64_t x_row_stride, const void* sum,
-                                  int64_t sum_row_stride, const void* weight, int32_t weight_is_f32,
-                                  const void* post_weight, int32_t post_weight_is_f32, const void* gate,
+                                  int64_t dsum_row_stride, const void* x, int64_t x_row_stride, const void* residual,
+                                  int64_t residual_row_stride, const float* stats, const void* weight,
+                                  int32_t weight_is_f32, const void* post_weight, int32_t post_weight_is_f32, const void* gate,
                                   int64_t gate_stride, const void* scale, int64_t scale_stride, const void* shift,
                                   int64_t shift_stride, int32_t modulation_is_f32, int64_t rows, int64_t width,
                                   int64_t group_rows, int32_t is_f32, float residual_scale, float eps, void* dx,
@@ -1650,10 +1652,11 @@ int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, c
     return AVATTN_ERR_ARGUMENT;
   if (rows == 0) return AVATTN_ERR_BAD_SHAPE;  // its sums are zeros: the caller's to write
   const bool whole = gate || post_weight;      // dx is not the sum's gradient
-  if (!dnorm || !sum || !dx || (whole && !x)) return AVATTN_ERR_NULL_POINTER;
+  if (!dnorm || !x || !residual || !stats || !dx) return AVATTN_ERR_NULL_POINTER;
   if (!dresidual && (whole || residual_scale != 1.f)) return AVATTN_ERR_NULL_POINTER;
-  for (const void* q : {dnorm, dsum, x, sum, (const void*)dx, (const void*)dresidual})
+  for (const void* q : {dnorm, dsum, x, residual, (const void*)dx, (const void*)dresidual})
     if (!aligned_to(q, is_f32 ? 4 : 2)) return AVATTN_ERR_LAYOUT;
+  if (!aligned_to(stats, 8)) return AVATTN_ERR_LAYOUT;
   if (!aligned_to(dweight, weight_is_f32 ? 4 : 2) || !aligned_to(dpost_weight, post_weight_is_f32 ? 4 : 2))
     return AVATTN_ERR_LAYOUT;
   for (const void* q : {dgate, dscale, dshift})
@@ -1663,8 +1666,9 @@ int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, c
     return AVATTN_ERR_WORKSPACE;
   a.dn = dnorm, a.dns = dnorm_row_stride;
   a.dh = dsum, a.dhs = dsum ? dsum_row_stride : 0;
-  a.x = whole ? x : nullptr, a.xs = whole ? x_row_stride : 0;
-  a.hin = sum, a.hs = sum_row_stride;
+  a.x = x, a.xs = x_row_stride;
+  a.r = residual, a.rs = residual_row_stride;
+  a.stats = const_cast<float*>(stats);  // read
   a.dx = dx, a.dr = dresidual;
   a.dw = dweight, a.dp = dpost_weight, a.dg = dgate, a.ds = dscale, a.dt = dshift;
   a.part = static_cast<float*>(workspace);

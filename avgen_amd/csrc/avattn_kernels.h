@@ -711,11 +711,12 @@ hipError_t launch_add_norm(const AddNormArgs& a, bool f32, bool fp8, hipStream_t
 hipError_t launch_add_norm_bwd(const AddNormArgs& a, bool f32, void* dw, bool dw32, hipStream_t stream);
 
 // The gated residual step with its norms (gated_norm.hip, which has the
-// formulas).  Rows of x, r (forward) and hin, dn, dh (backward) their strides
-// apart; h, n, dx and dr contiguous.  w and p: (W), null for none; g, s, t: a row
-// for each group of R rows, gs, ss and ts apart (0: shared), null for none.
-// Backward: x null without g and p, dh null for none, dr null where it is dx;
-// ds, dt, dg (a contiguous row per group), dw and dp null where not wanted.
+// formulas).  Rows of x, r, dn and dh their strides apart; h, n, dx and dr
+// contiguous.  w and p: (W), null for none; g, s, t: a row for each group of R
+// rows, gs, ss and ts apart (0: shared), null for none.  stats: rx and rh of a
+// row, written by the forward if not null, read by the backward.
+// Backward: dh null for none, dr null where it is dx; ds, dt, dg (a contiguous
+// row per group), dw and dp null where not wanted.
 struct GatedNormArgs {
   const void* x;
   const void* r;
@@ -731,10 +732,10 @@ struct GatedNormArgs {
   float alpha, eps;
   void* h;
   void* n;
-  const void* hin;
+  float* stats;
   const void* dn;
   const void* dh;
-  int64_t hs, dns, dhs;
+  int64_t dns, dhs;
   void* dx;
   void* dr;
   void* dg;

@@ -6,15 +6,17 @@
 //   n = h * rh * w (1 + s) + t,  rh = 1 / sqrt(mean(h^2) + eps), the fp32 h
 // Without w, g, s or t: 1, 1, 0, 0.  g, s and t have a row for each group of R
 // consecutive rows (R = all of them: one row; R = 1: one per token).
-// Backward, given dn and dh (may be absent), from x and the stored h:
-//   A = w (1 + s),  d = dh + rh (dn A - h rh^2 mean(dn A h)),  dr = alpha d
+// Backward, given dn and dh (may be absent), from x and r, which give h again
+// without its rounding, and the forward's rx and rh:
+//   A = w (1 + s),  d = dh + rh (dn A - h rh^2 m),  m = mean(dn A h),  dr = alpha d
 //   b = g p,        dx = d b                            without p
-//                   dx = rx (d b - x rx^2 mean(d b x))  with it
+//                   dx = rx (d b - x rx^2 mean(d b x))  with it, where
+//   sum(d b x) = sum(b x (dh + rh dn A)) - rh^3 m sum(b x h): one pass of sums
 // and per column, over the rows of a group, the sums N = dn h rh, T = dn and
 // C = d x rx (without p: d x), from which ds = w N, dt = T, dg = p C, and over
 // the groups dw = sum (1 + s) N, dp = sum g C.
 // HBM-bound: the forward reads x and r and writes h and n, the backward reads x,
-// h, dn and dh and writes dx and dr (one tensor where they are alike).  A row
+// r, dn and dh and writes dx and dr (one tensor where they are alike).  A row
 // stays in the registers of the threads that share it (a wave, or a workgroup),
 // which keep their columns of A, b and t, and of the sums, over the rows of a
 // group that they take one after the other.  Sums are fp32, in a fixed order.
@@ -124,6 +126,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_kernel(GatedNorm
       if (col < a.W) store_chunk<T, CH>(hp + col, h[j]);
     }
     const float rh = row_rstd(row_reduce<WAVE, false>(ss, red), a);
+    if (a.stats != nullptr && t == 0) *reinterpret_cast<f32x2*>(a.stats + 2 * row) = f32x2{rx, rh};
     T* np = static_cast<T*>(a.n) + row * a.W;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -158,6 +161,7 @@ __global__ __launch_bounds__(256) void gated_norm_any_kernel(GatedNormArgs a) {
     ss = fmaf(h, h, ss);
   }
   const float rh = row_rstd(row_reduce<false, false>(ss, red), a);
+  if (a.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<f32x2*>(a.stats + 2 * row) = f32x2{rx, rh};
   for (int64_t c = threadIdx.x; c < a.W; c += 256) {
     float av, bv, tv;
     group_vectors<T, 1>(a, group, c, &av, &bv, &tv);
@@ -166,28 +170,34 @@ __global__ __launch_bounds__(256) void gated_norm_any_kernel(GatedNormArgs a) {
   }
 }
 
-// Two sums over the threads of a row.
-template <bool WAVE>
-__device__ __forceinline__ void row_sums(float& u, float& v, float (*red)[16], int waves) {
+// N sums over the threads of a row; red: a float per sum and wave.
+template <bool WAVE, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[16], int waves) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) u += __shfl_xor(u, off), v += __shfl_xor(v, off);
+  for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], off);
   if constexpr (!WAVE) {
-    if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = u, red[1][threadIdx.x >> 6] = v;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = v[k];
     __syncthreads();
-    u = red[0][0], v = red[1][0];
-    for (int i = 1; i < waves; ++i) u += red[0][i], v += red[1][i];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = red[k][0];
+      for (int i = 1; i < waves; ++i) v[k] += red[k][i];
+    }
   }
 }
 
 // Backward.  Workers take rows as in the forward; with a row of g, s and t per
 // token (TOKEN) every worker takes all rows in turn, writes that token's ds, dt
-// and dg and keeps the sums of dw and dp.  HASX: x is needed (a gate or a norm
-// behind the section); DH: a gradient of h is given.  The next row is loaded
-// before this one's sums.
-template <class T, int CH, int NV, bool WAVE, bool HASX, bool POST, bool DH, bool TOKEN>
+// and dg and keeps the sums of dw and dp.  DH: a gradient of h is given.  The
+// next row is loaded before this one's sums.
+template <class T, int CH, int NV, bool WAVE, bool POST, bool DH, bool TOKEN>
 __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(GatedNormArgs a) {
-  constexpr int RPB = WAVE ? 4 : 1;
-  __shared__ float red[2][2][2][16];
+  constexpr int RPB = WAVE ? 4 : 1, NS = POST ? 3 : 1;
+  __shared__ float red[2][NS][16];
   const int TPR = WAVE ? 64 : blockDim.x, waves = TPR / 64;
   const int t = threadIdx.x % TPR;
   const int64_t worker = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -210,16 +220,18 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
     for (int e = 0; e < CH; ++e) sn[j][e] = st[j][e] = sc[j][e] = 0.f;
   }
   struct Row {
-    RawChunk<T, CH> h[NV], g[NV], d[NV], x[NV];
+    RawChunk<T, CH> x[NV], r[NV], g[NV], d[NV];
+    f32x2 stats;
   };
   auto load = [&](int64_t row, Row& r) {
     row = row < end ? row : end - 1;
+    r.stats = *reinterpret_cast<const f32x2*>(a.stats + 2 * row);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      r.h[j] = read_chunk<T, CH>(static_cast<const T*>(a.hin) + row * a.hs + at[j]);
+      r.x[j] = read_chunk<T, CH>(static_cast<const T*>(a.x) + row * a.xs + at[j]);
+      r.r[j] = read_chunk<T, CH>(static_cast<const T*>(a.r) + row * a.rs + at[j]);
       r.g[j] = read_chunk<T, CH>(static_cast<const T*>(a.dn) + row * a.dns + at[j]);
       if constexpr (DH) r.d[j] = read_chunk<T, CH>(static_cast<const T*>(a.dh) + row * a.dhs + at[j]);
-      if constexpr (HASX) r.x[j] = read_chunk<T, CH>(static_cast<const T*>(a.x) + row * a.xs + at[j]);
     }
   };
   Row next;
@@ -232,62 +244,47 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
 #pragma unroll
       for (int j = 0; j < NV; ++j) group_vectors<T, CH>(a, row, at[j], av[j], bv[j], nullptr);
     }
+    const float rx = POST ? cur.stats[0] : 1.f, rh = cur.stats[1];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      cur.h[j] &= in[j], cur.g[j] &= in[j];
-      if constexpr (HASX) cur.x[j] &= in[j];
+      cur.x[j] &= in[j], cur.r[j] &= in[j], cur.g[j] &= in[j];
       if constexpr (DH) cur.d[j] &= in[j];
     }
-    float ssh = 0.f, dot = 0.f, ssx = 0.f;
+    auto value = [](const RawChunk<T, CH>& r, int e) { return chunk_value<T, CH>(r, e); };
+    auto sum_h = [&](int j, int e) { return fmaf(value(cur.x[j], e) * rx, bv[j][e], a.alpha * value(cur.r[j], e)); };
+    float sums[NS] = {};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < CH; ++e) {
-        const float h = chunk_value<T, CH>(cur.h[j], e);
-        ssh = fmaf(h, h, ssh);
-        dot = fmaf(chunk_value<T, CH>(cur.g[j], e) * av[j][e], h, dot);
+        const float h = sum_h(j, e), ga = value(cur.g[j], e) * av[j][e];
+        sums[0] = fmaf(ga, h, sums[0]);
         if constexpr (POST) {
-          const float x = chunk_value<T, CH>(cur.x[j], e);
-          ssx = fmaf(x, x, ssx);
+          const float bx = bv[j][e] * value(cur.x[j], e);
+          float u = rh * ga;
+          if constexpr (DH) u += value(cur.d[j], e);
+          sums[1] = fmaf(bx, u, sums[1]);
+          sums[2] = fmaf(bx, h, sums[2]);
         }
       }
-    row_sums<WAVE>(ssh, dot, red[buf][0], waves);
-    const float rh = row_rstd(ssh, a), m = dot / (float)a.W * rh * rh;
-    float d[NV][CH];
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < CH; ++e) {
-        const float h = chunk_value<T, CH>(cur.h[j], e), g = chunk_value<T, CH>(cur.g[j], e);
-        d[j][e] = rh * (g * av[j][e] - h * m);
-        if constexpr (DH) d[j][e] += chunk_value<T, CH>(cur.d[j], e);
-      }
-    float rx = 1.f, mx = 0.f;
-    if constexpr (POST) {
-      float dotx = 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < CH; ++e) dotx = fmaf(d[j][e] * bv[j][e], chunk_value<T, CH>(cur.x[j], e), dotx);
-      row_sums<WAVE>(ssx, dotx, red[buf][1], waves);
-      rx = row_rstd(ssx, a), mx = dotx / (float)a.W * rx * rx;
-    }
-    buf ^= 1;  // the next row's values go elsewhere: one barrier per sum
+    row_sums<WAVE, NS>(sums, red[buf], waves);
+    buf ^= 1;  // the next row's sums go elsewhere: one barrier a row
+    const float m = sums[0] / (float)a.W * rh * rh;
+    float mx = 0.f;
+    if constexpr (POST) mx = fmaf(-rh * m, sums[2], sums[1]) / (float)a.W * rx * rx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t col = (int64_t)(j * TPR + t) * CH;
       float dx[CH], dr[CH], tn[CH], tt[CH], tc[CH];
 #pragma unroll
       for (int e = 0; e < CH; ++e) {
-        const float h = chunk_value<T, CH>(cur.h[j], e), g = chunk_value<T, CH>(cur.g[j], e);
-        tn[e] = g * (h * rh), tt[e] = g;
-        dr[e] = a.alpha * d[j][e];
-        dx[e] = d[j][e] * bv[j][e];
-        if constexpr (HASX) {
-          const float x = chunk_value<T, CH>(cur.x[j], e);
-          tc[e] = d[j][e] * (x * rx);
-          if constexpr (POST) dx[e] = rx * (dx[e] - x * mx);
-        }
+        const float h = sum_h(j, e), g = value(cur.g[j], e), x = value(cur.x[j], e);
+        float d = rh * (g * av[j][e] - h * m);
+        if constexpr (DH) d += value(cur.d[j], e);
+        tn[e] = g * (h * rh), tt[e] = g, tc[e] = d * (x * rx);
+        dr[e] = a.alpha * d;
+        dx[e] = d * bv[j][e];
+        if constexpr (POST) dx[e] = rx * (dx[e] - x * mx);
       }
       if (col < a.W) {
         store_chunk<T, CH>(static_cast<T*>(a.dx) + row * a.W + col, dx);
@@ -303,24 +300,20 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
         for (int e = 0; e < CH; ++e) {
           sn[j][e] = fmaf(tn[e], 1.f + s[e], sn[j][e]);
           tn[e] *= w[e];
-          if constexpr (HASX) {
-            sc[j][e] = fmaf(tc[e], g[e], sc[j][e]);
-            tc[e] *= p[e];
-          }
+          sc[j][e] = fmaf(tc[e], g[e], sc[j][e]);
+          tc[e] *= p[e];
         }
         if (col < a.W) {
           if (a.ds) store_vector<T, CH>(a.ds, a.m32, row * a.W + col, tn);
           if (a.dt) store_vector<T, CH>(a.dt, a.m32, row * a.W + col, tt);
-          if constexpr (HASX) {
-            if (a.dg) store_vector<T, CH>(a.dg, a.m32, row * a.W + col, tc);
-          }
+          if (a.dg) store_vector<T, CH>(a.dg, a.m32, row * a.W + col, tc);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < CH; ++e) {
           sn[j][e] += tn[e];
           st[j][e] += tt[e];
-          if constexpr (HASX) sc[j][e] += tc[e];
+          sc[j][e] += tc[e];
         }
       }
     }
@@ -334,7 +327,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
     for (int e = 0; e < CH; ++e) {
       part[col + e] = sn[j][e];
       if (!TOKEN) part[a.W + col + e] = st[j][e];
-      if (HASX) part[2 * a.W + col + e] = sc[j][e];
+      part[2 * a.W + col + e] = sc[j][e];
     }
   }
 }
@@ -348,43 +341,38 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_any_kernel(GatedNormArgs a
   const int64_t group = TOKEN ? 0 : worker / a.per_group;
   const int64_t end = TOKEN ? a.rows : min((group + 1) * a.R, a.rows);
   float* part = a.part + worker * 3 * a.W;
-  for (int64_t c = threadIdx.x; c < 3 * a.W; c += 256) part[c] = 0.f;
-  __syncthreads();  // (a column's sums belong to one thread, its zeros may be another's)
+  for (int64_t c = threadIdx.x; c < a.W; c += 256) part[c] = part[a.W + c] = part[2 * a.W + c] = 0.f;
   for (int64_t row = TOKEN ? worker : group * a.R + worker % a.per_group; row < end; row += a.per_group) {
     const int64_t mine = TOKEN ? row : group;
-    const T* h = static_cast<const T*>(a.hin) + row * a.hs;
-    const T* g = static_cast<const T*>(a.dn) + row * a.dns;
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    const T* r = static_cast<const T*>(a.r) + row * a.rs;
+    const T* gr = static_cast<const T*>(a.dn) + row * a.dns;
     const T* dh = a.dh ? static_cast<const T*>(a.dh) + row * a.dhs : nullptr;
-    const T* x = a.x ? static_cast<const T*>(a.x) + row * a.xs : nullptr;
-    float ssh = 0.f, dot = 0.f, ssx = 0.f;
+    const float rx = a.p ? a.stats[2 * row] : 1.f, rh = a.stats[2 * row + 1];
+    float dot = 0.f, s1 = 0.f, s2 = 0.f;
     for (int64_t c = threadIdx.x; c < a.W; c += 256) {
       float av, bv;
       group_vectors<T, 1>(a, mine, c, &av, &bv, nullptr);
-      ssh = fmaf((float)h[c], (float)h[c], ssh);
-      dot = fmaf((float)g[c] * av, (float)h[c], dot);
-      if (a.p) ssx = fmaf((float)x[c], (float)x[c], ssx);
+      const float h = fmaf((float)x[c] * rx, bv, a.alpha * (float)r[c]), ga = (float)gr[c] * av;
+      const float bx = bv * (float)x[c];
+      dot = fmaf(ga, h, dot);
+      s1 = fmaf(bx, (dh ? (float)dh[c] : 0.f) + rh * ga, s1);
+      s2 = fmaf(bx, h, s2);
     }
-    ssh = row_reduce<false, false>(ssh, red);
     dot = row_reduce<false, false>(dot, red);
-    const float rh = row_rstd(ssh, a), m = dot / (float)a.W * rh * rh;
-    auto inner = [&](int64_t c, float av) { return (dh ? (float)dh[c] : 0.f) + rh * ((float)g[c] * av - (float)h[c] * m); };
-    float rx = 1.f, mx = 0.f;
+    const float m = dot / (float)a.W * rh * rh;
+    float mx = 0.f;
     if (a.p) {
-      float dotx = 0.f;
-      for (int64_t c = threadIdx.x; c < a.W; c += 256) {
-        float av, bv;
-        group_vectors<T, 1>(a, mine, c, &av, &bv, nullptr);
-        dotx = fmaf(inner(c, av) * bv, (float)x[c], dotx);
-      }
-      ssx = row_reduce<false, false>(ssx, red);
-      dotx = row_reduce<false, false>(dotx, red);
-      rx = row_rstd(ssx, a), mx = dotx / (float)a.W * rx * rx;
+      s1 = row_reduce<false, false>(s1, red);
+      s2 = row_reduce<false, false>(s2, red);
+      mx = fmaf(-rh * m, s2, s1) / (float)a.W * rx * rx;
     }
     for (int64_t c = threadIdx.x; c < a.W; c += 256) {
       float av, bv;
       group_vectors<T, 1>(a, mine, c, &av, &bv, nullptr);
-      const float d = inner(c, av), tn = (float)g[c] * ((float)h[c] * rh), xv = x ? (float)x[c] : 0.f;
-      const float tc = d * (xv * rx);
+      const float xv = (float)x[c], g = (float)gr[c], h = fmaf(xv * rx, bv, a.alpha * (float)r[c]);
+      const float d = rh * (g * av - h * m) + (dh ? (float)dh[c] : 0.f);
+      const float tn = g * (h * rh), tc = d * (xv * rx);
       float dx = d * bv;
       if (a.p) dx = rx * (dx - xv * mx);
       static_cast<T*>(a.dx)[row * a.W + c] = (T)dx;
@@ -397,13 +385,13 @@ __global__ __launch_bounds__(256) void gated_norm_bwd_any_kernel(GatedNormArgs a
         load_vector<T, 1>(a.g, a.m32, row * a.gs + c, 1.f, &gt);
         part[c] = fmaf(tn, 1.f + s, part[c]);
         part[2 * a.W + c] = fmaf(tc, gt, part[2 * a.W + c]);
-        const float ds = tn * w, dt = (float)g[c], dg = tc * p;
+        const float ds = tn * w, dg = tc * p;
         if (a.ds) store_vector<T, 1>(a.ds, a.m32, row * a.W + c, &ds);
-        if (a.dt) store_vector<T, 1>(a.dt, a.m32, row * a.W + c, &dt);
+        if (a.dt) store_vector<T, 1>(a.dt, a.m32, row * a.W + c, &g);
         if (a.dg) store_vector<T, 1>(a.dg, a.m32, row * a.W + c, &dg);
       } else {
         part[c] += tn;
-        part[a.W + c] += (float)g[c];
+        part[a.W + c] += g;
         part[2 * a.W + c] += tc;
       }
     }
@@ -508,11 +496,11 @@ __global__ __launch_bounds__(256) void gated_norm_gains_kernel(GatedNormArgs a, 
 bool chunked(const GatedNormArgs& a, int size) {
   const int64_t ch = 16 / size;
   uintptr_t p = 0;
-  for (const void* q : {a.x, a.r, a.hin, a.dn, a.dh, (const void*)a.h, (const void*)a.n, (const void*)a.dx,
+  for (const void* q : {a.x, a.r, a.dn, a.dh, (const void*)a.h, (const void*)a.n, (const void*)a.dx,
                         (const void*)a.dr, a.w, a.p, a.g, a.s, a.t})
     p |= reinterpret_cast<uintptr_t>(q);
   bool ok = p % 16 == 0 && a.W % ch == 0;
-  for (int64_t s : {a.xs, a.rs, a.hs, a.dns, a.dhs, a.gs, a.ss, a.ts}) ok = ok && s % ch == 0;
+  for (int64_t s : {a.xs, a.rs, a.dns, a.dhs, a.gs, a.ss, a.ts}) ok = ok && s % ch == 0;
   return ok;
 }
 
@@ -588,25 +576,14 @@ template <class T, int NV, bool WAVE, bool TOKEN>
 void backward_shape(const GatedNormArgs& a, int tpr, unsigned grid, hipStream_t stream) {
   constexpr int CH = 16 / (int)sizeof(T);
   const dim3 block(WAVE ? 256 : tpr);
-  auto go = [&](auto hasx, auto post, auto dh) {
-    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, decltype(hasx)::value, decltype(post)::value,
-                                              decltype(dh)::value, TOKEN>),
-                       dim3(grid), block, 0, stream, a);
-  };
-  using Y = std::true_type;
-  using N = std::false_type;
   if (a.p && a.dh)
-    go(Y(), Y(), Y());
+    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, true, true, TOKEN>), dim3(grid), block, 0, stream, a);
   else if (a.p)
-    go(Y(), Y(), N());
-  else if (a.x && a.dh)
-    go(Y(), N(), Y());
-  else if (a.x)
-    go(Y(), N(), N());
+    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, true, false, TOKEN>), dim3(grid), block, 0, stream, a);
   else if (a.dh)
-    go(N(), N(), Y());
+    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, false, true, TOKEN>), dim3(grid), block, 0, stream, a);
   else
-    go(N(), N(), N());
+    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, false, false, TOKEN>), dim3(grid), block, 0, stream, a);
 }
 
 template <class T, bool TOKEN>

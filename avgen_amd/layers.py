@@ -131,6 +131,10 @@ def _one_modulation(shape, *given):
     first = next((t for t in given if t is not None), None)
     if first is None:
         return given
+    if first.ndim == len(shape) and first.shape[-2] == 1 and first.shape[0] == shape[0] and first.ndim == 3:
+        # A row per sample, as a modulation's projection has it.
+        if first.shape[-1] == shape[-1] and all(t is None or t.shape == first.shape for t in given):
+            return given
     lead = tuple(shape[:-1])
     groups = 0  # leading sizes of x that some of them has a row for each of
     for t in given:
@@ -175,7 +179,7 @@ def gated_add_rms_norm(
     in place) or ``(batch, seq, width)``, all in their dtype or all float32.
     What is None leaves its step out.  The norm is that of the unrounded fp32
     ``h``; both results are rounded once.  Differentiable in every tensor; the
-    backward starts from the stored ``h``.
+    backward forms ``h`` again from ``x`` and ``residual``, which it keeps.
 
     Raises:
         ValueError: shapes that do not fit, a negative eps.

@@ -1163,15 +1163,17 @@ int avattn_paged_attention(const void* q, const int64_t* q_strides,
  *   y = x / sqrt(mean(x^2) + eps) * post_weight     (post_weight NULL: y = x)
  *   h = residual_scale * residual + gate * y,  sum_out = h,
  *   norm_out = h / sqrt(mean(h^2) + eps) * weight * (1 + scale) + shift
- * in fp32 (the norm from the unrounded h), each output rounded once.  Rows bf16,
- * or float32 with is_f32; x and residual rows their strides apart (elements),
- * outputs contiguous and not overlapping the inputs.  weight, post_weight
+ * in fp32 (the norm from the unrounded h), each output rounded once; stats_out
+ * (float32, may be NULL): the two factors 1 / sqrt(..) of each row, x's (1
+ * without post_weight) and h's, for the backward.  Rows bf16, or float32 with
+ * is_f32; x and residual rows their strides apart (elements), outputs contiguous
+ * and not overlapping the inputs.  weight, post_weight
  * (width) and gate, scale, shift (a row for each of the consecutive groups of
  * group_rows rows, which divide `rows`; their strides apart, 0: one row) in the
  * rows' type or float32 (always float32 for float32 rows); each may be NULL.
  *
- * Backward: from x (may be NULL without gate and post_weight), the stored sum and
- * the gradients of norm_out and sum_out (dsum may be NULL): dx and dresidual
+ * Backward: from x, residual, the stats and the gradients of norm_out and
+ * sum_out (dsum may be NULL): dx and dresidual
  * (contiguous, rows' type; dresidual NULL where it equals dx: no gate, no
  * post_weight, residual_scale 1), and where not NULL dweight, dpost_weight,
  * dgate, dscale, dshift (contiguous rows, one per group, the vectors' types),
@@ -1189,7 +1191,7 @@ int avattn_gated_add_rms_norm(const void* x, int64_t x_row_stride,
                               int64_t rows, int64_t width, int64_t group_rows,
                               int32_t is_f32, float residual_scale, float eps,
                               void* sum_out, void* norm_out,
-                              avattn_stream_t stream);
+                              float* stats_out, avattn_stream_t stream);
 
 size_t avattn_gated_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width,
                                                     int64_t group_rows,
@@ -1198,7 +1200,9 @@ size_t avattn_gated_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width,
 int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride,
                                   const void* dsum, int64_t dsum_row_stride,
                                   const void* x, int64_t x_row_stride,
-                                  const void* sum, int64_t sum_row_stride,
+                                  const void* residual,
+                                  int64_t residual_row_stride,
+                                  const float* stats,
                                   const void* weight, int32_t weight_is_f32,
                                   const void* post_weight,
                                   int32_t post_weight_is_f32,

@@ -90,26 +90,29 @@ def check_forward(st, alpha, n, h):
     close(n, want_n, half(dtype) * want_n.abs() + err_n + 1e-37, "norm")
 
 
-def check_backward(st, alpha, total, grads, with_dh=True):
-    """Against the formulas, from the stored sum."""
+def check_backward(st, alpha, grads, with_dh=True):
+    """Against the formulas, from the unrounded sum."""
     dtype = st["x"].dtype
     x, r, w, gate, scale, shift, p = doubles(st)
-    h, dn = total.detach().double(), st["dn"].double()
-    dh = st["dh"].double() if with_dh else torch.zeros_like(h)
+    dn = st["dn"].double()
+    dh = st["dh"].double() if with_dh else torch.zeros_like(r)
     one = torch.ones((), dtype=torch.float64, device="cuda")
     g, s = one if gate is None else gate, one if scale is None else 1 + scale
     wv, pv = one if w is None else w, one if p is None else p
-    W = h.shape[-1]
+    W = x.shape[-1]
     rx = torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) if p is not None else one
+    h = alpha * r + g * (x * rx * pv)
     rh = torch.rsqrt((h * h).mean(-1, keepdim=True) + EPS)
     nx, nh, t = x * rx, h * rh, dn * wv * s
     d = dh + rh * (t - nh * (t * nh).mean(-1, keepdim=True))
     b = d * g * pv
     dx = b if p is None else rx * (b - nx * (b * nx).mean(-1, keepdim=True))
     # float32 terms of d and dx: (a row's sums in at most W / 64 steps and a tree)
-    # times the sizes of the terms.
+    # times the sizes of the terms; h's is that of its two terms.
     unit = (W / 64 + 32) * UNIT
-    size_d = dh.abs() + rh * (t.abs() + nh.abs() * (t * nh).abs().mean(-1, keepdim=True))
+    size_h = (alpha * r).abs() + (g * nx * pv).abs()
+    size_n = size_h * rh
+    size_d = dh.abs() + rh * (t.abs() + size_n * (t.abs() * size_n).mean(-1, keepdim=True))
     size_b = size_d * (g * pv).abs()
     size_x = size_b if p is None else rx * (size_b + nx.abs() * (size_b * nx.abs()).mean(-1, keepdim=True) * 2)
     want = {"x": (dx, unit * size_x), "r": (alpha * d, unit * size_d * abs(alpha))}
@@ -119,11 +122,11 @@ def check_backward(st, alpha, total, grads, with_dh=True):
         return terms.sum_to_size(like.shape), (sizes * (unit + (n + 8) * UNIT)).sum_to_size(like.shape)
 
     if w is not None:
-        want["w"] = total_of(dn * s * nh, (dn * s * nh).abs(), w)
+        want["w"] = total_of(dn * s * nh, (dn * s).abs() * size_n, w)
     if gate is not None:
         want["gate"] = total_of(d * nx * pv, size_d * (nx * pv).abs(), gate)
     if scale is not None:
-        want["scale"] = total_of(dn * nh * wv, (dn * nh * wv).abs(), scale)
+        want["scale"] = total_of(dn * nh * wv, (dn * wv).abs() * size_n, scale)
     if shift is not None:
         want["shift"] = total_of(dn, dn.abs(), shift)
     if p is not None:
@@ -143,7 +146,7 @@ def check(lead, W, dtype, modulation, post, gain, alpha=1.0, seed=0, vectors=Non
     leaves = {n: st[n].detach().requires_grad_(True) for n in NAMES if st[n] is not None}
     n, h = call({**st, **leaves}, alpha)
     grads = torch.autograd.grad((n, h), list(leaves.values()), (st["dn"], st["dh"]))
-    check_backward(st, alpha, h, dict(zip(leaves, grads)))
+    check_backward(st, alpha, dict(zip(leaves, grads)))
     return st
 
 
@@ -210,7 +213,7 @@ def test_modulations_of_different_shapes():
     exact = torch.autograd.grad((pn, ph), want, (st["dn"].double(), st["dh"].double()))
     for name, e in zip(leaves, exact):
         rel = float((grads[name].double() - e).norm() / e.norm())
-        # stored sum (bf16), output and partial roundings: four half steps
+        # output and partial roundings: four half steps
         assert rel <= 4 * half(B16), (name, rel)
     assert st32["gate"] is not None
 
@@ -223,12 +226,12 @@ def test_one_output_used(which, post):
     n, h = call({**st, **leaves}, 0.5)
     if which == "norm":
         grads = torch.autograd.grad(n, list(leaves.values()), st["dn"])
-        check_backward(st, 0.5, h, dict(zip(leaves, grads)), with_dh=False)
+        check_backward(st, 0.5, dict(zip(leaves, grads)), with_dh=False)
     else:
         names = [k for k in leaves if k in ("x", "r", "gate", "p")]
         grads = torch.autograd.grad(h, [leaves[k] for k in names], st["dh"])
         st["dn"] = torch.zeros_like(st["dn"])
-        check_backward(st, 0.5, h, dict(zip(names, grads)))
+        check_backward(st, 0.5, dict(zip(names, grads)))
 
 
 @pytest.mark.parametrize("modulation", ["none", "batch", "token"])

@@ -18,6 +18,8 @@ B16, F8, I32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32
 class OffGpu:
     """What a PagedCache holds, on the CPU (which a PagedCache refuses)."""
 
+    _plan = None
+
     def __init__(self, dtype=B16, pages=6, heads=2, page=16, dim=64):
         self.key, self.value = (torch.zeros(pages, heads, page, dim).to(dtype) for _ in range(2))
         coded = dtype is F8
@@ -129,7 +131,7 @@ def test_paged_refusals(call, error):
         call()
 
 
-X, W = torch.zeros(2, 3, 32), torch.zeros(32)
+X, W, S = torch.zeros(2, 3, 32), torch.zeros(32), torch.zeros(6, 2)
 
 
 def gated(x=X, r=X, w=W, **more):
@@ -158,8 +160,10 @@ def gated(x=X, r=X, w=W, **more):
     (lambda: gated_ops.gated_add_rms_norm(X, X, W, None, torch.zeros(4, 32), None, None, 1.0, 1e-6), ValueError),
     (lambda: gated_ops.gated_add_rms_norm(X, X, W, None, torch.zeros(2, 32), torch.zeros(3, 32), None, 1.0, 1e-6),
      ValueError),
-    (lambda: gated_ops.gated_add_rms_norm_bwd(X, None, None, X, W, None, W, None, None, 1.0, 1e-6), ValueError),
-    (lambda: gated_ops.gated_add_rms_norm_bwd(X[:1], None, X, X, W, None, W, None, None, 1.0, 1e-6), ValueError),
+    (lambda: gated_ops.gated_add_rms_norm_bwd(X[:1], None, X, X, S, W, None, W, None, None, 1.0, 1e-6), ValueError),
+    (lambda: gated_ops.gated_add_rms_norm_bwd(X, None, X, X[:1], S, W, None, W, None, None, 1.0, 1e-6), ValueError),
+    (lambda: gated_ops.gated_add_rms_norm_bwd(X, X.bfloat16(), X, X, S, W, None, W, None, None, 1.0, 1e-6), ValueError),
+    (lambda: gated_ops.gated_add_rms_norm_bwd(X, None, X, X, S[:5], W, None, W, None, None, 1.0, 1e-6), ValueError),
 ])
 def test_gated_refusals(call, error):
     with pytest.raises(error):
@@ -255,14 +259,14 @@ def test_attention_status(changed, status):
 
 def norm_args(**c):
     a = dict(x=P, xs=32, r=P, rs=32, w=P, w32=0, p=P, p32=0, g=P, gs=96, s=P, ss=96, t=P, ts=96, m32=0, rows=6, W=32,
-             R=3, f32=0, alpha=1.0, eps=1e-6, h=P, n=P, stream=None)
+             R=3, f32=0, alpha=1.0, eps=1e-6, h=P, n=P, stats=P, stream=None)
     assert set(c) <= set(a)
     a.update(c)
     return list(a.values())
 
 
 def norm_bwd_args(**c):
-    a = dict(dn=P, dns=32, dh=P, dhs=32, x=P, xs=32, h=P, hs=32, w=P, w32=0, p=P, p32=0, g=P, gs=96, s=P, ss=96, t=P,
+    a = dict(dn=P, dns=32, dh=P, dhs=32, x=P, xs=32, r=P, rs=32, stats=P, w=P, w32=0, p=P, p32=0, g=P, gs=96, s=P, ss=96, t=P,
              ts=96, m32=0, rows=6, W=32, R=3, f32=0, alpha=1.0, eps=1e-6, dx=P, dr=P, dw=P, dp=P, dg=P, ds=P, dt=P,
              ws=P, wsb=1 << 20, stream=None)
     assert set(c) <= set(a)
@@ -282,6 +286,7 @@ SHARED = [
 @cpu_only
 @pytest.mark.parametrize("changed, status", SHARED + [
     (dict(x=None), _lib.ERR_NULL_POINTER), (dict(n=None), _lib.ERR_NULL_POINTER), (dict(h=P + 1), _lib.ERR_LAYOUT),
+    (dict(stats=P + 4), _lib.ERR_LAYOUT),
     (dict(rows=0), _lib.OK),
 ])
 def test_norm_status(changed, status):
@@ -290,7 +295,8 @@ def test_norm_status(changed, status):
 
 @cpu_only
 @pytest.mark.parametrize("changed, status", SHARED + [
-    (dict(rows=0), _lib.ERR_BAD_SHAPE), (dict(x=None), _lib.ERR_NULL_POINTER), (dict(dr=None), _lib.ERR_NULL_POINTER),
+    (dict(rows=0), _lib.ERR_BAD_SHAPE), (dict(x=None), _lib.ERR_NULL_POINTER), (dict(stats=None), _lib.ERR_NULL_POINTER),
+    (dict(r=None), _lib.ERR_NULL_POINTER), (dict(stats=P + 4), _lib.ERR_LAYOUT), (dict(dr=None), _lib.ERR_NULL_POINTER),
     (dict(dx=None), _lib.ERR_NULL_POINTER), (dict(w=None), _lib.ERR_ARGUMENT), (dict(g=None), _lib.ERR_ARGUMENT),
     (dict(ws=None), _lib.ERR_WORKSPACE), (dict(wsb=100), _lib.ERR_WORKSPACE), (dict(ws=P + 4), _lib.ERR_WORKSPACE),
     (dict(dg=P + 1), _lib.ERR_LAYOUT), (dict(dw=P + 1), _lib.ERR_LAYOUT), (dict(dh=P + 1), _lib.ERR_LAYOUT),
