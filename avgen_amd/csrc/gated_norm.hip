@@ -26,25 +26,41 @@ namespace avattn {
 
 namespace {
 
-// A per-column vector of the rows' type or fp32 (null: `otherwise`).
+// A per-column vector of the rows' type or fp32 (null: `otherwise`), CH columns
+// from `at` on; CH > 1: whole 16-byte chunks.
 template <class T, int CH>
 __device__ __forceinline__ void load_vector(const void* p, bool f32, int64_t at, float otherwise, float* v) {
-  if (p != nullptr) {
-    load_gain<T, CH>(p, f32, at, v);
-  } else {
+  if (p == nullptr) {
 #pragma unroll
     for (int e = 0; e < CH; ++e) v[e] = otherwise;
+  } else if (sizeof(T) == 2 && !f32) {
+    load_chunk<T, CH>(static_cast<const T*>(p) + at, v);
+  } else {
+    constexpr int C4 = CH > 1 ? 4 : 1;
+#pragma unroll
+    for (int e = 0; e < CH; e += C4) load_chunk<float, C4>(static_cast<const float*>(p) + at + e, v + e);
   }
 }
 template <class T, int CH>
 __device__ __forceinline__ void store_vector(void* p, bool f32, int64_t at, const float* v) {
+  if (sizeof(T) == 2 && !f32) {
+    store_chunk<T, CH>(static_cast<T*>(p) + at, v);
+  } else {
+    constexpr int C4 = CH > 1 ? 4 : 1;
 #pragma unroll
-  for (int e = 0; e < CH; ++e) {
-    if (f32)
-      static_cast<float*>(p)[at + e] = v[e];
-    else
-      static_cast<T*>(p)[at + e] = (T)v[e];
+    for (int e = 0; e < CH; e += C4) store_chunk<float, C4>(static_cast<float*>(p) + at + e, v + e);
   }
+}
+
+// A row's chunk at a byte offset, from the row's (uniform) address.
+template <class T, int CH>
+__device__ __forceinline__ RawChunk<T, CH> read_at(const void* base, int64_t row, int64_t stride, uint32_t off) {
+  return *reinterpret_cast<const RawChunk<T, CH>*>(static_cast<const char*>(base) + row * stride * (int64_t)sizeof(T) +
+                                                   off);
+}
+template <class T, int CH>
+__device__ __forceinline__ void write_at(void* base, int64_t row, int64_t stride, uint32_t off, const float* v) {
+  store_chunk<T, CH>(reinterpret_cast<T*>(static_cast<char*>(base) + row * stride * (int64_t)sizeof(T) + off), v);
 }
 
 // What a thread knows of its columns for the rows of a group: a = w (1 + s),
@@ -68,72 +84,94 @@ __device__ __forceinline__ float row_rstd(float ss, const GatedNormArgs& a) {
   return 1.f / __builtin_sqrtf(ss / (float)a.W + a.eps);
 }
 
+// Threads of a workgroup up to which a kernel is compiled, and its waves per SIMD.
+template <int SIZE>
+struct Threads;  // 0: four waves, a row each; 1, 2, 3: a row per workgroup
+template <>
+struct Threads<0> {
+  static constexpr int most = 256, fwd = 5, bwd = 3;
+};
+template <>
+struct Threads<1> {
+  static constexpr int most = 512, fwd = 5, bwd = 4;
+};
+template <>
+struct Threads<2> {
+  static constexpr int most = 768, fwd = 5, bwd = 3;
+};
+template <>
+struct Threads<3> {
+  static constexpr int most = 1024, fwd = 4, bwd = 4;
+};
+
 // Forward.  A worker, a wave (narrow rows, 4 per workgroup) or a workgroup, takes
-// every per_group-th row of a group.
-template <class T, int CH, int NV, bool WAVE, bool POST>
-__global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_kernel(GatedNormArgs a) {
+// every per_group-th row of a group, the next row loaded before this one's sums.
+template <class T, int CH, int NV, int SIZE, bool POST>
+__global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::fwd) void gated_norm_kernel(GatedNormArgs a) {
+  constexpr bool WAVE = SIZE == 0;
   constexpr int RPB = WAVE ? 4 : 1;
   __shared__ float red[16];
   const int TPR = WAVE ? 64 : blockDim.x;
   const int t = threadIdx.x % TPR;
-  const int64_t worker = a.first + (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int64_t worker = a.first + (int64_t)blockIdx.x * RPB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const int64_t group = worker / a.per_group, end = min((group + 1) * a.R, a.rows);
   int64_t row = group * a.R + worker % a.per_group;
   if (row >= end) return;  // whole waves or nobody
   float av[NV][CH], bv[NV][CH], tv[NV][CH];
+  uint32_t off[NV];  // this thread's columns, 0 past the end of the row,
+  uint32_t in[NV];   // where what is loaded is masked out
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int64_t col = (int64_t)(j * TPR + t) * CH;
-    if (col < a.W) {
-      group_vectors<T, CH>(a, group, col, av[j], bv[j], tv[j]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < CH; ++e) av[j][e] = bv[j][e] = tv[j][e] = 0.f;
-    }
+    const int64_t col = (int64_t)(j * TPR + t) * CH, at = col < a.W ? col : 0;
+    in[j] = col < a.W ? 0xffffffffu : 0u;
+    off[j] = (uint32_t)at * sizeof(T);
+    group_vectors<T, CH>(a, group, at, av[j], bv[j], tv[j]);
   }
-  for (; row < end; row += a.per_group) {
-    float h[NV][CH], x[NV][CH];
+  struct Row {
+    RawChunk<T, CH> x[NV], r[NV];
+  };
+  auto load = [&](int64_t row, Row& q) {
+    row = row < end ? row : end - 1;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t col = (int64_t)(j * TPR + t) * CH;
-      if (col < a.W) {
-        load_chunk<T, CH>(static_cast<const T*>(a.x) + row * a.xs + col, x[j]);
-        load_chunk<T, CH>(static_cast<const T*>(a.r) + row * a.rs + col, h[j]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < CH; ++e) x[j][e] = h[j][e] = 0.f;
-      }
+      q.x[j] = read_at<T, CH>(a.x, row, a.xs, off[j]);
+      q.r[j] = read_at<T, CH>(a.r, row, a.rs, off[j]);
     }
+  };
+  Row next;
+  load(row, next);
+  for (; row < end; row += a.per_group) {
+    Row cur = next;
+    load(row + a.per_group, next);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) cur.x[j] &= in[j], cur.r[j] &= in[j];
     float rx = 1.f;
     if constexpr (POST) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int e = 0; e < CH; ++e) ss = fmaf(x[j][e], x[j][e], ss);
+        for (int e = 0; e < CH; ++e) ss = fmaf(chunk_value<T, CH>(cur.x[j], e), chunk_value<T, CH>(cur.x[j], e), ss);
       rx = row_rstd(row_reduce<WAVE, false>(ss, red), a);
     }
     float ss = 0.f;
-    T* hp = static_cast<T*>(a.h) + row * a.W;
+    float h[NV][CH];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t col = (int64_t)(j * TPR + t) * CH;
 #pragma unroll
       for (int e = 0; e < CH; ++e) {
-        h[j][e] = fmaf(x[j][e] * rx, bv[j][e], a.alpha * h[j][e]);
+        h[j][e] = fmaf(chunk_value<T, CH>(cur.x[j], e) * rx, bv[j][e], a.alpha * chunk_value<T, CH>(cur.r[j], e));
         ss = fmaf(h[j][e], h[j][e], ss);
       }
-      if (col < a.W) store_chunk<T, CH>(hp + col, h[j]);
+      if (in[j]) write_at<T, CH>(a.h, row, a.W, off[j], h[j]);
     }
     const float rh = row_rstd(row_reduce<WAVE, false>(ss, red), a);
     if (a.stats != nullptr && t == 0) *reinterpret_cast<f32x2*>(a.stats + 2 * row) = f32x2{rx, rh};
-    T* np = static_cast<T*>(a.n) + row * a.W;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t col = (int64_t)(j * TPR + t) * CH;
 #pragma unroll
       for (int e = 0; e < CH; ++e) h[j][e] = fmaf(h[j][e] * rh, av[j][e], tv[j][e]);
-      if (col < a.W) store_chunk<T, CH>(np + col, h[j]);
+      if (in[j]) write_at<T, CH>(a.n, row, a.W, off[j], h[j]);
     }
   }
 }
@@ -194,13 +232,14 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[16], int wa
 // token (TOKEN) every worker takes all rows in turn, writes that token's ds, dt
 // and dg and keeps the sums of dw and dp.  DH: a gradient of h is given.  The
 // next row is loaded before this one's sums.
-template <class T, int CH, int NV, bool WAVE, bool POST, bool DH, bool TOKEN>
-__global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(GatedNormArgs a) {
+template <class T, int CH, int NV, int SIZE, bool POST, bool DH, bool TOKEN>
+__global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated_norm_bwd_kernel(GatedNormArgs a) {
+  constexpr bool WAVE = SIZE == 0;
   constexpr int RPB = WAVE ? 4 : 1, NS = POST ? 3 : 1;
   __shared__ float red[2][NS][16];
   const int TPR = WAVE ? 64 : blockDim.x, waves = TPR / 64;
   const int t = threadIdx.x % TPR;
-  const int64_t worker = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int64_t worker = (int64_t)blockIdx.x * RPB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const int64_t group = TOKEN ? 0 : worker / a.per_group;
   const int64_t end = TOKEN ? a.rows : min((group + 1) * a.R, a.rows);
   const int64_t step = a.per_group;
@@ -208,30 +247,28 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
   if (!TOKEN && group * a.R >= a.rows) return;  // whole waves or nobody
   float av[NV][CH], bv[NV][CH];
   float sn[NV][CH], st[NV][CH], sc[NV][CH];
-  int64_t at[NV];   // this thread's columns, 0 past the end of the row,
-  uint32_t in[NV];  // where what is loaded is masked out
+  uint32_t off[NV];  // this thread's columns, 0 past the end of the row,
+  uint32_t in[NV];   // where what is loaded is masked out
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int64_t col = (int64_t)(j * TPR + t) * CH;
-    at[j] = col < a.W ? col : 0;
+    const int64_t col = (int64_t)(j * TPR + t) * CH, at = col < a.W ? col : 0;
     in[j] = col < a.W ? 0xffffffffu : 0u;
-    if constexpr (!TOKEN) group_vectors<T, CH>(a, group, at[j], av[j], bv[j], nullptr);
+    off[j] = (uint32_t)at * sizeof(T);
+    if constexpr (!TOKEN) group_vectors<T, CH>(a, group, at, av[j], bv[j], nullptr);
 #pragma unroll
     for (int e = 0; e < CH; ++e) sn[j][e] = st[j][e] = sc[j][e] = 0.f;
   }
   struct Row {
     RawChunk<T, CH> x[NV], r[NV], g[NV], d[NV];
-    f32x2 stats;
   };
-  auto load = [&](int64_t row, Row& r) {
+  auto load = [&](int64_t row, Row& q) {
     row = row < end ? row : end - 1;
-    r.stats = *reinterpret_cast<const f32x2*>(a.stats + 2 * row);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      r.x[j] = read_chunk<T, CH>(static_cast<const T*>(a.x) + row * a.xs + at[j]);
-      r.r[j] = read_chunk<T, CH>(static_cast<const T*>(a.r) + row * a.rs + at[j]);
-      r.g[j] = read_chunk<T, CH>(static_cast<const T*>(a.dn) + row * a.dns + at[j]);
-      if constexpr (DH) r.d[j] = read_chunk<T, CH>(static_cast<const T*>(a.dh) + row * a.dhs + at[j]);
+      q.x[j] = read_at<T, CH>(a.x, row, a.xs, off[j]);
+      q.r[j] = read_at<T, CH>(a.r, row, a.rs, off[j]);
+      q.g[j] = read_at<T, CH>(a.dn, row, a.dns, off[j]);
+      if constexpr (DH) q.d[j] = read_at<T, CH>(a.dh, row, a.dhs, off[j]);
     }
   };
   Row next;
@@ -242,9 +279,10 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
     load(row + step, next);
     if constexpr (TOKEN) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) group_vectors<T, CH>(a, row, at[j], av[j], bv[j], nullptr);
+      for (int j = 0; j < NV; ++j) group_vectors<T, CH>(a, row, off[j] / sizeof(T), av[j], bv[j], nullptr);
     }
-    const float rx = POST ? cur.stats[0] : 1.f, rh = cur.stats[1];
+    const f32x2 stats = *reinterpret_cast<const f32x2*>(a.stats + 2 * row);
+    const float rx = POST ? stats[0] : 1.f, rh = stats[1];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur.x[j] &= in[j], cur.r[j] &= in[j], cur.g[j] &= in[j];
@@ -274,45 +312,60 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
     if constexpr (POST) mx = fmaf(-rh * m, sums[2], sums[1]) / (float)a.W * rx * rx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t col = (int64_t)(j * TPR + t) * CH;
-      float dx[CH], dr[CH], tn[CH], tt[CH], tc[CH];
+      float d[CH], out[CH];
 #pragma unroll
       for (int e = 0; e < CH; ++e) {
-        const float h = sum_h(j, e), g = value(cur.g[j], e), x = value(cur.x[j], e);
-        float d = rh * (g * av[j][e] - h * m);
-        if constexpr (DH) d += value(cur.d[j], e);
-        tn[e] = g * (h * rh), tt[e] = g, tc[e] = d * (x * rx);
-        dr[e] = a.alpha * d;
-        dx[e] = d * bv[j][e];
-        if constexpr (POST) dx[e] = rx * (dx[e] - x * mx);
+        const float h = sum_h(j, e), g = value(cur.g[j], e);
+        d[e] = rh * (g * av[j][e] - h * m);
+        if constexpr (DH) d[e] += value(cur.d[j], e);
+        out[e] = d[e] * bv[j][e];
+        if constexpr (POST) out[e] = rx * (out[e] - value(cur.x[j], e) * mx);
       }
-      if (col < a.W) {
-        store_chunk<T, CH>(static_cast<T*>(a.dx) + row * a.W + col, dx);
-        if (a.dr != nullptr) store_chunk<T, CH>(static_cast<T*>(a.dr) + row * a.W + col, dr);
+      if (in[j]) write_at<T, CH>(a.dx, row, a.W, off[j], out);
+      if (a.dr != nullptr) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) out[e] = a.alpha * d[e];
+        if (in[j]) write_at<T, CH>(a.dr, row, a.W, off[j], out);
+      }
+      float tn[CH], tc[CH];
+#pragma unroll
+      for (int e = 0; e < CH; ++e) {
+        tn[e] = value(cur.g[j], e) * (sum_h(j, e) * rh);
+        tc[e] = d[e] * (value(cur.x[j], e) * rx);
       }
       if constexpr (TOKEN) {
-        float w[CH], s[CH], p[CH], g[CH];
-        load_vector<T, CH>(a.w, a.w32, at[j], 1.f, w);
-        load_vector<T, CH>(a.s, a.m32, row * a.ss + at[j], 0.f, s);
-        load_vector<T, CH>(a.p, a.p32, at[j], 1.f, p);
-        load_vector<T, CH>(a.g, a.m32, row * a.gs + at[j], 1.f, g);
+        const int64_t at = off[j] / sizeof(T);
+        float v[CH];
+        load_vector<T, CH>(a.s, a.m32, row * a.ss + at, 0.f, v);
 #pragma unroll
-        for (int e = 0; e < CH; ++e) {
-          sn[j][e] = fmaf(tn[e], 1.f + s[e], sn[j][e]);
-          tn[e] *= w[e];
-          sc[j][e] = fmaf(tc[e], g[e], sc[j][e]);
-          tc[e] *= p[e];
-        }
-        if (col < a.W) {
-          if (a.ds) store_vector<T, CH>(a.ds, a.m32, row * a.W + col, tn);
-          if (a.dt) store_vector<T, CH>(a.dt, a.m32, row * a.W + col, tt);
-          if (a.dg) store_vector<T, CH>(a.dg, a.m32, row * a.W + col, tc);
+        for (int e = 0; e < CH; ++e) sn[j][e] = fmaf(tn[e], 1.f + v[e], sn[j][e]);
+        load_vector<T, CH>(a.g, a.m32, row * a.gs + at, 1.f, v);
+#pragma unroll
+        for (int e = 0; e < CH; ++e) sc[j][e] = fmaf(tc[e], v[e], sc[j][e]);
+        if (in[j]) {
+          if (a.ds) {
+            load_vector<T, CH>(a.w, a.w32, at, 1.f, v);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) tn[e] *= v[e];
+            store_vector<T, CH>(a.ds, a.m32, row * a.W + at, tn);
+          }
+          if (a.dt) {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) v[e] = value(cur.g[j], e);
+            store_vector<T, CH>(a.dt, a.m32, row * a.W + at, v);
+          }
+          if (a.dg) {
+            load_vector<T, CH>(a.p, a.p32, at, 1.f, v);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) tc[e] *= v[e];
+            store_vector<T, CH>(a.dg, a.m32, row * a.W + at, tc);
+          }
         }
       } else {
 #pragma unroll
         for (int e = 0; e < CH; ++e) {
           sn[j][e] += tn[e];
-          st[j][e] += tt[e];
+          st[j][e] += value(cur.g[j], e);
           sc[j][e] += tc[e];
         }
       }
@@ -321,14 +374,11 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void gated_norm_bwd_kernel(Gated
   float* part = a.part + worker * 3 * a.W;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int64_t col = (int64_t)(j * TPR + t) * CH;
-    if (col >= a.W) continue;
-#pragma unroll
-    for (int e = 0; e < CH; ++e) {
-      part[col + e] = sn[j][e];
-      if (!TOKEN) part[a.W + col + e] = st[j][e];
-      part[2 * a.W + col + e] = sc[j][e];
-    }
+    if (!in[j]) continue;
+    const int64_t col = off[j] / sizeof(T);
+    store_vector<float, CH>(part, true, col, sn[j]);
+    if (!TOKEN) store_vector<float, CH>(part, true, a.W + col, st[j]);
+    store_vector<float, CH>(part, true, 2 * a.W + col, sc[j]);
   }
 }
 
@@ -504,25 +554,35 @@ bool chunked(const GatedNormArgs& a, int size) {
   return ok;
 }
 
-// Threads per row and chunks per thread (nv 0: value by value).
+// Threads per row and chunks per thread (nv 0: value by value), and the Threads
+// to compile for.
 struct RowShape {
-  int tpr, nv;
+  int tpr, nv, size;
 };
 RowShape row_shape(int64_t chunks, int ch) {
-  if (chunks <= 64) return {64, 1};
+  if (chunks <= 64) return {64, 1, 0};
   const int nv = chunks <= 1024 ? 1 : (chunks <= 2048 ? 2 : 4);
-  if (chunks > 1024 * nv || nv * ch > 16) return {0, 0};
-  return {(int)((chunks + 64 * nv - 1) / (64 * nv)) * 64, nv};
+  if (chunks > 1024 * nv || nv * ch > 16) return {0, 0, 0};
+  const int tpr = (int)((chunks + 64 * nv - 1) / (64 * nv)) * 64;
+  return {tpr, nv, tpr <= 512 ? 1 : (tpr <= 768 ? 2 : 3)};
 }
 
-template <class T, int NV, bool WAVE>
-void forward_shape(const GatedNormArgs& a, int tpr, unsigned grid, hipStream_t stream) {
-  constexpr int CH = 16 / (int)sizeof(T);
-  const dim3 block(WAVE ? 256 : tpr);
-  if (a.p)
-    hipLaunchKernelGGL((gated_norm_kernel<T, CH, NV, WAVE, true>), dim3(grid), block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((gated_norm_kernel<T, CH, NV, WAVE, false>), dim3(grid), block, 0, stream, a);
+// f(chunks per thread, size) as compile-time constants.
+template <class T, class F>
+void with_shape(const RowShape& s, F&& f) {
+  using std::integral_constant;
+  if (s.size == 0)
+    f(integral_constant<int, 1>(), integral_constant<int, 0>());
+  else if (s.nv == 1 && s.size == 1)
+    f(integral_constant<int, 1>(), integral_constant<int, 1>());
+  else if (s.nv == 1 && s.size == 2)
+    f(integral_constant<int, 1>(), integral_constant<int, 2>());
+  else if (s.nv == 1)
+    f(integral_constant<int, 1>(), integral_constant<int, 3>());
+  else if (s.nv == 2)
+    f(integral_constant<int, 2>(), integral_constant<int, 3>());
+  else if constexpr (sizeof(T) == 4)
+    f(integral_constant<int, 4>(), integral_constant<int, 3>());
 }
 
 template <class T>
@@ -530,11 +590,11 @@ hipError_t forward(const GatedNormArgs& all, hipStream_t stream) {
   GatedNormArgs a = all;
   LaunchTimer timer(kKidGatedNorm, stream);
   constexpr int CH = 16 / (int)sizeof(T);
-  const RowShape s = chunked(a, sizeof(T)) ? row_shape(a.W / CH, CH) : RowShape{0, 0};
+  const RowShape s = chunked(a, sizeof(T)) ? row_shape(a.W / CH, CH) : RowShape{0, 0, 0};
   const int64_t groups = (a.rows + a.R - 1) / a.R;
   // Workers: 4 rows each where that leaves enough of them.
   a.per_group = a.rows <= 16384 || s.nv == 0 ? a.R : (a.R + 3) / 4;
-  const int rpb = s.nv > 0 && s.tpr == 64 ? 4 : 1;
+  const int rpb = s.nv > 0 && s.size == 0 ? 4 : 1;
   // Any number of rows: the threads of a grid (up to 1,024 a row) stay below 2^32.
   constexpr int64_t kMost = 1 << 21;
   const int64_t blocks = (groups * a.per_group + rpb - 1) / rpb;
@@ -543,14 +603,16 @@ hipError_t forward(const GatedNormArgs& all, hipStream_t stream) {
     const unsigned grid = (unsigned)(blocks - done < kMost ? blocks - done : kMost);
     if (s.nv == 0)
       hipLaunchKernelGGL(gated_norm_any_kernel<T>, dim3(grid), dim3(256), 0, stream, a);
-    else if (s.tpr == 64)
-      forward_shape<T, 1, true>(a, 64, grid, stream);
-    else if (s.nv == 1)
-      forward_shape<T, 1, false>(a, s.tpr, grid, stream);
-    else if (s.nv == 2)
-      forward_shape<T, 2, false>(a, s.tpr, grid, stream);
-    else if constexpr (sizeof(T) == 4)
-      forward_shape<T, 4, false>(a, s.tpr, grid, stream);
+    else
+      with_shape<T>(s, [&](auto nv, auto size) {
+        const dim3 block(size == 0 ? 256 : s.tpr);
+        if (a.p)
+          hipLaunchKernelGGL((gated_norm_kernel<T, CH, decltype(nv)::value, decltype(size)::value, true>), dim3(grid),
+                             block, 0, stream, a);
+        else
+          hipLaunchKernelGGL((gated_norm_kernel<T, CH, decltype(nv)::value, decltype(size)::value, false>), dim3(grid),
+                             block, 0, stream, a);
+      });
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -562,7 +624,7 @@ struct Workers {
   int64_t groups, per_group;
   bool token;
 };
-constexpr int64_t kMostWorkers = 1024, kMostNarrow = 4096;
+constexpr int64_t kMostWorkers = 512, kMostNarrow = 4096;
 Workers bwd_workers(int64_t rows, int64_t R, int64_t W, bool modulated) {
   const int64_t most = W <= 1024 ? kMostNarrow : kMostWorkers, groups = (rows + R - 1) / R;
   if (R == 1 && modulated && rows > 1) return {1, rows < most ? (rows + 3) / 4 * 4 : most, true};
@@ -572,39 +634,32 @@ Workers bwd_workers(int64_t rows, int64_t R, int64_t W, bool modulated) {
   return {groups, per, false};
 }
 
-template <class T, int NV, bool WAVE, bool TOKEN>
-void backward_shape(const GatedNormArgs& a, int tpr, unsigned grid, hipStream_t stream) {
-  constexpr int CH = 16 / (int)sizeof(T);
-  const dim3 block(WAVE ? 256 : tpr);
-  if (a.p && a.dh)
-    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, true, true, TOKEN>), dim3(grid), block, 0, stream, a);
-  else if (a.p)
-    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, true, false, TOKEN>), dim3(grid), block, 0, stream, a);
-  else if (a.dh)
-    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, false, true, TOKEN>), dim3(grid), block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, WAVE, false, false, TOKEN>), dim3(grid), block, 0, stream, a);
-}
-
 template <class T, bool TOKEN>
 void backward_rows(const GatedNormArgs& a, const RowShape& s, int64_t workers, hipStream_t stream) {
-  if (s.nv == 0)
+  constexpr int CH = 16 / (int)sizeof(T);
+  if (s.nv == 0) {
     hipLaunchKernelGGL((gated_norm_bwd_any_kernel<T, TOKEN>), dim3((unsigned)workers), dim3(256), 0, stream, a);
-  else if (s.tpr == 64)
-    backward_shape<T, 1, true, TOKEN>(a, 64, (unsigned)((workers + 3) / 4), stream);
-  else if (s.nv == 1)
-    backward_shape<T, 1, false, TOKEN>(a, s.tpr, (unsigned)workers, stream);
-  else if (s.nv == 2)
-    backward_shape<T, 2, false, TOKEN>(a, s.tpr, (unsigned)workers, stream);
-  else if constexpr (sizeof(T) == 4)
-    backward_shape<T, 4, false, TOKEN>(a, s.tpr, (unsigned)workers, stream);
+    return;
+  }
+  with_shape<T>(s, [&](auto nv, auto size) {
+    constexpr int NV = decltype(nv)::value, S = decltype(size)::value;
+    const dim3 grid((unsigned)(S == 0 ? (workers + 3) / 4 : workers)), block(S == 0 ? 256 : s.tpr);
+    if (a.p && a.dh)
+      hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, true, true, TOKEN>), grid, block, 0, stream, a);
+    else if (a.p)
+      hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, true, false, TOKEN>), grid, block, 0, stream, a);
+    else if (a.dh)
+      hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, false, true, TOKEN>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, false, false, TOKEN>), grid, block, 0, stream, a);
+  });
 }
 
 template <class T>
 hipError_t backward(const GatedNormArgs& all, hipStream_t stream) {
   GatedNormArgs a = all;
   constexpr int CH = 16 / (int)sizeof(T);
-  const RowShape s = chunked(a, sizeof(T)) ? row_shape(a.W / CH, CH) : RowShape{0, 0};
+  const RowShape s = chunked(a, sizeof(T)) ? row_shape(a.W / CH, CH) : RowShape{0, 0, 0};
   const Workers w = bwd_workers(a.rows, a.R, a.W, a.g || a.s || a.t);
   a.per_group = w.per_group;
   {
