@@ -12,6 +12,8 @@ import os
 import threading
 from pathlib import Path
 
+import torch
+
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("AVATTN_LIB", _PKG / "libavattn.so"))
 
@@ -437,6 +439,40 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_calls = None
+
+
+def direct_calls(t):
+    """The module of direct calls (``csrc/direct_calls.cpp``), for a call on ``t``;
+    None where the call is to go through the registered ops: not on the GPU, being
+    compiled, inside a function transform, or with forward-mode tangents."""
+    if (torch.compiler.is_compiling() or not t.is_cuda or torch.autograd.forward_ad._current_level >= 0
+            or torch._C._functorch.peek_interpreter_stack() is not None):
+        return None
+    return _calls if _calls is not None else _load_calls()
+
+
+def _load_calls():
+    global _calls
+    lib = load()
+    from .cache_ops import MAX_WINDOW
+    from .scored_ops import MAX_SLOPE_GROUP, MAX_SOFTCAP_BF16
+
+    with _lock:
+        if _calls is None:
+            try:
+                from . import _direct_calls
+            except ImportError as e:
+                raise RuntimeError("avgen_amd/_direct_calls.so is missing or older than this torch; build it with "
+                                   "`python -m avgen_amd.build` (no fallback path exists)") from e
+            names = ("append_paged", "page_values", "paged_attention_workspace_size", "paged_attention",
+                     "gated_add_rms_norm", "gated_add_rms_norm_bwd_workspace_size", "gated_add_rms_norm_bwd")
+            _direct_calls.bind(tuple(ctypes.cast(getattr(lib, f"avattn_{n}"), ctypes.c_void_p).value for n in names),
+                               torch.nn.Parameter, MAX_WINDOW, MAX_SOFTCAP_BF16, MAX_SLOPE_GROUP)
+            _calls = _direct_calls
+    return _calls
 
 
 def strerror(status: int) -> str:

@@ -1,4 +1,5 @@
-"""Build ``libavattn.so`` (the C-ABI HIP library) in-tree with hipcc for gfx950.
+"""Build ``libavattn.so`` (the C-ABI HIP library) in-tree with hipcc for gfx950,
+and ``_direct_calls.so`` (the direct calls of some of its functions from torch).
 
 Usage: ``python -m avgen_amd.build`` (or ``__graft_entry__.build()``).  Each
 ``csrc/*.hip`` is compiled to an object under ``avgen_amd/_build/`` in
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -20,6 +22,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libavattn.so"
+CALLS = PKG / "_direct_calls.so"
 ARCH = "gfx950"
 
 # Packed-fp32 VALU forms stay disabled (plain scalar fp32 code only).
@@ -62,15 +65,40 @@ def _compile(src: Path, extra: list[str]) -> Path:
     return obj
 
 
+def _build_calls() -> None:
+    """Host code against the installed torch, whose libraries are loaded when it is
+    imported."""
+    import torch
+
+    home = Path(torch.__file__).parent
+    include = home / "include"
+    tmp = CALLS.with_suffix(".so.tmp")
+    cmd = [hipcc(), "-x", "c++", "-O2", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-shared", "-Wall",
+           "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-I{INCLUDE}",
+           *(f"-isystem{d}" for d in (include, include / "torch/csrc/api/include", "/opt/rocm/include",
+                                      sysconfig.get_paths()["include"])),
+           str(CSRC / "direct_calls.cpp"), "-o", str(tmp), f"-L{home / 'lib'}",
+           "-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-lc10_hip", "-lc10"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"hipcc failed for direct_calls.cpp:\n{proc.stdout}{proc.stderr}")
+    if proc.stderr.strip():
+        print(proc.stderr, file=sys.stderr)
+    os.replace(tmp, CALLS)
+
+
 def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
-    """Compile every kernel source and link the shared library; return its path."""
+    """Compile every kernel source and link the shared library; build the direct calls;
+    return the library's path."""
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.hip"))
     extra = list(extra_flags or [])
     if verbose:
         extra += ["-Rpass-analysis=kernel-resource-usage"]
     with ThreadPoolExecutor(max_workers=min(8, len(sources))) as pool:
+        calls = pool.submit(_build_calls)
         objs = list(pool.map(lambda s: _compile(s, extra), sources))
+        calls.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     proc = subprocess.run(cmd, capture_output=True, text=True)

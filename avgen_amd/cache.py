@@ -51,11 +51,8 @@ class PagedCache:
 
     def __post_init__(self) -> None:
         tensors = (self.key, self.value, self.key_exponent, self.value_exponent)
-        plan = cache_ops.check_pool("PagedCache", *tensors)
+        cache_ops.check_pool("PagedCache", *tensors)
         _one_device("PagedCache", *tensors)
-        # The pool's strides, where its tensors are ordinary ones: calls then look
-        # at their other arguments only.
-        object.__setattr__(self, "_plan", plan if ops._plain_eager(*tensors) else None)
 
     @classmethod
     def empty(
@@ -145,7 +142,7 @@ def append_paged(
         rotated = None
     out = cache_ops.append_paged(key, value, query if tables is not None else None, cos, sin, int(start), half,
                                  block_table, lengths, counts, cache.key, cache.value, cache.key_exponent,
-                                 cache.value_exponent, cache._plan)
+                                 cache.value_exponent)
     return out if rotated is None else rotated
 
 
@@ -192,9 +189,8 @@ def paged_attention(
         raise ValueError(f"softcap must be positive or None; got {softcap}")
     if window is not None and window < 1:
         raise ValueError(f"window must be positive or None; got {window}")
-    out, _ = cache_ops.paged_attention(
+    return cache_ops.paged_attention(
         query, cache.key, cache.value, cache.key_exponent, cache.value_exponent, block_table, lengths, counts,
         distance_slopes, 0 if window is None else int(window),
         ops.default_scale(query.shape[-1]) if scale is None else float(scale),
-        0.0 if softcap is None else float(softcap), cache._plan, rows=False)
-    return out
+        0.0 if softcap is None else float(softcap))

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .block_ops import _on, _one_device, _packed_last
-from .ops import SUPPORTED_HEAD_DIMS, _direct, _plain_eager, _ptr, _stream, _Strides3, _workspace
+from .ops import SUPPORTED_HEAD_DIMS, _ptr, _stream, _Strides3, _workspace
 from .scored_ops import MAX_SLOPE_GROUP, MAX_SOFTCAP_BF16, _deliver, _laid_out, _new_like
 
 __all__ = ["MAX_WINDOW", "PAGE_SIZES", "append_paged", "page_values", "paged_attention"]
@@ -133,11 +133,10 @@ def _check_tables(name, B, block_table, lengths, counts):
 
 
 def _append_impl(k, v, query, cos, sin, start, half, block_table, lengths, counts, key_pages, value_pages,
-                 key_exponent, value_exponent, plan=None):
+                 key_exponent, value_exponent):
     name = "avgen_amd.append_paged"
     pool = (key_pages, value_pages, key_exponent, value_exponent)
-    if plan is None:
-        plan = check_pool(name, *pool)
+    plan = check_pool(name, *pool)
     pages, heads, page, D = key_pages.shape
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError(f"{name}: key and value must be (batch, heads, length, head_dim) and agree; got "
@@ -216,21 +215,17 @@ def _no_gradient(name, *tensors) -> None:
 
 
 def append_paged(k, v, query, cos, sin, start: int, half: bool, block_table, lengths, counts, key_pages, value_pages,
-                 key_exponent, value_exponent, plan=None):
-    """Writes keys and values to their pages; the rotated query, None for none.
-    ``plan``: that of the pool's :func:`check_pool`, its tensors being
-    :func:`avgen_amd.ops._plain_eager`'s."""
-    name = "avgen_amd.append_paged"
-    pool = (key_pages, value_pages, key_exponent, value_exponent)
-    args = (k, v, query, cos, sin, start, half, block_table, lengths, counts, *pool)
-    _no_gradient(name, k, v, query, cos, sin, key_pages, value_pages)
-    given = (k, v, query, cos, sin, block_table, lengths, counts)
-    if _plain_eager(*given) if plan is not None else _plain_eager(*given, *pool):
-        out = _append_impl(*args, plan)
-        # (As the op does for what it writes.)
-        torch.autograd.graph.increment_version(pool[:2] if key_exponent is None else pool)
-        return out
-    out = _append_op(*args)
+                 key_exponent, value_exponent):
+    """Writes keys and values to their pages; the rotated query, None for none."""
+    calls = _lib.direct_calls(k)
+    if calls is not None:
+        out = calls.append_paged(k, v, query, cos, sin, block_table, lengths, counts, key_pages, value_pages,
+                                 key_exponent, value_exponent, start, half)
+        if out is not NotImplemented:
+            return out
+    _no_gradient("avgen_amd.append_paged", k, v, query, cos, sin, key_pages, value_pages)
+    out = _append_op(k, v, query, cos, sin, start, half, block_table, lengths, counts, key_pages, value_pages,
+                     key_exponent, value_exponent)
     return None if query is None else out
 
 
@@ -272,7 +267,12 @@ def _(key_pages, value_pages, key_exponent, value_exponent):
 def page_values(key_pages, value_pages, key_exponent, value_exponent):
     """The bf16 values of an e4m3 pool: ``(key, value)``."""
     args = (key_pages, value_pages, key_exponent, value_exponent)
-    return _direct(None, _values_op, _values_impl, args, args)
+    calls = _lib.direct_calls(key_pages)
+    if calls is not None:
+        out = calls.page_values(*args)
+        if out is not NotImplemented:
+            return out
+    return _values_op(*args)
 
 
 # ---------------------------------------------------------------------------
@@ -286,12 +286,10 @@ def _attention_workspace_size(*sizes: int) -> int:
 
 
 def _attention_impl(q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes,
-                    window, scale, softcap, plan=None, rows=True):
-    """``(out, lse)``; without ``rows`` the lse is scratch, and None."""
+                    window, scale, softcap):
     name = "avgen_amd.paged_attention"
     pool = (key_pages, value_pages, key_exponent, value_exponent)
-    if plan is None:
-        plan = check_pool(name, *pool)
+    plan = check_pool(name, *pool)
     pages, Hkv, page, D = key_pages.shape
     if q.ndim != 4 or q.shape[3] != D:
         raise ValueError(f"{name}: query must be (batch, heads, length, {D}); got {tuple(q.shape)}")
@@ -321,20 +319,13 @@ def _attention_impl(q, key_pages, value_pages, key_exponent, value_exponent, blo
     o = _new_like(given, q, qs, False)
     blocks = block_table.shape[1]
     need = _attention_workspace_size(B, Hq, Hkv, Lq, D, blocks, page, window, key_exponent is not None)
-    lse = None
-    if rows:
-        lse = torch.empty((B, Hq, Lq), device=device, dtype=torch.float32)
-        ws = _workspace(need, device)
-        at, lse_at = ws.data_ptr(), lse.data_ptr()
-    else:
-        ws = _workspace(need + 4 * B * Hq * Lq, device)  # what is needed is whole 16 bytes
-        at = ws.data_ptr()
-        lse_at = at + need
+    lse = torch.empty((B, Hq, Lq), device=device, dtype=torch.float32)
+    ws = _workspace(need, device)
     with _on(device):
         st = _lib.load().avattn_paged_attention(
             q.data_ptr(), qs, B, Hq, Hkv, Lq, D, block_table.data_ptr(), bts, blocks, lengths.data_ptr(), _ptr(counts),
             *_pool_args(plan, *pool), pages, page, window, scale, softcap, _ptr(slopes),
-            o[1].data_ptr(), o[2], lse_at, at, max(need, 256) if rows else need, _stream(device))
+            o[1].data_ptr(), o[2], lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device))
     _lib.check(st, name)
     return _deliver(o)[0], lse
 
@@ -357,12 +348,15 @@ def _(q, key_pages, value_pages, key_exponent, value_exponent, block_table, leng
 
 
 def paged_attention(q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes,
-                    window: int, scale: float, softcap: float, plan=None, rows: bool = True):
-    """Attention of the newest tokens over pages: ``(out, lse)``.  ``plan`` as for
-    :func:`append_paged`; without ``rows`` the lse may be None."""
+                    window: int, scale: float, softcap: float):
+    """Attention of the newest tokens over pages: the output (the op gives the lse
+    too)."""
     args = (q, key_pages, value_pages, key_exponent, value_exponent, block_table, lengths, counts, slopes, window,
             scale, softcap)
+    calls = _lib.direct_calls(q)
+    if calls is not None:
+        out = calls.paged_attention(*args)
+        if out is not NotImplemented:
+            return out
     _no_gradient("avgen_amd.paged_attention", q, key_pages, value_pages, slopes)
-    if _plain_eager(q, block_table, lengths, counts, slopes, *(args[1:5] if plan is None else ())):
-        return _attention_impl(*args, plan, rows)
-    return _attention_op(*args)
+    return _attention_op(*args)[0]

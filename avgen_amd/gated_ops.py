@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from .block_ops import _FLOATS, _on, _one_device, _rows
-from .ops import _direct, _grad_direct, _ptr, _stream, _workspace
+from .ops import _grad_direct, _ptr, _stream, _workspace
 
 __all__ = ["gated_add_rms_norm", "gated_add_rms_norm_bwd"]
 
@@ -96,7 +96,7 @@ def _vectors(weight, post_weight, gate, scale, shift):
             first is not None and first.dtype is f32), (w, p, g, s, t)
 
 
-def _impl(x, residual, weight, post_weight, gate, scale, shift, residual_scale, eps, stats=True):
+def _impl(x, residual, weight, post_weight, gate, scale, shift, residual_scale, eps):
     rows, group = _check_vectors(_NAME, x, weight, post_weight, gate, scale, shift, eps, residual_scale)
     shape, dtype, device = x.shape, x.dtype, x.device
     if residual is not x:
@@ -107,22 +107,17 @@ def _impl(x, residual, weight, post_weight, gate, scale, shift, residual_scale, 
     _one_device(_NAME, x, residual, weight, post_weight, gate, scale, shift)
     total = torch.empty(shape, dtype=dtype, device=device)
     norm = torch.empty(shape, dtype=dtype, device=device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=device) if stats else None
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=device)
     if rows:
         vectors, _held = _vectors(weight, post_weight, gate, scale, shift)
         (x, xs), (residual, rs) = _rows(x), _rows(residual)
         with _on(device):
             st = _lib.load().avattn_gated_add_rms_norm(
                 x.data_ptr(), xs, residual.data_ptr(), rs, *vectors, rows, shape[-1], group,
-                dtype is torch.float32, residual_scale, eps, total.data_ptr(), norm.data_ptr(), _ptr(stats),
+                dtype is torch.float32, residual_scale, eps, total.data_ptr(), norm.data_ptr(), stats.data_ptr(),
                 _stream(device))
         _lib.check(st, _NAME)
     return norm, total, stats
-
-
-def _plain_impl(*args):
-    """Without a backward to come."""
-    return _impl(*args, stats=False)
 
 
 @lru_cache(maxsize=256)
@@ -147,14 +142,7 @@ def _bwd_impl(dnorm, dsum, x, residual, stats, weight, post_weight, gate, scale,
     if stats.shape != (rows, 2) or stats.dtype is not torch.float32:
         raise ValueError(f"{name}: stats must be float32 ({rows}, 2)")
     _one_device(name, x, residual, stats, dnorm, dsum, weight, post_weight, gate, scale, shift)
-    return _bwd_run(name, rows, group, dnorm, dsum, x, residual, stats.contiguous(), weight, post_weight, gate, scale,
-                    shift, residual_scale, eps)
-
-
-def _bwd_run(name, rows, group, dnorm, dsum, x, residual, stats, weight, post_weight, gate, scale, shift,
-             residual_scale, eps):
-    """The backward of checked arguments."""
-    shape, dtype, device = x.shape, x.dtype, x.device
+    stats = stats.contiguous()
     W = shape[-1]
     dx = torch.empty(shape, dtype=dtype, device=device)
     dr = dx if _alike(post_weight, gate, residual_scale) else torch.empty(shape, dtype=dtype, device=device)
@@ -219,8 +207,13 @@ def _(dnorm, dsum, x, residual, stats, weight, post_weight, gate, scale, shift, 
 def gated_add_rms_norm(x, residual, weight, post_weight, gate, scale, shift, residual_scale: float,
                        eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """``(norm, sum)`` of the gated residual step; differentiable."""
-    tensors = (x, residual, weight, post_weight, gate, scale, shift)
-    return _direct(_GatedAddRmsNorm, _op, _plain_impl, (*tensors, residual_scale, eps), tensors)[:2]
+    args = (x, residual, weight, post_weight, gate, scale, shift, residual_scale, eps)
+    calls = _lib.direct_calls(x)
+    if calls is not None:
+        out = calls.gated_add_rms_norm(*args)
+        if out is not NotImplemented:
+            return out
+    return _op(*args)[:2]
 
 
 def gated_add_rms_norm_bwd(dnorm, dsum, x, residual, stats, weight, post_weight, gate, scale, shift,
@@ -255,25 +248,3 @@ def _backward(ctx, dnorm, dsum, _dstats=None):
 
 
 torch.library.register_autograd("avgen_amd::gated_add_rms_norm", _backward, setup_context=_setup)
-
-
-class _GatedAddRmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, *args):
-        result = _impl(*args)
-        ctx.set_materialize_grads(False)
-        _setup(ctx, args, result)
-        return result
-
-    @staticmethod
-    def backward(ctx, dnorm, dsum, _dstats):
-        if dnorm is None or not _grad_direct(dnorm, dsum):
-            return _backward(ctx, dnorm, dsum)
-        # The forward was a plain call, its arguments are checked: so is this one.
-        x, residual, stats, weight, post_weight, gate, scale, shift = ctx.saved_tensors
-        first = gate if gate is not None else scale if scale is not None else shift
-        rows = stats.shape[0]
-        group = rows if first is None or not rows else x.numel() // first.numel()
-        grads = _bwd_run(_NAME + "_bwd", rows, group, dnorm, dsum, x, residual, stats, weight, post_weight, gate,
-                         scale, shift, ctx.residual_scale, ctx.eps)
-        return (*grads, None, None)
