@@ -57,7 +57,10 @@ static bool use_small(int B, int Hq, int Lq, int Lk, int head_dim) {
 // (20,000 keys 0.94-1.02 of the whole).
 FwdSplit fwd_split_plan(int B, int Hq, int Lq, int Lk, int D, bool fp8, bool windows) {
   FwdSplit best{0, 0, 0};
-  if (windows) return best;  // the tiles of a row block are known on the device only
+  // The tiles of a row block are known on the device only.  (Over pages, where
+  // the rows are a sequence's newest tokens, they are about all of them: 1,024 rows
+  // of 64 heads x 12,001 keys 313 -> 267 us.)
+  if (windows) return best;
   const bool small = !fp8 && use_small(B, Hq, Lq, Lk, D);
   const int bm = small ? 128 : 256;
   const int per_cu = small ? (D == 64 ? 3 : 2) : 1;
@@ -116,7 +119,7 @@ static hipError_t launch_fwd_d(const FwdArgs& args, hipStream_t stream) {
   const bool small = !fp8 && use_small(a.B, a.Hq, a.Lq, a.Lk, D);
   const int bm = small ? 128 : 256;
   const int64_t blocks = (int64_t)((a.Lq + bm - 1) / bm) * a.B * a.Hq;
-  const FwdSplit sp = fwd_split_plan(a.B, a.Hq, a.Lq, a.Lk, D, fp8, a.wlo != nullptr && a.score.mode == 0);
+  const FwdSplit sp = fwd_split_plan(a.B, a.Hq, a.Lq, a.Lk, D, fp8, a.wlo != nullptr && a.score.mode == 0 && !a.paged);
   if (a.part != nullptr) {
     a.nsplit = sp.nsplit;
     a.nparts = sp.nparts;

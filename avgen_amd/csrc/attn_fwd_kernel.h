@@ -225,7 +225,9 @@ void attn_fwd_kernel(FwdArgs a) {
   if ((int)blockIdx.x < nfull) {
     bid = xcd_remap_pairs(blockIdx.x, nfull, nqt * (a.Hq / a.Hkv), a.mask != nullptr);
   } else {
-    const int i = blockIdx.x - nfull;
+    int i = blockIdx.x - nfull;
+    // (Split here only over pages; the parts of a kv head's blocks on one XCD.)
+    if constexpr (WIN && !SCORE) i = xcd_remap(i, a.nsplit * a.nparts);
     bid = nfull + i / a.nparts;
     part = i % a.nparts;
   }

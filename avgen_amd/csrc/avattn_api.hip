@@ -1390,13 +1390,14 @@ int table_args(const int32_t* table, int64_t stride, int32_t blocks, const int32
 }
 
 struct PagedWorkspace {
-  size_t windows, offsets, total;
+  size_t windows, offsets, parts, total;
 };
-PagedWorkspace paged_general_workspace(int32_t B, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D) {
+PagedWorkspace paged_general_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t Lq, int32_t Lk, int32_t D) {
   PagedWorkspace w;
   w.windows = round256(fwd_workspace(B, Hkv, Lk, D).total);
   w.offsets = w.windows + round256((size_t)B * Lq * 2 * sizeof(int));
-  w.total = w.offsets + round256((size_t)B * sizeof(int));
+  w.parts = w.offsets + round256((size_t)B * sizeof(int));
+  w.total = w.parts + fwd_split_plan(B, Hq, Lq, Lk, D, false, false).bytes;
   return w;
 }
 
@@ -1486,7 +1487,7 @@ size_t avattn_paged_attention_workspace_size(int32_t batch, int32_t heads_q, int
   if (check_dims(batch, heads_q, heads_kv, len_q, cap, head_dim) != AVATTN_OK) return 0;
   if ((int64_t)batch * heads_q * len_q == 0 || cap == 0) return 0;
   const FewPlan few = paged_plan(batch, heads_q, heads_kv, len_q, cap, window, head_dim, is_e4m3 != 0);
-  return few.nsplit > 0 ? few.bytes : paged_general_workspace(batch, heads_kv, len_q, cap, head_dim).total;
+  return few.nsplit > 0 ? few.bytes : paged_general_workspace(batch, heads_q, heads_kv, len_q, cap, head_dim).total;
 }
 
 int avattn_paged_attention(const void* q, const int64_t* q_strides, int32_t batch, int32_t heads_q, int32_t heads_kv,
@@ -1522,7 +1523,7 @@ int avattn_paged_attention(const void* q, const int64_t* q_strides, int32_t batc
     return launch_status(launch_empty(static_cast<bf16*>(out), out_strides[0], out_strides[1], out_strides[2], batch,
                                       heads_q, len_q, head_dim, lse, s));
   const FewPlan plan = paged_plan(batch, heads_q, heads_kv, len_q, cap, window, head_dim, key_exponents != nullptr);
-  const PagedWorkspace wl = paged_general_workspace(batch, heads_kv, len_q, cap, head_dim);
+  const PagedWorkspace wl = paged_general_workspace(batch, heads_q, heads_kv, len_q, cap, head_dim);
   const size_t need = plan.nsplit > 0 ? plan.bytes : wl.total;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return AVATTN_ERR_WORKSPACE;
   c.q = q, c.o = out;
@@ -1562,6 +1563,7 @@ int avattn_paged_attention(const void* q, const int64_t* q_strides, int32_t batc
   a.wlo = reinterpret_cast<int*>(ws + wl.windows);
   a.whi = a.wlo + (int64_t)batch * len_q;
   a.wsb = len_q;
+  a.part = reinterpret_cast<float*>(ws + wl.parts);
   if (2 * (int64_t)batch * heads_kv * (a.Lkp / 64) + ((int64_t)batch * len_q + 255) / 256 >= (int64_t)1 << 24)
     return AVATTN_ERR_TOO_LARGE;  // the preparation's grid
   // Neither cap nor bias: the plain forward with windows.
