@@ -175,10 +175,10 @@ def paged_attention(
 
     Returns ``(batch, heads, length, head_dim)`` in the query's layout.  Rows of
     padding, and rows whose keys have no page, are zeros.  Slots outside the
-    hull of a sequence's windows may hold anything.  A few rows (up to 32
-    queries, or 64 rows over the heads of a kv head) read the pages in place,
-    the keys split over the chip; more rows go over a copy in bfloat16 of the
-    pages that the table has room for, so pass the part of the table that is in
+    hull of a sequence's windows may hold anything.  Up to some hundred rows (by
+    an estimate of both ways' times, from the sizes) read the pages in place, the
+    keys split over the chip; more go over a copy in bfloat16 of the pages
+    that the table has room for, so pass the part of the table that is in
     use.  Not differentiable.
 
     Raises:

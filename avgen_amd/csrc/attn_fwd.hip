@@ -56,7 +56,7 @@ static bool use_small(int B, int Hq, int Lq, int Lk, int head_dim) {
 // (1,20,1792,128) x 10,752 keys from 221 to 234 us, (1,24,1537) 245 to 253
 // (20,000 keys 0.94-1.02 of the whole).
 FwdSplit fwd_split_plan(int B, int Hq, int Lq, int Lk, int D, bool fp8, bool windows) {
-  FwdSplit best{0, 0, 0};
+  FwdSplit best{0, 0, 0, 0.f};
   // The tiles of a row block are known on the device only.  (Over pages, where
   // the rows are a sequence's newest tokens, they are about all of them: 1,024 rows
   // of 64 heads x 12,001 keys 313 -> 267 us.)
@@ -66,7 +66,8 @@ FwdSplit fwd_split_plan(int B, int Hq, int Lq, int Lk, int D, bool fp8, bool win
   const int per_cu = small ? (D == 64 ? 3 : 2) : 1;
   const int slots = kCus * per_cu;
   const int ntile = (Lk + 63) / 64;
-  const int r = (int)((int64_t)((Lq + bm - 1) / bm) * B * Hq % slots);
+  const int64_t blocks = (int64_t)((Lq + bm - 1) / bm) * B * Hq;
+  const int r = (int)(blocks % slots);
   const float tile_us = fp8 ? 1.25f : (D == 64 ? 1.55f : 1.7f), fixed_us = 8.f;
   // Rounds n workgroups take.  A partial round is shorter than a full one:
   // one workgroup on a CU by itself takes less than per_cu sharing it, and
@@ -83,13 +84,15 @@ FwdSplit fwd_split_plan(int B, int Hq, int Lq, int Lk, int D, bool fp8, bool win
   // The parts cost their partial sums, written and read at 4 TB/s, and the
   // combining launch.
   const float slot_bytes = 4.f * fwd_slot_floats(bm, D);
-  if (!small && r == (int64_t)((Lq + bm - 1) / bm) * B * Hq && r > kCus / 2) return best;
-  float cost = rounds(r) * (ntile * tile_us + fixed_us) - 4.f;
+  const float whole = ntile * tile_us + fixed_us;
+  best.us = blocks / slots * whole + rounds(r) * whole;
+  if (!small && r == blocks && r > kCus / 2) return best;
+  float cost = rounds(r) * whole - 4.f;
   for (int p = 2; p <= 8 && ntile / p >= 8; ++p) {
     const float c = rounds(r * p) * (ntile * tile_us / p + fixed_us) + 5.f + r * p * slot_bytes * 0.5e-6f;
     if (c < cost) {
       cost = c;
-      best = FwdSplit{r, p, (size_t)r * p * fwd_slot_floats(bm, D) * sizeof(float)};
+      best = FwdSplit{r, p, (size_t)r * p * fwd_slot_floats(bm, D) * sizeof(float), blocks / slots * whole + c};
     }
   }
   return best;

@@ -1,11 +1,12 @@
 // Attention forward over a cache of pages (PageTable), bf16 or e4m3 with an
 // exponent per page and head.
 //
-// Few query rows per kv head (a decode step, drafted tokens): the few-row forward
+// Few query rows per kv head (a decode step, drafted tokens, a piece of a prompt;
+// paged_plan): the few-row forward
 // of attn_few.hip, whose waves stage their 32-key tiles from two runs of 16 slots
-// each, since a page is a multiple of 16.  The entries of the block table are read
-// two tiles ahead of their use and the exponents one, so neither adds a latency
-// to the tile's.  e4m3 codes stay codes in LDS (half the bytes, two workgroups
+// each, since a page is a multiple of 16.  The entries of the block table and the
+// exponents are read for 32 tiles at once, a lane each half tile, so that they add
+// a latency per 32 tiles.  e4m3 codes stay codes in LDS (half the bytes, two workgroups
 // on a CU) and become bf16 on the way into the MFMAs, c 2^e exactly: K as 16
 // bytes of a key's row, V by transposed 8-bit reads.  HBM-bound: the pages are
 // read once.
@@ -42,19 +43,44 @@ __device__ __forceinline__ i32x2 lds_read_tr8(const bf16* p) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(const_cast<bf16*>(p)));
 }
 
+// A value that is the same in the whole wave, by a scalar load.
+__device__ __forceinline__ int load_uniform(const int* p) {
+  return *(const __attribute__((address_space(4))) int*)p;
+}
+// A sequence's tokens and how many of them are the call's; `uniform`: b is the
+// whole wave's.
+struct PagedSequence {
+  int len, count;
+  __device__ __forceinline__ PagedSequence(const PagedArgs& p, int b, bool uniform = false) {
+    len = max(uniform ? load_uniform(p.lengths + b) : p.lengths[b], 0);
+    count = p.few.Lq;
+    if (p.counts) count = min(max(uniform ? load_uniform(p.counts + b) : p.counts[b], 0), count);
+  }
+};
 // A query's position and keys.
 struct PagedRow {
   int pos, lo, hi;
 };
-__device__ __forceinline__ PagedRow paged_row(const PagedArgs& p, int b, int i) {
-  const int len = max(p.lengths[b], 0), count = p.counts ? min(max(p.counts[b], 0), p.few.Lq) : p.few.Lq;
-  const int64_t pos = (int64_t)len - count + i;
-  PagedRow r{(int)pos, 0, 0};  // (a row behind the last one: any position)
-  if (i >= count || pos < 0) return r;
-  const int64_t lo = p.window > 0 ? pos - p.window + 1 : 0;
-  r.hi = (int)(pos + 1 < p.few.Lk ? pos + 1 : p.few.Lk);
-  r.lo = (int)(lo < 0 ? 0 : (lo < r.hi ? lo : r.hi));
+__device__ __forceinline__ PagedRow paged_row(const PagedArgs& p, const PagedSequence& s, int i) {
+  const int pos = (int)((unsigned)(s.len - s.count) + (unsigned)i);
+  PagedRow r{pos, 0, 0};                // (a row behind the last one: any position)
+  if (i >= s.count || pos < 0) return r;
+  r.hi = pos < p.few.Lk ? pos + 1 : p.few.Lk;
+  r.lo = p.window > 0 ? min(max(pos - p.window + 1, 0), r.hi) : 0;
   return r;
+}
+
+// The hull of the keys of rows i0 .. i1 (a block's), whose windows never move
+// back, and the keys that all of them see.
+__device__ __forceinline__ void paged_hull(const PagedArgs& p, const PagedSequence& s, int i0, int i1,
+                                           BlockWindows& w) {
+  w.glo = w.ghi = w.all_lo = w.all_hi = 0;
+  if (i0 >= s.count) return;
+  const PagedRow first = paged_row(p, s, i0), last = paged_row(p, s, min(i1, s.count - 1));
+  w.ghi = last.hi;
+  w.glo = min(first.lo, last.hi);
+  w.all_lo = last.lo;
+  w.all_hi = i1 < s.count ? first.hi : 0;
 }
 
 template <int D, bool FP8>
@@ -78,12 +104,11 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
   const int unit = blockIdx.x / a.nsplit, split = blockIdx.x % a.nsplit;
   const int rb = unit % a.row_blocks, bhk = unit / a.row_blocks;
   const int b = bhk / a.Hkv, hk = bhk % a.Hkv;
-  const int rows = min(a.Lq * (a.Hq / a.Hkv) - rb * kTile, kTile);  // of this block
+  const PagedSequence seq(p, b, true);
+  const int group = a.Hq / a.Hkv;
+  const int rows = min(a.Lq * group - rb * kTile, kTile);  // of this block
   const bool valid = l32 < rows;
   const RowPlace rp = row_place(a, hk, rb * kTile + (valid ? l32 : 0));
-  const PagedRow pr = paged_row(p, b, rp.i);
-  const BlockWindows w = block_windows(pr.lo, pr.hi, valid);
-
   // This lane's row of Q: per 16-channel step channels 16*ks + 8*hh + [0, 8); with
   // codes, whose rows are read 16 bytes at a time, 32*(ks/2) + 16*hh + 8*(ks%2).
   bf16x8 qf[KS];
@@ -101,48 +126,53 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
   if (a.score.slopes != nullptr) {
     rbias.slope = a.score.slopes[rp.h];
     rbias.slope2 = rbias.slope * kLog2e;
-    rbias.measure(pr.pos, pr.lo, pr.hi);
   }
-  const int qpos = rbias.at.pos;
-  const float slope2 = rbias.slope2, ref = (float)rbias.at.ref;
+  const PagedRow pr = paged_row(p, seq, rp.i);
+  BlockWindows w{pr.lo, pr.hi, 0, 0, 0, 0};
+  paged_hull(p, seq, rb * kTile / group, (rb * kTile + rows - 1) / group, w);
 
   // Tiles of this wave: the block's tiles, a range per workgroup, every
   // fourth of it per wave.
   const int tile0 = w.glo / kTile, ntile = w.ghi > w.glo ? (w.ghi + kTile - 1) / kTile - tile0 : 0;
-  const int t0 = tile0 + (int)((int64_t)ntile * split / a.nsplit) + wave;
-  const int t1 = tile0 + (int)((int64_t)ntile * (split + 1) / a.nsplit);
+  const int each = ntile / a.nsplit, more = ntile % a.nsplit;
+  const int first = tile0 + each * split + min(split, more);
+  const int t0 = first + wave, t1 = first + each + (split < more);
 
   TileStager<16, RL, 1> rows16;  // both tensors' slots are D apart
   rows16.init(RL, 0, lane);
   constexpr int ES = FP8 ? 1 : 2;
+  constexpr int kLoads = 4 * decltype(rows16)::kPer;  // of a stage
   const char* kp = static_cast<const char*>(p.kp) + hk * p.kph * ES;
   const char* vp = static_cast<const char*>(p.vp) + hk * p.vph * ES;
-  // The table entry of slots t*32 + 16*(lane % 2) .. + 15 (-1: none of them is
-  // looked at), as loaded: checked where it is used.
-  auto load_entry = [&](int t) {
-    const int key0 = t * kTile + 16 * (lane & 1);
-    if (t >= t1 || key0 >= w.ghi || key0 + 16 <= w.glo) return -1;
-    return p.pages.table[b * p.pages.tsb + (key0 >> p.pages.shift)];
+  // The pages of 32 of the wave's tiles at once, batch n: lane 2i + g has that of
+  // slots 16*g .. + 15 of tile t0 + kWaves*(32n + i) (-1: none of them is looked
+  // at, or the entry names no page) and its exponents.  A batch is loaded when its
+  // first tile is staged, before the last batch's last tile is computed.
+  int page = -1, ke = 0, ve = 0, old_ke = 0, old_ve = 0;
+  auto load_batch = [&](int n) {
+    const int key0 = (t0 + kWaves * (32 * n + (lane >> 1))) * kTile + 16 * (lane & 1);
+    const bool in = key0 < w.ghi && key0 + 16 > w.glo;
+    const int entry = p.pages.table[b * p.pages.tsb + (in ? key0 >> p.pages.shift : 0)];
+    page = in && entry >= 0 && entry < p.pages.pages ? entry : -1;
+    if constexpr (FP8) {
+      old_ke = ke, old_ve = ve;
+      const int64_t at = page < 0 ? 0 : page;
+      ke = p.ke[at * p.kes + hk], ve = p.ve[at * p.ves + hk];
+    }
   };
-  int ke = 0, ve = 0;  // exponents of the staged tile, by lane % 2
-  // Stages tile t from pages `entry`; returns which of its keys have a page.
-  auto stage = [&](int t, int entry, Stage& sg) {
-    if (entry < 0 || entry >= p.pages.pages) entry = -1;
+  // Stages the wave's tile i (of this batch, at t); returns which of its keys have
+  // a page.
+  auto stage = [&](int i, int t, Stage& sg) {
     uint32_t has = 0;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int page = __builtin_amdgcn_readlane(entry, g);
-      const int64_t at = page < 0 ? 0 : page;
+      const int pg = __builtin_amdgcn_readlane(page, 2 * (i % 32) + g);
+      const int64_t at = pg < 0 ? 0 : pg;
       const int slot = (t * kTile + 16 * g) & ((1 << p.pages.shift) - 1);
-      const uint32_t bytes = page < 0 ? 0u : 16u * D * ES;  // no page: zeros
-      has |= page < 0 ? 0u : 0xffffu << (16 * g);
+      const uint32_t bytes = pg < 0 ? 0u : 16u * D * ES;  // no page: zeros
+      has |= pg < 0 ? 0u : 0xffffu << (16 * g);
       rows16.stage(sg.k + 16 * g * RL, make_rsrc(kp + (at * p.kps + slot * D) * ES, bytes), 0u);
       rows16.stage(sg.v + 16 * g * RL, make_rsrc(vp + (at * p.vps + slot * D) * ES, bytes), 0u);
-    }
-    if constexpr (FP8) {
-      const int64_t at = entry < 0 ? 0 : entry;
-      ke = p.ke[at * p.kes + hk];
-      ve = p.ve[at * p.ves + hk];
     }
     return has;
   };
@@ -152,33 +182,32 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
 
+  // Two tiles of the wave are in flight: while one is computed the other, then
+  // both.
+  uint32_t has = 0, has_next = 0;
+  load_batch(0);
   retire_prologue_loads();
-  uint32_t has = 0;
-  int entry = -1;
-  if (t0 < t1) {
-    entry = load_entry(t0);
-    wait_vmem_n<0>();
-    has = stage(t0, opaque(entry), sm.st[wave][0]);
-    entry = load_entry(t0 + kWaves);
-  }
-  for (int t = t0, buf = 0; t < t1; t += kWaves, buf ^= 1) {
-    Stage& sg = sm.st[wave][buf];
-    // Everything in flight belongs to this tile (its rows, its exponents) or is
-    // the next one's table entry.
-    wait_vmem_n<0>();
+  if (t0 < t1) has = stage(0, t0, sm.st[wave][0]);
+  if (t0 + kWaves < t1) has_next = stage(1, t0 + kWaves, sm.st[wave][1]);
+  if (a.score.slopes != nullptr) rbias.measure(pr.pos, pr.lo, pr.hi);
+  const int qpos = rbias.at.pos;
+  const float slope2 = rbias.slope2, ref = (float)rbias.at.ref;
+  for (int t = t0, i = 0; t < t1; t += kWaves, ++i) {
+    Stage& sg = sm.st[wave][i & 1];
+    // This tile's rows; the next one's may be on the way.
+    if (t + kWaves < t1)
+      wait_vmem_n<kLoads>();
+    else
+      wait_vmem_n<0>();
     uint32_t keys = has;
-    const int next = opaque(entry);
     float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f;
     if constexpr (FP8) {
-      const int ek = opaque(ke), ev = opaque(ve);
-      ks0 = exponent_scale(__builtin_amdgcn_readlane(ek, 0)), ks1 = exponent_scale(__builtin_amdgcn_readlane(ek, 1));
-      vs0 = exponent_scale(__builtin_amdgcn_readlane(ev, 0)), vs1 = exponent_scale(__builtin_amdgcn_readlane(ev, 1));
-    }
-    if (t + kWaves < t1) {
-      // The other stage's reads have returned before it is filled again.
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      has = stage(t + kWaves, next, sm.st[wave][buf ^ 1]);
-      entry = load_entry(t + 2 * kWaves);
+      const bool old = i % 32 == 31 && t + kWaves < t1;
+      const int ek = old ? old_ke : ke, ev = old ? old_ve : ve, lane0 = 2 * (i % 32);
+      ks0 = exponent_scale(__builtin_amdgcn_readlane(ek, lane0));
+      ks1 = exponent_scale(__builtin_amdgcn_readlane(ek, lane0 + 1));
+      vs0 = exponent_scale(__builtin_amdgcn_readlane(ev, lane0));
+      vs1 = exponent_scale(__builtin_amdgcn_readlane(ev, lane0 + 1));
     }
     {
       const int from = w.glo - t * kTile, to = w.ghi - t * kTile;
@@ -260,6 +289,13 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
           acc[dt] = mfma32(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[k2], acc[dt]);
         }
       }
+    has = has_next;
+    if (t + 2 * kWaves < t1) {
+      if ((i + 2) % 32 == 0) load_batch((i + 2) / 32);
+      // The stage's reads have returned before it is filled again.
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      has_next = stage(i + 2, t + 2 * kWaves, sg);
+    }
   }
 
   // Join the waves: each leaves its rows' maxima, sums and outputs.
@@ -297,10 +333,10 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(FwdArgs a, PagedArgs p,
     const int64_t u = ((int64_t)blockIdx.x - 2 * nk) * 256 + tid;
     if (u >= (int64_t)a.B * a.Lq) return;
     const int b = (int)(u / a.Lq), i = (int)(u % a.Lq);
-    PagedRow r = paged_row(p, b, i);
-    const int count = p.counts ? min(max(p.counts[b], 0), a.Lq) : a.Lq;
+    const PagedSequence seq(p, b);
+    PagedRow r = paged_row(p, seq, i);
     // Non-decreasing in the row: a row behind the last token ends where it ends.
-    if (i >= count && count > 0) r.lo = r.hi = paged_row(p, b, count - 1).hi;
+    if (i >= seq.count && seq.count > 0) r.lo = r.hi = paged_row(p, seq, seq.count - 1).hi;
     wlo[u] = r.lo, whi[u] = r.hi;
     if (offsets != nullptr && i == 0) offsets[b] = r.pos;
     return;
@@ -309,9 +345,9 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(FwdArgs a, PagedArgs p,
   const int u = is_k ? blockIdx.x : blockIdx.x - nk;
   const int t = u % nt, bh = u / nt;
   const int b = bh / a.Hkv, h = bh % a.Hkv, s0 = S * t;
-  const int count = p.counts ? min(max(p.counts[b], 0), a.Lq) : a.Lq;
+  const PagedSequence seq(p, b, true);
   int lo = 0, hi = 0;
-  if (count > 0) lo = paged_row(p, b, 0).lo, hi = paged_row(p, b, count - 1).hi;
+  if (seq.count > 0) lo = paged_row(p, seq, 0).lo, hi = paged_row(p, seq, seq.count - 1).hi;
   if (s0 + S <= lo || s0 >= hi) {
     if (is_k && tid == 0) a.kmax2[(int64_t)bh * nt + t] = 0;
     if (!is_k && h == 0 && tid < 64) {
@@ -386,21 +422,50 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(FwdArgs a, PagedArgs p,
 
 }  // namespace
 
+// Few rows or many: the smaller of two estimates, both within about a sixth of
+// what was measured (us, few-row against general):
+//   e4m3, 32 heads over 8 of 128, 12,000 keys: 33 tokens 29, 65; 128 56, 69; 192 92, 72; 512 169, 110
+//   the same twice: 96 tokens 92, 106; 192 166, 113; bf16: 64 tokens 85, 112; 96 147, 115
+//   e4m3, 64 heads over 8, 1,000 keys: 96 tokens 21, 30; 256 23, 33; 512 40, 34
+//   e4m3, 16 heads over 2 of 64, 12,000 keys: 128 tokens 33, 41; 192 45, 43; 512 85, 49
+// The few-row kernel computes no row that is not there (its blocks hold rows of all
+// heads of a kv head) and needs no copy; the general one has twice its rate.
+// Its split n of a block's keys is the fastest by the same estimate: whole rounds
+// of workgroups, and no parts to join where the keys are few (128 blocks of 1,000
+// keys 18 us, split in 4 19; 304 of 6,000 keys 88 whole, 72 in 3).
 FewPlan paged_plan(int B, int Hq, int Hkv, int Lq, int64_t cap, int window, int D, bool fp8) {
   FewPlan p{};
   const int64_t rows = (int64_t)Lq * (Hq / Hkv);
-  if (cap < 1 || !(Lq <= kFewQueries || rows <= kFewRows)) return p;
-  int64_t reach = window > 0 && (int64_t)window + Lq - 1 < cap ? (int64_t)window + Lq - 1 : cap;
+  if (cap < 1) return p;
+  const int64_t reach = window > 0 && (int64_t)window + Lq - 1 < cap ? (int64_t)window + Lq - 1 : cap;
   p.block_rows = (int)(rows < kTile ? rows : kTile);
   p.row_blocks = (int)((rows + kTile - 1) / kTile);
   const int64_t units = (int64_t)B * Hkv * p.row_blocks;
-  const int64_t slots = D == 128 && !fp8 ? 256 : 512;
-  const int64_t tiles = reach / kTile + 1, most = (tiles + kWaves - 1) / kWaves;
-  int64_t n = units < slots ? slots / units : 1;
-  if (n > most) n = most;
-  p.nsplit = (int)n;
-  constexpr int64_t kMaxGrid = (1 << 24) - 1;
-  if (units * p.nsplit > kMaxGrid || units * p.block_rows > kMaxGrid) return FewPlan{};
+  constexpr int64_t kCus = 256, kMaxGrid = (1 << 24) - 1;
+  if (units > kMaxGrid || units * p.block_rows > kMaxGrid) return FewPlan{};
+  // Workgroups per CU, a wave's tile among them (and 0.7 of it with a CU to itself).
+  const int per_cu = D == 128 && !fp8 ? 1 : 2;
+  const float tile_us = D == 64 ? 1.6f : (fp8 ? 1.9f : 1.5f);
+  const float slot_bytes = 4.f * few_slot_floats(p.block_rows, D);
+  const int64_t slots = kCus * per_cu, tiles = reach / kTile + 1, most = (tiles + kWaves - 1) / kWaves;
+  float best = 0.f;
+  auto consider = [&](int64_t n) {
+    if (n > most) n = most;
+    if (n < 1 || units * n > kMaxGrid) return;
+    const int64_t grid = units * n, rem = grid % slots;
+    const float rounds = (float)(grid / slots) + (rem == 0 ? 0.f : (rem <= kCus && per_cu > 1 ? 0.7f : 1.f));
+    const int64_t mine = ((tiles + n - 1) / n + kWaves - 1) / kWaves;
+    const float us = 0.88f * (rounds * (mine * tile_us + 4.f) + 6.f +
+                              (n > 1 ? 3.f + grid * slot_bytes * 2.f / 3.5e6f : 0.f));
+    if (p.nsplit == 0 || us < best) best = us, p.nsplit = (int)n;
+  };
+  consider(1);
+  for (int64_t r = 1; r <= 4; ++r) consider(r * slots / units);  // whole rounds
+  if (per_cu > 1) consider(kCus / units);
+  // Three launches, the copy of the pages, the general forward.
+  const float copy = (float)(B * Hkv) * (float)reach * D * 2.f * (fp8 ? 3.f : 4.f) / 4.5e6f;
+  const float forward = 0.7f * fwd_split_plan(B, Hq, Lq, (int)reach, D, false, false).us;
+  if (rows > kFewRows && 12.f + copy + (forward > 10.f ? forward : 10.f) < best) return FewPlan{};
   p.bytes = p.nsplit > 1 ? (size_t)units * p.nsplit * few_slot_floats(p.block_rows, D) * sizeof(float) : 0;
   return p;
 }

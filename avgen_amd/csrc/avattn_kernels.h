@@ -225,10 +225,12 @@ struct FwdArgs {
 // Floats of one part of `rows` rows: the accumulators, then per 32 rows their
 // maxima and sums.
 constexpr int fwd_slot_floats(int rows, int D) { return rows * (D + 2); }
-// The forward's split for a shape (nsplit 0: none) and the bytes of its slots.
+// The forward's split for a shape (nsplit 0: none), the bytes of its slots and the
+// estimated time of the whole forward.
 struct FwdSplit {
   int nsplit, nparts;
   size_t bytes;
+  float us;
 };
 FwdSplit fwd_split_plan(int B, int Hq, int Lq, int Lk, int head_dim, bool fp8, bool windows);
 

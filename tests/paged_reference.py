@@ -107,25 +107,26 @@ def attend(q, key: torch.Tensor, value: torch.Tensor, block_table, lengths, coun
         if n == 0:
             continue
         pg, sl = torch.tensor([a[0] for a in at]), torch.tensor([a[1] for a in at])
-        j = torch.arange(n)
+        j, i = torch.arange(n), torch.arange(Lq)
+        distance = (last - count + i)[:, None] - j
+        seen = has & (distance >= 0) & (i < count)[:, None]
+        if window:
+            seen &= distance < window
+        rows = seen.any(1)  # the others have no key
         for h in range(Hq):
-            k, v = key[pg, h * H // Hq, sl], value[pg, h * H // Hq, sl]
-            for i in range(count):
-                p = last - count + i
-                seen = has & (j <= p)
-                if window:
-                    seen &= j > p - window
-                if not bool(seen.any()):
-                    continue
-                z = scale * (k[seen] @ q[b, h, i])
-                mag = scale * (k[seen].abs() @ q[b, h, i].abs())
-                if cap:
-                    z = cap * torch.tanh(z / cap)
-                if slopes is not None:
-                    z = z - float(slopes[h]) * (p - j[seen]).double()
-                w = torch.softmax(z, 0)
-                out[b, h, i] = w @ v[seen]
-                spread[b, h, i] = w @ v[seen].abs()
-                lse[b, h, i] = torch.logsumexp(z, 0)
-                score[b, h, i] = mag.max() + z.max().abs() + 1.0
+            # Values that no row sees may be anything.
+            used = seen.any(0)
+            k, v = (torch.where(used[:, None], t[pg, h * H // Hq, sl], 0.0) for t in (key, value))
+            z = scale * (q[b, h] @ k.T)
+            mag = scale * (q[b, h].abs() @ k.T.abs())
+            if cap:
+                z = cap * torch.tanh(z / cap)
+            if slopes is not None:
+                z = z - float(slopes[h]) * distance.double()
+            z = z.masked_fill(~seen, float("-inf"))[rows]
+            w = torch.softmax(z, 1)
+            out[b, h, rows] = w @ v
+            spread[b, h, rows] = w @ v.abs()
+            lse[b, h, rows] = torch.logsumexp(z, 1)
+            score[b, h, rows] = mag.masked_fill(~seen, 0.0)[rows].amax(1) + z.amax(1).abs() + 1.0
     return out, lse, spread, score

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from avgen_amd import rope
+from avgen_amd import _lib, rope
 from avgen_amd.cache import PagedCache, append_paged, paged_attention
 from avgen_amd.rope import RotaryTables
 
@@ -251,6 +251,49 @@ def test_far_positions_of_a_long_cache():
     append_paged(few, k, k, i32(moved), i32([150, 192]))
     for a, b in ((cache.key, few.key), (cache.value, few.value)):
         assert all(torch.equal(a[p].view(torch.uint8), b[n].view(torch.uint8)) for n, p in enumerate(names))
+
+
+def launched(name, call):
+    """Whether `call` launches the kernel."""
+    with _lib.LaunchTiming(64) as t:
+        call()
+        torch.cuda.synchronize()
+        return t.read(name)[1] > 0
+
+
+MANY = 300  # tokens that go over a copy of the pages, with 64 heads over one
+
+
+@pytest.mark.parametrize("dtype", [B16, F8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("options", [{}, {"window": 70}, {"window": 5}, {"cap": 15.0}, {"slopes": True},
+                                     {"window": 130, "cap": 15.0, "slopes": True}], ids=str)
+def test_many_rows_over_a_copy(options, D, dtype):
+    """Sequences of different lengths, one without the call's tokens, one without
+    any, padded rows, entries without a page and slots that hold anything."""
+    lengths, counts = [MANY + 700, 1203, 310, 0], [MANY, 211, 0, 0]
+    rows, pages = table_of(lengths, 32, seed=3)
+    cache = filled(pages, 1, 32, D, dtype, 17)
+    rows[1][3], rows[0][20] = -1, pages + 7
+    for page, n in ((rows[0][1000 // 32], 1000), (rows[1][1203 // 32], 1203)):
+        for pool in (cache.key, cache.value):
+            pool[page, :, n % 32:].view(torch.uint8).fill_(0xFF)
+    given = dict(options)
+    if given.pop("slopes", False):
+        given["slopes"] = torch.linspace(0.001, 0.2, 64, device="cuda")
+    q = heads(4, 64, MANY, D, 3, 2.0)
+    out = check_attention(q, cache, rows, lengths, counts, **given)
+    assert not bool(out[1, :, 211:].any()) and not bool(out[2:].any())
+    call = lambda: paged_attention(q, cache, i32(rows), i32(lengths), counts=i32(counts))  # noqa: E731
+    assert launched("prep_paged", call)
+
+
+def test_few_rows_are_read_in_place():
+    rows, pages = table_of([900], 16)
+    cache = filled(pages, 2, 16, 128, F8, 4)
+    for Lq in (1, 40, 70):
+        q = heads(1, 8, Lq, 128, 5)
+        assert not launched("prep_paged", lambda: paged_attention(q, cache, i32(rows), i32([900])))
 
 
 # ---------------------------------------------------------------------------

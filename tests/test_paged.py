@@ -248,8 +248,8 @@ def test_append_status(changed, status):
     (dict(cap=2000.0), _lib.ERR_ARGUMENT), (dict(slopes=P + 2), _lib.ERR_LAYOUT),
     (dict(blocks=1 << 27, bts=1 << 27), _lib.ERR_TOO_LARGE), (dict(blocks=1 << 21, bts=1 << 21), _lib.ERR_TOO_LARGE),
     (dict(lengths=None), _lib.ERR_NULL_POINTER), (dict(counts=P + 1), _lib.ERR_LAYOUT),
-    (dict(L=40, Hq=64, ws=None, qs=strides(4096 * 40, 64, 4096)), _lib.ERR_WORKSPACE),
-    (dict(L=40, Hq=64, wsb=1000, qs=strides(4096 * 40, 64, 4096)), _lib.ERR_WORKSPACE),
+    (dict(L=4000, Hq=64, ws=None, qs=strides(4096 * 4000, 64, 4096)), _lib.ERR_WORKSPACE),
+    (dict(L=4000, Hq=64, wsb=1000, qs=strides(4096 * 4000, 64, 4096)), _lib.ERR_WORKSPACE),
     (dict(blocks=300, bts=300, ws=P + 8), _lib.ERR_WORKSPACE), (dict(blocks=300, bts=300, wsb=8), _lib.ERR_WORKSPACE),
     (dict(B=0), _lib.OK), (dict(L=0), _lib.OK),
 ])
