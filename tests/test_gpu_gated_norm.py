@@ -317,3 +317,14 @@ def test_same_tensor_twice_and_repeatable():
     n2, h2 = layers.gated_add_rms_norm(*two, gate=st["gate"])
     a, b = torch.autograd.grad((n2, h2), two, (st["dn"], st["dh"]))
     assert torch.equal(h, h2) and torch.equal(got, a + b)
+
+
+@pytest.mark.parametrize("dtype", [B16, F32])
+@pytest.mark.parametrize("W", [1, 5, 8, 24, 33, 64, 65, 129, 200, 257, 512, 513, 777, 1025, 2056, 4097, 6152, 8191, 8200,
+                               12288, 16381, 16384, 16392])
+@pytest.mark.parametrize("lead, modulation", [((3, 37), "batch"), ((1, 600), "shared"), ((2, 9), "token"),
+                                              ((70, 3), "batch")])
+def test_every_way_of_sharing_a_row(lead, modulation, W, dtype):
+    """Several rows in a wave, one in a wave or in a workgroup of any size, with and
+    without whole 16-byte chunks, and rows of any width; one workgroup and many."""
+    check(lead, W, dtype, modulation, W % 3 != 0, True, 0.5, seed=W)
