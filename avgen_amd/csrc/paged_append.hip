@@ -23,8 +23,7 @@ namespace {
 
 constexpr int kItem = 16;  // channels a thread rotates at once: two chunks of 8
 
-__device__ __forceinline__ void load8(const bf16* p, float* v) {
-  const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+__device__ __forceinline__ void unpack8(const u32x4& w, float* v) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
 }
@@ -50,62 +49,95 @@ __device__ __forceinline__ ItemPlace item_place(const AppendRotation& r, int u) 
   return {c0, c1, false};
 }
 
-// Rotates 8 consecutive channels from `ch` on in interleaved pairs.
-__device__ __forceinline__ void turn_pairs(const AppendRotation& r, int64_t t, int ch, float* v) {
-#pragma clang fp contract(off)
-  if (ch < r.start || ch >= r.start + 2 * r.pairs) return;
-  const int p = (ch - r.start) / 2;
-  const f32x4 c = *reinterpret_cast<const f32x4*>(r.cos + t + p), s = *reinterpret_cast<const f32x4*>(r.sin + t + p);
+// The factors of an item of whole chunks, the same for all heads: of a pair of
+// chunks all eight, else four for each chunk that is rotated.
+struct Turn {
+  float c[8] = {}, s[8] = {};
+  bool on0 = false, on1 = false;
+  __device__ __forceinline__ void load4(const AppendRotation& r, int64_t at, int j) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(r.cos + at), y = *reinterpret_cast<const f32x4*>(r.sin + at);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float e = v[2 * j], f = v[2 * j + 1];
-    v[2 * j] = e * c[j] - f * s[j];
-    v[2 * j + 1] = e * s[j] + f * c[j];
+    for (int i = 0; i < 4; ++i) c[j + i] = x[i], s[j + i] = y[i];
   }
-}
+  // t: the row's place in the tables.
+  __device__ __forceinline__ void load(const AppendRotation& r, int64_t t, int u, const ItemPlace& at) {
+    on0 = on1 = at.pair;
+    if (r.cos == nullptr) return;
+    if (at.pair) {
+      load4(r, t + 8 * u, 0);
+      load4(r, t + 8 * u + 4, 4);
+    } else if (!r.half) {
+      auto in = [&](int ch) { return ch >= r.start && ch < r.start + 2 * r.pairs; };
+      on0 = in(at.c0), on1 = in(at.c1);
+      if (on0) load4(r, t + (at.c0 - r.start) / 2, 0);
+      if (on1) load4(r, t + (at.c1 - r.start) / 2, 4);
+    }
+  }
+  // Every product rounded separately, as rotate_kernel does.
+  __device__ __forceinline__ void apply(const ItemPlace& at, float* v) const {
+#pragma clang fp contract(off)
+    if (at.pair) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = v[i], f = v[8 + i];
+        v[i] = e * c[i] - f * s[i];
+        v[8 + i] = e * s[i] + f * c[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = v[2 * i], f = v[2 * i + 1];
+        const bool on = i < 4 ? on0 : on1;
+        v[2 * i] = on ? e * c[i] - f * s[i] : e;
+        v[2 * i + 1] = on ? e * s[i] + f * c[i] : f;
+      }
+    }
+  }
+};
 
-// Item u of the row at x, rotated (ROT) by the table row at t; every product
-// rounded separately, as rotate_kernel does.  VEC: whole 16-byte chunks; else
-// channel by channel, any pairs, start and strides.
-template <bool VEC, bool ROT>
-__device__ __forceinline__ void load_item(const AppendRotation& r, const bf16* x, int64_t t, int u, float* v) {
+// Item u of the rows of HB heads, `hs` apart from x on (those below `heads`), rotated
+// (ROT) by the table row at t.  VEC: whole 16-byte chunks; else channel by channel,
+// any pairs, start and strides.
+template <bool VEC, bool ROT, int HB>
+__device__ __forceinline__ void load_items(const AppendRotation& r, const bf16* x, int64_t hs, int heads, int64_t t,
+                                           int u, float (*v)[kItem]) {
 #pragma clang fp contract(off)
   if constexpr (VEC) {
     ItemPlace at{kItem * u, kItem * u + 8, false};
     if (ROT) at = item_place(r, u);
-    load8(x + at.c0, v);
-    load8(x + at.c1, v + 8);
-    if (ROT && r.cos != nullptr) {
-      if (at.pair) {
+    Turn turn;
+    if (ROT) turn.load(r, t, u, at);
+    u32x4 r0[HB], r1[HB];
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const f32x4 c = *reinterpret_cast<const f32x4*>(r.cos + t + 8 * u + j);
-          const f32x4 s = *reinterpret_cast<const f32x4*>(r.sin + t + 8 * u + j);
+    for (int e = 0; e < HB; ++e) {
+      const bf16* row = x + (e < heads ? e : 0) * hs;  // (past the last head: the first one again)
+      r0[e] = *reinterpret_cast<const u32x4*>(row + at.c0);
+      r1[e] = *reinterpret_cast<const u32x4*>(row + at.c1);
+    }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = v[j + i], f = v[8 + j + i];
-            v[j + i] = e * c[i] - f * s[i];
-            v[8 + j + i] = e * s[i] + f * c[i];
-          }
-        }
-      } else if (!r.half) {
-        turn_pairs(r, t, at.c0, v);
-        turn_pairs(r, t, at.c1, v + 8);
-      }
+    for (int e = 0; e < HB; ++e) {
+      unpack8(r0[e], v[e]);
+      unpack8(r1[e], v[e] + 8);
+      if (ROT) turn.apply(at, v[e]);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < kItem; ++j) {
-      const int ch = kItem * u + j, at = ch - r.start;
-      float y = (float)x[ch];
-      if (ROT && r.cos != nullptr && at >= 0 && at < 2 * r.pairs) {
-        const int p = r.half ? at % r.pairs : at / 2;
-        const bool second = r.half ? at >= r.pairs : at & 1;
-        const int mate = r.half ? (second ? ch - r.pairs : ch + r.pairs) : (second ? ch - 1 : ch + 1);
-        const float o = (float)x[mate], c = r.cos[t + p], s = r.sin[t + p];
-        y = second ? o * s + y * c : y * c - o * s;
+    for (int e = 0; e < HB; ++e) {
+      if (e >= heads) continue;
+#pragma unroll
+      for (int j = 0; j < kItem; ++j) {
+        const int ch = kItem * u + j, at = ch - r.start;
+        const bf16* row = x + e * hs;
+        float y = (float)row[ch];
+        if (ROT && r.cos != nullptr && at >= 0 && at < 2 * r.pairs) {
+          const int p = r.half ? at % r.pairs : at / 2;
+          const bool second = r.half ? at >= r.pairs : at & 1;
+          const int mate = r.half ? (second ? ch - r.pairs : ch + r.pairs) : (second ? ch - 1 : ch + 1);
+          const float o = (float)row[mate], c = r.cos[t + p], s = r.sin[t + p];
+          y = second ? o * s + y * c : y * c - o * s;
+        }
+        v[e][j] = y;
       }
-      v[j] = y;
     }
   }
 }
@@ -167,31 +199,47 @@ __device__ __forceinline__ PagePlace page_place(const AppendArgs& a, int b, int 
   return p;
 }
 
-// Workgroups [0, nkv): (b, block, kv head, key or value); then the query's rows.
+// Heads that a thread takes together (the factors of the rotation are read once
+// for them, and their rows are in flight together): of the query, and of bf16 pages
+// as far as registers allow (two prompts of 8,192 tokens, 32 heads of 128: 187 ->
+// 151 us).  A page and head of codes needs its maximum before the first is written;
+// beside it more of the query's heads cost waves (four of 4,133 tokens, 32 query
+// heads: 80 us, with 4 together 93).
+template <bool FP8>
+constexpr int kQueryHeads = FP8 ? 1 : 4;
+template <bool FP8, int NI>
+constexpr int kPageHeads = FP8 ? 1 : (NI == 1 ? 4 : (NI == 2 ? 2 : 1));
+
+// Workgroups [0, nkv): (b, block, kv heads, key or value); then the query's rows.
 template <int D, bool FP8, bool VEC, int NI>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
   constexpr int IPR = D / kItem;  // items of a row
+  constexpr int HB = kPageHeads<FP8, NI>, HQ = kQueryHeads<FP8>;
   const int tid = threadIdx.x, n = blockDim.x;
   if ((int)blockIdx.x >= nkv) {
-    const int64_t rows = (int64_t)a.B * a.L * a.Hq;
     const int64_t u0 = ((int64_t)blockIdx.x - nkv) * n + tid;
-    const int64_t row = u0 / IPR;
     const int u = (int)(u0 % IPR);
-    if (row >= rows) return;
-    const int h = (int)(row % a.Hq);
-    const int64_t bi = row / a.Hq;
+    const int nh = (a.Hq + HQ - 1) / HQ;
+    const int64_t bi = u0 / IPR / nh;
+    if (bi >= (int64_t)a.B * a.L) return;
+    const int h0 = (int)(u0 / IPR - bi * nh);  // heads h0, h0 + nh, ..
     const int b = (int)(bi / a.L), i = (int)(bi - (int64_t)b * a.L);
-    float v[kItem];
-    load_item<VEC, true>(a.rot, a.q + b * a.qsb + h * a.qsh + i * a.qsl, b * a.rot.tsb + (int64_t)i * a.rot.pairs, u,
-                         v);
+    const int heads = (a.Hq - h0 + nh - 1) / nh;
+    float v[HQ][kItem];
+    load_items<VEC, true, HQ>(a.rot, a.q + b * a.qsb + h0 * a.qsh + i * a.qsl, nh * a.qsh, heads,
+                                       b * a.rot.tsb + (int64_t)i * a.rot.pairs, u, v);
     const ItemPlace at = stored_place<VEC, true>(a.rot, u);
-    bf16* o = a.q_out + b * a.osb + h * a.osh + i * a.osl;
-    if constexpr (VEC) {
-      store8(o + at.c0, v);
-      store8(o + at.c1, v + 8);
-    } else {
 #pragma unroll
-      for (int j = 0; j < kItem; ++j) o[kItem * u + j] = (bf16)v[j];
+    for (int e = 0; e < HQ; ++e) {
+      if (e >= heads) continue;
+      bf16* o = a.q_out + b * a.osb + (h0 + e * nh) * a.osh + i * a.osl;
+      if constexpr (VEC) {
+        store8(o + at.c0, v[e]);
+        store8(o + at.c1, v[e] + 8);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kItem; ++j) o[kItem * u + j] = (bf16)v[e][j];
+      }
     }
     return;
   }
@@ -199,34 +247,41 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
   int w = blockIdx.x;
   const int which = w & 1;
   w >>= 1;
-  const int h = w % a.Hkv;
-  w /= a.Hkv;
+  const int nh = (a.Hkv + HB - 1) / HB;
+  const int h = w % nh * HB;
+  w /= nh;
   const int j = w % a.nblocks, b = w / a.nblocks;
   const PagePlace pp = page_place(a, b, j);
   if (pp.page < 0) return;  // the whole workgroup
   const bool key = which == 0;
   const bf16* x = (key ? a.k + b * a.ksb + h * a.ksh : a.v + b * a.vsb + h * a.vsh);
-  const int64_t sl = key ? a.ksl : a.vsl;
-  float v[NI][kItem];
+  const int64_t sl = key ? a.ksl : a.vsl, sh = key ? a.ksh : a.vsh;
+  const int heads = min(HB, a.Hkv - h);
+  float v[NI][HB][kItem];
 #pragma unroll
   for (int m = 0; m < NI; ++m) {
     const int it = m * n + tid, slot = it / IPR, u = it % IPR;
     if (slot < pp.lo || slot >= pp.hi) continue;
     const int i = pp.i0 + slot;
     if (key)
-      load_item<VEC, true>(a.rot, x + i * sl, b * a.rot.tsb + (int64_t)i * a.rot.pairs, u, v[m]);
+      load_items<VEC, true, HB>(a.rot, x + i * sl, sh, heads, b * a.rot.tsb + (int64_t)i * a.rot.pairs, u, v[m]);
     else
-      load_item<VEC, false>(a.rot, x + i * sl, 0, u, v[m]);
+      load_items<VEC, false, HB>(a.rot, x + i * sl, sh, heads, 0, u, v[m]);
   }
   if constexpr (!FP8) {
-    bf16* out = static_cast<bf16*>(key ? a.kp : a.vp) + pp.page * (key ? a.kps : a.vps) + h * (key ? a.kph : a.vph);
+    const int64_t ph = key ? a.kph : a.vph;
+    bf16* out = static_cast<bf16*>(key ? a.kp : a.vp) + pp.page * (key ? a.kps : a.vps) + h * ph;
 #pragma unroll
     for (int m = 0; m < NI; ++m) {
       const int it = m * n + tid, slot = it / IPR, u = it % IPR;
       if (slot < pp.lo || slot >= pp.hi) continue;
       const ItemPlace at = key ? stored_place<VEC, true>(a.rot, u) : stored_place<VEC, false>(a.rot, u);
-      store8(out + slot * D + at.c0, v[m]);
-      store8(out + slot * D + at.c1, v[m] + 8);
+#pragma unroll
+      for (int e = 0; e < HB; ++e) {
+        if (e >= heads) continue;
+        store8(out + e * ph + slot * D + at.c0, v[m][e]);
+        store8(out + e * ph + slot * D + at.c1, v[m][e] + 8);
+      }
     }
   } else {
     float top = 0.f;
@@ -236,7 +291,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
       if (slot < pp.lo || slot >= pp.hi) continue;
 #pragma unroll
       for (int e = 0; e < kItem; ++e) {
-        const float y = fabsf(v[m][e]);
+        const float y = fabsf(v[m][0][e]);
         top = fmaxf(top, y < kPosInf ? y : 0.f);
       }
     }
@@ -267,8 +322,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
       const int it = m * n + tid, slot = it / IPR, u = it % IPR;
       if (slot < pp.lo || slot >= pp.hi) continue;
       const ItemPlace at = key ? stored_place<VEC, true>(a.rot, u) : stored_place<VEC, false>(a.rot, u);
-      *reinterpret_cast<u32x2*>(out + slot * D + at.c0) = codes8(v[m], unit);
-      *reinterpret_cast<u32x2*>(out + slot * D + at.c1) = codes8(v[m] + 8, unit);
+      *reinterpret_cast<u32x2*>(out + slot * D + at.c0) = codes8(v[m][0], unit);
+      *reinterpret_cast<u32x2*>(out + slot * D + at.c1) = codes8(v[m][0] + 8, unit);
     }
   }
 }
@@ -336,8 +391,11 @@ static AppendShape append_shape(const AppendArgs& a, int head_dim) {
   AppendShape s;
   s.threads = items < 256 ? (items + 63) / 64 * 64 : 256;
   s.ni = items > 256 ? items / 256 : 1;
-  s.nkv = 2 * (int64_t)a.B * ((a.L - 1) / page + 2) * a.Hkv;
-  s.nq = a.q ? ((int64_t)a.B * a.L * a.Hq * ipr + s.threads - 1) / s.threads : 0;
+  const int heads = a.ke ? 1 : (s.ni == 1 ? kPageHeads<false, 1> : (s.ni == 2 ? kPageHeads<false, 2> : 1));
+  s.nkv = 2 * (int64_t)a.B * ((a.L - 1) / page + 2) * ((a.Hkv + heads - 1) / heads);
+  const int together = a.ke ? kQueryHeads<true> : kQueryHeads<false>;
+  const int64_t nh = (a.Hq + together - 1) / together;
+  s.nq = a.q ? ((int64_t)a.B * a.L * nh * ipr + s.threads - 1) / s.threads : 0;
   return s;
 }
 
