@@ -746,9 +746,10 @@ struct GatedNormArgs {
   void* dw;
   void* dp;
   float* part;
-  int64_t first;      // a launch's first worker, and workers of a group, each with
-  int64_t per_group;  // every per_group-th of its rows (set by the launchers)
-  int tpr;  // threads per row, of those that share a wave (set by the launches)
+  // Set by the launchers: a launch's first worker (backward: workgroup), those of a
+  // group, and threads per row of the rows that share a wave.
+  int64_t first, per_group;
+  int tpr;
 };
 size_t gated_norm_bwd_workspace_bytes(int64_t rows, int64_t R, int64_t W, bool modulated);
 hipError_t launch_gated_norm(const GatedNormArgs& a, bool f32, hipStream_t stream);

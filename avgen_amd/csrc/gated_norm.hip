@@ -273,10 +273,10 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated
   __shared__ __attribute__((aligned(16))) float acc[LDS ? 2 * NV * MOST * CH : (WAVE ? 256 * NV * CH : 4)];
   const int TPR = WAVE ? a.tpr : (int)blockDim.x, RPB = WAVE ? 256 / TPR : 1;
   const int t = WAVE ? threadIdx.x & (TPR - 1) : threadIdx.x, sub = WAVE ? threadIdx.x / TPR : 0;
-  const int64_t group = TOKEN ? 0 : blockIdx.x / a.per_group;
+  const int64_t wg = a.first + blockIdx.x, group = TOKEN ? 0 : wg / a.per_group;
   const int64_t end = TOKEN ? a.rows : min((group + 1) * a.R, a.rows);
   const int64_t step = a.per_group * RPB;
-  const int64_t row0 = (TOKEN ? 0 : group * a.R) + (blockIdx.x - group * a.per_group) * RPB + sub;
+  const int64_t row0 = (TOKEN ? 0 : group * a.R) + (wg - group * a.per_group) * RPB + sub;
   float held_a[HOLD ? NV : 1][CH], held_b[HOLD ? NV : 1][CH];
   float sn[NV][CH], st[NV][CH], sc[NV][CH];
   uint32_t off[NV];  // this thread's columns, 0 past the end of the row,
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated
       }
     }
   }
-  float* part = a.part + blockIdx.x * 3 * a.W;
+  float* part = a.part + wg * 3 * a.W;
   if constexpr (WAVE) {
     // The workers' sums, in order.
     const int width = TPR * NV * CH;
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated
 template <class T, bool TOKEN>
 __global__ __launch_bounds__(kAny) void gated_norm_bwd_any_kernel(GatedNormArgs a) {
   __shared__ float red[16];
-  const int64_t worker = blockIdx.x;
+  const int64_t worker = a.first + blockIdx.x;
   const int64_t group = TOKEN ? 0 : worker / a.per_group;
   const int64_t end = TOKEN ? a.rows : min((group + 1) * a.R, a.rows);
   float* part = a.part + worker * 3 * a.W;
@@ -636,6 +636,9 @@ RowShape row_shape(int64_t W, int chunk, int64_t rows) {
   return {tpr, chunk, nv, nv > 1 ? 3 : (tpr <= 512 ? 1 : (tpr <= 768 ? 2 : 3))};
 }
 
+// Workgroups of a launch: the threads of a grid (up to 1,024 a row) stay below 2^32.
+constexpr int64_t kMostGrid = 1 << 21;
+
 // f(columns of a chunk, chunks per thread, size) as compile-time constants.
 template <class T, class F>
 void with_shape(const RowShape& s, F&& f) {
@@ -671,12 +674,10 @@ hipError_t forward(const GatedNormArgs& all, hipStream_t stream) {
   const int64_t most = s.size == 0 ? 16 : 8;
   mine = mine < 1 || s.nv == 0 ? 1 : (mine > most ? most : mine);
   a.per_group = (a.R + mine - 1) / mine;
-  // Any number of rows: the threads of a grid (up to 1,024 a row) stay below 2^32.
-  constexpr int64_t kMost = 1 << 21;
   const int64_t blocks = (groups * a.per_group + rpb - 1) / rpb;
-  for (int64_t done = 0; done < blocks; done += kMost) {
+  for (int64_t done = 0; done < blocks; done += kMostGrid) {
     a.first = done * rpb;
-    const unsigned grid = (unsigned)(blocks - done < kMost ? blocks - done : kMost);
+    const unsigned grid = (unsigned)(blocks - done < kMostGrid ? blocks - done : kMostGrid);
     if (s.nv == 0)
       hipLaunchKernelGGL(gated_norm_any_kernel<T>, dim3(grid), dim3(kAny), 0, stream, a);
     else
@@ -714,20 +715,26 @@ Workgroups bwd_workgroups(int64_t rows, int64_t R, int rpb, int waves, bool modu
 }
 
 template <class T, bool TOKEN>
-void backward_rows(const GatedNormArgs& a, const RowShape& s, int64_t workgroups, hipStream_t stream) {
-  const dim3 grid((unsigned)workgroups);
-  if (s.nv == 0) {
-    hipLaunchKernelGGL((gated_norm_bwd_any_kernel<T, TOKEN>), grid, dim3(kAny), 0, stream, a);
-    return;
-  }
-  with_shape<T>(s, [&](auto ch, auto nv, auto size) {
-    constexpr int CH = decltype(ch)::value, NV = decltype(nv)::value, S = decltype(size)::value;
-    const dim3 block(S == 0 ? 256 : s.tpr);
-    if (a.p)
-      hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, true, TOKEN>), grid, block, 0, stream, a);
+hipError_t backward_rows(const GatedNormArgs& all, const RowShape& s, int64_t workgroups, hipStream_t stream) {
+  GatedNormArgs a = all;
+  for (int64_t done = 0; done < workgroups; done += kMostGrid) {
+    a.first = done;
+    const dim3 grid((unsigned)(workgroups - done < kMostGrid ? workgroups - done : kMostGrid));
+    if (s.nv == 0)
+      hipLaunchKernelGGL((gated_norm_bwd_any_kernel<T, TOKEN>), grid, dim3(kAny), 0, stream, a);
     else
-      hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, false, TOKEN>), grid, block, 0, stream, a);
-  });
+      with_shape<T>(s, [&](auto ch, auto nv, auto size) {
+        constexpr int CH = decltype(ch)::value, NV = decltype(nv)::value, S = decltype(size)::value;
+        const dim3 block(S == 0 ? 256 : s.tpr);
+        if (a.p)
+          hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, true, TOKEN>), grid, block, 0, stream, a);
+        else
+          hipLaunchKernelGGL((gated_norm_bwd_kernel<T, CH, NV, S, false, TOKEN>), grid, block, 0, stream, a);
+      });
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <class T>
@@ -740,14 +747,12 @@ hipError_t backward(const GatedNormArgs& all, hipStream_t stream) {
   const Workgroups w = bwd_workgroups(a.rows, a.R, rpb, s.nv == 0 ? kAny / 64 : (s.size == 0 ? 4 : s.tpr / 64), modulated);
   a.per_group = w.per_group;
   a.tpr = s.tpr;
+  hipError_t e;
   {
     LaunchTimer timer(kKidGatedNormBwd, stream);
-    if (w.token)
-      backward_rows<T, true>(a, s, w.per_group, stream);
-    else
-      backward_rows<T, false>(a, s, w.groups * w.per_group, stream);
+    e = w.token ? backward_rows<T, true>(a, s, w.per_group, stream)
+                : backward_rows<T, false>(a, s, w.groups * w.per_group, stream);
   }
-  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   GatedNormArgs b = a;
   if (w.token) b.ds = b.dt = b.dg = nullptr;  // written

@@ -328,3 +328,20 @@ def test_every_way_of_sharing_a_row(lead, modulation, W, dtype):
     """Several rows in a wave, one in a wave or in a workgroup of any size, with and
     without whole 16-byte chunks, and rows of any width; one workgroup and many."""
     check(lead, W, dtype, modulation, W % 3 != 0, True, 0.5, seed=W)
+
+
+def test_more_workgroups_than_a_launch_takes():
+    """Groups of three rows of 8 values, 2^21 + 7 of them: a workgroup each in the
+    backward, in two launches."""
+    groups, W = 2**21 + 7, 8
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x, r, dn, dh = (torch.randn(groups, 3, W, generator=g, device="cuda", dtype=F32) for _ in range(4))
+    gate = torch.randn(groups, 1, W, generator=g, device="cuda", dtype=F32)
+    leaves = [t.requires_grad_(True) for t in (x, r, gate)]
+    n, h = layers.gated_add_rms_norm(x, r, gate=gate)
+    grads = torch.autograd.grad((n, h), leaves, (dn, dh))
+    at = torch.tensor([0, 1, 2**20, 2**21 - 1, 2**21, groups - 1], device="cuda")
+    st = dict.fromkeys(NAMES)
+    st.update({k: v.detach()[at] for k, v in dict(x=x, r=r, gate=gate, dn=dn, dh=dh).items()})
+    check_forward(st, 1.0, n.detach()[at], h.detach()[at])
+    check_backward(st, 1.0, {k: v[at] for k, v in zip(("x", "r", "gate"), grads)})

@@ -288,6 +288,31 @@ def test_many_rows_over_a_copy(options, D, dtype):
     assert launched("prep_paged", call)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("options", [{}, {"window": 700}, {"window": 30}, {"cap": 15.0}], ids=str)
+def test_many_rows_split_over_their_keys(options, D):
+    """A grid on half the CUs: parts of the keys (at 128), also parts without a key."""
+    rows, pages = table_of([6000], 64, seed=4)
+    cache = filled(pages, 1, 64, D, F8, 18)
+    q = heads(1, 64, MANY, D, 4, 2.0)
+    check_attention(q, cache, rows, [6000], **options)
+    call = lambda: paged_attention(q, cache, i32(rows), i32([6000]), window=options.get("window"))  # noqa: E731
+    if not options:
+        assert launched("prep_paged", call) and launched("lse_merge", call) == (D == 128)
+
+
+@pytest.mark.parametrize("dtype", [B16, F8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles_of_one_wave(D, dtype):
+    """Enough sequences that each is one workgroup's: a wave passes several batches
+    of 32 tiles.  They share their pages."""
+    B, H = 64, 8
+    lengths = [9000 - 131 * b for b in range(B)]
+    rows, pages = table_of(lengths[:1], 16, seed=5)
+    cache = filled(pages, H, 16, D, dtype, 19)
+    check_attention(heads(B, H, 1, D, 5, 2.0), cache, rows * B, lengths)
+
+
 def test_few_rows_are_read_in_place():
     rows, pages = table_of([900], 16)
     cache = filled(pages, 2, 16, 128, F8, 4)
@@ -340,6 +365,19 @@ def check_append(cache, k, v, rows, lengths, counts=None, tables=None, layout="i
     if tables is not None and query is not None:
         assert torch.equal(out, rope.rotate_heads(query, tables, layout=layout, start=start))
     return old
+
+
+@pytest.mark.parametrize("dtype", [B16, F8])
+@pytest.mark.parametrize("page", [16, 32, 256])
+@pytest.mark.parametrize("Hkv, Hq", [(1, 1), (5, 9), (8, 30)])
+def test_append_any_number_of_heads(Hkv, Hq, page, dtype):
+    """Heads that a thread takes together, and what is left of them."""
+    L, counts = 45, [45, 31]
+    lengths = [45, 31 + 70]
+    rows, pages = table_of(lengths, page)
+    cache = filled(pages, Hkv, page, 64, dtype, page)
+    k, v, q = heads(2, Hkv, L, 64, 50, 3.0), heads(2, Hkv, L, 64, 51), heads(2, Hq, L, 64, 52)
+    check_append(cache, k, v, rows, lengths, counts, tables_of(lengths, counts, L, 64), "interleaved", 0, q)
 
 
 @pytest.mark.parametrize("dtype", [B16, F8])
