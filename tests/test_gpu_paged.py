@@ -291,14 +291,14 @@ def test_many_rows_over_a_copy(options, D, dtype):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("options", [{}, {"window": 700}, {"window": 30}, {"cap": 15.0}], ids=str)
 def test_many_rows_split_over_their_keys(options, D):
-    """A grid on half the CUs: parts of the keys (at 128), also parts without a key."""
+    """A grid on half the CUs: parts of the keys, also parts without a key."""
     rows, pages = table_of([6000], 64, seed=4)
     cache = filled(pages, 1, 64, D, F8, 18)
     q = heads(1, 64, MANY, D, 4, 2.0)
     check_attention(q, cache, rows, [6000], **options)
     call = lambda: paged_attention(q, cache, i32(rows), i32([6000]), window=options.get("window"))  # noqa: E731
     if not options:
-        assert launched("prep_paged", call) and launched("lse_merge", call) == (D == 128)
+        assert launched("prep_paged", call) and launched("lse_merge", call)
 
 
 @pytest.mark.parametrize("dtype", [B16, F8])
