@@ -154,6 +154,8 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
     const bool in = key0 < w.ghi && key0 + 16 > w.glo;
     const int entry = p.pages.table[b * p.pages.tsb + (in ? key0 >> p.pages.shift : 0)];
     page = in && entry >= 0 && entry < p.pages.pages ? entry : -1;
+  };
+  auto load_exponents = [&] {
     if constexpr (FP8) {
       old_ke = ke, old_ve = ve;
       const int64_t at = page < 0 ? 0 : page;
@@ -189,6 +191,7 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
   retire_prologue_loads();
   if (t0 < t1) has = stage(0, t0, sm.st[wave][0]);
   if (t0 + kWaves < t1) has_next = stage(1, t0 + kWaves, sm.st[wave][1]);
+  load_exponents();  // (behind the tiles, which wait for the table's entries only)
   if (a.score.slopes != nullptr) rbias.measure(pr.pos, pr.lo, pr.hi);
   const int qpos = rbias.at.pos;
   const float slope2 = rbias.slope2, ref = (float)rbias.at.ref;
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
       }
     has = has_next;
     if (t + 2 * kWaves < t1) {
-      if ((i + 2) % 32 == 0) load_batch((i + 2) / 32);
+      if ((i + 2) % 32 == 0) load_batch((i + 2) / 32), load_exponents();
       // The stage's reads have returned before it is filled again.
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       has_next = stage(i + 2, t + 2 * kWaves, sg);

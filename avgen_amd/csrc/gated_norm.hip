@@ -17,8 +17,8 @@
 // the groups dw = sum (1 + s) N, dp = sum g C.
 // HBM-bound: the forward reads x and r and writes h and n, the backward reads x,
 // r, dn and dh and writes dx and dr (one tensor where they are alike).  A row
-// stays in the registers of the threads that share it (a wave, or a workgroup),
-// which keep their columns of A, b and t, and of the sums, over the rows of a
+// stays in the registers of the threads that share it (8 to 64 lanes of a wave, or a
+// workgroup), which keep their columns of A, b and t, and of the sums, over the rows of a
 // group that they take one after the other.  Sums are fp32, in a fixed order.
 #include "norm_parts.h"
 

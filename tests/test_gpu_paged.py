@@ -504,3 +504,21 @@ def test_no_gradient():
     seen = cache.key._version
     append_paged(cache, q.detach(), q.detach(), i32([[0]]), i32([3]))
     assert cache.key._version > seen
+
+
+@pytest.mark.parametrize("page, D", [(16, 64), (32, 128), (256, 128)])
+def test_values_of_every_code_and_exponent(page, D):
+    """All 256 codes with all 256 exponents: bf16(code * 2**exponent), exact but for
+    results below bf16's smallest normal number or past its largest."""
+    pages, H = 129, 2
+    cache = PagedCache.empty(pages, H, page, D, dtype=F8)
+    codes = torch.arange(page * D, device="cuda", dtype=torch.int32).remainder(256).to(torch.uint8)
+    for pool, shift in ((cache.key, 0), (cache.value, 7)):
+        pool.view(torch.uint8).copy_(codes.roll(shift).view(page, D).expand(pages, H, page, D))
+    e = (torch.arange(pages * H, device="cuda") % 256 - 128).to(torch.int8).view(pages, H)
+    cache.key_exponent.copy_(e)
+    cache.value_exponent.copy_(e.flip(0))
+    for pool, ex, got in zip((cache.key, cache.value), (cache.key_exponent, cache.value_exponent), cache.values()):
+        want = torch.ldexp(pool.double(), ex.double()[:, :, None, None]).to(torch.float32).to(B16)
+        same = (got == want) | (got.isnan() & want.isnan())
+        assert bool(same.all())
