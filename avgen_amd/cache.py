@@ -121,7 +121,7 @@ def append_paged(
     e4m3: the exponent of a page and head is the least with ``448 * 2 ** e >=``
     the largest finite magnitude of the tokens that this call writes to the page,
     and not below its present one if the page holds earlier tokens of the
-    sequence.  Where that raises it, their codes are rounded again, which changes
+    sequence.  Where that raises it, the page's other codes are rounded again, which changes
     subnormal codes alone; so a page filled token by token and one filled at once
     may differ in those, and in their exponent.  Codes are rounded to
     nearest even from the rotation's fp32 result; infinities become NaN.

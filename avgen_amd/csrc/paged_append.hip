@@ -7,7 +7,8 @@
 // slots of a page and head:
 //   e = least integer with 448 2^e >= max |x| over the new tokens of the page,
 //       and not below the page's exponent where earlier tokens are in it;
-//   if that raises the exponent, the earlier codes become e4m3(c 2^(e' - e)).
+//   if that raises the exponent, the page's other codes become e4m3(c 2^(e' - e)),
+//   those behind the new tokens too: what they stand for stays.
 // A power of two costs e4m3 nothing (its own steps are relative) and makes
 // c 2^e a bf16 value exactly, so readers convert without rounding, and a raised
 // exponent moves codes without rounding them, subnormal ones apart.
@@ -308,7 +309,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
     if (tid == 0) *ep = (int8_t)e;
     uint8_t* out = static_cast<uint8_t*>(key ? a.kp : a.vp) + pp.page * (key ? a.kps : a.vps) + h * (key ? a.kph : a.vph);
     if (pp.lo > 0 && e > e0) {
-      for (int it = tid; it < pp.lo * IPR; it += n) {
+      for (int it = tid; it < IPR << a.pages.shift; it += n) {
+        if (it >= pp.lo * IPR && it < pp.hi * IPR) continue;
         u32x4* c = reinterpret_cast<u32x4*>(out + it * kItem);
         u32x4 y = *c;
 #pragma unroll

@@ -1083,10 +1083,11 @@ int avattn_bwd_scored_row_lse(const void* dout, const void* q,
  * rounded separately, a result once) and writes q rotated to q_out (heads_q 0:
  * no q).  Every row of q is written, whatever counts says.  A token before
  * position 0, behind the table or without a page is left out, and no other
- * slot changes its code.  e4m3: the exponent of a page and head becomes the least e with 448 *
+ * slot changes its value.  e4m3: the exponent of a page and head becomes the least e with 448 *
  * 2^e >= the largest finite magnitude among its new tokens, but not below its
  * present one where earlier tokens of the sequence are in the page; if that
- * raises it, their codes become e4m3(code * 2^(old - e)).  Codes are rounded to
+ * raises it, the page's other codes become e4m3(code * 2^(old - e)).  (A page that the
+ * tokens begin takes its exponent from them alone.)  Codes are rounded to
  * nearest even; what is not finite becomes NaN.  No page may be written for two
  * sequences of a call.
  *

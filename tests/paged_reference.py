@@ -50,7 +50,7 @@ class Pool:
             if lo > 0:
                 e = max(e, old)
                 if e > old:
-                    self.data[page, h, :lo] = codes_of(self.data[page, h, :lo] * 2.0 ** (old - e))
+                    self.data[page, h] = codes_of(self.data[page, h] * 2.0 ** (old - e))
             self.data[page, h, lo:lo + n] = codes_of(rows[h] / 2.0**e)
             self.exponent[page, h] = e
 
