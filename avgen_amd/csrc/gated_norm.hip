@@ -101,6 +101,17 @@ __device__ __forceinline__ void group_vectors(const GatedNormArgs& a, int64_t gr
   if (tv) load_vector<T, CH>(a.t, a.m32, group * a.ts + col, 0.f, tv);
 }
 
+// The same of chunk j, zeros past the end of the row (in 0), where an infinite or
+// NaN entry of column 0 would reach the row's sums through 0 * inf.
+template <int CH>
+__device__ __forceinline__ void mask_vectors(uint32_t in, float* av, float* bv) {
+#pragma unroll
+  for (int e = 0; e < CH; ++e) {
+    av[e] = __uint_as_float(__float_as_uint(av[e]) & in);
+    bv[e] = __uint_as_float(__float_as_uint(bv[e]) & in);
+  }
+}
+
 __device__ __forceinline__ float row_rstd(float ss, const GatedNormArgs& a) {
   return 1.f / __builtin_sqrtf(ss / (float)a.W + a.eps);
 }
@@ -162,6 +173,7 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::fwd) void gated
     in[j] = col < a.W ? 0xffffffffu : 0u;
     off[j] = (uint32_t)at * sizeof(T);
     group_vectors<T, CH>(a, group, at, av[j], bv[j], tv[j]);
+    mask_vectors<CH>(in[j], av[j], bv[j]);
   }
   struct Row {
     Raw<CH> x[NV], r[NV];
@@ -287,7 +299,10 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated
     const int64_t col = (int64_t)(j * TPR + t) * CH, at = col < a.W ? col : 0;
     in[j] = col < a.W ? 0xffffffffu : 0u;
     off[j] = (uint32_t)at * sizeof(T);
-    if constexpr (HOLD) group_vectors<T, CH>(a, group, at, held_a[j], held_b[j], nullptr);
+    if constexpr (HOLD) {
+      group_vectors<T, CH>(a, group, at, held_a[j], held_b[j], nullptr);
+      mask_vectors<CH>(in[j], held_a[j], held_b[j]);
+    }
 #pragma unroll
     for (int e = 0; e < CH; ++e) {
       sn[j][e] = st[j][e] = sc[j][e] = 0.f;
@@ -330,6 +345,7 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated
         for (int e = 0; e < CH; ++e) av[e] = held_a[j][e], bv[e] = held_b[j][e];
       } else {
         group_vectors<T, CH>(a, TOKEN ? row : group, opaque(off[j]) / sizeof(T), av, bv, nullptr);
+        mask_vectors<CH>(in[j], av, bv);
       }
     };
     const f32x2 stats = *reinterpret_cast<const f32x2*>(a.stats + 2 * row);
