@@ -619,7 +619,8 @@ bool chunked(const GatedNormArgs& a, int size) {
   const int64_t ch = 16 / size;
   uintptr_t p = 0;
   for (const void* q : {a.x, a.r, a.dn, a.dh, (const void*)a.h, (const void*)a.n, (const void*)a.dx,
-                        (const void*)a.dr, a.w, a.p, a.g, a.s, a.t})
+                        (const void*)a.dr, a.w, a.p, a.g, a.s, a.t, (const void*)a.dg, (const void*)a.ds,
+                        (const void*)a.dt})
     p |= reinterpret_cast<uintptr_t>(q);
   bool ok = p % 16 == 0 && a.W % ch == 0;
   for (int64_t s : {a.xs, a.rs, a.dns, a.dhs, a.gs, a.ss, a.ts}) ok = ok && s % ch == 0;
