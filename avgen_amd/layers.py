@@ -131,7 +131,7 @@ def _one_modulation(shape, *given):
     first = next((t for t in given if t is not None), None)
     if first is None:
         return given
-    if first.ndim == len(shape) and first.shape[-2] == 1 and first.shape[0] == shape[0] and first.ndim == 3:
+    if first.ndim == 3 == len(shape) and first.shape[-2] == 1 and first.shape[0] == shape[0]:
         # A row per sample, as a modulation's projection has it.
         if first.shape[-1] == shape[-1] and all(t is None or t.shape == first.shape for t in given):
             return given
