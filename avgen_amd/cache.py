@@ -31,7 +31,10 @@ class PagedCache:
     Token ``t`` of a sequence is in slot ``t % page_size`` of the page that its
     block table names at ``t // page_size``.  With e4m3, ``key_exponent`` and
     ``value_exponent`` (int8 ``(pages, heads)``) scale a page's codes: a value is
-    ``code * 2 ** exponent``, which bfloat16 holds exactly.
+    ``code * 2 ** exponent``, which bfloat16 holds exactly for the exponents that
+    :func:`append_paged` chooses, -110 to 119.  Pages that a program fills itself may
+    have any: past 119 the largest values are infinite in bfloat16, and attention takes
+    -127 and -128 as -126.
 
     page_size is 16, 32, 64, 128 or 256, head_dim 64 or 128; the slots of a page
     and head are contiguous, pages and heads may have any strides of whole 16

@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
         *c = y;
       }
     }
-    const float unit = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float unit = ldexpf(1.f, -e);  // (a page's own exponent may be 127: 2^-127 is subnormal)
 #pragma unroll
     for (int m = 0; m < NI; ++m) {
       const int it = m * n + tid, slot = it / IPR, u = it % IPR;
