@@ -425,12 +425,16 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(FwdArgs a, PagedArgs p,
 
 }  // namespace
 
-// Few rows or many: the smaller of two estimates, both within about a sixth of
-// what was measured (us, few-row against general):
-//   e4m3, 32 heads over 8 of 128, 12,000 keys: 33 tokens 29, 65; 128 56, 69; 192 92, 72; 512 169, 110
-//   the same twice: 96 tokens 92, 106; 192 166, 113; bf16: 64 tokens 85, 112; 96 147, 115
-//   e4m3, 64 heads over 8, 1,000 keys: 96 tokens 21, 30; 256 23, 33; 512 40, 34
-//   e4m3, 16 heads over 2 of 64, 12,000 keys: 128 tokens 33, 41; 192 45, 43; 512 85, 49
+// Few rows or many: the smaller of two estimates, both for sequences that fill
+// their room (us, few-row against general):
+//   e4m3, 32 heads over 8 of 128, 12,000 keys: 33 tokens 27, 64; 128 54, 68; 192 86, 70; 512 164, 105
+//   the same twice: 96 tokens 89, 102; 192 140, 109; bf16: 64 tokens 88, 110; 96 128, 113
+//   bf16, eight sequences of 4,000: 48 tokens 130, 136; 96 160, 141; of 1,000: 64 49, 39
+//   e4m3, 64 heads over 8, 1,000 keys: 96 tokens 18, 31; 256 23, 33; 512 39, 34
+//   e4m3, 16 heads over 2 of 64, 12,000 keys: 128 tokens 33, 41; 192 44, 43; 512 82, 49
+// Of 460 such shapes (1 to 8 sequences, 17 to 512 tokens, both types) the slower way
+// is taken at seven by 8 to 15 %, else by 4 % at most.  Near the crossing nine of ten
+// estimates are within a quarter of what was measured.
 // The few-row kernel computes no row that is not there (its blocks hold rows of all
 // heads of a kv head) and needs no copy; the general one has twice its rate.
 // Its split n of a block's keys is the fastest by the same estimate: whole rounds
@@ -451,14 +455,9 @@ FewPlan paged_plan(int B, int Hq, int Hkv, int Lq, int64_t cap, int window, int 
   const float tile_us = D == 64 ? 1.6f : (fp8 ? 1.9f : 1.5f);
   const float slot_bytes = 4.f * few_slot_floats(p.block_rows, D);
   const int64_t slots = kCus * per_cu, tiles = reach / kTile + 1, most = (tiles + kWaves - 1) / kWaves;
-  // Of a batch, what the sequences hold of their room on the mean; the workgroups of the
-  // longest end last, so more rounds of smaller ones pay (16 sequences of 1,016 to
-  // 16,001 keys 126 us in one round, 106 in two; e4m3 77, 66; alike ones 104, 107).
-  const float filled = window > 0 ? 1.f : 0.75f;
-  float best = 0.f;
-  auto consider = [&](int64_t n) {
-    if (n > most) n = most;
-    if (n < 1 || units * n > kMaxGrid) return;
+  // A call's time with n parts, its sequences holding `filled` of their room on the
+  // mean and the longest all of it.
+  auto estimate = [&](int64_t n, float filled) {
     const int64_t grid = units * n, rem = grid % slots;
     const int64_t mine = ((tiles + n - 1) / n + kWaves - 1) / kWaves;
     float us;
@@ -470,16 +469,31 @@ FewPlan paged_plan(int B, int Hq, int Hkv, int Lq, int64_t cap, int window, int 
       const float mean = (float)grid / slots * (mine * tile_us * filled + 5.f) + 0.4f * longest;
       us = longest > mean ? longest : mean;
     }
-    us = 0.88f * (us + 6.f + (n > 1 ? 3.f + grid * slot_bytes * 2.f / 3.5e6f : 0.f));
+    return 0.88f * (us + 6.f + (n > 1 ? 3.f + grid * slot_bytes * 2.f / 3.5e6f : 0.f));
+  };
+  // The workgroups of a batch's longest sequences end last, so more rounds of smaller
+  // ones pay (16 sequences of 1,016 to 16,001 keys 126 us in one round, 106 in two; e4m3
+  // 77, 66; alike ones 104, 107).
+  const float filled = window > 0 ? 1.f : 0.75f;
+  float best = 0.f;
+  auto consider = [&](int64_t n) {
+    if (n > most) n = most;
+    if (n < 1 || units * n > kMaxGrid) return;
+    const float us = estimate(n, filled);
     if (p.nsplit == 0 || us < best) best = us, p.nsplit = (int)n;
   };
   consider(1);
   for (int64_t r = 1; r <= 4; ++r) consider(r * slots / units);  // whole rounds
   if (per_cu > 1) consider(kCus / units);
-  // Three launches, the copy of the pages, the general forward.
-  const float copy = (float)(B * Hkv) * (float)reach * D * 2.f * (fp8 ? 3.f : 4.f) / 4.5e6f;
-  const float forward = 0.7f * fwd_split_plan(B, Hq, Lq, (int)reach, D, false, false).us;
-  if (rows > kFewRows && 18.f + copy + (forward > 10.f ? forward : 10.f) < best) return FewPlan{};
+  // Against three launches, the copy of the pages (from and to caches in part) and the
+  // general forward, whose work follows the sequences' lengths likewise: so both with the
+  // room full.  Two workgroups on a CU fill each other's waits over a batch's many
+  // rounds; bf16 rows of 128 run into the caches' rate, each block reading all pages.
+  const float rate = per_cu == 1 ? 1.1f : (B == 1 ? 1.f : (D == 64 ? 0.82f : 0.78f));
+  const float copy = (float)(B * Hkv) * (float)reach * D * 2.f * (fp8 ? 3.f : 4.f) / 9e6f;
+  const float forward = fwd_split_plan(B, Hq, Lq, (int)reach, D, false, false).us;
+  const float general = 18.f + copy + 0.65f * (forward > 14.f ? forward : 14.f);
+  if (rows > kFewRows && general < rate * estimate(p.nsplit, 1.f)) return FewPlan{};
   p.bytes = p.nsplit > 1 ? (size_t)units * p.nsplit * few_slot_floats(p.block_rows, D) * sizeof(float) : 0;
   return p;
 }
