@@ -139,11 +139,14 @@ def append_paged(
     """
     half = _half_layout(layout)
     cos = sin = None
-    rotated = query
+    rotated, start = query, int(start)
     if tables is not None:
+        if not 0 <= start < max(ops.SUPPORTED_HEAD_DIMS):
+            raise ValueError(f"start must be a channel of the head; got {start}")
         cos, sin = tables.cos, tables.sin
         rotated = None
-    out = cache_ops.append_paged(key, value, query if tables is not None else None, cos, sin, int(start), half,
+    out = cache_ops.append_paged(key, value, query if tables is not None else None, cos, sin,
+                                 0 if tables is None else start, half,
                                  block_table, lengths, counts, cache.key, cache.value, cache.key_exponent,
                                  cache.value_exponent)
     return out if rotated is None else rotated
@@ -190,8 +193,8 @@ def paged_attention(
     """
     if softcap is not None and not softcap > 0.0:
         raise ValueError(f"softcap must be positive or None; got {softcap}")
-    if window is not None and window < 1:
-        raise ValueError(f"window must be positive or None; got {window}")
+    if window is not None and not 1 <= window <= cache_ops.MAX_WINDOW:
+        raise ValueError(f"window must be from 1 to {cache_ops.MAX_WINDOW} or None; got {window}")
     return cache_ops.paged_attention(
         query, cache.key, cache.value, cache.key_exponent, cache.value_exponent, block_table, lengths, counts,
         distance_slopes, 0 if window is None else int(window),
