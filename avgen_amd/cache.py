@@ -191,7 +191,7 @@ def paged_attention(
         ValueError, TypeError: shapes, types or values other than these.
         RuntimeError: a tensor not on the GPU, or one that requires grad.
     """
-    if softcap is not None and not softcap > 0.0:
+    if softcap is not None and not softcap >= torch.finfo(torch.float32).smallest_normal:  # (0 would be none)
         raise ValueError(f"softcap must be positive or None; got {softcap}")
     if window is not None and not 1 <= window <= cache_ops.MAX_WINDOW:
         raise ValueError(f"window must be from 1 to {cache_ops.MAX_WINDOW} or None; got {window}")

@@ -21,3 +21,10 @@ def test_starts_out_of_range(start):
         append_paged(POOL, K, K, TABLE, LEN, tables=T, start=start)
     with pytest.raises(RuntimeError, match="no CPU path"):  # no rotation: no channel to start at
         append_paged(POOL, K, K, TABLE, LEN, start=start)
+
+
+@pytest.mark.parametrize("softcap", [0.0, -1.0, 1e-60, 1e-40, float("nan"), float("inf"), 1025.0])
+def test_caps_out_of_range(softcap):
+    """Also those that are 0 in float32, which stands for none."""
+    with pytest.raises(ValueError, match="softcap"):
+        paged_attention(Q, POOL, TABLE, LEN, softcap=softcap)
