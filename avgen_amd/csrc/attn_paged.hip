@@ -222,7 +222,8 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
 #pragma unroll
       for (int i = 0; i < TE / 8 / 64; ++i) {
         const int c = i * 64 + lane, row = c / (RL / 8);
-        if (!(keys >> row & 1)) *reinterpret_cast<u32x4*>(sg.v + TileLayout<RL>::off(row, 8 * (c % (RL / 8)))) = u32x4{};
+        if (!(keys >> row & 1))
+          *reinterpret_cast<u32x4*>(sg.v + TileLayout<RL>::off(row, 8 * (c % (RL / 8)))) = u32x4{};
       }
     }
     // Register 8*k2 + e of lane l: key 16*k2 + 8*hh + e of the tile, row l32.

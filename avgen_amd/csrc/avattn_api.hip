@@ -1638,12 +1638,13 @@ size_t avattn_gated_add_rms_norm_bwd_workspace_size(int64_t rows, int64_t width,
 int avattn_gated_add_rms_norm_bwd(const void* dnorm, int64_t dnorm_row_stride, const void* dsum,
                                   int64_t dsum_row_stride, const void* x, int64_t x_row_stride, const void* residual,
                                   int64_t residual_row_stride, const float* stats, const void* weight,
-                                  int32_t weight_is_f32, const void* post_weight, int32_t post_weight_is_f32, const void* gate,
-                                  int64_t gate_stride, const void* scale, int64_t scale_stride, const void* shift,
-                                  int64_t shift_stride, int32_t modulation_is_f32, int64_t rows, int64_t width,
-                                  int64_t group_rows, int32_t is_f32, float residual_scale, float eps, void* dx,
-                                  void* dresidual, void* dweight, void* dpost_weight, void* dgate, void* dscale,
-                                  void* dshift, void* workspace, size_t workspace_bytes, avattn_stream_t stream) {
+                                  int32_t weight_is_f32, const void* post_weight, int32_t post_weight_is_f32,
+                                  const void* gate, int64_t gate_stride, const void* scale, int64_t scale_stride,
+                                  const void* shift, int64_t shift_stride, int32_t modulation_is_f32, int64_t rows,
+                                  int64_t width, int64_t group_rows, int32_t is_f32, float residual_scale, float eps,
+                                  void* dx, void* dresidual, void* dweight, void* dpost_weight, void* dgate,
+                                  void* dscale, void* dshift, void* workspace, size_t workspace_bytes,
+                                  avattn_stream_t stream) {
   GatedNormArgs a{};
   const int st = gated_args(weight, weight_is_f32, post_weight, post_weight_is_f32, gate, gate_stride, scale,
                             scale_stride, shift, shift_stride, modulation_is_f32, rows, width, group_rows, is_f32,

@@ -62,8 +62,8 @@ Bound bound;
 // see.)
 bool ordinary_state() {
   return c10::impl::TorchDispatchModeTLS::stack_len() == 0 && at::impl::PythonTorchFunctionTLS::stack_len() == 0 &&
-         !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) && !torch::jit::tracer::isTracing() &&
-         !torch::profiler::impl::profilerEnabled();
+         !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) &&
+         !torch::jit::tracer::isTracing() && !torch::profiler::impl::profilerEnabled();
 }
 
 // On the current device, with the key set of an ordinary tensor (made in or out of

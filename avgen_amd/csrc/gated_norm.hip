@@ -761,7 +761,8 @@ hipError_t backward(const GatedNormArgs& all, hipStream_t stream) {
   const RowShape s = row_shape(a.W, chunked(a, sizeof(T)) ? 16 / (int)sizeof(T) : 1,
                                a.R == 1 && modulated ? a.rows : a.R);
   const int rpb = s.nv > 0 && s.size == 0 ? 256 / s.tpr : 1;
-  const Workgroups w = bwd_workgroups(a.rows, a.R, rpb, s.nv == 0 ? kAny / 64 : (s.size == 0 ? 4 : s.tpr / 64), modulated);
+  const int waves = s.nv == 0 ? kAny / 64 : (s.size == 0 ? 4 : s.tpr / 64);
+  const Workgroups w = bwd_workgroups(a.rows, a.R, rpb, waves, modulated);
   a.per_group = w.per_group;
   a.tpr = s.tpr;
   hipError_t e;

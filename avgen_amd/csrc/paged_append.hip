@@ -307,7 +307,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int nkv) {
     int e = code_exponent(top);
     if (pp.lo > 0) e = max(e, e0);
     if (tid == 0) *ep = (int8_t)e;
-    uint8_t* out = static_cast<uint8_t*>(key ? a.kp : a.vp) + pp.page * (key ? a.kps : a.vps) + h * (key ? a.kph : a.vph);
+    uint8_t* out = static_cast<uint8_t*>(key ? a.kp : a.vp);
+    out += pp.page * (key ? a.kps : a.vps) + h * (key ? a.kph : a.vph);
     if (pp.lo > 0 && e > e0) {
       for (int it = tid; it < IPR << a.pages.shift; it += n) {
         if (it >= pp.lo * IPR && it < pp.hi * IPR) continue;

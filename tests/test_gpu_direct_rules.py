@@ -48,9 +48,9 @@ def append_args(dtype):
 
 def norm_args(dtype):
     one = lambda n: normal((1, 1, 40), n, dtype)  # noqa: E731
-    return dict(x=normal((B, L, 40), 10, dtype), residual=normal((B, L, 40), 11, dtype), weight=normal((40,), 12, dtype),
-                post_weight=normal((40,), 13, dtype), gate=one(14), scale=one(15), shift=one(16), residual_scale=0.5,
-                eps=1e-6)
+    return dict(x=normal((B, L, 40), 10, dtype), residual=normal((B, L, 40), 11, dtype),
+                weight=normal((40,), 12, dtype), post_weight=normal((40,), 13, dtype), gate=one(14), scale=one(15),
+                shift=one(16), residual_scale=0.5, eps=1e-6)
 
 
 def copied(args):
@@ -85,7 +85,7 @@ def run(kind, args, direct):
         return [out if direct else out[0]]
     if kind == "norm":
         return list(out[:2])
-    written = [a["key_pages"], a["value_pages"]] + [a[n] for n in ("key_exponent", "value_exponent") if a[n] is not None]
+    written = [a[n] for n in ("key_pages", "value_pages", "key_exponent", "value_exponent") if a[n] is not None]
     return ([out] if a["query"] is not None else []) + written
 
 
@@ -172,7 +172,8 @@ ATTEND = [
     ("refuse", "a query without a batch", lambda a: dict(q=a["q"][0])),
     ("refuse", "another head size", lambda a: dict(q=torch.cat([a["q"]] * 2, 3))),
     ("refuse", "heads that do not divide", lambda a: dict(q=a["q"][:, :7], slopes=None)),
-    ("refuse", "too many heads with slopes", lambda a: dict(q=normal((B, 130, L, D), 3), slopes=normal((130,), 4, F32))),
+    ("refuse", "too many heads with slopes", lambda a: dict(q=normal((B, 130, L, D), 3),
+                                                               slopes=normal((130,), 4, F32))),
 ]
 APPEND = [
     ("take", "no query", lambda a: dict(query=None)),
@@ -186,7 +187,8 @@ APPEND = [
     ("refuse", "one table", lambda a: dict(sin=None)),
     ("refuse", "tables of another length", lambda a: {n: a[n][:, :, :2].contiguous() for n in ("cos", "sin")}),
     ("refuse", "tables of heads", lambda a: {n: a[n].expand(-1, 2, -1, -1).contiguous() for n in ("cos", "sin")}),
-    ("refuse", "tables of another batch", lambda a: {n: a[n].expand(3, -1, -1, -1).contiguous() for n in ("cos", "sin")}),
+    ("refuse", "tables of another batch", lambda a: {n: a[n].expand(3, -1, -1, -1).contiguous()
+                                                     for n in ("cos", "sin")}),
     ("refuse", "tables of different sizes", lambda a: dict(sin=a["sin"][..., :8].contiguous())),
     ("refuse", "float64 tables", lambda a: {n: a[n].double() for n in ("cos", "sin")}),
     ("refuse", "no pairs", lambda a: {n: a[n][..., :0] for n in ("cos", "sin")}),
@@ -204,7 +206,8 @@ NORM = [
     ("take", "a row per sample", lambda a: {n: a[n].expand(B, 1, 40).contiguous() for n in ("gate", "scale", "shift")}),
     ("take", "one row for all samples", lambda a: {n: a[n].expand(B, 1, 40) for n in ("gate", "scale", "shift")}),
     ("take", "a row per token", lambda a: {n: a[n].expand(B, L, 40).contiguous() for n in ("gate", "scale", "shift")}),
-    ("take", "float32 vectors", lambda a: {n: a[n].float() for n in ("weight", "post_weight", "gate", "scale", "shift")}),
+    ("take", "float32 vectors", lambda a: {n: a[n].float()
+                                           for n in ("weight", "post_weight", "gate", "scale", "shift")}),
     ("take", "unaligned rows", lambda a: dict(x=other(a["x"]))),
     ("take", "rows apart", lambda a: dict(x=torch.cat([a["x"]] * 2, 2)[..., :40])),
     ("take", "the same twice", lambda a: dict(residual=a["x"])),
@@ -225,7 +228,8 @@ NORM = [
     ("refuse", "a gate and a scale of two shapes", lambda a: dict(gate=a["gate"].expand(B, 1, 40).contiguous())),
     ("refuse", "rows that no groups divide", lambda a: {n: a[n].expand(4, 1, 40).contiguous()
                                                         for n in ("gate", "scale", "shift")}),
-    ("refuse", "a gate of another width", lambda a: {n: a[n][..., :39].contiguous() for n in ("gate", "scale", "shift")}),
+    ("refuse", "a gate of another width", lambda a: {n: a[n][..., :39].contiguous()
+                                                     for n in ("gate", "scale", "shift")}),
     *(("refuse", f"eps {e}", lambda a, e=e: dict(eps=e)) for e in (-1.0, NAN, INF, 1e39)),
     *(("refuse", f"factor {e}", lambda a, e=e: dict(residual_scale=e)) for e in (NAN, INF, -1e39)),
     ("refuse", "a residual on the CPU", lambda a: dict(residual=a["residual"].cpu())),
@@ -280,7 +284,8 @@ def test_vmap_over_a_pool(dtype):
     before = bits(cache.key).clone()
     k = normal((B, 1, H, L, D), 21)
     with pytest.raises(RuntimeError, match="[Bb]atching rule"):
-        torch.vmap(lambda k, t, n: append_paged(cache, k, k, t[None], n[None], query=k))(k, a["block_table"], a["lengths"])
+        torch.vmap(lambda k, t, n: append_paged(cache, k, k, t[None], n[None], query=k))(k, a["block_table"],
+                                                                                        a["lengths"])
     assert torch.equal(bits(cache.key), before)
 
 
