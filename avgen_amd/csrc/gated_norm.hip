@@ -271,15 +271,16 @@ __global__ __launch_bounds__(kAny) void gated_norm_any_kernel(GatedNormArgs a) {
 // Backward.  Workgroups take rows of a group in turn, as many at once as they
 // have workers, and leave a part of the sums each; with a row of g, s and t per token
 // (TOKEN) they take all rows, write that token's ds, dt and dg and keep the sums of
-// dw and dp.  Rows are loaded ahead of their sums (two of them ahead where the
-// registers are there: (18,900, 5,120) bf16 285 -> 256 us; with p they are not: 250 ->
-// 274).  Rows of up to a workgroup of 1,024 threads leave room for 128 registers a
-// thread: two of the three sums are in LDS then, and A and b are read again
-// for each row of two or more chunks a thread.
+// dw and dp.  A row is loaded ahead of the last one's sums ((18,900, 5,120) bf16 233
+// us; two ahead are no faster, nor with p: 244).  Rows of up to a workgroup of 1,024
+// threads leave room for 128 registers a thread: two of the three sums are in LDS then,
+// and of two or more chunks a thread, A and b are read again for each row and none is
+// loaded ahead (2,000 rows of 16,384, bf16 148 us, float32 367, where their bytes take 77
+// and 155).
 template <class T, int CH, int NV, int SIZE, bool POST, bool TOKEN>
 __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated_norm_bwd_kernel(GatedNormArgs a) {
   constexpr bool WAVE = SIZE == 0, LDS = SIZE == 3, HOLD = !TOKEN && NV * CH <= 8;
-  constexpr int AHEAD = SIZE == 3 && NV > 1 ? 0 : (SIZE == 2 && !POST && !TOKEN ? 2 : 1);
+  constexpr bool AHEAD = SIZE != 3 || NV == 1;
   constexpr int NS = POST ? 3 : 1, MOST = Threads<SIZE>::most;
   __shared__ float red[2][NS][16];
   __shared__ __attribute__((aligned(16))) float acc[LDS ? 2 * NV * MOST * CH : (WAVE ? 256 * NV * CH : 4)];
@@ -323,16 +324,12 @@ __global__ __launch_bounds__(Threads<SIZE>::most, Threads<SIZE>::bwd) void gated
       if (a.dh != nullptr) q.d[j] = read_at<T, CH>(a.dh, row, a.dhs, off[j]);
     }
   };
-  Row next, later;
-  if (AHEAD > 0) load(row0, next);
-  if (AHEAD > 1) load(row0 + step, later);
+  Row next;
+  if (AHEAD) load(row0, next);
   int buf = 0;
   for (int64_t row = row0; row < end; row += step) {  // the same for a row's threads
     Row cur;
-    if constexpr (AHEAD > 1) {
-      cur = next, next = later;
-      load(row + 2 * step, later);
-    } else if constexpr (AHEAD > 0) {
+    if constexpr (AHEAD) {
       cur = next;
       load(row + step, next);
     } else {
@@ -713,8 +710,8 @@ hipError_t forward(const GatedNormArgs& all, hipStream_t stream) {
 }
 
 // Workgroups of the backward: of a group (TOKEN: in all).  A round of them: more
-// leave more parts of the sums ((18,900, 5,120) bf16 420 us forward and backward
-// with two rounds, 410 with one), and no fewer than two rows for each worker.
+// leave more parts of the sums ((18,900, 5,120) bf16 402 us forward and backward
+// with two rounds, 393 with one; (8,000, 2,560) with both norms 130, 123), and no fewer than two rows for each worker.
 struct Workgroups {
   int64_t groups, per_group;
   bool token;
