@@ -121,13 +121,15 @@ def append_paged(
         query: bf16 ``(batch, query heads, length, head_dim)``.  Every row is
             rotated, padding included.
 
-    e4m3: the exponent of a page and head is the least with ``448 * 2 ** e >=``
-    the largest finite magnitude of the tokens that this call writes to the page,
-    and not below its present one if the page holds earlier tokens of the
-    sequence.  Where that raises it, the page's other codes are rounded again, which changes
-    subnormal codes alone; so a page filled token by token and one filled at once
-    may differ in those, and in their exponent.  Codes are rounded to
-    nearest even from the rotation's fp32 result; infinities become NaN.
+    e4m3: the exponent of a page and head is the least from -110 to 119 with ``448 *
+    2 ** e >=`` the largest finite magnitude of the tokens that this call writes to the
+    page (past that they saturate), and not below its present one if the page holds
+    earlier tokens of the sequence.  Where that raises it, the page's other codes are
+    rounded again, which changes subnormal codes alone; so a page filled token by token
+    and one filled at once may differ in those, and in their exponent.  Of a page that
+    the tokens begin, slots behind them keep their codes under the new exponent: they
+    hold no token.  Codes are rounded to nearest even from the rotation's fp32 result;
+    infinities become NaN.
 
     A page belongs to one sequence while it is written: sequences may share pages
     that are full.  Writing the same tokens again gives the same pages.  Not
@@ -170,8 +172,8 @@ def paged_attention(
     Args:
         query: bf16 ``(batch, heads, length, head_dim)``, heads a multiple of
             the cache's.
-        block_table, lengths, counts: as for :func:`append_paged`.  Query ``i`` is at position ``p =
-            lengths - counts + i`` and sees the keys ``0 .. p``.
+        block_table, lengths, counts: as for :func:`append_paged`.  Query ``i`` is at
+            position ``p = lengths - counts + i`` and sees the keys ``0 .. p``.
         window: see the keys ``p - window + 1 .. p`` only.  Pages in front
             of every query's window are not read: their entries may be ``-1``.
         softcap, distance_slopes, scale: as for
@@ -183,9 +185,14 @@ def paged_attention(
     padding, and rows whose keys have no page, are zeros.  Slots outside the
     hull of a sequence's windows may hold anything.  Up to some hundred rows (by
     an estimate of both ways' times, from the sizes) read the pages in place, the
-    keys split over the chip; more go over a copy in bfloat16 of the pages
-    that the table has room for, so pass the part of the table that is in
-    use.  Not differentiable.
+    keys split over the chip; more go over a copy in bfloat16 of the pages, with
+    memory for all that the table has room for.  Which way, how the keys are split and
+    that memory follow the table's room, since the host does not know the lengths: pass
+    the part of the table that is in use.  A captured step needs the room of the
+    longest sequence that it is to serve, and shorter ones pay for it: with 16 times the
+    room in use single tokens take up to a third longer, 64 tokens up to twice as long,
+    512 a quarter to nine tenths (and 4 bytes of copies for each channel and slot of that
+    room); so capture one for each of a few rooms.  Not differentiable.
 
     Raises:
         ValueError, TypeError: shapes, types or values other than these.

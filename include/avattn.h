@@ -1082,14 +1082,16 @@ int avattn_bwd_scored_row_lse(const void* dout, const void* q,
  * slots, the keys rotated as by avattn_rotate (cos_tab NULL: not; a product
  * rounded separately, a result once) and writes q rotated to q_out (heads_q 0:
  * no q).  Every row of q is written, whatever counts says.  A token before
- * position 0, behind the table or without a page is left out, and no other
- * slot changes its value.  e4m3: the exponent of a page and head becomes the least e with 448 *
- * 2^e >= the largest finite magnitude among its new tokens, but not below its
- * present one where earlier tokens of the sequence are in the page; if that
- * raises it, the page's other codes become e4m3(code * 2^(old - e)).  (A page that the
- * tokens begin takes its exponent from them alone.)  Codes are rounded to
- * nearest even; what is not finite becomes NaN.  No page may be written for two
- * sequences of a call.
+ * position 0, behind the table or without a page is left out.  Other slots of a
+ * bf16 page stay as they are.  e4m3: the exponent of a page and head becomes the
+ * least e from -110 to 119 with 448 * 2^e >= the largest finite magnitude among its
+ * new tokens (larger ones saturate), but not below its present one where earlier
+ * tokens of the sequence are in the page; if that raises it, the page's other codes
+ * become e4m3(code * 2^(old - e)), those behind the new tokens too, so that all keep
+ * their values but for subnormal codes' roundings.  A page that the tokens begin
+ * takes its exponent from them alone, and the codes behind them stay, so that their
+ * values change with it: no token is there.  Codes are rounded to nearest even; what
+ * is not finite becomes NaN.  No page may be written for two sequences of a call.
  *
  * avattn_page_values: bf16 values of all pages of an e4m3 pool, contiguous
  * (pages, heads, page_size, head_dim).
