@@ -275,7 +275,10 @@ __global__ __launch_bounds__(256, FP8 || D == 64 ? 2 : 1) void attn_paged_kernel
         const float p0 = __builtin_amdgcn_exp2f(s[8 * k2 + 2 * e2] - mc);
         const float p1 = __builtin_amdgcn_exp2f(s[8 * k2 + 2 * e2 + 1] - mc);
         l += p0 + p1;
-        u[e2] = pack_bf16x2(p0, p1);  // the PV operand, rounded as in the general forward
+        // The PV operand in bf16, as in the general forward, for the bf16 products: as
+        // much of the result's error (0.0010 of 0.0020) as its own rounding leaves room
+        // for.  The sum takes the unrounded ones.
+        u[e2] = pack_bf16x2(p0, p1);
       }
       pf[k2] = bits_to_bf16x8(u);
     }
@@ -433,9 +436,9 @@ __global__ __launch_bounds__(256) void prep_paged_kernel(FwdArgs a, PagedArgs p,
 //   bf16, eight sequences of 4,000: 48 tokens 130, 136; 96 160, 141; of 1,000: 64 49, 39
 //   e4m3, 64 heads over 8, 1,000 keys: 96 tokens 18, 31; 256 23, 33; 512 39, 34
 //   e4m3, 16 heads over 2 of 64, 12,000 keys: 128 tokens 33, 41; 192 44, 43; 512 82, 49
-// Of 460 such shapes (1 to 8 sequences, 17 to 512 tokens, both types) the slower way
-// is taken at seven by 8 to 15 %, else by 4 % at most.  Near the crossing nine of ten
-// estimates are within a quarter of what was measured.
+// Of 576 such shapes (1 to 16 sequences, alike, of a quarter of their room on, or with
+// windows; up to 512 tokens, both types) the slower way is taken at 17 by 5 to 25 %.  Near
+// the crossing nine of ten estimates are within a quarter of what was measured.
 // The few-row kernel computes no row that is not there (its blocks hold rows of all
 // heads of a kv head) and needs no copy; the general one has twice its rate.
 // Its split n of a block's keys is the fastest by the same estimate: whole rounds
@@ -487,10 +490,12 @@ FewPlan paged_plan(int B, int Hq, int Hkv, int Lq, int64_t cap, int window, int 
   for (int64_t r = 1; r <= 4; ++r) consider(r * slots / units);  // whole rounds
   if (per_cu > 1) consider(kCus / units);
   // Against three launches, the copy of the pages (from and to caches in part) and the
-  // general forward, whose work follows the sequences' lengths likewise: so both with the
-  // room full.  Two workgroups on a CU fill each other's waits over a batch's many
-  // rounds; bf16 rows of 128 run into the caches' rate, each block reading all pages.
-  const float rate = per_cu == 1 ? 1.1f : (B == 1 ? 1.f : (D == 64 ? 0.82f : 0.78f));
+  // general forward, both for sequences that fill their room.  Two workgroups on a CU
+  // fill each other's waits over a batch's many rounds; bf16 rows of 128 run into the
+  // caches' rate, each block reading all pages, though of a batch's shorter sequences less,
+  // while the general forward's time is that of the longest (four sequences of 3,000 to
+  // 12,000 keys, 64 tokens: 158 in place, 188; all of 12,000: 228, 212).
+  const float rate = per_cu == 1 ? (B == 1 ? 1.16f : 1.04f) : (B == 1 ? 1.f : (D == 64 ? 0.82f : 0.78f));
   const float copy = (float)(B * Hkv) * (float)reach * D * 2.f * (fp8 ? 3.f : 4.f) / 9e6f;
   const float forward = fwd_split_plan(B, Hq, Lq, (int)reach, D, false, false).us;
   const float general = 18.f + copy + 0.65f * (forward > 14.f ? forward : 14.f);
